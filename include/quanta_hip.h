@@ -271,6 +271,98 @@ int qh_sample_ws(const float* logits, int32_t n_valid, const int32_t* rows, cons
                  const int32_t* history, int32_t n_hist, const qh_sampler_params* params, uint64_t* state,
                  int32_t* out_id, void* ws, size_t ws_bytes, void* stream);
 
+/* ------------------------------------------------------------------ 8-bit paged key / value cache */
+
+/* A key / value cache in 8 bits for many sequences, in pages that sequences may share. A block is 16 tokens of one KV
+ * head, keys and values apart: int8 codes and one f32 scale d, which stand for code * d. A page holds page_tokens tokens
+ * of every KV head (its layout is the library's own; qh_kv8_read gives values back). One page number names the same
+ * tokens in every layer. All memory is the caller's; the calls below only enqueue work, take no memory of their own and
+ * can be captured in a HIP graph (the lists they read are DEVICE arrays, read when the work runs). Calls that change one
+ * cache have to be in order; calls that overlap must not share a workspace.
+ * No counterpart in the reference, whose cache holds one sequence in f16 or f32 (model.cpp:96-104, 197-204). */
+#define QH_KV8_BLOCK 16
+#define QH_KV8_MAX_SEQS 32768
+#define QH_KV8_MAX_PAGES (1 << 20)
+
+typedef struct qh_kv8_cache {
+    void* pages;     /* [n_layers][n_pages][qh_kv8_page_bytes(page_tokens, n_kv_heads, head_dim)], 16-byte aligned */
+    int32_t* table;  /* [n_seqs][seq_pages]: the page of a sequence's tokens [j * page_tokens, (j + 1) * page_tokens) */
+    int32_t* lens;   /* [n_seqs]: tokens of the sequence */
+    int32_t* refs;   /* [n_pages]: how many sequences hold the page; 0: free */
+    int32_t* status; /* one: QH_KV8_* bits that calls on this cache have set (cleared by qh_kv8_reset or the caller) */
+    int32_t n_layers, n_pages;
+    int32_t page_tokens; /* a power of two, 16 to 256 */
+    int32_t n_kv_heads;
+    int32_t head_dim; /* 64 or 128 */
+    int32_t n_seqs, seq_pages;
+} qh_kv8_cache;
+
+/* Bits of *status. */
+enum {
+    QH_KV8_NO_PAGES = 1, /* resize or fork: too few free pages */
+    QH_KV8_BAD_LIST = 2, /* a sequence number or length out of range, or a sequence named twice: the call did nothing */
+    QH_KV8_SHARED = 4    /* append: tokens in a page that other sequences hold were not stored */
+};
+
+/* Bytes of one page (0 for an unsupported shape). */
+size_t qh_kv8_page_bytes(int page_tokens, int n_kv_heads, int head_dim);
+
+/* Every page free, every sequence empty, status 0 (page contents are left). A new cache's state arrays need it. */
+int qh_kv8_reset(const qh_kv8_cache* c, void* stream);
+
+/* Workspace bytes of qh_kv8_resize, qh_kv8_fork and qh_kv8_compact (4-byte aligned, no initialisation). */
+size_t qh_kv8_pages_workspace_bytes(const qh_kv8_cache* c);
+
+/* Sequence seqs[i] gets length lens[i] (DEVICE arrays of n; each sequence once), for every i of the list at once. First
+ * the shorter ones give back the pages past their new length (0: all of them); then the longer ones take the lowest free
+ * pages, in the list's order. A last page that is partly filled and also held by other sequences is replaced by a copy of
+ * it when its sequence grows, so that new tokens go into the sequence's own page. With fewer free pages than the longer
+ * ones need, none of them grows and QH_KV8_NO_PAGES is set. Tokens between the old and the new length have no values
+ * until qh_kv8_append stores them. */
+int qh_kv8_resize(const qh_kv8_cache* c, const int32_t* seqs, const int32_t* lens, int n, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
+/* Sequence dst[i] becomes a fork of src[i] (DEVICE arrays of n; each dst once and in no place of src): its pages are
+ * given back, and it holds src[i]'s tokens: src[i]'s pages, shared (copy 0), or copies of them in the lowest free pages
+ * (copy 1; with too few of them every listed dst stays empty and QH_KV8_NO_PAGES is set). */
+int qh_kv8_fork(const qh_kv8_cache* c, const int32_t* src, const int32_t* dst, int n, int copy, void* workspace,
+                size_t workspace_bytes, void* stream);
+
+/* Moves the pages in use to the front: with L of them, those numbered L and above move, in order, to the free numbers
+ * below L, in every layer, and the tables follow. *live (DEVICE, may be NULL) = L: the pages from L on are free. */
+int qh_kv8_compact(const qh_kv8_cache* c, int32_t* live, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The ragged batch of the calls below: n entries over n_tok rows. Entry b is the rows [start[b], start[b + 1]) (start:
+ * DEVICE [n + 1], ascending; NULL: n == n_tok and one row each), the LAST tokens of sequence seqs[b] (DEVICE [n]; NULL:
+ * sequence b), whose length qh_kv8_resize has set before: row i of m is at position lens - m + i. Rows outside
+ * the entries are neither read nor written. Entries whose sequence number is out of range are empty sequences. Rows are
+ * ld elements apart, a row's heads contiguous; dtype QH_F32 or QH_F16. Bases and row strides: multiples of 16 bytes. */
+
+/* Stores k and v, rows of [n_kv_heads][head_dim], into layer `layer`: per block d = max|x| / 127 (rounded to f32) and
+ * the codes nearest to x / d, halves away from zero. A block that holds earlier tokens keeps the larger of its scale and
+ * the new ones', and where that grows its codes are rounded to it. An infinite or NaN value makes its block's scale NaN,
+ * so that all 16 tokens of that head read as NaN. Each sequence in one entry at most. Tokens in a page that other
+ * sequences hold are left out (QH_KV8_SHARED). */
+int qh_kv8_append(const qh_kv8_cache* c, int layer, const void* k, const void* v, int dtype, int64_t ldk, int64_t ldv,
+                  const int32_t* start, const int32_t* seqs, int n, int n_tok, void* stream);
+
+/* The stored values of the entries' tokens: code * d rounded to f32, then to dtype. Tokens without a page read as 0. */
+int qh_kv8_read(const qh_kv8_cache* c, int layer, void* k, void* v, int dtype, int64_t ldk, int64_t ldv,
+                const int32_t* start, const int32_t* seqs, int n, int n_tok, void* stream);
+
+/* Workspace bytes of qh_kv8_attention for up to n entries over n_tok rows (no initialisation). */
+size_t qh_kv8_attention_workspace_bytes(const qh_kv8_cache* c, int n_heads, int n, int n_tok);
+
+/* Attention of query rows q [n_heads][head_dim] over their sequences: out = sum_j p_j v_j with p = softmax(scale *
+ * q . k_j) over the positions j that the row sees: up to its own (causal 1), or the whole sequence (causal 0, for states
+ * that are not the queries' own: an entry may then have more rows than the sequence has tokens). Query head h reads KV
+ * head h / (n_heads / n_kv_heads). A row that sees nothing (an empty sequence, or a position below 0) is 0. out may not
+ * overlap q. Sums in f32; f32 queries and weights go through the matrix instructions as two f16 each, f16 calls' weights
+ * as one. */
+int qh_kv8_attention(const qh_kv8_cache* c, int layer, const void* q, void* out, int dtype, int n_heads, int64_t ldq,
+                     int64_t ldo, const int32_t* start, const int32_t* seqs, int n, int n_tok, int causal, float scale,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ GPU-resident decoder */
 
 /* FLAG_HADAMARD_DOWN (reference engine/src/model_file.h:19-21): the down projection's input is rotated by the

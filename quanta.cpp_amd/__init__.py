@@ -71,6 +71,15 @@ def sampler_params(temperature=0.7, top_k=20, top_p=0.8, min_p=0.0, repeat_penal
     return qh_sampler_params(temperature, top_k, top_p, min_p, repeat_penalty, repeat_window)
 
 
+KV8_BLOCK = 16  # QH_KV8_BLOCK: tokens that share a scale
+KV8_NO_PAGES, KV8_BAD_LIST, KV8_SHARED = 1, 2, 4  # bits of KV8Cache.status
+
+
+class qh_kv8_cache(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("pages", "table", "lens", "refs", "status")] + [
+        (n, C.c_int32) for n in ("n_layers", "n_pages", "page_tokens", "n_kv_heads", "head_dim", "n_seqs", "seq_pages")]
+
+
 STAGE_QKV, STAGE_ATTENTION, STAGE_O, STAGE_GATE_UP, STAGE_DOWN, STAGES_PER_LAYER = 0, 1, 2, 3, 4, 8
 STAGE_FINAL_NORM, STAGE_HEAD, STAGE_PICK = 1 << 20, (1 << 20) + 1, (1 << 20) + 2
 
@@ -81,7 +90,10 @@ EXPORTS = ("qh_last_error", "qh_version", "qh_init", "qh_quant_bytes", "qh_tenso
            "qh_quantize_q8", "qh_matvec_q", "qh_matvec_ref", "qh_matmul_q", "qh_argmax_workspace_bytes", "qh_argmax",
            "qh_shortlist_workspace_bytes", "qh_shortlist_head", "qh_shortlist_head_noalloc",
            "qh_head_planes", "qh_shortlist_planes",
-           "qh_sampler_state", "qh_sample", "qh_sample_workspace_bytes", "qh_sample_ws", "qh_decoder_create",
+           "qh_sampler_state", "qh_sample", "qh_sample_workspace_bytes", "qh_sample_ws",
+           "qh_kv8_page_bytes", "qh_kv8_reset", "qh_kv8_pages_workspace_bytes", "qh_kv8_resize", "qh_kv8_fork",
+           "qh_kv8_compact", "qh_kv8_append", "qh_kv8_read", "qh_kv8_attention_workspace_bytes", "qh_kv8_attention",
+           "qh_decoder_create",
            "qh_decoder_destroy",
            "qh_decoder_prefill", "qh_decoder_begin", "qh_decoder_step", "qh_decoder_views",
            "qh_decoder_set_prefill_stack", "qh_decoder_step_timed",
@@ -96,6 +108,7 @@ def build() -> None:
 
 def _bind(lib):
     vp, i32, sz = C.c_void_p, C.c_int, C.c_size_t
+    kv8 = C.POINTER(qh_kv8_cache)
     sig = {
         "qh_last_error": ([], C.c_char_p), "qh_version": ([], C.c_char_p), "qh_init": ([i32], i32),
         "qh_quant_bytes": ([i32, i32, i32], sz), "qh_tensor_bytes": ([i32, i32, i32], sz),
@@ -118,6 +131,17 @@ def _bind(lib):
         "qh_head_planes": ([C.POINTER(qh_tensor), vp, vp], i32),
         "qh_shortlist_planes": ([C.POINTER(qh_tensor), vp, vp, C.POINTER(qh_head_query), C.POINTER(qh_head_out), vp,
                                  sz, vp], i32),
+        "qh_kv8_page_bytes": ([i32, i32, i32], sz),
+        "qh_kv8_reset": ([kv8, vp], i32),
+        "qh_kv8_pages_workspace_bytes": ([kv8], sz),
+        "qh_kv8_resize": ([kv8, vp, vp, i32, vp, sz, vp], i32),
+        "qh_kv8_fork": ([kv8, vp, vp, i32, i32, vp, sz, vp], i32),
+        "qh_kv8_compact": ([kv8, vp, vp, sz, vp], i32),
+        "qh_kv8_append": ([kv8, i32, vp, vp, i32, C.c_int64, C.c_int64, vp, vp, i32, i32, vp], i32),
+        "qh_kv8_read": ([kv8, i32, vp, vp, i32, C.c_int64, C.c_int64, vp, vp, i32, i32, vp], i32),
+        "qh_kv8_attention_workspace_bytes": ([kv8, i32, i32, i32], sz),
+        "qh_kv8_attention": ([kv8, i32, vp, vp, i32, i32, C.c_int64, C.c_int64, vp, vp, i32, i32, i32, C.c_float, vp, sz,
+                              vp], i32),
         "qh_decoder_create": ([C.POINTER(qh_model_desc), C.POINTER(qh_tensor), i32, C.POINTER(vp)], i32),
         "qh_decoder_destroy": ([vp], i32),
         "qh_decoder_prefill": ([vp, vp, i32, i32, i32, vp], i32),
@@ -351,6 +375,154 @@ class ShortlistHead:
         raw = self.stats_dev.cpu().numpy()
         s = qh_head_stats.from_buffer_copy(raw.tobytes())
         return {f: getattr(s, f) for f, _ in qh_head_stats._fields_}
+
+
+# ------------------------------------------------------------------------------------ 8-bit paged key / value cache
+
+class KV8Cache:
+    """A key / value cache in 8 bits for many sequences, in pages that they may share (qh_kv8_*). State on the device:
+    ``table`` [n_seqs][seq_pages], ``lens`` [n_seqs], ``refs`` [n_pages], ``status`` [1] (KV8_* bits) and ``pages``
+    [n_layers][n_pages][page_bytes]. Calls run on the current stream of the cache's device and read their lists there.
+
+    A batch's rows are the last tokens of its sequences: ``start`` (int32 [n + 1], on the device) gives each entry's rows,
+    None one row each; ``seqs`` (int32 [n]) their sequences, None sequence b for entry b. So a step is: ``resize`` to the
+    new lengths, then for each layer ``append`` the new rows and ``attention`` of their queries."""
+
+    def __init__(self, n_layers: int, n_pages: int, page_tokens: int, n_kv_heads: int, head_dim: int, n_seqs: int,
+                 seq_pages: int, device="cuda"):
+        torch = _torch()
+        page_bytes = lib().qh_kv8_page_bytes(page_tokens, n_kv_heads, head_dim)
+        if page_bytes == 0:
+            raise QHError(f"unsupported cache shape: pages of {page_tokens} tokens, {n_kv_heads} KV heads of {head_dim}")
+        if min(n_layers, n_pages, n_seqs, seq_pages) < 1:
+            raise QHError(f"{n_layers} layers of {n_pages} pages, {n_seqs} sequences of {seq_pages} pages")
+        self.n_layers, self.n_pages, self.page_tokens = n_layers, n_pages, page_tokens
+        self.n_kv_heads, self.head_dim, self.n_seqs, self.seq_pages = n_kv_heads, head_dim, n_seqs, seq_pages
+        self.pages = torch.empty((n_layers, n_pages, page_bytes), dtype=torch.uint8, device=device)
+        self.device = self.pages.device
+        self.table = torch.empty((n_seqs, seq_pages), dtype=torch.int32, device=device)
+        self.lens = torch.empty(n_seqs, dtype=torch.int32, device=device)
+        self.refs = torch.empty(n_pages, dtype=torch.int32, device=device)
+        self.status = torch.empty(1, dtype=torch.int32, device=device)
+        self.view = qh_kv8_cache(_ptr(self.pages), _ptr(self.table), _ptr(self.lens), _ptr(self.refs), _ptr(self.status),
+                                 n_layers, n_pages, page_tokens, n_kv_heads, head_dim, n_seqs, seq_pages)
+        self._ref = C.byref(self.view)
+        self.reset()
+
+    def _here(self) -> int:
+        """The current stream, on the cache's device."""
+        torch = _torch()
+        if torch.cuda.current_device() != self.device.index:
+            raise QHError(f"the cache is on {self.device}, the current device is cuda:{torch.cuda.current_device()}")
+        return _stream()
+
+    def _ints(self, t, n, what):
+        torch = _torch()
+        if t.dtype != torch.int32 or t.device != self.device or t.dim() != 1 or not t.is_contiguous():
+            raise QHError(f"{what} must be a contiguous int32 vector on {self.device}")
+        if n is not None and t.numel() != n:
+            raise QHError(f"{what} has {t.numel()} entries, expected {n}")
+        return _ptr(t)
+
+    def _batch(self, n_tok, start, seqs):
+        """(start, seqs, n) of a batch as the C calls take them."""
+        if start is None:
+            n = n_tok if seqs is None else seqs.numel()
+            if n != n_tok:
+                raise QHError(f"{n} sequences for {n_tok} rows: entries of more than one row need start")
+        else:
+            n = start.numel() - 1
+            if n < 0:
+                raise QHError("start has no entries")
+        if seqs is None and n > self.n_seqs:
+            raise QHError(f"{n} entries for {self.n_seqs} sequences")
+        return (None if start is None else self._ints(start, n + 1, "start"),
+                None if seqs is None else self._ints(seqs, n, "seqs"), n)
+
+    def _rows(self, t, heads, what):
+        """(dtype, row stride) of rows [n_tok][heads][head_dim], or [n_tok][heads * head_dim], with contiguous heads."""
+        torch = _torch()
+        if t.device != self.device or t.dtype not in (torch.float32, torch.float16):
+            raise QHError(f"{what} must be float32 or float16 on {self.device}")
+        hd = self.head_dim
+        if t.dim() == 3 and t.shape[1:] == (heads, hd):
+            ok = t.stride(2) == 1 and (heads == 1 or t.stride(1) == hd)
+        elif t.dim() == 2 and t.shape[1] == heads * hd:
+            ok = t.stride(1) == 1
+        else:
+            raise QHError(f"{what} is {tuple(t.shape)}, expected [rows][{heads}][{hd}]")
+        if not ok:
+            raise QHError(f"the heads of a row of {what} must be contiguous")
+        return (F32 if t.dtype == torch.float32 else F16), (t.stride(0) if t.shape[0] > 1 else heads * hd)
+
+    def _workspace(self, nbytes):
+        # a tensor for each call: nothing of one call (or captured graph) is shared with the next
+        return _torch().empty(max(int(nbytes), 16), dtype=_torch().uint8, device=self.device)
+
+    def reset(self) -> None:
+        """Every page free, every sequence empty, status 0."""
+        _check(lib().qh_kv8_reset(self._ref, self._here()))
+
+    def _pages_call(self, name, *args):
+        ws = self._workspace(lib().qh_kv8_pages_workspace_bytes(self._ref))
+        _check(getattr(lib(), name)(self._ref, *args, _ptr(ws), ws.numel(), self._here()))
+
+    def resize(self, seqs, lens) -> None:
+        """Sequence seqs[i] gets length lens[i] (int32 device vectors): pages past it are given back, missing ones taken."""
+        n = seqs.numel()
+        self._pages_call("qh_kv8_resize", self._ints(seqs, None, "seqs"), self._ints(lens, n, "lens"), n)
+
+    def fork(self, src, dst, copy: bool = False) -> None:
+        """Sequence dst[i] becomes a fork of src[i]: it shares its pages, or (copy) holds copies of them."""
+        n = src.numel()
+        self._pages_call("qh_kv8_fork", self._ints(src, None, "src"), self._ints(dst, n, "dst"), n, int(copy))
+
+    def compact(self):
+        """Moves the pages in use to the front of the pool; returns how many there are (int32 device tensor [1])."""
+        live = _torch().empty(1, dtype=_torch().int32, device=self.device)
+        self._pages_call("qh_kv8_compact", _ptr(live))
+        return live
+
+    def append(self, layer: int, k, v, start=None, seqs=None) -> None:
+        """Stores the rows k and v ([rows][n_kv_heads][head_dim], float32 or float16; views of a wider row are fine)."""
+        dtype, ldk = self._rows(k, self.n_kv_heads, "k")
+        dtype_v, ldv = self._rows(v, self.n_kv_heads, "v")
+        if dtype != dtype_v or k.shape[0] != v.shape[0]:
+            raise QHError("k and v differ in dtype or rows")
+        start, seqs, n = self._batch(k.shape[0], start, seqs)
+        _check(lib().qh_kv8_append(self._ref, layer, _ptr(k), _ptr(v), dtype, ldk, ldv, start, seqs, n, k.shape[0],
+                                   self._here()))
+
+    def read(self, layer: int, n_tok: int, start=None, seqs=None, dtype=None):
+        """The stored values (k, v) of the batch's tokens, [n_tok][n_kv_heads][head_dim] of dtype (float32)."""
+        torch = _torch()
+        out = torch.zeros((2, n_tok, self.n_kv_heads, self.head_dim), dtype=dtype or torch.float32, device=self.device)
+        code, ld = self._rows(out[0], self.n_kv_heads, "read")
+        start, seqs, n = self._batch(n_tok, start, seqs)
+        _check(lib().qh_kv8_read(self._ref, layer, _ptr(out[0]), _ptr(out[1]), code, ld, ld, start, seqs, n, n_tok,
+                                 self._here()))
+        return out[0], out[1]
+
+    def attention(self, layer: int, q, start=None, seqs=None, causal: bool = True, scale: float | None = None, out=None):
+        """Attention of the rows q ([rows][n_heads][head_dim]) over their sequences, each row up to its own position
+        (causal) or over all of its sequence; scale: 1 / sqrt(head_dim). Rows outside the entries keep out's values (zeros
+        in a new one)."""
+        torch = _torch()
+        heads = q.shape[1] if q.dim() == 3 else q.shape[-1] // self.head_dim
+        dtype, ldq = self._rows(q, heads, "q")
+        if out is None:
+            # single tokens fill every row; with starts, rows behind the last entry stay zero
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if start is None else \
+                torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape or out.dtype != q.dtype:
+            raise QHError("out differs from q in shape or dtype")
+        _, ldo = self._rows(out, heads, "out")
+        start, seqs, n = self._batch(q.shape[0], start, seqs)
+        ws = self._workspace(lib().qh_kv8_attention_workspace_bytes(self._ref, heads, n, q.shape[0]))
+        _check(lib().qh_kv8_attention(self._ref, layer, _ptr(q), _ptr(out), dtype, heads, ldq, ldo, start, seqs, n,
+                                      q.shape[0], int(causal), self.head_dim ** -0.5 if scale is None else scale, _ptr(ws),
+                                      ws.numel(), self._here()))
+        return out
 
 
 # ------------------------------------------------------------------------------------------------ decoder

@@ -8,6 +8,7 @@
 #include <mutex>
 
 #include "qh_internal.h"
+#include "qh_kv8.h"
 
 namespace qh {
 
@@ -92,6 +93,81 @@ int check_sampler(const qh_sampler_params& p, int n_valid, const char* who, bool
                         k);
     }
     return QH_OK;
+}
+
+// Supported page shapes of the 8-bit cache.
+bool kv8_shape_ok(int page_tokens, int n_kv, int hd) {
+    return page_tokens >= 16 && page_tokens <= 256 && (page_tokens & (page_tokens - 1)) == 0 && n_kv > 0 && n_kv <= 4096 &&
+           (hd == 64 || hd == 128);
+}
+
+int validate_kv8(const qh_kv8_cache* c, const char* who) {
+    if (!c || !c->pages || !c->table || !c->lens || !c->refs || !c->status)
+        return fail(QH_ERR_ARG, "%s: null cache or cache array", who);
+    if (!kv8_shape_ok(c->page_tokens, c->n_kv_heads, c->head_dim))
+        return fail(QH_ERR_SHAPE, "%s: pages of %d tokens (a power of two, 16 to 256), %d KV heads of %d (64 or 128)", who,
+                    c->page_tokens, c->n_kv_heads, c->head_dim);
+    if (c->n_layers <= 0 || c->n_pages <= 0 || c->n_pages > QH_KV8_MAX_PAGES || c->n_seqs <= 0 ||
+        c->n_seqs > QH_KV8_MAX_SEQS || c->seq_pages <= 0 || (int64_t)c->seq_pages * c->page_tokens > (1 << 30) ||
+        (int64_t)c->n_seqs * c->seq_pages > (1 << 30))
+        return fail(QH_ERR_SHAPE, "%s: %d layers of %d pages, %d sequences of %d pages", who, c->n_layers, c->n_pages,
+                    c->n_seqs, c->seq_pages);
+    if (!aligned16(c->pages)) return fail(QH_ERR_ALIGN, "%s: pages not 16-byte aligned", who);
+    return QH_OK;
+}
+
+// The sequence lists and workspace of the page calls.
+int validate_kv8_list(const qh_kv8_cache& c, const void* a, const void* b, int n, const void* ws, size_t ws_bytes,
+                      const char* who) {
+    if (n < 0 || n > c.n_seqs || !a || !b) return fail(QH_ERR_ARG, "%s: a list of %d of %d sequences", who, n, c.n_seqs);
+    const size_t need = kv8_pages_workspace_bytes(c.n_pages, c.n_seqs);
+    if (!ws || ws_bytes < need)
+        return fail(QH_ERR_NOMEM, "%s: workspace of %zu bytes, needs %zu", who, ws ? ws_bytes : 0, need);
+    if (!aligned16(ws)) return fail(QH_ERR_ALIGN, "%s: workspace not 16-byte aligned", who);
+    return QH_OK;
+}
+
+int validate_kv8_batch(const qh_kv8_cache& c, int layer, const int32_t* start, int n, int n_tok, const char* who) {
+    if (layer < 0 || layer >= c.n_layers) return fail(QH_ERR_ARG, "%s: layer %d of %d", who, layer, c.n_layers);
+    if (n < 0 || n_tok < 0 || n > (1 << 24)) return fail(QH_ERR_ARG, "%s: %d entries over %d rows", who, n, n_tok);
+    if (!start && n != n_tok) return fail(QH_ERR_ARG, "%s: %d entries over %d rows without starts", who, n, n_tok);
+    return QH_OK;
+}
+
+int validate_kv8_heads(const qh_kv8_cache& c, int n_heads, int n_tok, const char* who) {
+    if (n_heads <= 0 || n_heads % c.n_kv_heads != 0)
+        return fail(QH_ERR_SHAPE, "%s: %d query heads over %d KV heads", who, n_heads, c.n_kv_heads);
+    if ((int64_t)n_heads / c.n_kv_heads * (n_tok > 0 ? n_tok : 0) > (1 << 30) || (int64_t)n_heads * c.head_dim > (1 << 24))
+        return fail(QH_ERR_SHAPE, "%s: %d rows of %d heads", who, n_tok, n_heads);
+    return QH_OK;
+}
+
+// Rows of `width` elements, ld apart.
+int validate_kv8_rows(const void* p, int dtype, int64_t ld, int64_t width, const char* who) {
+    if (dtype != QH_F32 && dtype != QH_F16) return fail(QH_ERR_DTYPE, "%s: dtype %d is not f32 (0) or f16 (1)", who, dtype);
+    if (!p) return fail(QH_ERR_ARG, "%s: null rows", who);
+    if (ld < width || ld > (int64_t)1 << 32) return fail(QH_ERR_ARG, "%s: rows %lld apart, %lld wide", who, (long long)ld,
+                                                         (long long)width);
+    if (!aligned16(p) || ld % (dtype == QH_F32 ? 4 : 8) != 0)
+        return fail(QH_ERR_ALIGN, "%s: rows not on multiples of 16 bytes", who);
+    return QH_OK;
+}
+
+Kv8View kv8_view(const qh_kv8_cache& c, int layer) {
+    Kv8View v{};
+    v.page_bytes = kv8_page_bytes(c.page_tokens, c.n_kv_heads, c.head_dim);
+    v.pages = static_cast<uint8_t*>(c.pages) + (size_t)layer * c.n_pages * v.page_bytes;
+    v.table = c.table;
+    v.lens = c.lens;
+    v.refs = c.refs;
+    v.status = c.status;
+    v.n_pages = c.n_pages;
+    v.n_kv = c.n_kv_heads;
+    v.hd = c.head_dim;
+    v.n_seqs = c.n_seqs;
+    v.seq_pages = c.seq_pages;
+    v.page_shift = __builtin_ctz((unsigned)c.page_tokens);
+    return v;
 }
 
 // Device checks of qh_init for the current device (gfx950), once per device.
@@ -454,6 +530,100 @@ int qh_shortlist_head_noalloc(const qh_tensor* head8, const qh_tensor* head4, co
     must.n = query->n_must;
     return check_hip(launch_shortlist_head(*head8, *head4, *err, xq, xd, *query, must, *out, ws, as_stream(stream)),
                      "qh_shortlist_head_noalloc launch");
+}
+
+size_t qh_kv8_page_bytes(int page_tokens, int n_kv_heads, int head_dim) {
+    return kv8_shape_ok(page_tokens, n_kv_heads, head_dim) ? kv8_page_bytes(page_tokens, n_kv_heads, head_dim) : 0;
+}
+
+int qh_kv8_reset(const qh_kv8_cache* c, void* stream) {
+    if (int rc = validate_kv8(c, "qh_kv8_reset")) return rc;
+    return check_hip(launch_kv8_reset(kv8_view(*c, 0), as_stream(stream)), "qh_kv8_reset");
+}
+
+size_t qh_kv8_pages_workspace_bytes(const qh_kv8_cache* c) {
+    return validate_kv8(c, "qh_kv8_pages_workspace_bytes") ? 0 : kv8_pages_workspace_bytes(c->n_pages, c->n_seqs);
+}
+
+int qh_kv8_resize(const qh_kv8_cache* c, const int32_t* seqs, const int32_t* lens, int n, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+    const char* who = "qh_kv8_resize";
+    if (int rc = validate_kv8(c, who)) return rc;
+    if (n == 0) return QH_OK;
+    if (int rc = validate_kv8_list(*c, seqs, lens, n, workspace, workspace_bytes, who)) return rc;
+    return check_hip(launch_kv8_resize(kv8_view(*c, 0), c->n_layers, seqs, lens, n, workspace, as_stream(stream)), who);
+}
+
+int qh_kv8_fork(const qh_kv8_cache* c, const int32_t* src, const int32_t* dst, int n, int copy, void* workspace,
+                size_t workspace_bytes, void* stream) {
+    const char* who = "qh_kv8_fork";
+    if (int rc = validate_kv8(c, who)) return rc;
+    if (n == 0) return QH_OK;
+    if (int rc = validate_kv8_list(*c, src, dst, n, workspace, workspace_bytes, who)) return rc;
+    if (copy != 0 && copy != 1) return fail(QH_ERR_ARG, "%s: copy = %d", who, copy);
+    return check_hip(launch_kv8_fork(kv8_view(*c, 0), c->n_layers, src, dst, n, copy != 0, workspace, as_stream(stream)),
+                     who);
+}
+
+int qh_kv8_compact(const qh_kv8_cache* c, int32_t* live, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "qh_kv8_compact";
+    if (int rc = validate_kv8(c, who)) return rc;
+    if (int rc = validate_kv8_list(*c, c->lens, c->lens, 1, workspace, workspace_bytes, who)) return rc;
+    return check_hip(launch_kv8_compact(kv8_view(*c, 0), c->n_layers, live, workspace, as_stream(stream)), who);
+}
+
+int qh_kv8_append(const qh_kv8_cache* c, int layer, const void* k, const void* v, int dtype, int64_t ldk, int64_t ldv,
+                  const int32_t* start, const int32_t* seqs, int n, int n_tok, void* stream) {
+    const char* who = "qh_kv8_append";
+    if (int rc = validate_kv8(c, who)) return rc;
+    if (int rc = validate_kv8_batch(*c, layer, start, n, n_tok, who)) return rc;
+    if (n == 0 || n_tok == 0) return QH_OK;
+    const int64_t width = (int64_t)c->n_kv_heads * c->head_dim;
+    if (int rc = validate_kv8_rows(k, dtype, ldk, width, who)) return rc;
+    if (int rc = validate_kv8_rows(v, dtype, ldv, width, who)) return rc;
+    return check_hip(launch_kv8_append(kv8_view(*c, layer), k, v, dtype, ldk, ldv, start, seqs, n, n_tok,
+                                       as_stream(stream)), who);
+}
+
+int qh_kv8_read(const qh_kv8_cache* c, int layer, void* k, void* v, int dtype, int64_t ldk, int64_t ldv,
+                const int32_t* start, const int32_t* seqs, int n, int n_tok, void* stream) {
+    const char* who = "qh_kv8_read";
+    if (int rc = validate_kv8(c, who)) return rc;
+    if (int rc = validate_kv8_batch(*c, layer, start, n, n_tok, who)) return rc;
+    if (n == 0 || n_tok == 0) return QH_OK;
+    const int64_t width = (int64_t)c->n_kv_heads * c->head_dim;
+    if (int rc = validate_kv8_rows(k, dtype, ldk, width, who)) return rc;
+    if (int rc = validate_kv8_rows(v, dtype, ldv, width, who)) return rc;
+    return check_hip(launch_kv8_read(kv8_view(*c, layer), k, v, dtype, ldk, ldv, start, seqs, n, n_tok,
+                                     as_stream(stream)), who);
+}
+
+size_t qh_kv8_attention_workspace_bytes(const qh_kv8_cache* c, int n_heads, int n, int n_tok) {
+    const char* who = "qh_kv8_attention_workspace_bytes";
+    if (validate_kv8(c, who) || validate_kv8_heads(*c, n_heads, n_tok, who)) return 0;
+    if (n <= 0 || n_tok <= 0) return 0;
+    return kv8_attention_workspace_bytes(n_heads, c->n_kv_heads, c->head_dim, n, n_tok);
+}
+
+int qh_kv8_attention(const qh_kv8_cache* c, int layer, const void* q, void* out, int dtype, int n_heads, int64_t ldq,
+                     int64_t ldo, const int32_t* start, const int32_t* seqs, int n, int n_tok, int causal, float scale,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "qh_kv8_attention";
+    if (int rc = validate_kv8(c, who)) return rc;
+    if (int rc = validate_kv8_heads(*c, n_heads, n_tok, who)) return rc;
+    if (int rc = validate_kv8_batch(*c, layer, start, n, n_tok, who)) return rc;
+    if (causal != 0 && causal != 1) return fail(QH_ERR_ARG, "%s: causal = %d", who, causal);
+    if (!(scale - scale == 0.0f)) return fail(QH_ERR_ARG, "%s: scale is not finite", who);
+    if (n == 0 || n_tok == 0) return QH_OK;
+    const int64_t width = (int64_t)n_heads * c->head_dim;
+    if (int rc = validate_kv8_rows(q, dtype, ldq, width, who)) return rc;
+    if (int rc = validate_kv8_rows(out, dtype, ldo, width, who)) return rc;
+    const size_t need = kv8_attention_workspace_bytes(n_heads, c->n_kv_heads, c->head_dim, n, n_tok);
+    if (!workspace || workspace_bytes < need)
+        return fail(QH_ERR_NOMEM, "%s: workspace of %zu bytes, needs %zu", who, workspace ? workspace_bytes : 0, need);
+    if (!aligned16(workspace)) return fail(QH_ERR_ALIGN, "%s: workspace not 16-byte aligned", who);
+    return check_hip(launch_kv8_attention(kv8_view(*c, layer), q, out, dtype, n_heads, ldq, ldo, start, seqs, n, n_tok,
+                                          causal != 0, scale, workspace, as_stream(stream)), who);
 }
 
 int qh_decoder_create(const qh_model_desc* hp, const qh_tensor* tensors, int n_tensors, qh_decoder** out) {

@@ -1,0 +1,104 @@
+// The 8-bit paged key / value cache: its layout, and what the kernels that read and write it share.
+//
+// A block is 16 tokens of one KV head, keys and values apart: 16 * head_dim codes (int8) and one f32 scale. A page holds
+// page_tokens / 16 blocks of every KV head: the key blocks [n_kv][page_tokens / 16], the value blocks likewise, then the
+// scales f32 [key, value][n_kv][page_tokens / 16]; pages are padded to 128 bytes. Within a block the codes lie in the
+// order in which a wave's 64 lanes take them as matrix operands, 16 bytes to a lane, so that every load of a block is one
+// contiguous KB per 64 dimensions, without a transposition of the values:
+//   keys    [head_dim / 64][4 groups][16 tokens][16 dims]: lane 16 g + t holds dims 64 c + 16 g .. + 15 of token t
+//   values  [head_dim / 64][4 groups][16][4 dims][4 tokens]: lane 16 g + j holds dims 64 c + 4 j .. + 3 of tokens
+//           4 g .. 4 g + 3, the tokens whose weights the same lane holds after the product of keys and queries
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "qh_internal.h"
+
+namespace qh {
+
+constexpr int kBlk = QH_KV8_BLOCK;
+
+// What the kernels need of a qh_kv8_cache for one layer.
+struct Kv8View {
+    uint8_t* pages;  // the layer's first page
+    int32_t *table, *lens, *refs, *status;
+    size_t page_bytes;
+    int n_pages, n_kv, hd, n_seqs, seq_pages;
+    int page_shift;  // log2(page_tokens)
+};
+
+__host__ __device__ __forceinline__ size_t kv8_page_bytes(int page_tokens, int n_kv, int hd) {
+    const size_t raw = 2 * (size_t)n_kv * page_tokens * hd + 8 * (size_t)n_kv * (page_tokens / kBlk);
+    return (raw + 127) / 128 * 128;
+}
+
+#if defined(__HIPCC__)
+// Tokens of a sequence, never more than its table row can hold.
+__device__ __forceinline__ int kv8_len(const Kv8View& c, int seq) {
+    return min(max(c.lens[seq], 0), c.seq_pages << c.page_shift);
+}
+
+// The codes of block `blk` (of the page) of KV head h, which = 0 keys, 1 values.
+__device__ __forceinline__ uint8_t* kv8_codes(const Kv8View& c, int page, int which, int h, int blk) {
+    const int per = 1 << (c.page_shift - 4);
+    return c.pages + (size_t)page * c.page_bytes + ((size_t)((which * c.n_kv + h) * per + blk) * (kBlk * c.hd));
+}
+__device__ __forceinline__ float* kv8_scale(const Kv8View& c, int page, int which, int h, int blk) {
+    const int per = 1 << (c.page_shift - 4);
+    uint8_t* s = c.pages + (size_t)page * c.page_bytes + 2 * ((size_t)c.n_kv * c.hd << c.page_shift);
+    return reinterpret_cast<float*>(s) + (which * c.n_kv + h) * per + blk;
+}
+
+// A ragged batch: entry b is the last rows [start[b], start[b + 1]) of sequence seqs[b] (null: b); start null: one row
+// each. Whatever the arrays hold, rows stay in [0, n_tok) and sequences outside the cache have none.
+struct Kv8Batch {
+    const int32_t *start, *seqs;
+    int n, n_tok;
+    __device__ __forceinline__ int at(int b) const {
+        return start ? min(max(start[b], 0), n_tok) : min(b, n_tok);
+    }
+    __device__ __forceinline__ int seq(int b) const { return seqs ? seqs[b] : b; }
+};
+
+// Work items of a ragged batch without a prefix sum: entry b's items begin at floor(start[b] * mul / unit) + pad * b,
+// which leaves every entry floor(rows * mul / unit) + pad of them at least. The entry of `item` (a wave calls it, all
+// lanes with one item; the start array is read 64 entries at a time): the last one that begins at or before it.
+__device__ __forceinline__ int kv8_entry_of(const Kv8Batch& q, int item, int mul, int unit, int pad, int* first) {
+    const int lane = (int)threadIdx.x & 63;
+    int b = -1;
+    for (int base = 0; base < q.n; base += 64) {
+        const int i = base + lane;
+        const int key = i < q.n ? (int)((long)q.at(i) * mul / unit) + pad * i : 0x7fffffff;
+        const uint64_t m = __ballot(key <= item);
+        if (m == 0) break;
+        b = base + 63 - __builtin_clzll(m);
+        const int k = __builtin_amdgcn_readlane(key, b - base);
+        *first = k;
+        if (b < base + 63) break;
+    }
+    return __builtin_amdgcn_readfirstlane(b);
+}
+#endif
+
+// qh_kv8.hip
+hipError_t launch_kv8_append(const Kv8View& c, const void* k, const void* v, int dtype, int64_t ldk, int64_t ldv,
+                             const int32_t* start, const int32_t* seqs, int n, int n_tok, hipStream_t s);
+hipError_t launch_kv8_read(const Kv8View& c, void* k, void* v, int dtype, int64_t ldk, int64_t ldv, const int32_t* start,
+                           const int32_t* seqs, int n, int n_tok, hipStream_t s);
+size_t kv8_pages_workspace_bytes(int n_pages, int n_seqs);
+// pages: the first layer's; n_layers of them lie layer_bytes apart.
+hipError_t launch_kv8_reset(const Kv8View& c, hipStream_t s);
+hipError_t launch_kv8_resize(const Kv8View& c, int n_layers, const int32_t* seqs, const int32_t* lens, int n, void* ws,
+                             hipStream_t s);
+hipError_t launch_kv8_fork(const Kv8View& c, int n_layers, const int32_t* src, const int32_t* dst, int n, bool copy,
+                           void* ws, hipStream_t s);
+hipError_t launch_kv8_compact(const Kv8View& c, int n_layers, int32_t* live, void* ws, hipStream_t s);
+// qh_kv8_attn.hip
+size_t kv8_attention_workspace_bytes(int n_heads, int n_kv, int hd, int n, int n_tok);
+hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int dtype, int n_heads, int64_t ldq,
+                                int64_t ldo, const int32_t* start, const int32_t* seqs, int n, int n_tok, bool causal,
+                                float scale, void* ws, hipStream_t s);
+
+}  // namespace qh

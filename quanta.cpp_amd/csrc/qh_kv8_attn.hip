@@ -1,0 +1,873 @@
+// Attention over the 8-bit paged key / value cache (layout in qh_kv8.h).
+//
+// For query row q of a head and the positions j it sees:  o = sum_j e_j d_j v_j / sum_j e_j,  e_j = 2^(x_j - max x),
+// x_j = (q . k_j) c_j scale log2(e), with k_j, v_j the integer codes and c_j, d_j the scales of their blocks. One pass
+// over the cache with the running maximum and sum: 64 positions (a tile) at a time, in f32.
+//
+// Both products run on the f16 matrix instructions (16 x 16 x 32): a code in [-127, 127] is exact in f16, so a tile's
+// codes become f16 operands (five instructions for four of them) and the block scales are applied to the scores and to
+// the weights, whose tokens a lane holds next to each other. Scores are computed transposed (codes . queries), so that a
+// lane's weights are already the operand of the second product (values . weights, transposed too): no weight passes
+// through shared memory, and a row's maximum and sum belong to one lane column.
+//   f32 queries are split into two f16 (22 bits), scaled by a power of two so that the row's largest value has exponent
+//   13: what the split drops is below 2^-22 of each value, about what f32 sums round off. Weights likewise, in f32 calls;
+//   f16 calls round each weight to f16 once, half an ulp of the result's own type, in errors that average out over the
+//   positions. A weight carries the value scale of its block divided by a running power of two at least as large as all
+//   of them, times 2^14, so that small weights stay clear of f16's subnormals.
+#include <type_traits>
+
+#include "qh_device.h"
+#include "qh_kv8.h"
+
+namespace qh {
+namespace {
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+constexpr int kTile = 64;            // positions of one step
+constexpr int kRowTile = 16;         // query rows of a workgroup of the row kernel
+constexpr int kBigTile = 128;        // and of the tile kernel
+constexpr int kMaxItems = 1024;      // row tiles of one launch of the row kernel
+constexpr float kWeight = 16384.0f;  // 2^14
+
+// Four codes as f16: the bytes biased by 128 under the high byte 0x64 are the numbers 1024 + 128 + code.
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t* out) {
+    const uint32_t x = w ^ 0x80808080u;
+    const h2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+    out[0] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) - bias);
+    out[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) - bias);
+}
+__device__ __forceinline__ h8 codes8_to_f16(uint32_t a, uint32_t b) {
+    uint32_t r[4];
+    codes_to_f16(a, r);
+    codes_to_f16(b, r + 2);
+    return __builtin_bit_cast(h8, make_uint4(r[0], r[1], r[2], r[3]));
+}
+
+// v combined over the four lanes that hold one query column (lane, lane ^ 16, lane ^ 32, lane ^ 48).
+template <typename Op>
+__device__ __forceinline__ float over_groups(float v, Op op) {
+    uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    v = op(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+    u = __builtin_bit_cast(uint32_t, v);
+    const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return op(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
+}
+__device__ __forceinline__ float fmax2(float a, float b) { return __builtin_fmaxf(a, b); }
+
+// 16 query rows as the operand of the score product: lane 16 g + r holds dims 64 c + 16 g .. + 15 of row r.
+template <typename T, int kC>
+struct Query {
+    static constexpr bool kSplit = std::is_same<T, float>::value;
+    h8 hi[kC][2], lo[kSplit ? kC : 1][2];
+    float unit;  // x = product * unit * key scale
+
+    __device__ __forceinline__ void load(const T* p, bool valid, float scale_log2e) {
+        if constexpr (kSplit) {
+            float v[kC][16], top = 0.0f;
+#pragma unroll
+            for (int c = 0; c < kC; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float4 a = valid ? reinterpret_cast<const float4*>(p + 64 * c)[i] : make_float4(0, 0, 0, 0);
+                    v[c][4 * i] = a.x, v[c][4 * i + 1] = a.y, v[c][4 * i + 2] = a.z, v[c][4 * i + 3] = a.w;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) top = __builtin_fmaxf(top, __builtin_fabsf(v[c][4 * i + j]));
+                }
+            top = over_groups(top, fmax2);
+            // the power of two that takes the largest value to [2^13, 2^14); an infinite row becomes NaN
+            const int e = max((int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -100);
+            const float up = top < __builtin_inff() ? __builtin_ldexpf(1.0f, 13 - e) : __builtin_nanf("");
+            unit = __builtin_ldexpf(scale_log2e, e - 13);
+#pragma unroll
+            for (int c = 0; c < kC; ++c)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float x = v[c][8 * h + j] * up;
+                        hi[c][h][j] = (_Float16)x;
+                        lo[c][h][j] = (_Float16)(x - (float)hi[c][h][j]);
+                    }
+        } else {
+            unit = scale_log2e;
+#pragma unroll
+            for (int c = 0; c < kC; ++c)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    hi[c][h] = h8{};
+                    if (valid) hi[c][h] = reinterpret_cast<const h8*>(p + 64 * c)[h];
+                }
+        }
+    }
+
+    __device__ __forceinline__ f4 dot(h8 k, int c, int h, f4 acc) const {
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, hi[c][h], acc, 0, 0, 0);
+        if constexpr (kSplit) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, lo[c][h], acc, 0, 0, 0);
+        return acc;
+    }
+};
+
+// The page and scales of 64 blocks, one to a lane: 16 tiles, lane 4 j + b block b of the j-th.
+struct Blocks {
+    int page;
+    float ck, cv;
+    uint64_t ok;  // lanes whose block exists
+
+    // tile: this lane's; blocks at or past len, or without a page, are left out.
+    __device__ __forceinline__ void load(const Kv8View& c, int seq, int h, int tile, bool in_range, int len) {
+        const int pos = tile * kTile + ((int)threadIdx.x & 3) * kBlk;
+        page = -1;
+        if (in_range && pos < len) page = c.table[(size_t)seq * c.seq_pages + (pos >> c.page_shift)];
+        const bool good = page >= 0 && page < c.n_pages;
+        ok = __ballot(good);
+        ck = cv = 0.0f;
+        const int blk = (pos >> 4) & ((1 << (c.page_shift - 4)) - 1);
+        if (good) {
+            ck = *kv8_scale(c, page, 0, h, blk);
+            cv = *kv8_scale(c, page, 1, h, blk);
+        }
+        page = good ? page : 0;
+    }
+    __device__ __forceinline__ int page_of(int i) const { return __builtin_amdgcn_readlane(page, i); }
+    __device__ __forceinline__ float key(int i) const {
+        return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ck), i));
+    }
+    __device__ __forceinline__ float value(int i) const {
+        return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, cv), i));
+    }
+};
+
+// The running state of 16 query rows: maximum and this lane's share of the sum, and the output, transposed: lane
+// 16 g + r holds row r, register [4 c + i][s] dimension 64 c + 16 g + 4 s + i.
+template <typename T, int kC>
+struct Rows {
+    static constexpr bool kSplit = std::is_same<T, float>::value;
+    float m = -__builtin_inff(), l = 0.0f;
+    f4 o[4 * kC];
+
+    __device__ __forceinline__ void clear() {
+        m = -__builtin_inff();
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4 * kC; ++i) o[i] = f4{0, 0, 0, 0};
+    }
+
+    // x: the scores of a tile (log2), [block][token 4 g + s], -inf where masked. weight[b]: value scale of block b over
+    // the running power of two, shrink: what that power grew by (<= 1). Leaves the weights as operands w (and their low
+    // halves lo). masked: some x may be masked, and then has weight 0 whatever its block's scale is.
+    template <bool kMasked>
+    __device__ __forceinline__ void step(float (&x)[4][4], const float (&weight)[4], float shrink, h8 (&w)[2],
+                                         h8 (&lo)[2]) {
+        float top = x[0][0];
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) top = __builtin_fmaxf(top, x[b][s]);
+        top = __builtin_fmaxf(m, over_groups(top, fmax2));
+        // a row that has seen nothing yet: subtract 0, so that its weights are 2^-inf = 0 and not NaN
+        const float base = top == -__builtin_inff() ? 0.0f : top;
+        const float alpha = __builtin_amdgcn_exp2f(m - base);
+        m = top;
+        float sum = 0.0f;
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const bool out = kMasked && x[b][s] == -__builtin_inff();
+                const float p = __builtin_amdgcn_exp2f(x[b][s] - base);
+                sum += p;
+                const float v = out ? 0.0f : p * weight[b];
+                const _Float16 hi = (_Float16)v;
+                w[b >> 1][4 * (b & 1) + s] = hi;
+                if constexpr (kSplit) lo[b >> 1][4 * (b & 1) + s] = (_Float16)(v - (float)hi);
+            }
+        l = __builtin_fmaf(l, alpha, sum);
+        const float a = alpha * shrink;
+        if (__any(a != 1.0f)) {
+#pragma unroll
+            for (int i = 0; i < 4 * kC; ++i) o[i] *= a;
+        }
+    }
+};
+
+// A power of two above v (and at least 2^-110), as f32: the value scales' running unit.
+__device__ __forceinline__ float unit_above(float v) {
+    const uint32_t u = (__builtin_bit_cast(uint32_t, v) & 0x7f800000u) + 0x00800000u;
+    return __builtin_fmaxf(__builtin_bit_cast(float, min(u, 0x7e800000u)), 0x1p-110f);
+}
+
+// The value scales of a tile's blocks as weights over the running unit (grown where it has to be); returns by what
+// factor the output so far shrinks.
+__device__ __forceinline__ float tile_weights(const Blocks& bl, int i0, float& unit, float (&weight)[4]) {
+    float v[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) v[b] = bl.value(i0 + b);
+    // from 0 up: a NaN scale, which some rows may not see, leaves the unit alone
+    const float top = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(0.0f, v[0]), v[1]), __builtin_fmaxf(v[2], v[3]));
+    float shrink = 1.0f;
+    if (!(top < unit)) {  // also the first tile (unit 0)
+        const float grown = __builtin_fmaxf(unit, unit_above(top));
+        shrink = unit / grown;
+        unit = grown;
+    }
+    const float inv = kWeight / unit;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) weight[b] = v[b] * inv;
+    return shrink;
+}
+
+// What a launch needs besides the cache.
+struct AttnArgs {
+    const void* q;
+    void* out;
+    int64_t ldq, ldo;
+    Kv8Batch batch;
+    int group;  // query heads to a KV head; the rows of an entry are (token, head of the group)
+    int causal;
+    float scale_log2e;
+    float* part_o;   // partial outputs [slot][n_kv][rows][hd], with their maximum and sum [slot][n_kv][rows][2]
+    float* part_ml;
+    int4* rec;       // [items] where an item's partials are: first slot, how many (0: none), first row, rows
+    int items, splits;
+};
+
+// Entry b's rows: global rows (token * group + head) from first on, and the positions its tokens see.
+struct Entry {
+    int seq, len, tokens, row0, rows;
+};
+__device__ __forceinline__ Entry entry_of(const Kv8View& c, const AttnArgs& a, int b) {
+    const int s0 = a.batch.at(b), s1 = max(s0, a.batch.at(b + 1)), seq = a.batch.seq(b);
+    const bool known = seq >= 0 && seq < c.n_seqs;
+    return {known ? seq : 0, known ? kv8_len(c, seq) : 0, s1 - s0, s0 * a.group, (s1 - s0) * a.group};
+}
+// Positions that row r of the entry sees.
+__device__ __forceinline__ int visible(const Entry& e, const AttnArgs& a, int r) {
+    return a.causal ? min(max(e.len - e.tokens + r / a.group + 1, 0), e.len) : e.len;
+}
+
+// A row's share of the output, 4 values at dimension d: divided by the row's sum, zero where it saw nothing.
+template <typename T>
+__device__ __forceinline__ void store_out(T* out, float4 o, float m, float l) {
+    const float inv = m == -__builtin_inff() ? 0.0f : 1.0f / l;
+    if constexpr (std::is_same<T, float>::value) {
+        *reinterpret_cast<float4*>(out) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    } else {
+        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<h4*>(out) = h4{(_Float16)(o.x * inv), (_Float16)(o.y * inv), (_Float16)(o.z * inv),
+                                         (_Float16)(o.w * inv)};
+    }
+}
+template <typename T>
+__device__ __forceinline__ T* out_row(const AttnArgs& a, const Kv8View& c, int grow, int kvh) {
+    const int tok = grow / a.group, head = kvh * a.group + (grow - tok * a.group);
+    return static_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * c.hd;
+}
+template <typename T>
+__device__ __forceinline__ const T* q_row(const AttnArgs& a, const Kv8View& c, int grow, int kvh) {
+    const int tok = grow / a.group, head = kvh * a.group + (grow - tok * a.group);
+    return static_cast<const T*>(a.q) + (int64_t)tok * a.ldq + (int64_t)head * c.hd;
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+
+// Row tiles of 16 (single tokens: the query heads of one KV head) over long caches, bound by reading the codes. The
+// tiles of all items lie end to end, and each of the gridDim.x workgroups of a KV head takes an equal share of them,
+// whatever the lengths are: a share may end inside an item (the parts are joined by kv8_join_kernel) or span several.
+// Every workgroup finds its share from the lengths itself. Its four waves take every fourth tile of a share, each with
+// its own running maximum, straight from global memory into registers (one contiguous KB a load, the next tile's loads
+// in flight while one is computed), and meet in shared memory at the end of an item.
+template <typename T, int kC>
+__global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8View c, AttnArgs a) {
+    constexpr int kHd = 64 * kC, kPad = kHd + 4;
+    __shared__ int pre[kMaxItems + 1];
+    __shared__ uint16_t ent[kMaxItems];
+    __shared__ int wave_sum[4];
+    __shared__ __align__(16) float so[4][kRowTile][kPad];
+    __shared__ float sm[4][kRowTile], sl[4][kRowTile];
+    const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4,
+              col = lane & 15;
+    const int kvh = (int)blockIdx.y, tiles_per_token = (a.group + kRowTile - 1) / kRowTile;
+    auto first_item = [&](const Entry& e, int b) {
+        return a.batch.start ? (int)((long)e.row0 / kRowTile) + b : b * tiles_per_token;
+    };
+
+    // the items' tile counts, then their prefix sums
+    for (int i = tid; i < a.items; i += 256) pre[i] = 0;
+    __syncthreads();
+    for (int b = tid; b < a.batch.n; b += 256) {
+        const Entry e = entry_of(c, a, b);
+        const int at = first_item(e, b);
+        for (int t = 0; t * kRowTile < e.rows && at + t < a.items; ++t) {
+            const int last = min((t + 1) * kRowTile, e.rows) - 1;
+            pre[at + t] = max(1, (visible(e, a, last) + kTile - 1) / kTile);
+            ent[at + t] = (uint16_t)b;
+        }
+    }
+    __syncthreads();
+    constexpr int kPer = kMaxItems / 256;
+    int mine[kPer], sum = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        mine[j] = tid * kPer + j < a.items ? pre[tid * kPer + j] : 0;
+        sum += mine[j];
+    }
+    int incl = sum;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+        const int y = __shfl_up(incl, s);
+        incl += lane >= s ? y : 0;
+    }
+    if (lane == 63) wave_sum[wave] = incl;
+    __syncthreads();
+    int at = incl - sum, total = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        at += i < wave ? wave_sum[i] : 0;
+        total += wave_sum[i];
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        if (tid * kPer + j < a.items) pre[tid * kPer + j] = at;
+        at += mine[j];
+    }
+    if (tid == 0) pre[a.items] = total;
+    __syncthreads();
+
+    // shares: whole rounds of the four waves
+    const int shares = (int)gridDim.x;
+    const int share = max(4, ((total + shares - 1) / shares + 3) & ~3);
+    if (blockIdx.x == 0 && kvh == 0) {
+        for (int i = tid; i < a.items; i += 256) {
+            int4 r = make_int4(0, 0, 0, 0);
+            if (pre[i + 1] > pre[i]) {
+                const int b = ent[i];
+                const Entry e = entry_of(c, a, b);
+                const int t = i - first_item(e, b), w0 = pre[i] / share, w1 = (pre[i + 1] - 1) / share;
+                r = make_int4(2 * w0 + (pre[i] > w0 * share ? 1 : 0), w1 > w0 ? w1 - w0 + 1 : 0, e.row0 + t * kRowTile,
+                              min(kRowTile, e.rows - t * kRowTile));
+            }
+            a.rec[i] = r;
+        }
+    }
+    const int from = (int)blockIdx.x * share, to = min(total, from + share);
+    if (from >= to) return;
+
+    // the item that holds tile `from`: the last one whose prefix is at or below it (items without tiles have the
+    // following item's prefix)
+    int item = 0;
+    {
+        int lo = 0, hi = a.items - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (pre[mid] <= from) lo = mid;
+            else hi = mid - 1;
+        }
+        item = __builtin_amdgcn_readfirstlane(lo);
+    }
+
+    for (int done = from; done < to; ++item) {
+        const int p0 = pre[item], p1 = pre[item + 1];
+        if (p1 <= done) continue;
+        const int t0 = done - p0, t1 = min(to, p1) - p0;  // this item's tiles of the share
+        const int b = __builtin_amdgcn_readfirstlane((int)ent[item]);
+        const Entry e = entry_of(c, a, b);
+        const int r0 = (item - first_item(e, b)) * kRowTile, r = r0 + col;
+        const bool valid = r < e.rows;
+        const int vis = valid ? visible(e, a, r) : 0;
+        const int all_see = visible(e, a, r0);  // positions that every row sees: the first row's
+        Query<T, kC> q;
+        q.load(q_row<T>(a, c, e.row0 + (valid ? r : r0), kvh) + 16 * g, valid, a.scale_log2e);
+        Rows<T, kC> st;
+        st.clear();
+        float unit = 0.0f;
+
+        uint4 kr[2][4][kC], vr[2][4][kC];
+        Blocks bl;
+        const int n_mine = t1 - t0 > wave ? (t1 - t0 - wave + 3) / 4 : 0;  // tiles t0 + wave + 4 j
+        auto fetch = [&](int buf, int j) {
+            if ((j & 15) == 0) {
+                const int jl = j + (lane >> 2);
+                bl.load(c, e.seq, kvh, t0 + wave + 4 * jl, jl < n_mine, e.len);
+            }
+            const int tile = t0 + wave + 4 * j;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int page = bl.page_of(4 * (j & 15) + k), blk = (tile * 4 + k) & ((1 << (c.page_shift - 4)) - 1);
+                const uint4* kp = reinterpret_cast<const uint4*>(kv8_codes(c, page, 0, kvh, blk)) + lane;
+                const uint4* vp = reinterpret_cast<const uint4*>(kv8_codes(c, page, 1, kvh, blk)) + lane;
+#pragma unroll
+                for (int cc = 0; cc < kC; ++cc) {
+                    kr[buf][k][cc] = kp[64 * cc];
+                    vr[buf][k][cc] = vp[64 * cc];
+                }
+            }
+        };
+        // scales and masks of tile j, kept across the fetch of the next tile's blocks
+        struct TileInfo {
+            float key[4], weight[4], shrink;
+            uint32_t ok;
+        };
+        auto info = [&](int j) {
+            TileInfo ti;
+            const int i0 = 4 * (j & 15);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) ti.key[k] = bl.key(i0 + k);
+            ti.shrink = tile_weights(bl, i0, unit, ti.weight);
+            ti.ok = (uint32_t)(bl.ok >> i0) & 15u;
+            return ti;
+        };
+        auto compute = [&](int buf, int j, const TileInfo& ti) {
+            const int pos0 = (t0 + wave + 4 * j) * kTile;
+            float x[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                f4 acc = {0, 0, 0, 0};
+#pragma unroll
+                for (int cc = 0; cc < kC; ++cc) {
+                    acc = q.dot(codes8_to_f16(kr[buf][k][cc].x, kr[buf][k][cc].y), cc, 0, acc);
+                    acc = q.dot(codes8_to_f16(kr[buf][k][cc].z, kr[buf][k][cc].w), cc, 1, acc);
+                }
+                const float f = ti.key[k] * q.unit;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) x[k][s] = acc[s] * f;
+            }
+            h8 w[2], lo[2];
+            if (pos0 + kTile > all_see || ti.ok != 15u) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int s = 0; s < 4; ++s)
+                        if (pos0 + 16 * k + 4 * g + s >= vis || !((ti.ok >> k) & 1u)) x[k][s] = -__builtin_inff();
+                st.template step<true>(x, ti.weight, ti.shrink, w, lo);
+            } else {
+                st.template step<false>(x, ti.weight, ti.shrink, w, lo);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int cc = 0; cc < kC; ++cc) {
+                    const uint4 v0 = vr[buf][2 * u][cc], v1 = vr[buf][2 * u + 1][cc];
+                    const uint32_t a0[4] = {v0.x, v0.y, v0.z, v0.w}, a1[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const h8 v = codes8_to_f16(a0[i], a1[i]);
+                        f4& o = st.o[4 * cc + i];
+                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[u], o, 0, 0, 0);
+                        if constexpr (Query<T, kC>::kSplit) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[u], o, 0, 0, 0);
+                    }
+                }
+        };
+        if (n_mine > 0) fetch(0, 0);
+        for (int j = 0; j < n_mine; j += 2) {
+            const TileInfo t_a = info(j);
+            if (j + 1 < n_mine) fetch(1, j + 1);
+            compute(0, j, t_a);
+            if (j + 1 < n_mine) {
+                const TileInfo t_b = info(j + 1);
+                if (j + 2 < n_mine) fetch(0, j + 2);
+                compute(1, j + 1, t_b);
+            }
+        }
+
+        // the four waves' results of this item together
+        const float l = over_groups(st.l, [](float p, float q2) { return p + q2; });
+        const float back = unit * (1.0f / kWeight);
+        if (g == 0) {
+            sm[wave][col] = st.m;
+            sl[wave][col] = l;
+        }
+#pragma unroll
+        for (int cc = 0; cc < kC; ++cc)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                *reinterpret_cast<float4*>(&so[wave][col][64 * cc + 16 * g + 4 * s]) =
+                    make_float4(st.o[4 * cc][s] * back, st.o[4 * cc + 1][s] * back, st.o[4 * cc + 2][s] * back,
+                                st.o[4 * cc + 3][s] * back);
+        __syncthreads();
+        const int rr = tid >> 4, d0 = 4 * (tid & 15);
+        if (r0 + rr < e.rows) {
+            float top = sm[0][rr];
+#pragma unroll
+            for (int w2 = 1; w2 < 4; ++w2) top = __builtin_fmaxf(top, sm[w2][rr]);
+            const float base = top == -__builtin_inff() ? 0.0f : top;
+            float f[4], lsum = 0.0f;
+#pragma unroll
+            for (int w2 = 0; w2 < 4; ++w2) {
+                f[w2] = __builtin_amdgcn_exp2f(sm[w2][rr] - base);
+                lsum = __builtin_fmaf(f[w2], sl[w2][rr], lsum);
+            }
+            const bool whole = t0 == 0 && t1 == p1 - p0;
+            const int slot = 2 * (int)blockIdx.x + (done > from ? 1 : 0);
+            const size_t pr = ((size_t)slot * c.n_kv + kvh) * kRowTile + rr;
+#pragma unroll
+            for (int cc = 0; cc < kC; ++cc) {
+                float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll
+                for (int w2 = 0; w2 < 4; ++w2) {
+                    const float4 v = *reinterpret_cast<const float4*>(&so[w2][rr][64 * cc + d0]);
+                    o.x = __builtin_fmaf(f[w2], v.x, o.x);
+                    o.y = __builtin_fmaf(f[w2], v.y, o.y);
+                    o.z = __builtin_fmaf(f[w2], v.z, o.z);
+                    o.w = __builtin_fmaf(f[w2], v.w, o.w);
+                }
+                if (whole)
+                    store_out(out_row<T>(a, c, e.row0 + r0 + rr, kvh) + 64 * cc + d0, o, top, lsum);
+                else
+                    *reinterpret_cast<float4*>(a.part_o + pr * kHd + 64 * cc + d0) = o;
+            }
+            if (!whole && (tid & 15) == 0) {
+                a.part_ml[2 * pr] = top;
+                a.part_ml[2 * pr + 1] = lsum;
+            }
+        }
+        __syncthreads();
+        done = min(to, p1);
+    }
+}
+
+// Joins an item's partial results: one workgroup per item, KV head and row; hd / 4 threads to a partial, the workgroup's
+// groups of them take every (256 / (hd / 4))-th one. Partial k is slot first (k = 0) or the k-th multiple of stride after.
+template <typename T, int kC>
+__global__ __launch_bounds__(256) void kv8_join_kernel(Kv8View c, AttnArgs a, int rows, int stride) {
+    constexpr int kHd = 64 * kC, kThr = kHd / 4, kGroups = 256 / kThr;
+    __shared__ __align__(16) float so[kGroups][kHd];
+    __shared__ float sm[kGroups], sl[kGroups];
+    const int4 rec = a.rec[blockIdx.x];
+    const int row = (int)blockIdx.z, kvh = (int)blockIdx.y, tid = (int)threadIdx.x, grp = tid / kThr, d = 4 * (tid % kThr);
+    if (rec.y == 0 || row >= rec.w) return;
+    auto at = [&](int k) {
+        const int slot = k == 0 ? rec.x : rec.x / stride * stride + k * stride;
+        return ((size_t)slot * c.n_kv + kvh) * rows + row;
+    };
+    float m = -__builtin_inff(), l = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+    for (int k = grp; k < rec.y; k += kGroups) {
+        const size_t p = at(k);
+        const float mk = a.part_ml[2 * p], lk = a.part_ml[2 * p + 1];
+        const float4 v = *reinterpret_cast<const float4*>(a.part_o + p * kHd + d);
+        const float top = __builtin_fmaxf(m, mk), base = top == -__builtin_inff() ? 0.0f : top;
+        const float f0 = __builtin_amdgcn_exp2f(m - base), f1 = __builtin_amdgcn_exp2f(mk - base);
+        o.x = __builtin_fmaf(o.x, f0, v.x * f1);
+        o.y = __builtin_fmaf(o.y, f0, v.y * f1);
+        o.z = __builtin_fmaf(o.z, f0, v.z * f1);
+        o.w = __builtin_fmaf(o.w, f0, v.w * f1);
+        l = __builtin_fmaf(l, f0, lk * f1);
+        m = top;
+    }
+    *reinterpret_cast<float4*>(&so[grp][d]) = o;
+    if (d == 0) {
+        sm[grp] = m;
+        sl[grp] = l;
+    }
+    __syncthreads();
+    if (grp != 0) return;
+    float top = sm[0];
+#pragma unroll
+    for (int k = 1; k < kGroups; ++k) top = __builtin_fmaxf(top, sm[k]);
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    float lsum = 0.0f;
+    o = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+        const float f = __builtin_amdgcn_exp2f(sm[k] - base);
+        const float4 v = *reinterpret_cast<const float4*>(&so[k][d]);
+        o.x = __builtin_fmaf(f, v.x, o.x);
+        o.y = __builtin_fmaf(f, v.y, o.y);
+        o.z = __builtin_fmaf(f, v.z, o.z);
+        o.w = __builtin_fmaf(f, v.w, o.w);
+        lsum = __builtin_fmaf(f, sl[k], lsum);
+    }
+    store_out(out_row<T>(a, c, rec.z + row, kvh) + d, o, top, lsum);
+}
+
+// ------------------------------------------------------------------------------------------------ many rows
+
+// Row tiles of 128 (a prompt's tokens times the query heads of a KV head), bound by the matrix instructions and, next to
+// them, by the exponentials. Each of the four waves holds 32 rows; a tile's codes become f16 once per workgroup, into
+// shared memory, in the order in which the waves read them as operands (1 KB a read, no bank conflicts), in two buffers:
+// one barrier a tile, the next tile's codes converted and the one after that in flight while one is computed. The KV head
+// is the fastest grid index, so that the workgroups of one head share an XCD's L2 where there are eight heads, and the
+// last row tiles (which see the most positions) start first. splits > 1: that many workgroups share a row tile's
+// positions and leave partials.
+template <typename T, int kC>
+__global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a) {
+    constexpr int kHd = 64 * kC;
+    constexpr int kUnits = 4 * kC * 2 * 64;  // 16-byte units of a tile's keys (and values) in f16
+    extern __shared__ __align__(16) uint4 lds[];  // [buffer][keys, values][kUnits]
+    const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4,
+              col = lane & 15;
+    const int kvh = (int)(blockIdx.x % (unsigned)c.n_kv), split = (int)blockIdx.y;
+    const int item = a.items - 1 - (int)(blockIdx.x / (unsigned)c.n_kv);
+    int from = 0, b = item;
+    b = kv8_entry_of(a.batch, item, a.group, kBigTile, 1, &from);
+    Entry e{0, 0, 0, 0, 0};
+    if (b >= 0) e = entry_of(c, a, b);
+    const int r0 = b < 0 ? 0 : (item - from) * kBigTile;
+    if (a.splits > 1 && split == 0 && kvh == 0 && tid == 0)
+        a.rec[item] = r0 < e.rows ? make_int4(item * a.splits, a.splits, e.row0 + r0, min(kBigTile, e.rows - r0))
+                                  : make_int4(0, 0, 0, 0);
+    if (r0 >= e.rows) return;
+    const int last = min(r0 + kBigTile, e.rows) - 1;
+    const int tiles = (visible(e, a, last) + kTile - 1) / kTile;
+    const int t0 = (int)((long)tiles * split / a.splits), t1 = (int)((long)tiles * (split + 1) / a.splits);
+
+    Query<T, kC> q[2];
+    Rows<T, kC> st[2];
+    int vis[2];
+#pragma unroll
+    for (int ct = 0; ct < 2; ++ct) {
+        const int r = r0 + wave * 32 + ct * 16 + col;
+        const bool valid = r < e.rows;
+        vis[ct] = valid ? visible(e, a, r) : 0;
+        q[ct].load(q_row<T>(a, c, e.row0 + (valid ? r : r0), kvh) + 16 * g, valid, a.scale_log2e);
+        st[ct].clear();
+    }
+    const int w0 = r0 + wave * 32, w1 = min(w0 + 31, last);
+    const int all_see = w0 <= last ? visible(e, a, w0) : 0;   // positions that each row of the wave sees
+    const int some_see = w0 <= last ? visible(e, a, w1) : 0;  // and that any of them does
+    float unit = 0.0f;
+
+    Blocks bl, bl_next;
+    uint4 kr[kC], vr[2];
+    // Wave w stages key block w and a quarter of the values: pair u = w / 2 of the blocks, dimensions by w % 2.
+    auto fetch = [&](int t) {
+        const int j = (t - t0) & 15;
+        if (j == 0) {
+            const int tl = t + (lane >> 2);
+            bl_next.load(c, e.seq, kvh, tl, tl < t1, e.len);
+        }
+        const int per = (1 << (c.page_shift - 4)) - 1;
+        const uint4* kp =
+            reinterpret_cast<const uint4*>(kv8_codes(c, bl_next.page_of(4 * j + wave), 0, kvh, (t * 4 + wave) & per)) + lane;
+#pragma unroll
+        for (int cc = 0; cc < kC; ++cc) kr[cc] = kp[64 * cc];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int blk = 2 * (wave >> 1) + k;
+            const uint8_t* vp = kv8_codes(c, bl_next.page_of(4 * j + blk), 1, kvh, (t * 4 + blk) & per);
+            if constexpr (kC == 2) {
+                vr[k] = reinterpret_cast<const uint4*>(vp)[64 * (wave & 1) + lane];
+            } else {
+                const uint2 h = reinterpret_cast<const uint2*>(vp)[2 * lane + (wave & 1)];
+                vr[k].x = h.x;
+                vr[k].y = h.y;
+            }
+        }
+    };
+    auto stage = [&](int buf) {
+        uint4* ks = lds + (size_t)buf * 2 * kUnits;
+        uint4* vs = ks + kUnits;
+#pragma unroll
+        for (int cc = 0; cc < kC; ++cc) {
+            ks[((wave * kC + cc) * 2 + 0) * 64 + lane] = __builtin_bit_cast(uint4, codes8_to_f16(kr[cc].x, kr[cc].y));
+            ks[((wave * kC + cc) * 2 + 1) * 64 + lane] = __builtin_bit_cast(uint4, codes8_to_f16(kr[cc].z, kr[cc].w));
+        }
+        const int u = wave >> 1;
+        const uint32_t a0[4] = {vr[0].x, vr[0].y, vr[0].z, vr[0].w}, a1[4] = {vr[1].x, vr[1].y, vr[1].z, vr[1].w};
+#pragma unroll
+        for (int i = 0; i < 2 * kC; ++i) {
+            const int at = kC == 2 ? (u * 2 + (wave & 1)) * 4 + i : u * 4 + 2 * (wave & 1) + i;
+            vs[at * 64 + lane] = __builtin_bit_cast(uint4, codes8_to_f16(a0[i], a1[i]));
+        }
+    };
+    auto compute = [&](int buf, int t) {
+        const int pos0 = t * kTile, i0 = 4 * ((t - t0) & 15);
+        float weight[4];
+        const float shrink = tile_weights(bl, i0, unit, weight);
+        if (pos0 >= some_see) {  // nothing here for this wave's rows; the unit has moved all the same
+            if (shrink != 1.0f) {
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+                    for (int i = 0; i < 4 * kC; ++i) st[ct].o[i] *= shrink;
+            }
+            return;
+        }
+        const uint32_t ok = (uint32_t)(bl.ok >> i0) & 15u;
+        const uint4* ks = lds + (size_t)buf * 2 * kUnits;
+        const uint4* vs = ks + kUnits;
+        float x[2][4][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            f4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+            for (int cc = 0; cc < kC; ++cc)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const h8 kk = __builtin_bit_cast(h8, ks[((k * kC + cc) * 2 + h) * 64 + lane]);
+#pragma unroll
+                    for (int ct = 0; ct < 2; ++ct) acc[ct] = q[ct].dot(kk, cc, h, acc[ct]);
+                }
+            const float key = bl.key(i0 + k);
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct) {
+                const float f = key * q[ct].unit;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) x[ct][k][s] = acc[ct][s] * f;
+            }
+        }
+        h8 w[2][2], lo[2][2];
+        if (pos0 + kTile > all_see || ok != 15u) {
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int s = 0; s < 4; ++s)
+                        if (pos0 + 16 * k + 4 * g + s >= vis[ct] || !((ok >> k) & 1u)) x[ct][k][s] = -__builtin_inff();
+                st[ct].template step<true>(x[ct], weight, shrink, w[ct], lo[ct]);
+            }
+        } else {
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct) st[ct].template step<false>(x[ct], weight, shrink, w[ct], lo[ct]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4 * kC; ++i) {
+                const h8 v = __builtin_bit_cast(h8, vs[(u * kC * 4 + i) * 64 + lane]);
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct) {
+                    f4& o = st[ct].o[i];
+                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[ct][u], o, 0, 0, 0);
+                    if constexpr (Query<T, kC>::kSplit)
+                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[ct][u], o, 0, 0, 0);
+                }
+            }
+    };
+
+    if (t0 < t1) {
+        fetch(t0);
+        bl = bl_next;
+        stage(0);
+        if (t0 + 1 < t1) fetch(t0 + 1);
+        for (int t = t0; t < t1; ++t) {
+            __syncthreads();  // tile t is staged, and tile t - 1 (whose buffer comes next) has been read
+            if (t > t0 && ((t - t0) & 15) == 0) bl = bl_next;
+            if (t + 1 < t1) stage((t + 1 - t0) & 1);
+            const bool more = t + 2 < t1;
+            // the blocks of the tiles in flight replace those in use only after the last of these
+            if (more) fetch(t + 2);
+            compute((t - t0) & 1, t);
+        }
+    }
+
+    const float back = unit * (1.0f / kWeight);
+#pragma unroll
+    for (int ct = 0; ct < 2; ++ct) {
+        const int rr = wave * 32 + ct * 16 + col, r = r0 + rr;
+        const float l = over_groups(st[ct].l, [](float p, float q2) { return p + q2; });
+        if (r >= e.rows) continue;
+        const size_t pr = ((size_t)(item * a.splits + split) * c.n_kv + kvh) * kBigTile + rr;
+        T* out = out_row<T>(a, c, e.row0 + r, kvh);
+#pragma unroll
+        for (int cc = 0; cc < kC; ++cc)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const float4 o = make_float4(st[ct].o[4 * cc][s] * back, st[ct].o[4 * cc + 1][s] * back,
+                                             st[ct].o[4 * cc + 2][s] * back, st[ct].o[4 * cc + 3][s] * back);
+                const int d = 64 * cc + 16 * g + 4 * s;
+                if (a.splits == 1)
+                    store_out(out + d, o, st[ct].m, l);
+                else
+                    *reinterpret_cast<float4*>(a.part_o + pr * kHd + d) = o;
+            }
+        if (a.splits > 1 && g == 0) {
+            a.part_ml[2 * pr] = st[ct].m;
+            a.part_ml[2 * pr + 1] = l;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ launches
+
+// How a call is split: few rows to an entry take the row kernel (shares over all lengths), many the tile kernel.
+struct Plan {
+    bool rows;
+    int items, shares, splits;
+    size_t part_rows;  // rows of partial results (per KV head)
+    size_t bytes(int n_kv, int hd) const {
+        return sizeof(int4) * (size_t)items + sizeof(float) * part_rows * n_kv * (hd + 2);
+    }
+};
+Plan plan_of(int group, int n_kv, int n, int n_tok, bool single) {
+    const long rows = (long)n_tok * group;
+    const long few = single ? (long)n * ((group + kRowTile - 1) / kRowTile) : rows / kRowTile + n;
+    const int cus = device_cus();
+    Plan p{};
+    if (few <= kMaxItems && rows <= 32l * n) {
+        p.rows = true;
+        p.items = (int)few;
+        p.shares = (2 * cus + n_kv - 1) / n_kv;
+        p.splits = 1;
+        p.part_rows = 2 * (size_t)p.shares * kRowTile;
+        return p;
+    }
+    p.items = (int)(rows / kBigTile + n);
+    const long wgs = (long)p.items * n_kv;
+    p.splits = wgs >= cus ? 1 : (int)((2 * cus + wgs - 1) / wgs);
+    if (p.splits > 16) p.splits = 16;
+    p.part_rows = p.splits > 1 ? (size_t)p.items * p.splits * kBigTile : 0;
+    return p;
+}
+
+}  // namespace
+
+size_t kv8_attention_workspace_bytes(int n_heads, int n_kv, int hd, int n, int n_tok) {
+    const int group = n_heads / n_kv;
+    size_t b = plan_of(group, n_kv, n, n_tok, false).bytes(n_kv, hd);
+    if (n == n_tok) {
+        const size_t single = plan_of(group, n_kv, n, n_tok, true).bytes(n_kv, hd);
+        b = b > single ? b : single;
+    }
+    return b;
+}
+
+hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int dtype, int n_heads, int64_t ldq,
+                                int64_t ldo, const int32_t* start, const int32_t* seqs, int n, int n_tok, bool causal,
+                                float scale, void* ws, hipStream_t s) {
+    AttnArgs a{};
+    a.q = q;
+    a.out = out;
+    a.ldq = ldq;
+    a.ldo = ldo;
+    a.batch = Kv8Batch{start, seqs, n, n_tok};
+    a.group = n_heads / c.n_kv;
+    a.causal = causal ? 1 : 0;
+    a.scale_log2e = scale * 1.44269504088896340736f;
+    const Plan p = plan_of(a.group, c.n_kv, n, n_tok, start == nullptr);
+    a.items = p.items;
+    a.splits = p.splits;
+    a.rec = static_cast<int4*>(ws);
+    a.part_o = reinterpret_cast<float*>(a.rec + p.items);
+    a.part_ml = a.part_o + p.part_rows * c.n_kv * c.hd;
+    auto go = [&](auto* t, auto kc) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        constexpr int kC = decltype(kc)::value;
+        if (p.rows) {
+            qh_launch((kv8_rows_kernel<T, kC>), dim3((unsigned)p.shares, (unsigned)c.n_kv), dim3(256), 0, s, c, a);
+            qh_launch((kv8_join_kernel<T, kC>), dim3((unsigned)p.items, (unsigned)c.n_kv, kRowTile), dim3(256), 0, s, c, a,
+                      kRowTile, 2);
+        } else {
+            constexpr size_t lds = 2 * 2 * (size_t)kTile * 64 * kC * 2;
+            qh_launch((kv8_tile_kernel<T, kC>), dim3((unsigned)c.n_kv * (unsigned)p.items, (unsigned)p.splits), dim3(256), lds, s, c,
+                      a);
+            if (p.splits > 1)
+                qh_launch((kv8_join_kernel<T, kC>), dim3((unsigned)p.items, (unsigned)c.n_kv, kBigTile), dim3(256), 0, s, c,
+                          a, kBigTile, 1);
+        }
+    };
+    using std::integral_constant;
+    if (dtype == QH_F32 && c.hd == 64) go((float*)nullptr, integral_constant<int, 1>{});
+    else if (dtype == QH_F32 && c.hd == 128) go((float*)nullptr, integral_constant<int, 2>{});
+    else if (dtype == QH_F16 && c.hd == 64) go((_Float16*)nullptr, integral_constant<int, 1>{});
+    else if (dtype == QH_F16 && c.hd == 128) go((_Float16*)nullptr, integral_constant<int, 2>{});
+    else return hipErrorInvalidValue;
+    return hipGetLastError();
+}
+
+}  // namespace qh
