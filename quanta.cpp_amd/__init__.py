@@ -407,79 +407,85 @@ class KV8Cache:
         self.view = qh_kv8_cache(_ptr(self.pages), _ptr(self.table), _ptr(self.lens), _ptr(self.refs), _ptr(self.status),
                                  n_layers, n_pages, page_tokens, n_kv_heads, head_dim, n_seqs, seq_pages)
         self._ref = C.byref(self.view)
+        # what every call looks up, kept here: the calls on a small batch take a few microseconds
+        self._index = self.device.index
+        self._int32, self._uint8, self._empty = torch.int32, torch.uint8, torch.empty
+        self._dtypes = {torch.float32: F32, torch.float16: F16}
+        self._pages_ws = lib().qh_kv8_pages_workspace_bytes(self._ref)
+        self._attention_ws = {}  # bytes by (heads, entries, rows)
         self.reset()
 
     def _here(self) -> int:
         """The current stream, on the cache's device."""
-        torch = _torch()
-        if torch.cuda.current_device() != self.device.index:
-            raise QHError(f"the cache is on {self.device}, the current device is cuda:{torch.cuda.current_device()}")
-        return _stream()
+        raw = _torch()._C
+        device = raw._cuda_getDevice()
+        if device != self._index:
+            raise QHError(f"the cache is on {self.device}, the current device is cuda:{device}")
+        return raw._cuda_getCurrentRawStream(device)
 
     def _ints(self, t, n, what):
-        torch = _torch()
-        if t.dtype != torch.int32 or t.device != self.device or t.dim() != 1 or not t.is_contiguous():
+        if t.dtype is not self._int32 or t.device != self.device or t.dim() != 1 or not t.is_contiguous():
             raise QHError(f"{what} must be a contiguous int32 vector on {self.device}")
-        if n is not None and t.numel() != n:
-            raise QHError(f"{what} has {t.numel()} entries, expected {n}")
-        return _ptr(t)
+        if t.shape[0] != n:
+            raise QHError(f"{what} has {t.shape[0]} entries, expected {n}")
+        return t.data_ptr()
 
     def _batch(self, n_tok, start, seqs):
         """(start, seqs, n) of a batch as the C calls take them."""
-        if start is None:
-            n = n_tok if seqs is None else seqs.numel()
-            if n != n_tok:
-                raise QHError(f"{n} sequences for {n_tok} rows: entries of more than one row need start")
-        else:
-            n = start.numel() - 1
+        if start is not None:
+            n = start.shape[0] - 1 if start.dim() == 1 else -1
             if n < 0:
                 raise QHError("start has no entries")
-        if seqs is None and n > self.n_seqs:
+            start = self._ints(start, n + 1, "start")
+        else:
+            n = n_tok
+        if seqs is not None:
+            return start, self._ints(seqs, n, "seqs"), n
+        if n > self.n_seqs:
             raise QHError(f"{n} entries for {self.n_seqs} sequences")
-        return (None if start is None else self._ints(start, n + 1, "start"),
-                None if seqs is None else self._ints(seqs, n, "seqs"), n)
+        return start, None, n
 
     def _rows(self, t, heads, what):
         """(dtype, row stride) of rows [n_tok][heads][head_dim], or [n_tok][heads * head_dim], with contiguous heads."""
-        torch = _torch()
-        if t.device != self.device or t.dtype not in (torch.float32, torch.float16):
+        dtype = self._dtypes.get(t.dtype)
+        if dtype is None or t.device != self.device:
             raise QHError(f"{what} must be float32 or float16 on {self.device}")
-        hd = self.head_dim
-        if t.dim() == 3 and t.shape[1:] == (heads, hd):
-            ok = t.stride(2) == 1 and (heads == 1 or t.stride(1) == hd)
-        elif t.dim() == 2 and t.shape[1] == heads * hd:
-            ok = t.stride(1) == 1
+        shape, stride, hd = t.shape, t.stride(), self.head_dim
+        if len(shape) == 3 and shape[1] == heads and shape[2] == hd:
+            ok = stride[2] == 1 and (heads == 1 or stride[1] == hd)
+        elif len(shape) == 2 and shape[1] == heads * hd:
+            ok = stride[1] == 1
         else:
-            raise QHError(f"{what} is {tuple(t.shape)}, expected [rows][{heads}][{hd}]")
+            raise QHError(f"{what} is {tuple(shape)}, expected [rows][{heads}][{hd}]")
         if not ok:
             raise QHError(f"the heads of a row of {what} must be contiguous")
-        return (F32 if t.dtype == torch.float32 else F16), (t.stride(0) if t.shape[0] > 1 else heads * hd)
+        return dtype, (stride[0] if shape[0] > 1 else heads * hd)
 
     def _workspace(self, nbytes):
         # a tensor for each call: nothing of one call (or captured graph) is shared with the next
-        return _torch().empty(max(int(nbytes), 16), dtype=_torch().uint8, device=self.device)
+        return self._empty(max(nbytes, 16), dtype=self._uint8, device=self.device)
 
     def reset(self) -> None:
         """Every page free, every sequence empty, status 0."""
         _check(lib().qh_kv8_reset(self._ref, self._here()))
 
     def _pages_call(self, name, *args):
-        ws = self._workspace(lib().qh_kv8_pages_workspace_bytes(self._ref))
-        _check(getattr(lib(), name)(self._ref, *args, _ptr(ws), ws.numel(), self._here()))
+        ws = self._workspace(self._pages_ws)
+        _check(getattr(lib(), name)(self._ref, *args, ws.data_ptr(), self._pages_ws, self._here()))
 
     def resize(self, seqs, lens) -> None:
         """Sequence seqs[i] gets length lens[i] (int32 device vectors): pages past it are given back, missing ones taken."""
         n = seqs.numel()
-        self._pages_call("qh_kv8_resize", self._ints(seqs, None, "seqs"), self._ints(lens, n, "lens"), n)
+        self._pages_call("qh_kv8_resize", self._ints(seqs, n, "seqs"), self._ints(lens, n, "lens"), n)
 
     def fork(self, src, dst, copy: bool = False) -> None:
         """Sequence dst[i] becomes a fork of src[i]: it shares its pages, or (copy) holds copies of them."""
         n = src.numel()
-        self._pages_call("qh_kv8_fork", self._ints(src, None, "src"), self._ints(dst, n, "dst"), n, int(copy))
+        self._pages_call("qh_kv8_fork", self._ints(src, n, "src"), self._ints(dst, n, "dst"), n, int(copy))
 
     def compact(self):
         """Moves the pages in use to the front of the pool; returns how many there are (int32 device tensor [1])."""
-        live = _torch().empty(1, dtype=_torch().int32, device=self.device)
+        live = self._empty(1, dtype=self._int32, device=self.device)
         self._pages_call("qh_kv8_compact", _ptr(live))
         return live
 
@@ -487,41 +493,49 @@ class KV8Cache:
         """Stores the rows k and v ([rows][n_kv_heads][head_dim], float32 or float16; views of a wider row are fine)."""
         dtype, ldk = self._rows(k, self.n_kv_heads, "k")
         dtype_v, ldv = self._rows(v, self.n_kv_heads, "v")
-        if dtype != dtype_v or k.shape[0] != v.shape[0]:
+        rows = k.shape[0]
+        if dtype != dtype_v or rows != v.shape[0]:
             raise QHError("k and v differ in dtype or rows")
-        start, seqs, n = self._batch(k.shape[0], start, seqs)
-        _check(lib().qh_kv8_append(self._ref, layer, _ptr(k), _ptr(v), dtype, ldk, ldv, start, seqs, n, k.shape[0],
+        start, seqs, n = self._batch(rows, start, seqs)
+        _check(lib().qh_kv8_append(self._ref, layer, k.data_ptr(), v.data_ptr(), dtype, ldk, ldv, start, seqs, n, rows,
                                    self._here()))
 
     def read(self, layer: int, n_tok: int, start=None, seqs=None, dtype=None):
-        """The stored values (k, v) of the batch's tokens, [n_tok][n_kv_heads][head_dim] of dtype (float32)."""
-        torch = _torch()
-        out = torch.zeros((2, n_tok, self.n_kv_heads, self.head_dim), dtype=dtype or torch.float32, device=self.device)
-        code, ld = self._rows(out[0], self.n_kv_heads, "read")
+        """The stored values (k, v) of the batch's tokens, [n_tok][n_kv_heads][head_dim] of dtype (float32). Rows outside
+        the entries are undefined."""
+        out = self._empty((2, n_tok, self.n_kv_heads, self.head_dim), dtype=dtype or _torch().float32, device=self.device)
+        k, v = out[0], out[1]
+        code, ld = self._rows(k, self.n_kv_heads, "read")
         start, seqs, n = self._batch(n_tok, start, seqs)
-        _check(lib().qh_kv8_read(self._ref, layer, _ptr(out[0]), _ptr(out[1]), code, ld, ld, start, seqs, n, n_tok,
+        _check(lib().qh_kv8_read(self._ref, layer, k.data_ptr(), v.data_ptr(), code, ld, ld, start, seqs, n, n_tok,
                                  self._here()))
-        return out[0], out[1]
+        return k, v
 
     def attention(self, layer: int, q, start=None, seqs=None, causal: bool = True, scale: float | None = None, out=None):
         """Attention of the rows q ([rows][n_heads][head_dim]) over their sequences, each row up to its own position
-        (causal) or over all of its sequence; scale: 1 / sqrt(head_dim). Rows outside the entries keep out's values (zeros
-        in a new one)."""
-        torch = _torch()
+        (causal) or over all of its sequence; scale: 1 / sqrt(head_dim). Rows outside the entries keep out's values (a new
+        out's are undefined)."""
+        rows = q.shape[0]
         heads = q.shape[1] if q.dim() == 3 else q.shape[-1] // self.head_dim
         dtype, ldq = self._rows(q, heads, "q")
         if out is None:
-            # single tokens fill every row; with starts, rows behind the last entry stay zero
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if start is None else \
-                torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != q.dtype:
-            raise QHError("out differs from q in shape or dtype")
-        _, ldo = self._rows(out, heads, "out")
-        start, seqs, n = self._batch(q.shape[0], start, seqs)
-        ws = self._workspace(lib().qh_kv8_attention_workspace_bytes(self._ref, heads, n, q.shape[0]))
-        _check(lib().qh_kv8_attention(self._ref, layer, _ptr(q), _ptr(out), dtype, heads, ldq, ldo, start, seqs, n,
-                                      q.shape[0], int(causal), self.head_dim ** -0.5 if scale is None else scale, _ptr(ws),
-                                      ws.numel(), self._here()))
+            out = self._empty(q.shape, dtype=q.dtype, device=self.device)
+            ldo = heads * self.head_dim
+        else:
+            if out.shape != q.shape or out.dtype != q.dtype:
+                raise QHError("out differs from q in shape or dtype")
+            _, ldo = self._rows(out, heads, "out")
+        start, seqs, n = self._batch(rows, start, seqs)
+        need = self._attention_ws.get((heads, n, rows))
+        if need is None:
+            need = lib().qh_kv8_attention_workspace_bytes(self._ref, heads, n, rows)
+            if len(self._attention_ws) > 4096:
+                self._attention_ws.clear()
+            self._attention_ws[heads, n, rows] = need
+        ws = self._workspace(need)
+        _check(lib().qh_kv8_attention(self._ref, layer, q.data_ptr(), out.data_ptr(), dtype, heads, ldq, ldo, start, seqs, n,
+                                      rows, 1 if causal else 0, self.head_dim ** -0.5 if scale is None else scale,
+                                      ws.data_ptr(), need, self._here()))
         return out
 
 

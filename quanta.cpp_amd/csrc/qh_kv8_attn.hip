@@ -30,6 +30,7 @@ constexpr int kTile = 64;            // positions of one step
 constexpr int kRowTile = 16;         // query rows of a workgroup of the row kernel
 constexpr int kBigTile = 128;        // and of the tile kernel
 constexpr int kMaxItems = 1024;      // row tiles of one launch of the row kernel
+constexpr int kMaxParts = 1024;      // partial results of a row: shares of the row kernel, splits of the tile kernel
 constexpr float kWeight = 16384.0f;  // 2^14
 
 // Four codes as f16: the bytes biased by 128 under the high byte 0x64 are the numbers 1024 + 128 + code.
@@ -65,17 +66,30 @@ struct Query {
     h8 hi[kC][2], lo[kSplit ? kC : 1][2];
     float unit;  // x = product * unit * key scale
 
-    __device__ __forceinline__ void load(const T* p, bool valid, float scale_log2e) {
+    // The row's values as loaded; convert() makes the operands of them, so that other loads can be issued in between.
+    using Raw = std::conditional_t<kSplit, float4, h8>;
+    static constexpr int kRaw = kSplit ? 4 : 2;
+    __device__ __forceinline__ static void fetch(Raw (&r)[kC][kRaw], const T* p) {
+#pragma unroll
+        for (int c = 0; c < kC; ++c)
+#pragma unroll
+            for (int i = 0; i < kRaw; ++i) r[c][i] = reinterpret_cast<const Raw*>(p + 64 * c)[i];
+    }
+
+    __device__ __forceinline__ void convert(const Raw (&r)[kC][kRaw], bool valid, float scale_log2e) {
         if constexpr (kSplit) {
             float v[kC][16], top = 0.0f;
 #pragma unroll
             for (int c = 0; c < kC; ++c)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float4 a = valid ? reinterpret_cast<const float4*>(p + 64 * c)[i] : make_float4(0, 0, 0, 0);
-                    v[c][4 * i] = a.x, v[c][4 * i + 1] = a.y, v[c][4 * i + 2] = a.z, v[c][4 * i + 3] = a.w;
+                    v[c][4 * i] = r[c][i].x, v[c][4 * i + 1] = r[c][i].y, v[c][4 * i + 2] = r[c][i].z,
+                              v[c][4 * i + 3] = r[c][i].w;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) top = __builtin_fmaxf(top, __builtin_fabsf(v[c][4 * i + j]));
+                    for (int j = 0; j < 4; ++j) {
+                        if (!valid) v[c][4 * i + j] = 0.0f;
+                        top = __builtin_fmaxf(top, __builtin_fabsf(v[c][4 * i + j]));
+                    }
                 }
             top = over_groups(top, fmax2);
             // the power of two that takes the largest value to [2^13, 2^14); an infinite row becomes NaN
@@ -97,10 +111,7 @@ struct Query {
 #pragma unroll
             for (int c = 0; c < kC; ++c)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    hi[c][h] = h8{};
-                    if (valid) hi[c][h] = reinterpret_cast<const h8*>(p + 64 * c)[h];
-                }
+                for (int h = 0; h < 2; ++h) hi[c][h] = valid ? r[c][h] : h8{};
         }
     }
 
@@ -281,10 +292,11 @@ __device__ __forceinline__ const T* q_row(const AttnArgs& a, const Kv8View& c, i
 // its own running maximum, straight from global memory into registers (one contiguous KB a load, the next tile's loads
 // in flight while one is computed), and meet in shared memory at the end of an item.
 template <typename T, int kC>
-__global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8View c, AttnArgs a) {
+__global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a) {
     constexpr int kHd = 64 * kC, kPad = kHd + 4;
     __shared__ int pre[kMaxItems + 1];
     __shared__ uint16_t ent[kMaxItems];
+    __shared__ Entry entries[kMaxItems];
     __shared__ int wave_sum[4];
     __shared__ __align__(16) float so[4][kRowTile][kPad];
     __shared__ float sm[4][kRowTile], sl[4][kRowTile];
@@ -300,6 +312,7 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8View c, AttnArgs a) {
     __syncthreads();
     for (int b = tid; b < a.batch.n; b += 256) {
         const Entry e = entry_of(c, a, b);
+        entries[b] = e;
         const int at = first_item(e, b);
         for (int t = 0; t * kRowTile < e.rows && at + t < a.items; ++t) {
             const int last = min((t + 1) * kRowTile, e.rows) - 1;
@@ -345,7 +358,7 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8View c, AttnArgs a) {
             int4 r = make_int4(0, 0, 0, 0);
             if (pre[i + 1] > pre[i]) {
                 const int b = ent[i];
-                const Entry e = entry_of(c, a, b);
+                const Entry e = entries[b];
                 const int t = i - first_item(e, b), w0 = pre[i] / share, w1 = (pre[i + 1] - 1) / share;
                 r = make_int4(2 * w0 + (pre[i] > w0 * share ? 1 : 0), w1 > w0 ? w1 - w0 + 1 : 0, e.row0 + t * kRowTile,
                               min(kRowTile, e.rows - t * kRowTile));
@@ -374,83 +387,88 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8View c, AttnArgs a) {
         if (p1 <= done) continue;
         const int t0 = done - p0, t1 = min(to, p1) - p0;  // this item's tiles of the share
         const int b = __builtin_amdgcn_readfirstlane((int)ent[item]);
-        const Entry e = entry_of(c, a, b);
+        const Entry el = entries[b];
+        const Entry e{__builtin_amdgcn_readfirstlane(el.seq), __builtin_amdgcn_readfirstlane(el.len),
+                      __builtin_amdgcn_readfirstlane(el.tokens), __builtin_amdgcn_readfirstlane(el.row0),
+                      __builtin_amdgcn_readfirstlane(el.rows)};
         const int r0 = (item - first_item(e, b)) * kRowTile, r = r0 + col;
         const bool valid = r < e.rows;
-        const int vis = valid ? visible(e, a, r) : 0;
-        const int all_see = visible(e, a, r0);  // positions that every row sees: the first row's
-        Query<T, kC> q;
-        q.load(q_row<T>(a, c, e.row0 + (valid ? r : r0), kvh) + 16 * g, valid, a.scale_log2e);
-        Rows<T, kC> st;
-        st.clear();
-        float unit = 0.0f;
-
-        uint4 kr[2][4][kC], vr[2][4][kC];
-        Blocks bl;
         const int n_mine = t1 - t0 > wave ? (t1 - t0 - wave + 3) / 4 : 0;  // tiles t0 + wave + 4 j
-        auto fetch = [&](int buf, int j) {
-            if ((j & 15) == 0) {
-                const int jl = j + (lane >> 2);
-                bl.load(c, e.seq, kvh, t0 + wave + 4 * jl, jl < n_mine, e.len);
-            }
+        Blocks bl;
+        auto blocks = [&](int j) {
+            const int jl = j + (lane >> 2);
+            bl.load(c, e.seq, kvh, t0 + wave + 4 * jl, jl < n_mine, e.len);
+        };
+        uint4 kr[4][kC], vr[4][kC];
+        auto fetch = [&](uint4 (&to)[4][kC], int which, int j) {
             const int tile = t0 + wave + 4 * j;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int page = bl.page_of(4 * (j & 15) + k), blk = (tile * 4 + k) & ((1 << (c.page_shift - 4)) - 1);
-                const uint4* kp = reinterpret_cast<const uint4*>(kv8_codes(c, page, 0, kvh, blk)) + lane;
-                const uint4* vp = reinterpret_cast<const uint4*>(kv8_codes(c, page, 1, kvh, blk)) + lane;
+                const uint4* p = reinterpret_cast<const uint4*>(kv8_codes(c, page, which, kvh, blk)) + lane;
 #pragma unroll
-                for (int cc = 0; cc < kC; ++cc) {
-                    kr[buf][k][cc] = kp[64 * cc];
-                    vr[buf][k][cc] = vp[64 * cc];
-                }
+                for (int cc = 0; cc < kC; ++cc) to[k][cc] = p[64 * cc];
             }
         };
-        // scales and masks of tile j, kept across the fetch of the next tile's blocks
-        struct TileInfo {
-            float key[4], weight[4], shrink;
-            uint32_t ok;
-        };
-        auto info = [&](int j) {
-            TileInfo ti;
-            const int i0 = 4 * (j & 15);
+        typename Query<T, kC>::Raw raw[kC][Query<T, kC>::kRaw];
+        blocks(0);
+        Query<T, kC>::fetch(raw, q_row<T>(a, c, e.row0 + (valid ? r : r0), kvh) + 16 * g);
+        if (n_mine > 0) {
+            fetch(kr, 0, 0);
+            fetch(vr, 1, 0);
+        }
+        const int vis = valid ? visible(e, a, r) : 0;
+        const int all_see = visible(e, a, r0);  // positions that every row sees: the first row's
+        Query<T, kC> q;
+        q.convert(raw, valid, a.scale_log2e);
+        Rows<T, kC> st;
+        st.clear();
+        float unit = 0.0f;
+
+        for (int j = 0; j < n_mine; ++j) {
+            const int pos0 = (t0 + wave + 4 * j) * kTile, i0 = 4 * (j & 15);
+            float weight[4], key[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) ti.key[k] = bl.key(i0 + k);
-            ti.shrink = tile_weights(bl, i0, unit, ti.weight);
-            ti.ok = (uint32_t)(bl.ok >> i0) & 15u;
-            return ti;
-        };
-        auto compute = [&](int buf, int j, const TileInfo& ti) {
-            const int pos0 = (t0 + wave + 4 * j) * kTile;
+            for (int k = 0; k < 4; ++k) key[k] = bl.key(i0 + k);
+            const float shrink = tile_weights(bl, i0, unit, weight);
+            const uint32_t ok = (uint32_t)(bl.ok >> i0) & 15u;
             float x[4][4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 f4 acc = {0, 0, 0, 0};
 #pragma unroll
                 for (int cc = 0; cc < kC; ++cc) {
-                    acc = q.dot(codes8_to_f16(kr[buf][k][cc].x, kr[buf][k][cc].y), cc, 0, acc);
-                    acc = q.dot(codes8_to_f16(kr[buf][k][cc].z, kr[buf][k][cc].w), cc, 1, acc);
+                    acc = q.dot(codes8_to_f16(kr[k][cc].x, kr[k][cc].y), cc, 0, acc);
+                    acc = q.dot(codes8_to_f16(kr[k][cc].z, kr[k][cc].w), cc, 1, acc);
                 }
-                const float f = ti.key[k] * q.unit;
+                const float f = key[k] * q.unit;
 #pragma unroll
                 for (int s = 0; s < 4; ++s) x[k][s] = acc[s] * f;
             }
+            // the next tile's keys are in flight from here on, its values from the end of the step
+            __builtin_amdgcn_sched_barrier(0);
+            const bool more = j + 1 < n_mine;
+            if (more) {
+                if (((j + 1) & 15) == 0) blocks(j + 1);
+                fetch(kr, 0, j + 1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
             h8 w[2], lo[2];
-            if (pos0 + kTile > all_see || ti.ok != 15u) {
+            if (pos0 + kTile > all_see || ok != 15u) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
 #pragma unroll
                     for (int s = 0; s < 4; ++s)
-                        if (pos0 + 16 * k + 4 * g + s >= vis || !((ti.ok >> k) & 1u)) x[k][s] = -__builtin_inff();
-                st.template step<true>(x, ti.weight, ti.shrink, w, lo);
+                        if (pos0 + 16 * k + 4 * g + s >= vis || !((ok >> k) & 1u)) x[k][s] = -__builtin_inff();
+                st.template step<true>(x, weight, shrink, w, lo);
             } else {
-                st.template step<false>(x, ti.weight, ti.shrink, w, lo);
+                st.template step<false>(x, weight, shrink, w, lo);
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int cc = 0; cc < kC; ++cc) {
-                    const uint4 v0 = vr[buf][2 * u][cc], v1 = vr[buf][2 * u + 1][cc];
+                    const uint4 v0 = vr[2 * u][cc], v1 = vr[2 * u + 1][cc];
                     const uint32_t a0[4] = {v0.x, v0.y, v0.z, v0.w}, a1[4] = {v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -460,17 +478,8 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8View c, AttnArgs a) {
                         if constexpr (Query<T, kC>::kSplit) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[u], o, 0, 0, 0);
                     }
                 }
-        };
-        if (n_mine > 0) fetch(0, 0);
-        for (int j = 0; j < n_mine; j += 2) {
-            const TileInfo t_a = info(j);
-            if (j + 1 < n_mine) fetch(1, j + 1);
-            compute(0, j, t_a);
-            if (j + 1 < n_mine) {
-                const TileInfo t_b = info(j + 1);
-                if (j + 2 < n_mine) fetch(0, j + 2);
-                compute(1, j + 1, t_b);
-            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) fetch(vr, 1, j + 1);
         }
 
         // the four waves' results of this item together
@@ -529,13 +538,15 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(Kv8View c, AttnArgs a) {
     }
 }
 
-// Joins an item's partial results: one workgroup per item, KV head and row; hd / 4 threads to a partial, the workgroup's
-// groups of them take every (256 / (hd / 4))-th one. Partial k is slot first (k = 0) or the k-th multiple of stride after.
+// Joins an item's partial results: one workgroup per item, KV head and row. First the partials' maxima, a thread to each,
+// and from them every partial's factor; then hd / 4 threads to a partial's row, the workgroup's groups of them taking
+// turns, so that the loads are independent of each other. Partial k is slot first (k = 0) or the k-th multiple of stride
+// after.
 template <typename T, int kC>
 __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8View c, AttnArgs a, int rows, int stride) {
     constexpr int kHd = 64 * kC, kThr = kHd / 4, kGroups = 256 / kThr;
     __shared__ __align__(16) float so[kGroups][kHd];
-    __shared__ float sm[kGroups], sl[kGroups];
+    __shared__ float factor[kMaxParts], wave_top[4], wave_sum[4];
     const int4 rec = a.rec[blockIdx.x];
     const int row = (int)blockIdx.z, kvh = (int)blockIdx.y, tid = (int)threadIdx.x, grp = tid / kThr, d = 4 * (tid % kThr);
     if (rec.y == 0 || row >= rec.w) return;
@@ -543,45 +554,51 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8View c, AttnArgs a, in
         const int slot = k == 0 ? rec.x : rec.x / stride * stride + k * stride;
         return ((size_t)slot * c.n_kv + kvh) * rows + row;
     };
-    float m = -__builtin_inff(), l = 0.0f;
-    float4 o = make_float4(0, 0, 0, 0);
-    for (int k = grp; k < rec.y; k += kGroups) {
-        const size_t p = at(k);
-        const float mk = a.part_ml[2 * p], lk = a.part_ml[2 * p + 1];
-        const float4 v = *reinterpret_cast<const float4*>(a.part_o + p * kHd + d);
-        const float top = __builtin_fmaxf(m, mk), base = top == -__builtin_inff() ? 0.0f : top;
-        const float f0 = __builtin_amdgcn_exp2f(m - base), f1 = __builtin_amdgcn_exp2f(mk - base);
-        o.x = __builtin_fmaf(o.x, f0, v.x * f1);
-        o.y = __builtin_fmaf(o.y, f0, v.y * f1);
-        o.z = __builtin_fmaf(o.z, f0, v.z * f1);
-        o.w = __builtin_fmaf(o.w, f0, v.w * f1);
-        l = __builtin_fmaf(l, f0, lk * f1);
-        m = top;
+    float m[kMaxParts / 256], top = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < kMaxParts / 256; ++j) {
+        const int k = tid + 256 * j;
+        m[j] = k < rec.y ? a.part_ml[2 * at(k)] : -__builtin_inff();
+        top = __builtin_fmaxf(top, m[j]);
     }
-    *reinterpret_cast<float4*>(&so[grp][d]) = o;
-    if (d == 0) {
-        sm[grp] = m;
-        sl[grp] = l;
-    }
+    top = wave_reduce32x2(top, fmax2);
+    if ((tid & 63) == 0) wave_top[tid >> 6] = top;
     __syncthreads();
-    if (grp != 0) return;
-    float top = sm[0];
-#pragma unroll
-    for (int k = 1; k < kGroups; ++k) top = __builtin_fmaxf(top, sm[k]);
+    top = __builtin_fmaxf(__builtin_fmaxf(wave_top[0], wave_top[1]), __builtin_fmaxf(wave_top[2], wave_top[3]));
     const float base = top == -__builtin_inff() ? 0.0f : top;
-    float lsum = 0.0f;
-    o = make_float4(0, 0, 0, 0);
+    float l = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kGroups; ++k) {
-        const float f = __builtin_amdgcn_exp2f(sm[k] - base);
-        const float4 v = *reinterpret_cast<const float4*>(&so[k][d]);
+    for (int j = 0; j < kMaxParts / 256; ++j) {
+        const int k = tid + 256 * j;
+        if (k < rec.y) {
+            const float f = __builtin_amdgcn_exp2f(m[j] - base);
+            factor[k] = f;
+            l = __builtin_fmaf(f, a.part_ml[2 * at(k) + 1], l);
+        }
+    }
+    l = wave_reduce32x2(l, [](float p, float q) { return p + q; });
+    if ((tid & 63) == 0) wave_sum[tid >> 6] = l;
+    __syncthreads();
+    l = (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]);
+    float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int k = grp; k < rec.y; k += kGroups) {
+        const float4 v = *reinterpret_cast<const float4*>(a.part_o + at(k) * kHd + d);
+        const float f = factor[k];
         o.x = __builtin_fmaf(f, v.x, o.x);
         o.y = __builtin_fmaf(f, v.y, o.y);
         o.z = __builtin_fmaf(f, v.z, o.z);
         o.w = __builtin_fmaf(f, v.w, o.w);
-        lsum = __builtin_fmaf(f, sl[k], lsum);
     }
-    store_out(out_row<T>(a, c, rec.z + row, kvh) + d, o, top, lsum);
+    *reinterpret_cast<float4*>(&so[grp][d]) = o;
+    __syncthreads();
+    if (grp != 0) return;
+#pragma unroll
+    for (int k = 1; k < kGroups; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(&so[k][d]);
+        o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+    }
+    store_out(out_row<T>(a, c, rec.z + row, kvh) + d, o, top, l);
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
@@ -623,7 +640,9 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
         const int r = r0 + wave * 32 + ct * 16 + col;
         const bool valid = r < e.rows;
         vis[ct] = valid ? visible(e, a, r) : 0;
-        q[ct].load(q_row<T>(a, c, e.row0 + (valid ? r : r0), kvh) + 16 * g, valid, a.scale_log2e);
+        typename Query<T, kC>::Raw raw[kC][Query<T, kC>::kRaw];
+        Query<T, kC>::fetch(raw, q_row<T>(a, c, e.row0 + (valid ? r : r0), kvh) + 16 * g);
+        q[ct].convert(raw, valid, a.scale_log2e);
         st[ct].clear();
     }
     const int w0 = r0 + wave * 32, w1 = min(w0 + 31, last);
@@ -803,6 +822,7 @@ Plan plan_of(int group, int n_kv, int n, int n_tok, bool single) {
         p.rows = true;
         p.items = (int)few;
         p.shares = (2 * cus + n_kv - 1) / n_kv;
+        if (p.shares > kMaxParts) p.shares = kMaxParts;
         p.splits = 1;
         p.part_rows = 2 * (size_t)p.shares * kRowTile;
         return p;
