@@ -31,7 +31,6 @@ constexpr int kRowTile = 16;         // query rows of a workgroup of the row ker
 constexpr int kBigTile = 128;        // and of the tile kernel
 constexpr int kMaxItems = 1024;      // row tiles of one launch of the row kernel
 constexpr int kMaxParts = 1024;      // partial results of a row: shares of the row kernel, splits of the tile kernel
-constexpr float kWeight = 16384.0f;  // 2^14
 
 // Four codes as f16: the bytes biased by 128 under the high byte 0x64 are the numbers 1024 + 128 + code.
 __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t* out) {
@@ -170,8 +169,7 @@ struct Rows {
     // x: the scores of a tile (log2), [block][token 4 g + s], -inf where masked. weight[b]: value scale of block b over
     // the running power of two, shrink: what that power grew by (<= 1). Leaves the weights as operands w (and their low
     // halves lo). masked: some x may be masked, and then has weight 0 whatever its block's scale is.
-    template <bool kMasked>
-    __device__ __forceinline__ void step(float (&x)[4][4], const float (&weight)[4], float shrink, h8 (&w)[2],
+    __device__ __forceinline__ void step(float (&x)[4][4], const float (&weight)[4], float shrink, bool masked, h8 (&w)[2],
                                          h8 (&lo)[2]) {
         float top = x[0][0];
 #pragma unroll
@@ -183,53 +181,62 @@ struct Rows {
         const float base = top == -__builtin_inff() ? 0.0f : top;
         const float alpha = __builtin_amdgcn_exp2f(m - base);
         m = top;
-        float sum = 0.0f;
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const bool out = kMasked && x[b][s] == -__builtin_inff();
-                const float p = __builtin_amdgcn_exp2f(x[b][s] - base);
-                sum += p;
-                const float v = out ? 0.0f : p * weight[b];
-                const _Float16 hi = (_Float16)v;
-                w[b >> 1][4 * (b & 1) + s] = hi;
-                if constexpr (kSplit) lo[b >> 1][4 * (b & 1) + s] = (_Float16)(v - (float)hi);
-            }
-        l = __builtin_fmaf(l, alpha, sum);
         const float a = alpha * shrink;
         if (__any(a != 1.0f)) {
 #pragma unroll
             for (int i = 0; i < 4 * kC; ++i) o[i] *= a;
         }
+        float sum = 0.0f, v[4][4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const float p = __builtin_amdgcn_exp2f(x[b][s] - base);
+                sum += p;
+                v[b][s] = p * weight[b];
+            }
+        if (masked) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) v[b][s] = x[b][s] == -__builtin_inff() ? 0.0f : v[b][s];
+        }
+        l = __builtin_fmaf(l, alpha, sum);
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const _Float16 hi = (_Float16)v[b][s];
+                w[b >> 1][4 * (b & 1) + s] = hi;
+                if constexpr (kSplit) lo[b >> 1][4 * (b & 1) + s] = (_Float16)(v[b][s] - (float)hi);
+            }
     }
 };
 
-// A power of two above v (and at least 2^-110), as f32: the value scales' running unit.
-__device__ __forceinline__ float unit_above(float v) {
-    const uint32_t u = (__builtin_bit_cast(uint32_t, v) & 0x7f800000u) + 0x00800000u;
-    return __builtin_fmaxf(__builtin_bit_cast(float, min(u, 0x7e800000u)), 0x1p-110f);
-}
-
-// The value scales of a tile's blocks as weights over the running unit (grown where it has to be); returns by what
-// factor the output so far shrinks.
-__device__ __forceinline__ float tile_weights(const Blocks& bl, int i0, float& unit, float (&weight)[4]) {
-    float v[4];
+// The value scales' running unit, a power of two above all of them so far and at least 2^-110, as its biased exponent (0:
+// none yet). All of it is scalar arithmetic: the scales of a tile are the same for every lane.
+struct Unit {
+    int e = 0;
+    // The scales of a tile's blocks (first one: lane i0 of bl) as weights over the unit, grown where it has to be; returns
+    // by what factor the output so far shrinks. A NaN scale, which some rows may not see, leaves the unit alone.
+    __device__ __forceinline__ float weights(const Blocks& bl, int i0, float (&weight)[4]) {
+        int v[4], top = 17 << 23;
 #pragma unroll
-    for (int b = 0; b < 4; ++b) v[b] = bl.value(i0 + b);
-    // from 0 up: a NaN scale, which some rows may not see, leaves the unit alone
-    const float top = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(0.0f, v[0]), v[1]), __builtin_fmaxf(v[2], v[3]));
-    float shrink = 1.0f;
-    if (!(top < unit)) {  // also the first tile (unit 0)
-        const float grown = __builtin_fmaxf(unit, unit_above(top));
-        shrink = unit / grown;
-        unit = grown;
+        for (int b = 0; b < 4; ++b) {
+            v[b] = __builtin_amdgcn_readlane(__builtin_bit_cast(int, bl.cv), i0 + b);
+            top = max(top, v[b] < 0x7f800000 ? v[b] : 0);
+        }
+        const int grown = max(e, min((top >> 23) + 1, 253));
+        const float shrink = __builtin_bit_cast(float, max(127 + e - grown, 0) << 23);
+        e = grown;
+        const float inv = __builtin_bit_cast(float, (127 + 14 + 127 - grown) << 23);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) weight[b] = __builtin_bit_cast(float, v[b]) * inv;
+        return shrink;
     }
-    const float inv = kWeight / unit;
-#pragma unroll
-    for (int b = 0; b < 4; ++b) weight[b] = v[b] * inv;
-    return shrink;
-}
+    // What the output is multiplied by at the end.
+    __device__ __forceinline__ float back() const { return e ? __builtin_bit_cast(float, (e - 14) << 23) : 0.0f; }
+};
 
 // What a launch needs besides the cache.
 struct AttnArgs {
@@ -297,7 +304,7 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
     __shared__ int pre[kMaxItems + 1];
     __shared__ uint16_t ent[kMaxItems];
     __shared__ Entry entries[kMaxItems];
-    __shared__ int wave_sum[4];
+    __shared__ int wave_sum[12];
     __shared__ __align__(16) float so[4][kRowTile][kPad];
     __shared__ float sm[4][kRowTile], sl[4][kRowTile];
     const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4,
@@ -322,44 +329,68 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
     }
     __syncthreads();
     constexpr int kPer = kMaxItems / 256;
+    const int shares = (int)gridDim.x;
     int mine[kPer], sum = 0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
         mine[j] = tid * kPer + j < a.items ? pre[tid * kPer + j] : 0;
         sum += mine[j];
     }
+    sum = wave_sum_i32(sum);
+    if (lane == 0) wave_sum[wave] = sum;
+    __syncthreads();
+    // a share is whole rounds of the four waves
+    const int share = max(4, ((wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3] + shares - 1) / shares + 3) & ~3);
+    // items that begin on a share of their own where the shares suffice for that: no workgroup then has two items in turn
+    int padded[kPer];
+    sum = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        padded[j] = (mine[j] + share - 1) / share * share;
+        sum += padded[j];
+    }
+    sum = wave_sum_i32(sum);
+    if (lane == 0) wave_sum[4 + wave] = sum;
+    __syncthreads();
+    const bool apart = wave_sum[4] + wave_sum[5] + wave_sum[6] + wave_sum[7] <= shares * share;
+    sum = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) sum += apart ? padded[j] : mine[j];
     int incl = sum;
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
         const int y = __shfl_up(incl, s);
         incl += lane >= s ? y : 0;
     }
-    if (lane == 63) wave_sum[wave] = incl;
+    if (lane == 63) wave_sum[8 + wave] = incl;
     __syncthreads();
     int at = incl - sum, total = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        at += i < wave ? wave_sum[i] : 0;
-        total += wave_sum[i];
+        at += i < wave ? wave_sum[8 + i] : 0;
+        total += wave_sum[8 + i];
     }
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
         if (tid * kPer + j < a.items) pre[tid * kPer + j] = at;
-        at += mine[j];
+        at += apart ? padded[j] : mine[j];
     }
     if (tid == 0) pre[a.items] = total;
     __syncthreads();
 
-    // shares: whole rounds of the four waves
-    const int shares = (int)gridDim.x;
-    const int share = max(4, ((total + shares - 1) / shares + 3) & ~3);
+    // tiles of an item: its own, without what pads it
+    auto tiles_of = [&](int i) {
+        const Entry e = entries[ent[i]];
+        const int r1 = min((i - first_item(e, ent[i]) + 1) * kRowTile, e.rows) - 1;
+        return max(1, (visible(e, a, r1) + kTile - 1) / kTile);
+    };
     if (blockIdx.x == 0 && kvh == 0) {
         for (int i = tid; i < a.items; i += 256) {
             int4 r = make_int4(0, 0, 0, 0);
             if (pre[i + 1] > pre[i]) {
                 const int b = ent[i];
                 const Entry e = entries[b];
-                const int t = i - first_item(e, b), w0 = pre[i] / share, w1 = (pre[i + 1] - 1) / share;
+                const int t = i - first_item(e, b), w0 = pre[i] / share, w1 = (min(pre[i] + tiles_of(i), pre[i + 1]) - 1) / share;
                 r = make_int4(2 * w0 + (pre[i] > w0 * share ? 1 : 0), w1 > w0 ? w1 - w0 + 1 : 0, e.row0 + t * kRowTile,
                               min(kRowTile, e.rows - t * kRowTile));
             }
@@ -385,7 +416,10 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
     for (int done = from; done < to; ++item) {
         const int p0 = pre[item], p1 = pre[item + 1];
         if (p1 <= done) continue;
-        const int t0 = done - p0, t1 = min(to, p1) - p0;  // this item's tiles of the share
+        const int n_tiles = __builtin_amdgcn_readfirstlane(tiles_of(item));
+        const int t0 = done - p0, t1 = min(min(to, p1) - p0, n_tiles);  // this item's tiles of the share
+        done = min(to, p1);
+        if (t0 >= t1) continue;  // only what pads the item
         const int b = __builtin_amdgcn_readfirstlane((int)ent[item]);
         const Entry el = entries[b];
         const Entry e{__builtin_amdgcn_readfirstlane(el.seq), __builtin_amdgcn_readfirstlane(el.len),
@@ -423,14 +457,14 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
         q.convert(raw, valid, a.scale_log2e);
         Rows<T, kC> st;
         st.clear();
-        float unit = 0.0f;
+        Unit unit;
 
         for (int j = 0; j < n_mine; ++j) {
             const int pos0 = (t0 + wave + 4 * j) * kTile, i0 = 4 * (j & 15);
             float weight[4], key[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) key[k] = bl.key(i0 + k);
-            const float shrink = tile_weights(bl, i0, unit, weight);
+            const float shrink = unit.weights(bl, i0, weight);
             const uint32_t ok = (uint32_t)(bl.ok >> i0) & 15u;
             float x[4][4];
 #pragma unroll
@@ -454,16 +488,15 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
             }
             __builtin_amdgcn_sched_barrier(0);
             h8 w[2], lo[2];
-            if (pos0 + kTile > all_see || ok != 15u) {
+            const bool masked = pos0 + kTile > all_see || ok != 15u;
+            if (masked) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
 #pragma unroll
                     for (int s = 0; s < 4; ++s)
                         if (pos0 + 16 * k + 4 * g + s >= vis || !((ok >> k) & 1u)) x[k][s] = -__builtin_inff();
-                st.template step<true>(x, weight, shrink, w, lo);
-            } else {
-                st.template step<false>(x, weight, shrink, w, lo);
             }
+            st.step(x, weight, shrink, masked, w, lo);
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -484,7 +517,7 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
 
         // the four waves' results of this item together
         const float l = over_groups(st.l, [](float p, float q2) { return p + q2; });
-        const float back = unit * (1.0f / kWeight);
+        const float back = unit.back();
         if (g == 0) {
             sm[wave][col] = st.m;
             sl[wave][col] = l;
@@ -509,8 +542,8 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
                 f[w2] = __builtin_amdgcn_exp2f(sm[w2][rr] - base);
                 lsum = __builtin_fmaf(f[w2], sl[w2][rr], lsum);
             }
-            const bool whole = t0 == 0 && t1 == p1 - p0;
-            const int slot = 2 * (int)blockIdx.x + (done > from ? 1 : 0);
+            const bool whole = t0 == 0 && t1 == n_tiles;
+            const int slot = 2 * (int)blockIdx.x + (p0 + t0 > from ? 1 : 0);
             const size_t pr = ((size_t)slot * c.n_kv + kvh) * kRowTile + rr;
 #pragma unroll
             for (int cc = 0; cc < kC; ++cc) {
@@ -534,7 +567,6 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
             }
         }
         __syncthreads();
-        done = min(to, p1);
     }
 }
 
@@ -648,7 +680,7 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
     const int w0 = r0 + wave * 32, w1 = min(w0 + 31, last);
     const int all_see = w0 <= last ? visible(e, a, w0) : 0;   // positions that each row of the wave sees
     const int some_see = w0 <= last ? visible(e, a, w1) : 0;  // and that any of them does
-    float unit = 0.0f;
+    Unit unit;
 
     Blocks bl, bl_next;
     uint4 kr[kC], vr[2];
@@ -696,7 +728,7 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
     auto compute = [&](int buf, int t) {
         const int pos0 = t * kTile, i0 = 4 * ((t - t0) & 15);
         float weight[4];
-        const float shrink = tile_weights(bl, i0, unit, weight);
+        const float shrink = unit.weights(bl, i0, weight);
         if (pos0 >= some_see) {  // nothing here for this wave's rows; the unit has moved all the same
             if (shrink != 1.0f) {
 #pragma unroll
@@ -730,19 +762,17 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
             }
         }
         h8 w[2][2], lo[2][2];
-        if (pos0 + kTile > all_see || ok != 15u) {
+        const bool masked = pos0 + kTile > all_see || ok != 15u;
 #pragma unroll
-            for (int ct = 0; ct < 2; ++ct) {
+        for (int ct = 0; ct < 2; ++ct) {
+            if (masked) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
 #pragma unroll
                     for (int s = 0; s < 4; ++s)
                         if (pos0 + 16 * k + 4 * g + s >= vis[ct] || !((ok >> k) & 1u)) x[ct][k][s] = -__builtin_inff();
-                st[ct].template step<true>(x[ct], weight, shrink, w[ct], lo[ct]);
             }
-        } else {
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) st[ct].template step<false>(x[ct], weight, shrink, w[ct], lo[ct]);
+            st[ct].step(x[ct], weight, shrink, masked, w[ct], lo[ct]);
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -775,7 +805,7 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
         }
     }
 
-    const float back = unit * (1.0f / kWeight);
+    const float back = unit.back();
 #pragma unroll
     for (int ct = 0; ct < 2; ++ct) {
         const int rr = wave * 32 + ct * 16 + col, r = r0 + rr;
@@ -808,6 +838,7 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
 struct Plan {
     bool rows;
     int items, shares, splits;
+    int join_rows;     // rows that an item can have
     size_t part_rows;  // rows of partial results (per KV head)
     size_t bytes(int n_kv, int hd) const {
         return sizeof(int4) * (size_t)items + sizeof(float) * part_rows * n_kv * (hd + 2);
@@ -824,6 +855,7 @@ Plan plan_of(int group, int n_kv, int n, int n_tok, bool single) {
         p.shares = (2 * cus + n_kv - 1) / n_kv;
         if (p.shares > kMaxParts) p.shares = kMaxParts;
         p.splits = 1;
+        p.join_rows = single && group < kRowTile ? group : kRowTile;
         p.part_rows = 2 * (size_t)p.shares * kRowTile;
         return p;
     }
@@ -870,8 +902,8 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
         constexpr int kC = decltype(kc)::value;
         if (p.rows) {
             qh_launch((kv8_rows_kernel<T, kC>), dim3((unsigned)p.shares, (unsigned)c.n_kv), dim3(256), 0, s, c, a);
-            qh_launch((kv8_join_kernel<T, kC>), dim3((unsigned)p.items, (unsigned)c.n_kv, kRowTile), dim3(256), 0, s, c, a,
-                      kRowTile, 2);
+            qh_launch((kv8_join_kernel<T, kC>), dim3((unsigned)p.items, (unsigned)c.n_kv, (unsigned)p.join_rows), dim3(256), 0,
+                      s, c, a, kRowTile, 2);
         } else {
             constexpr size_t lds = 2 * 2 * (size_t)kTile * 64 * kC * 2;
             qh_launch((kv8_tile_kernel<T, kC>), dim3((unsigned)c.n_kv * (unsigned)p.items, (unsigned)p.splits), dim3(256), lds, s, c,
