@@ -602,7 +602,7 @@ size_t qh_kv8_attention_workspace_bytes(const qh_kv8_cache* c, int n_heads, int 
     const char* who = "qh_kv8_attention_workspace_bytes";
     if (validate_kv8(c, who) || validate_kv8_heads(*c, n_heads, n_tok, who)) return 0;
     if (n <= 0 || n_tok <= 0) return 0;
-    return kv8_attention_workspace_bytes(n_heads, c->n_kv_heads, c->head_dim, n, n_tok);
+    return kv8_attention_workspace_bytes(n_heads, c->n_kv_heads, c->head_dim, c->seq_pages * c->page_tokens, n, n_tok);
 }
 
 int qh_kv8_attention(const qh_kv8_cache* c, int layer, const void* q, void* out, int dtype, int n_heads, int64_t ldq,
@@ -618,7 +618,7 @@ int qh_kv8_attention(const qh_kv8_cache* c, int layer, const void* q, void* out,
     const int64_t width = (int64_t)n_heads * c->head_dim;
     if (int rc = validate_kv8_rows(q, dtype, ldq, width, who)) return rc;
     if (int rc = validate_kv8_rows(out, dtype, ldo, width, who)) return rc;
-    const size_t need = kv8_attention_workspace_bytes(n_heads, c->n_kv_heads, c->head_dim, n, n_tok);
+    const size_t need = kv8_attention_workspace_bytes(n_heads, c->n_kv_heads, c->head_dim, c->seq_pages * c->page_tokens, n, n_tok);
     if (!workspace || workspace_bytes < need)
         return fail(QH_ERR_NOMEM, "%s: workspace of %zu bytes, needs %zu", who, workspace ? workspace_bytes : 0, need);
     if (!aligned16(workspace)) return fail(QH_ERR_ALIGN, "%s: workspace not 16-byte aligned", who);

@@ -2,8 +2,9 @@
 //
 // A block is 16 tokens of one KV head, keys and values apart: 16 * head_dim codes (int8) and one f32 scale. A page holds
 // page_tokens / 16 blocks of every KV head: the key blocks [n_kv][page_tokens / 16], the value blocks likewise, then the
-// scales f32 [key, value][n_kv][page_tokens / 16]; pages are padded to 128 bytes. Within a block the codes lie in the
-// order in which a wave's 64 lanes take them as matrix operands, 16 bytes to a lane, so that every load of a block is one
+// scales f32 [key, value][n_kv][page_tokens / 16]; pages are padded to 128 bytes. A code is stored as code + 128 (the
+// attention makes f16 of it with one instruction less a word). Within a block the codes lie in the order in
+// which a wave's 64 lanes take them as matrix operands, 16 bytes to a lane, so that every load of a block is one
 // contiguous KB per 64 dimensions, without a transposition of the values:
 //   keys    [head_dim / 64][4 groups][16 tokens][16 dims]: lane 16 g + t holds dims 64 c + 16 g .. + 15 of token t
 //   values  [head_dim / 64][4 groups][16][4 dims][4 tokens]: lane 16 g + j holds dims 64 c + 4 j .. + 3 of tokens
@@ -96,7 +97,8 @@ hipError_t launch_kv8_fork(const Kv8View& c, int n_layers, const int32_t* src, c
                            void* ws, hipStream_t s);
 hipError_t launch_kv8_compact(const Kv8View& c, int n_layers, int32_t* live, void* ws, hipStream_t s);
 // qh_kv8_attn.hip
-size_t kv8_attention_workspace_bytes(int n_heads, int n_kv, int hd, int n, int n_tok);
+// capacity: positions that a sequence can have.
+size_t kv8_attention_workspace_bytes(int n_heads, int n_kv, int hd, int capacity, int n, int n_tok);
 hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int dtype, int n_heads, int64_t ldq,
                                 int64_t ldo, const int32_t* start, const int32_t* seqs, int n, int n_tok, bool causal,
                                 float scale, void* ws, hipStream_t s);

@@ -8,6 +8,8 @@ namespace {
 
 // ------------------------------------------------------------------------------------------- append and read back
 
+constexpr uint32_t kBias = 0x80808080u;  // the 128 that stored codes carry, in each byte of a word
+
 // 16 consecutive values at p as f32.
 __device__ __forceinline__ void load_row16(const float* p, float* x) {
 #pragma unroll
@@ -145,7 +147,7 @@ __device__ __forceinline__ void append_block(const Kv8View& c, const T* __restri
             }
         }
         if (held) {
-            const uint32_t o[4] = {old[k].x, old[k].y, old[k].z, old[k].w};
+            const uint32_t o[4] = {old[k].x ^ kBias, old[k].y ^ kBias, old[k].z ^ kBias, old[k].w ^ kBias};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint32_t keep = o[j];
@@ -166,7 +168,7 @@ __device__ __forceinline__ void append_block(const Kv8View& c, const T* __restri
                 w[j] = (keep & mask) | (w[j] & ~mask);
             }
         }
-        codes[64 * k] = make_uint4(w[0], w[1], w[2], w[3]);
+        codes[64 * k] = make_uint4(w[0] ^ kBias, w[1] ^ kBias, w[2] ^ kBias, w[3] ^ kBias);
     }
     if (lane == 0) *scale = d;
 }
@@ -224,8 +226,8 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8View c, T* __restrict_
     const uint4* codes = reinterpret_cast<const uint4*>(kv8_codes(c, ok ? page : 0, hw & 1, h, bp)) + lane;
 #pragma unroll
     for (int kk = 0; kk < kC; ++kk) {
-        const uint4 w4 = ok ? codes[64 * kk] : make_uint4(0, 0, 0, 0);
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+        const uint4 w4 = ok ? codes[64 * kk] : make_uint4(kBias, kBias, kBias, kBias);
+        const uint32_t w[4] = {w4.x ^ kBias, w4.y ^ kBias, w4.z ^ kBias, w4.w ^ kBias};
         float x[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = (float)(int8_t)(w[e >> 2] >> (8 * (e & 3))) * d;

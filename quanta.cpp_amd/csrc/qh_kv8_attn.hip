@@ -5,7 +5,7 @@
 // over the cache with the running maximum and sum: 64 positions (a tile) at a time, in f32.
 //
 // Both products run on the f16 matrix instructions (16 x 16 x 32): a code in [-127, 127] is exact in f16, so a tile's
-// codes become f16 operands (five instructions for four of them) and the block scales are applied to the scores and to
+// codes become f16 operands (four instructions for four of them) and the block scales are applied to the scores and to
 // the weights, whose tokens a lane holds next to each other. Scores are computed transposed (codes . queries), so that a
 // lane's weights are already the operand of the second product (values . weights, transposed too): no weight passes
 // through shared memory, and a row's maximum and sum belong to one lane column.
@@ -13,7 +13,7 @@
 //   13: what the split drops is below 2^-22 of each value, about what f32 sums round off. Weights likewise, in f32 calls;
 //   f16 calls round each weight to f16 once, half an ulp of the result's own type, in errors that average out over the
 //   positions. A weight carries the value scale of its block divided by a running power of two at least as large as all
-//   of them, times 2^14, so that small weights stay clear of f16's subnormals.
+//   of them, times 2^14 (2^6 in f16 calls), so that small weights stay clear of f16's subnormals.
 #include <type_traits>
 
 #include "qh_device.h"
@@ -28,13 +28,11 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 64;            // positions of one step
 constexpr int kRowTile = 16;         // query rows of a workgroup of the row kernel
-constexpr int kBigTile = 128;        // and of the tile kernel
 constexpr int kMaxItems = 1024;      // row tiles of one launch of the row kernel
 constexpr int kMaxParts = 1024;      // partial results of a row: shares of the row kernel, splits of the tile kernel
 
-// Four codes as f16: the bytes biased by 128 under the high byte 0x64 are the numbers 1024 + 128 + code.
-__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t* out) {
-    const uint32_t x = w ^ 0x80808080u;
+// Four codes as f16: the stored bytes, code + 128, under the high byte 0x64 are the numbers 1024 + 128 + code.
+__device__ __forceinline__ void codes_to_f16(uint32_t x, uint32_t* out) {
     const h2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
     out[0] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) - bias);
     out[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) - bias);
@@ -63,7 +61,7 @@ template <typename T, int kC>
 struct Query {
     static constexpr bool kSplit = std::is_same<T, float>::value;
     h8 hi[kC][2], lo[kSplit ? kC : 1][2];
-    float unit;  // x = product * unit * key scale
+    float unit;  // x = product * unit * key scale, positive: a negative scale's sign goes into the operands
 
     // The row's values as loaded; convert() makes the operands of them, so that other loads can be issued in between.
     using Raw = std::conditional_t<kSplit, float4, h8>;
@@ -93,8 +91,9 @@ struct Query {
             top = over_groups(top, fmax2);
             // the power of two that takes the largest value to [2^13, 2^14); an infinite row becomes NaN
             const int e = max((int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -100);
-            const float up = top < __builtin_inff() ? __builtin_ldexpf(1.0f, 13 - e) : __builtin_nanf("");
-            unit = __builtin_ldexpf(scale_log2e, e - 13);
+            const float up = top < __builtin_inff() ? __builtin_copysignf(__builtin_ldexpf(1.0f, 13 - e), scale_log2e)
+                                                    : __builtin_nanf("");
+            unit = __builtin_ldexpf(__builtin_fabsf(scale_log2e), e - 13);
 #pragma unroll
             for (int c = 0; c < kC; ++c)
 #pragma unroll
@@ -106,11 +105,11 @@ struct Query {
                         lo[c][h][j] = (_Float16)(x - (float)hi[c][h][j]);
                     }
         } else {
-            unit = scale_log2e;
+            unit = __builtin_fabsf(scale_log2e);
 #pragma unroll
             for (int c = 0; c < kC; ++c)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) hi[c][h] = valid ? r[c][h] : h8{};
+                for (int h = 0; h < 2; ++h) hi[c][h] = valid ? (scale_log2e < 0.0f ? -r[c][h] : r[c][h]) : h8{};
         }
     }
 
@@ -151,11 +150,16 @@ struct Blocks {
     }
 };
 
-// The running state of 16 query rows: maximum and this lane's share of the sum, and the output, transposed: lane
-// 16 g + r holds row r, register [4 c + i][s] dimension 64 c + 16 g + 4 s + i.
+// The running state of 16 query rows: the base that exponents are relative to, this lane's share of the sum, and the
+// output, transposed: lane 16 g + r holds row r, register [4 c + i][s] dimension 64 c + 16 g + 4 s + i.
+// The base is the row's maximum, in f16 calls at most kSlack below it: a maximum that grows by less leaves the output as
+// it is (a rescaling is 16 registers per 64 dimensions and row tile), and the weights, up to 2^kSlack then, stay clear of
+// f16's largest number because their unit leaves that much room.
 template <typename T, int kC>
 struct Rows {
     static constexpr bool kSplit = std::is_same<T, float>::value;
+    static constexpr float kSlack = kSplit ? 0.0f : 8.0f;
+    static constexpr int kRoom = kSplit ? 14 : 6;  // weights are below 2^(kRoom + kSlack)
     float m = -__builtin_inff(), l = 0.0f;
     f4 o[4 * kC];
 
@@ -166,42 +170,48 @@ struct Rows {
         for (int i = 0; i < 4 * kC; ++i) o[i] = f4{0, 0, 0, 0};
     }
 
-    // x: the scores of a tile (log2), [block][token 4 g + s], -inf where masked. weight[b]: value scale of block b over
-    // the running power of two, shrink: what that power grew by (<= 1). Leaves the weights as operands w (and their low
-    // halves lo). masked: some x may be masked, and then has weight 0 whatever its block's scale is.
-    __device__ __forceinline__ void step(float (&x)[4][4], const float (&weight)[4], float shrink, bool masked, h8 (&w)[2],
-                                         h8 (&lo)[2]) {
-        float top = x[0][0];
+    // x: a tile's products of codes and queries, [block][token 4 g + s], -inf where masked; x * f[b] is the score (log2).
+    // weight[b]: value scale of block b over the running unit, shrink: what that unit grew by (<= 1). Leaves the weights
+    // as operands w (and their low halves lo). masked: some x may be masked, and then counts nothing whatever its block's
+    // scales are.
+    __device__ __forceinline__ void step(const f4 (&x)[4], const float (&f)[4], const float (&weight)[4], float shrink,
+                                         bool masked, h8 (&w)[2], h8 (&lo)[2]) {
+        float top = -__builtin_inff();
 #pragma unroll
         for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int s = 0; s < 4; ++s) top = __builtin_fmaxf(top, x[b][s]);
-        top = __builtin_fmaxf(m, over_groups(top, fmax2));
-        // a row that has seen nothing yet: subtract 0, so that its weights are 2^-inf = 0 and not NaN
-        const float base = top == -__builtin_inff() ? 0.0f : top;
-        const float alpha = __builtin_amdgcn_exp2f(m - base);
-        m = top;
-        const float a = alpha * shrink;
-        if (__any(a != 1.0f)) {
+            top = __builtin_fmaxf(top, fmax2(fmax2(x[b][0], x[b][1]), fmax2(x[b][2], x[b][3])) * f[b]);
+        top = over_groups(top, fmax2);
+        if (__any(top > m + kSlack) || shrink != 1.0f) {
+            const float was = m;
+            m = __builtin_fmaxf(m, top);
+            const float alpha = m == was ? 1.0f : __builtin_amdgcn_exp2f(was - m);
+            l *= alpha;
+            const float a = alpha * shrink;
 #pragma unroll
             for (int i = 0; i < 4 * kC; ++i) o[i] *= a;
         }
-        float sum = 0.0f, v[4][4];
+        // a row that has seen nothing yet: subtract 0, so that its weights are 2^-inf = 0 and not NaN
+        const float base = m == -__builtin_inff() ? 0.0f : m;
+        float p[4][4], v[4][4];
 #pragma unroll
         for (int b = 0; b < 4; ++b)
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                const float p = __builtin_amdgcn_exp2f(x[b][s] - base);
-                sum += p;
-                v[b][s] = p * weight[b];
+                p[b][s] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][s], f[b], -base));
+                v[b][s] = p[b][s] * weight[b];
             }
         if (masked) {
 #pragma unroll
             for (int b = 0; b < 4; ++b)
 #pragma unroll
-                for (int s = 0; s < 4; ++s) v[b][s] = x[b][s] == -__builtin_inff() ? 0.0f : v[b][s];
+                for (int s = 0; s < 4; ++s) {
+                    const bool out = x[b][s] == -__builtin_inff();
+                    p[b][s] = out ? 0.0f : p[b][s];
+                    v[b][s] = out ? 0.0f : v[b][s];
+                }
         }
-        l = __builtin_fmaf(l, alpha, sum);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) l += (p[b][0] + p[b][1]) + (p[b][2] + p[b][3]);
 #pragma unroll
         for (int b = 0; b < 4; ++b)
 #pragma unroll
@@ -214,7 +224,8 @@ struct Rows {
 };
 
 // The value scales' running unit, a power of two above all of them so far and at least 2^-110, as its biased exponent (0:
-// none yet). All of it is scalar arithmetic: the scales of a tile are the same for every lane.
+// none yet). All of it is scalar arithmetic: the scales of a tile are the same for every lane. Weights carry 2^kRoom more.
+template <int kRoom>
 struct Unit {
     int e = 0;
     // The scales of a tile's blocks (first one: lane i0 of bl) as weights over the unit, grown where it has to be; returns
@@ -229,13 +240,13 @@ struct Unit {
         const int grown = max(e, min((top >> 23) + 1, 253));
         const float shrink = __builtin_bit_cast(float, max(127 + e - grown, 0) << 23);
         e = grown;
-        const float inv = __builtin_bit_cast(float, (127 + 14 + 127 - grown) << 23);
+        const float inv = __builtin_bit_cast(float, (127 + kRoom + 127 - grown) << 23);
 #pragma unroll
         for (int b = 0; b < 4; ++b) weight[b] = __builtin_bit_cast(float, v[b]) * inv;
         return shrink;
     }
     // What the output is multiplied by at the end.
-    __device__ __forceinline__ float back() const { return e ? __builtin_bit_cast(float, (e - 14) << 23) : 0.0f; }
+    __device__ __forceinline__ float back() const { return e ? __builtin_bit_cast(float, (e - kRoom) << 23) : 0.0f; }
 };
 
 // What a launch needs besides the cache.
@@ -457,7 +468,7 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
         q.convert(raw, valid, a.scale_log2e);
         Rows<T, kC> st;
         st.clear();
-        Unit unit;
+        Unit<Rows<T, kC>::kRoom> unit;
 
         for (int j = 0; j < n_mine; ++j) {
             const int pos0 = (t0 + wave + 4 * j) * kTile, i0 = 4 * (j & 15);
@@ -466,7 +477,8 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
             for (int k = 0; k < 4; ++k) key[k] = bl.key(i0 + k);
             const float shrink = unit.weights(bl, i0, weight);
             const uint32_t ok = (uint32_t)(bl.ok >> i0) & 15u;
-            float x[4][4];
+            f4 x[4];
+            float f[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 f4 acc = {0, 0, 0, 0};
@@ -475,9 +487,8 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
                     acc = q.dot(codes8_to_f16(kr[k][cc].x, kr[k][cc].y), cc, 0, acc);
                     acc = q.dot(codes8_to_f16(kr[k][cc].z, kr[k][cc].w), cc, 1, acc);
                 }
-                const float f = key[k] * q.unit;
-#pragma unroll
-                for (int s = 0; s < 4; ++s) x[k][s] = acc[s] * f;
+                x[k] = acc;
+                f[k] = key[k] * q.unit;
             }
             // the next tile's keys are in flight from here on, its values from the end of the step
             __builtin_amdgcn_sched_barrier(0);
@@ -496,7 +507,7 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
                     for (int s = 0; s < 4; ++s)
                         if (pos0 + 16 * k + 4 * g + s >= vis || !((ok >> k) & 1u)) x[k][s] = -__builtin_inff();
             }
-            st.step(x, weight, shrink, masked, w, lo);
+            st.step(x, f, weight, shrink, masked, w, lo);
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -635,16 +646,16 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8View c, AttnArgs a, in
 
 // ------------------------------------------------------------------------------------------------ many rows
 
-// Row tiles of 128 (a prompt's tokens times the query heads of a KV head), bound by the matrix instructions and, next to
-// them, by the exponentials. Each of the four waves holds 32 rows; a tile's codes become f16 once per workgroup, into
+// Row tiles of 64 kCt (a prompt's tokens times the query heads of a KV head), bound by the matrix instructions and, next to
+// them, by the exponentials. Each of the four waves holds 16 kCt rows; a tile's codes become f16 once per workgroup, into
 // shared memory, in the order in which the waves read them as operands (1 KB a read, no bank conflicts), in two buffers:
 // one barrier a tile, the next tile's codes converted and the one after that in flight while one is computed. The KV head
 // is the fastest grid index, so that the workgroups of one head share an XCD's L2 where there are eight heads, and the
 // last row tiles (which see the most positions) start first. splits > 1: that many workgroups share a row tile's
 // positions and leave partials.
-template <typename T, int kC>
+template <typename T, int kC, int kCt>
 __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a) {
-    constexpr int kHd = 64 * kC;
+    constexpr int kHd = 64 * kC, kRows = 64 * kCt;
     constexpr int kUnits = 4 * kC * 2 * 64;  // 16-byte units of a tile's keys (and values) in f16
     extern __shared__ __align__(16) uint4 lds[];  // [buffer][keys, values][kUnits]
     const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4,
@@ -652,24 +663,24 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
     const int kvh = (int)(blockIdx.x % (unsigned)c.n_kv), split = (int)blockIdx.y;
     const int item = a.items - 1 - (int)(blockIdx.x / (unsigned)c.n_kv);
     int from = 0, b = item;
-    b = kv8_entry_of(a.batch, item, a.group, kBigTile, 1, &from);
+    b = kv8_entry_of(a.batch, item, a.group, kRows, 1, &from);
     Entry e{0, 0, 0, 0, 0};
     if (b >= 0) e = entry_of(c, a, b);
-    const int r0 = b < 0 ? 0 : (item - from) * kBigTile;
+    const int r0 = b < 0 ? 0 : (item - from) * kRows;
     if (a.splits > 1 && split == 0 && kvh == 0 && tid == 0)
-        a.rec[item] = r0 < e.rows ? make_int4(item * a.splits, a.splits, e.row0 + r0, min(kBigTile, e.rows - r0))
+        a.rec[item] = r0 < e.rows ? make_int4(item * a.splits, a.splits, e.row0 + r0, min(kRows, e.rows - r0))
                                   : make_int4(0, 0, 0, 0);
     if (r0 >= e.rows) return;
-    const int last = min(r0 + kBigTile, e.rows) - 1;
+    const int last = min(r0 + kRows, e.rows) - 1;
     const int tiles = (visible(e, a, last) + kTile - 1) / kTile;
     const int t0 = (int)((long)tiles * split / a.splits), t1 = (int)((long)tiles * (split + 1) / a.splits);
 
-    Query<T, kC> q[2];
-    Rows<T, kC> st[2];
-    int vis[2];
+    Query<T, kC> q[kCt];
+    Rows<T, kC> st[kCt];
+    int vis[kCt];
 #pragma unroll
-    for (int ct = 0; ct < 2; ++ct) {
-        const int r = r0 + wave * 32 + ct * 16 + col;
+    for (int ct = 0; ct < kCt; ++ct) {
+        const int r = r0 + wave * (16 * kCt) + ct * 16 + col;
         const bool valid = r < e.rows;
         vis[ct] = valid ? visible(e, a, r) : 0;
         typename Query<T, kC>::Raw raw[kC][Query<T, kC>::kRaw];
@@ -677,10 +688,10 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
         q[ct].convert(raw, valid, a.scale_log2e);
         st[ct].clear();
     }
-    const int w0 = r0 + wave * 32, w1 = min(w0 + 31, last);
+    const int w0 = r0 + wave * (16 * kCt), w1 = min(w0 + 16 * kCt - 1, last);
     const int all_see = w0 <= last ? visible(e, a, w0) : 0;   // positions that each row of the wave sees
     const int some_see = w0 <= last ? visible(e, a, w1) : 0;  // and that any of them does
-    Unit unit;
+    Unit<Rows<T, kC>::kRoom> unit;
 
     Blocks bl, bl_next;
     uint4 kr[kC], vr[2];
@@ -732,7 +743,7 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
         if (pos0 >= some_see) {  // nothing here for this wave's rows; the unit has moved all the same
             if (shrink != 1.0f) {
 #pragma unroll
-                for (int ct = 0; ct < 2; ++ct)
+                for (int ct = 0; ct < kCt; ++ct)
 #pragma unroll
                     for (int i = 0; i < 4 * kC; ++i) st[ct].o[i] *= shrink;
             }
@@ -741,30 +752,32 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
         const uint32_t ok = (uint32_t)(bl.ok >> i0) & 15u;
         const uint4* ks = lds + (size_t)buf * 2 * kUnits;
         const uint4* vs = ks + kUnits;
-        float x[2][4][4];
+        f4 x[kCt][4];
+        float f[kCt][4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            f4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+            f4 acc[kCt];
+#pragma unroll
+            for (int ct = 0; ct < kCt; ++ct) acc[ct] = f4{0, 0, 0, 0};
 #pragma unroll
             for (int cc = 0; cc < kC; ++cc)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const h8 kk = __builtin_bit_cast(h8, ks[((k * kC + cc) * 2 + h) * 64 + lane]);
 #pragma unroll
-                    for (int ct = 0; ct < 2; ++ct) acc[ct] = q[ct].dot(kk, cc, h, acc[ct]);
+                    for (int ct = 0; ct < kCt; ++ct) acc[ct] = q[ct].dot(kk, cc, h, acc[ct]);
                 }
             const float key = bl.key(i0 + k);
 #pragma unroll
-            for (int ct = 0; ct < 2; ++ct) {
-                const float f = key * q[ct].unit;
-#pragma unroll
-                for (int s = 0; s < 4; ++s) x[ct][k][s] = acc[ct][s] * f;
+            for (int ct = 0; ct < kCt; ++ct) {
+                x[ct][k] = acc[ct];
+                f[ct][k] = key * q[ct].unit;
             }
         }
-        h8 w[2][2], lo[2][2];
+        h8 w[kCt][2], lo[kCt][2];
         const bool masked = pos0 + kTile > all_see || ok != 15u;
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct) {
+        for (int ct = 0; ct < kCt; ++ct) {
             if (masked) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
@@ -772,7 +785,7 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
                     for (int s = 0; s < 4; ++s)
                         if (pos0 + 16 * k + 4 * g + s >= vis[ct] || !((ok >> k) & 1u)) x[ct][k][s] = -__builtin_inff();
             }
-            st[ct].step(x[ct], weight, shrink, masked, w[ct], lo[ct]);
+            st[ct].step(x[ct], f[ct], weight, shrink, masked, w[ct], lo[ct]);
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -780,7 +793,7 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
             for (int i = 0; i < 4 * kC; ++i) {
                 const h8 v = __builtin_bit_cast(h8, vs[(u * kC * 4 + i) * 64 + lane]);
 #pragma unroll
-                for (int ct = 0; ct < 2; ++ct) {
+                for (int ct = 0; ct < kCt; ++ct) {
                     f4& o = st[ct].o[i];
                     o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[ct][u], o, 0, 0, 0);
                     if constexpr (Query<T, kC>::kSplit)
@@ -807,11 +820,11 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
 
     const float back = unit.back();
 #pragma unroll
-    for (int ct = 0; ct < 2; ++ct) {
-        const int rr = wave * 32 + ct * 16 + col, r = r0 + rr;
+    for (int ct = 0; ct < kCt; ++ct) {
+        const int rr = wave * (16 * kCt) + ct * 16 + col, r = r0 + rr;
         const float l = over_groups(st[ct].l, [](float p, float q2) { return p + q2; });
         if (r >= e.rows) continue;
-        const size_t pr = ((size_t)(item * a.splits + split) * c.n_kv + kvh) * kBigTile + rr;
+        const size_t pr = ((size_t)(item * a.splits + split) * c.n_kv + kvh) * kRows + rr;
         T* out = out_row<T>(a, c, e.row0 + r, kvh);
 #pragma unroll
         for (int cc = 0; cc < kC; ++cc)
@@ -838,13 +851,15 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
 struct Plan {
     bool rows;
     int items, shares, splits;
-    int join_rows;     // rows that an item can have
+    int tile;          // rows of an item
+    int join_rows;     // rows of an item that can be used
     size_t part_rows;  // rows of partial results (per KV head)
     size_t bytes(int n_kv, int hd) const {
         return sizeof(int4) * (size_t)items + sizeof(float) * part_rows * n_kv * (hd + 2);
     }
 };
-Plan plan_of(int group, int n_kv, int n, int n_tok, bool single) {
+// capacity: positions that a sequence can have.
+Plan plan_of(int group, int n_kv, int capacity, int n, int n_tok, bool single) {
     const long rows = (long)n_tok * group;
     const long few = single ? (long)n * ((group + kRowTile - 1) / kRowTile) : rows / kRowTile + n;
     const int cus = device_cus();
@@ -855,25 +870,32 @@ Plan plan_of(int group, int n_kv, int n, int n_tok, bool single) {
         p.shares = (2 * cus + n_kv - 1) / n_kv;
         if (p.shares > kMaxParts) p.shares = kMaxParts;
         p.splits = 1;
+        p.tile = kRowTile;
         p.join_rows = single && group < kRowTile ? group : kRowTile;
         p.part_rows = 2 * (size_t)p.shares * kRowTile;
         return p;
     }
-    p.items = (int)(rows / kBigTile + n);
+    // 128 rows to a workgroup, or 64 where that leaves compute units idle
+    p.tile = rows / 128 * n_kv >= cus ? 128 : 64;
+    p.items = (int)(rows / p.tile + n);
     const long wgs = (long)p.items * n_kv;
+    // splits for two workgroups to a compute unit, but none of fewer than four tiles
     p.splits = wgs >= cus ? 1 : (int)((2 * cus + wgs - 1) / wgs);
+    const int most = capacity / (4 * kTile);
     if (p.splits > 16) p.splits = 16;
-    p.part_rows = p.splits > 1 ? (size_t)p.items * p.splits * kBigTile : 0;
+    if (p.splits > most) p.splits = most > 1 ? most : 1;
+    p.join_rows = p.tile;
+    p.part_rows = p.splits > 1 ? (size_t)p.items * p.splits * p.tile : 0;
     return p;
 }
 
 }  // namespace
 
-size_t kv8_attention_workspace_bytes(int n_heads, int n_kv, int hd, int n, int n_tok) {
+size_t kv8_attention_workspace_bytes(int n_heads, int n_kv, int hd, int capacity, int n, int n_tok) {
     const int group = n_heads / n_kv;
-    size_t b = plan_of(group, n_kv, n, n_tok, false).bytes(n_kv, hd);
+    size_t b = plan_of(group, n_kv, capacity, n, n_tok, false).bytes(n_kv, hd);
     if (n == n_tok) {
-        const size_t single = plan_of(group, n_kv, n, n_tok, true).bytes(n_kv, hd);
+        const size_t single = plan_of(group, n_kv, capacity, n, n_tok, true).bytes(n_kv, hd);
         b = b > single ? b : single;
     }
     return b;
@@ -891,7 +913,7 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
     a.group = n_heads / c.n_kv;
     a.causal = causal ? 1 : 0;
     a.scale_log2e = scale * 1.44269504088896340736f;
-    const Plan p = plan_of(a.group, c.n_kv, n, n_tok, start == nullptr);
+    const Plan p = plan_of(a.group, c.n_kv, c.seq_pages << c.page_shift, n, n_tok, start == nullptr);
     a.items = p.items;
     a.splits = p.splits;
     a.rec = static_cast<int4*>(ws);
@@ -906,11 +928,14 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
                       s, c, a, kRowTile, 2);
         } else {
             constexpr size_t lds = 2 * 2 * (size_t)kTile * 64 * kC * 2;
-            qh_launch((kv8_tile_kernel<T, kC>), dim3((unsigned)c.n_kv * (unsigned)p.items, (unsigned)p.splits), dim3(256), lds, s, c,
-                      a);
+            const dim3 grid((unsigned)c.n_kv * (unsigned)p.items, (unsigned)p.splits);
+            if (p.tile == 128)
+                qh_launch((kv8_tile_kernel<T, kC, 2>), grid, dim3(256), lds, s, c, a);
+            else
+                qh_launch((kv8_tile_kernel<T, kC, 1>), grid, dim3(256), lds, s, c, a);
             if (p.splits > 1)
-                qh_launch((kv8_join_kernel<T, kC>), dim3((unsigned)p.items, (unsigned)c.n_kv, kBigTile), dim3(256), 0, s, c,
-                          a, kBigTile, 1);
+                qh_launch((kv8_join_kernel<T, kC>), dim3((unsigned)p.items, (unsigned)c.n_kv, (unsigned)p.join_rows),
+                          dim3(256), 0, s, c, a, p.tile, 1);
         }
     };
     using std::integral_constant;
