@@ -273,6 +273,12 @@ __device__ __forceinline__ Entry entry_of(const Kv8View& c, const AttnArgs& a, i
     const bool known = seq >= 0 && seq < c.n_seqs;
     return {known ? seq : 0, known ? kv8_len(c, seq) : 0, s1 - s0, s0 * a.group, (s1 - s0) * a.group};
 }
+// The same in scalar registers (every lane has the same entry).
+__device__ __forceinline__ Entry uniform(const Entry& e) {
+    return {__builtin_amdgcn_readfirstlane(e.seq), __builtin_amdgcn_readfirstlane(e.len),
+            __builtin_amdgcn_readfirstlane(e.tokens), __builtin_amdgcn_readfirstlane(e.row0),
+            __builtin_amdgcn_readfirstlane(e.rows)};
+}
 // Positions that row r of the entry sees.
 __device__ __forceinline__ int visible(const Entry& e, const AttnArgs& a, int r) {
     return a.causal ? min(max(e.len - e.tokens + r / a.group + 1, 0), e.len) : e.len;
@@ -432,10 +438,7 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
         done = min(to, p1);
         if (t0 >= t1) continue;  // only what pads the item
         const int b = __builtin_amdgcn_readfirstlane((int)ent[item]);
-        const Entry el = entries[b];
-        const Entry e{__builtin_amdgcn_readfirstlane(el.seq), __builtin_amdgcn_readfirstlane(el.len),
-                      __builtin_amdgcn_readfirstlane(el.tokens), __builtin_amdgcn_readfirstlane(el.row0),
-                      __builtin_amdgcn_readfirstlane(el.rows)};
+        const Entry e = uniform(entries[b]);
         const int r0 = (item - first_item(e, b)) * kRowTile, r = r0 + col;
         const bool valid = r < e.rows;
         const int n_mine = t1 - t0 > wave ? (t1 - t0 - wave + 3) / 4 : 0;  // tiles t0 + wave + 4 j
@@ -665,8 +668,8 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
     int from = 0, b = item;
     b = kv8_entry_of(a.batch, item, a.group, kRows, 1, &from);
     Entry e{0, 0, 0, 0, 0};
-    if (b >= 0) e = entry_of(c, a, b);
-    const int r0 = b < 0 ? 0 : (item - from) * kRows;
+    if (b >= 0) e = uniform(entry_of(c, a, b));
+    const int r0 = b < 0 ? 0 : (item - __builtin_amdgcn_readfirstlane(from)) * kRows;
     if (a.splits > 1 && split == 0 && kvh == 0 && tid == 0)
         a.rec[item] = r0 < e.rows ? make_int4(item * a.splits, a.splits, e.row0 + r0, min(kRows, e.rows - r0))
                                   : make_int4(0, 0, 0, 0);
@@ -688,9 +691,8 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
         q[ct].convert(raw, valid, a.scale_log2e);
         st[ct].clear();
     }
-    const int w0 = r0 + wave * (16 * kCt), w1 = min(w0 + 16 * kCt - 1, last);
-    const int all_see = w0 <= last ? visible(e, a, w0) : 0;   // positions that each row of the wave sees
-    const int some_see = w0 <= last ? visible(e, a, w1) : 0;  // and that any of them does
+    const int w0 = r0 + wave * (16 * kCt);
+    const int all_see = w0 <= last ? visible(e, a, w0) : 0;  // positions that each row of the wave sees
     Unit<Rows<T, kC>::kRoom> unit;
 
     Blocks bl, bl_next;
@@ -736,43 +738,51 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
             vs[at * 64 + lane] = __builtin_bit_cast(uint4, codes8_to_f16(a0[i], a1[i]));
         }
     };
+    // One tile from buffer buf, while the next tile's codes go into the other one. The matrix instructions run in the
+    // background of a wave, four issue slots each: the conversion of the next tile fills them in the first product, and
+    // each operand is read from shared memory several matrix instructions before its use.
+    constexpr int kMm = kCt * (Query<T, kC>::kSplit ? 2 : 1);  // matrix instructions to an operand read
+    h8 kk[4], vv[4];
     auto compute = [&](int buf, int t) {
         const int pos0 = t * kTile, i0 = 4 * ((t - t0) & 15);
-        float weight[4];
-        const float shrink = unit.weights(bl, i0, weight);
-        if (pos0 >= some_see) {  // nothing here for this wave's rows; the unit has moved all the same
-            if (shrink != 1.0f) {
-#pragma unroll
-                for (int ct = 0; ct < kCt; ++ct)
-#pragma unroll
-                    for (int i = 0; i < 4 * kC; ++i) st[ct].o[i] *= shrink;
-            }
-            return;
-        }
-        const uint32_t ok = (uint32_t)(bl.ok >> i0) & 15u;
-        const uint4* ks = lds + (size_t)buf * 2 * kUnits;
+        const uint4* ks = lds + (size_t)buf * 2 * kUnits + lane;
         const uint4* vs = ks + kUnits;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) kk[r] = __builtin_bit_cast(h8, ks[r * 64]);
         f4 x[kCt][4];
-        float f[kCt][4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            f4 acc[kCt];
-#pragma unroll
-            for (int ct = 0; ct < kCt; ++ct) acc[ct] = f4{0, 0, 0, 0};
-#pragma unroll
-            for (int cc = 0; cc < kC; ++cc)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const h8 kk = __builtin_bit_cast(h8, ks[((k * kC + cc) * 2 + h) * 64 + lane]);
-#pragma unroll
-                    for (int ct = 0; ct < kCt; ++ct) acc[ct] = q[ct].dot(kk, cc, h, acc[ct]);
-                }
-            const float key = bl.key(i0 + k);
+        for (int r = 0; r < 8 * kC; ++r) {  // operand r: key block r / (2 kC), dimensions by r % (2 kC)
+            const int k = r / (2 * kC), cc = r / 2 % kC, h = r & 1;
 #pragma unroll
             for (int ct = 0; ct < kCt; ++ct) {
-                x[ct][k] = acc[ct];
-                f[ct][k] = key * q[ct].unit;
+                if (r % (2 * kC) == 0) x[ct][k] = f4{0, 0, 0, 0};
+                x[ct][k] = q[ct].dot(kk[r & 3], cc, h, x[ct][k]);
             }
+            if (r + 4 < 8 * kC) kk[r & 3] = __builtin_bit_cast(h8, ks[(r + 4) * 64]);
+        }
+        stage(buf ^ 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int r = 0; r < 8 * kC; ++r) {
+            __builtin_amdgcn_sched_group_barrier(0x008, kMm, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+            if (r & 1) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (t + 2 < t1) fetch(t + 2);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) vv[r] = __builtin_bit_cast(h8, vs[r * 64]);
+        __builtin_amdgcn_sched_barrier(0);
+        float weight[4], f[kCt][4];
+        const float shrink = unit.weights(bl, i0, weight);
+        const uint32_t ok = (uint32_t)(bl.ok >> i0) & 15u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float key = bl.key(i0 + k);
+#pragma unroll
+            for (int ct = 0; ct < kCt; ++ct) f[ct][k] = key * q[ct].unit;
         }
         h8 w[kCt][2], lo[kCt][2];
         const bool masked = pos0 + kTile > all_see || ok != 15u;
@@ -787,19 +797,25 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
             }
             st[ct].step(x[ct], f[ct], weight, shrink, masked, w[ct], lo[ct]);
         }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int r = 0; r < 8 * kC; ++r) {  // operand r: token pair of blocks r / (4 kC), dimensions by r % (4 kC)
+            const int u = r / (4 * kC), i = r % (4 * kC);
 #pragma unroll
-            for (int i = 0; i < 4 * kC; ++i) {
-                const h8 v = __builtin_bit_cast(h8, vs[(u * kC * 4 + i) * 64 + lane]);
-#pragma unroll
-                for (int ct = 0; ct < kCt; ++ct) {
-                    f4& o = st[ct].o[i];
-                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[ct][u], o, 0, 0, 0);
-                    if constexpr (Query<T, kC>::kSplit)
-                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[ct][u], o, 0, 0, 0);
-                }
+            for (int ct = 0; ct < kCt; ++ct) {
+                f4& o = st[ct].o[i];
+                o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv[r & 3], w[ct][u], o, 0, 0, 0);
+                if constexpr (Query<T, kC>::kSplit)
+                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv[r & 3], lo[ct][u], o, 0, 0, 0);
             }
+            if (r + 4 < 8 * kC) vv[r & 3] = __builtin_bit_cast(h8, vs[(r + 4) * 64]);
+        }
+#pragma unroll
+        for (int r = 0; r < 8 * kC; ++r) {
+            __builtin_amdgcn_sched_group_barrier(0x008, kMm, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
     };
 
     if (t0 < t1) {
@@ -810,11 +826,7 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
         for (int t = t0; t < t1; ++t) {
             __syncthreads();  // tile t is staged, and tile t - 1 (whose buffer comes next) has been read
             if (t > t0 && ((t - t0) & 15) == 0) bl = bl_next;
-            if (t + 1 < t1) stage((t + 1 - t0) & 1);
-            const bool more = t + 2 < t1;
-            // the blocks of the tiles in flight replace those in use only after the last of these
-            if (more) fetch(t + 2);
-            compute((t - t0) & 1, t);
+            compute((t - t0) & 1, t);  // past the last tile it stages what it has once more, for nobody
         }
     }
 
