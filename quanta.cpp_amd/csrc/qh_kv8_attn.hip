@@ -13,7 +13,7 @@
 //   13: what the split drops is below 2^-22 of each value, about what f32 sums round off. Weights likewise, in f32 calls;
 //   f16 calls round each weight to f16 once, half an ulp of the result's own type, in errors that average out over the
 //   positions. A weight carries the value scale of its block divided by a running power of two at least as large as all
-//   of them, times 2^14 (2^6 in f16 calls), so that small weights stay clear of f16's subnormals.
+//   of them, times 2^6, so that small weights stay clear of f16's subnormals and large ones of its infinity.
 #include <type_traits>
 
 #include "qh_device.h"
@@ -29,7 +29,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 constexpr int kTile = 64;            // positions of one step
 constexpr int kRowTile = 16;         // query rows of a workgroup of the row kernel
 constexpr int kMaxItems = 1024;      // row tiles of one launch of the row kernel
-constexpr int kMaxParts = 1024;      // partial results of a row: shares of the row kernel, splits of the tile kernel
+constexpr int kMaxParts = 1024;      // shares of the row kernel: partial results of a row
 
 // Four codes as f16: the stored bytes, code + 128, under the high byte 0x64 are the numbers 1024 + 128 + code.
 __device__ __forceinline__ void codes_to_f16(uint32_t x, uint32_t* out) {
@@ -152,14 +152,16 @@ struct Blocks {
 
 // The running state of 16 query rows: the base that exponents are relative to, this lane's share of the sum, and the
 // output, transposed: lane 16 g + r holds row r, register [4 c + i][s] dimension 64 c + 16 g + 4 s + i.
-// The base is the row's maximum, in f16 calls at most kSlack below it: a maximum that grows by less leaves the output as
-// it is (a rescaling is 16 registers per 64 dimensions and row tile), and the weights, up to 2^kSlack then, stay clear of
-// f16's largest number because their unit leaves that much room.
+// The base is a maximum that the row has had, and no later score exceeds it by more than 2^kSlack: only then does it move
+// and the output with it (16 registers per 64 dimensions and row tile), so that most tiles need neither that nor the
+// maximum over the row's four lanes. Weights, up to 2^kSlack, stay clear of f16's largest number because their unit leaves
+// that much room; their smallest step is 2^-31 of the base's weight.
+constexpr float kSlack = 8.0f;
+constexpr int kRoom = 6;  // weights are below 2^(kRoom + kSlack)
+
 template <typename T, int kC>
 struct Rows {
     static constexpr bool kSplit = std::is_same<T, float>::value;
-    static constexpr float kSlack = kSplit ? 0.0f : 8.0f;
-    static constexpr int kRoom = kSplit ? 14 : 6;  // weights are below 2^(kRoom + kSlack)
     float m = -__builtin_inff(), l = 0.0f;
     f4 o[4 * kC];
 
@@ -180,10 +182,9 @@ struct Rows {
 #pragma unroll
         for (int b = 0; b < 4; ++b)
             top = __builtin_fmaxf(top, fmax2(fmax2(x[b][0], x[b][1]), fmax2(x[b][2], x[b][3])) * f[b]);
-        top = over_groups(top, fmax2);
         if (__any(top > m + kSlack) || shrink != 1.0f) {
             const float was = m;
-            m = __builtin_fmaxf(m, top);
+            m = __builtin_fmaxf(m, over_groups(top, fmax2));
             const float alpha = m == was ? 1.0f : __builtin_amdgcn_exp2f(was - m);
             l *= alpha;
             const float a = alpha * shrink;
@@ -225,7 +226,6 @@ struct Rows {
 
 // The value scales' running unit, a power of two above all of them so far and at least 2^-110, as its biased exponent (0:
 // none yet). All of it is scalar arithmetic: the scales of a tile are the same for every lane. Weights carry 2^kRoom more.
-template <int kRoom>
 struct Unit {
     int e = 0;
     // The scales of a tile's blocks (first one: lane i0 of bl) as weights over the unit, grown where it has to be; returns
@@ -471,7 +471,7 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
         q.convert(raw, valid, a.scale_log2e);
         Rows<T, kC> st;
         st.clear();
-        Unit<Rows<T, kC>::kRoom> unit;
+        Unit unit;
 
         for (int j = 0; j < n_mine; ++j) {
             const int pos0 = (t0 + wave + 4 * j) * kTile, i0 = 4 * (j & 15);
@@ -586,10 +586,9 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
 
 // Joins an item's partial results: one workgroup per item, KV head and row. First the partials' maxima, a thread to each,
 // and from them every partial's factor; then hd / 4 threads to a partial's row, the workgroup's groups of them taking
-// turns, so that the loads are independent of each other. Partial k is slot first (k = 0) or the k-th multiple of stride
-// after.
+// turns, so that the loads are independent of each other. Partial k is slot first (k = 0) or the k-th even one after.
 template <typename T, int kC>
-__global__ __launch_bounds__(256) void kv8_join_kernel(Kv8View c, AttnArgs a, int rows, int stride) {
+__global__ __launch_bounds__(256) void kv8_join_kernel(Kv8View c, AttnArgs a) {
     constexpr int kHd = 64 * kC, kThr = kHd / 4, kGroups = 256 / kThr;
     __shared__ __align__(16) float so[kGroups][kHd];
     __shared__ float factor[kMaxParts], wave_top[4], wave_sum[4];
@@ -597,8 +596,8 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8View c, AttnArgs a, in
     const int row = (int)blockIdx.z, kvh = (int)blockIdx.y, tid = (int)threadIdx.x, grp = tid / kThr, d = 4 * (tid % kThr);
     if (rec.y == 0 || row >= rec.w) return;
     auto at = [&](int k) {
-        const int slot = k == 0 ? rec.x : rec.x / stride * stride + k * stride;
-        return ((size_t)slot * c.n_kv + kvh) * rows + row;
+        const int slot = k == 0 ? rec.x : (rec.x & ~1) + 2 * k;
+        return ((size_t)slot * c.n_kv + kvh) * kRowTile + row;
     };
     float m[kMaxParts / 256], top = -__builtin_inff();
 #pragma unroll
@@ -643,6 +642,34 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8View c, AttnArgs a, in
     for (int k = 1; k < kGroups; ++k) {
         const float4 v = *reinterpret_cast<const float4*>(&so[k][d]);
         o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+    }
+    store_out(out_row<T>(a, c, rec.z + row, kvh) + d, o, top, l);
+}
+
+// The same for few partials (the splits of the tile kernel): every group of hd / 4 threads joins a row of its own.
+template <typename T, int kC>
+__global__ __launch_bounds__(256) void kv8_join_splits_kernel(Kv8View c, AttnArgs a, int rows) {
+    constexpr int kHd = 64 * kC, kThr = kHd / 4, kGroups = 256 / kThr;
+    const int4 rec = a.rec[blockIdx.x];
+    const int row = (int)blockIdx.z * kGroups + (int)threadIdx.x / kThr, kvh = (int)blockIdx.y;
+    const int d = 4 * ((int)threadIdx.x % kThr);
+    if (rec.y == 0 || row >= rec.w) return;
+    const size_t first = ((size_t)rec.x * c.n_kv + kvh) * rows + row, next = (size_t)c.n_kv * rows;
+    float top = -__builtin_inff();
+    for (int k = 0; k < rec.y; ++k) top = __builtin_fmaxf(top, a.part_ml[2 * (first + k * next)]);
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    float l = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int k = 0; k < rec.y; ++k) {
+        const size_t p = first + k * next;
+        const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * p] - base);
+        const float4 v = *reinterpret_cast<const float4*>(a.part_o + p * kHd + d);
+        l = __builtin_fmaf(f, a.part_ml[2 * p + 1], l);
+        o.x = __builtin_fmaf(f, v.x, o.x);
+        o.y = __builtin_fmaf(f, v.y, o.y);
+        o.z = __builtin_fmaf(f, v.z, o.z);
+        o.w = __builtin_fmaf(f, v.w, o.w);
     }
     store_out(out_row<T>(a, c, rec.z + row, kvh) + d, o, top, l);
 }
@@ -693,7 +720,7 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
     }
     const int w0 = r0 + wave * (16 * kCt);
     const int all_see = w0 <= last ? visible(e, a, w0) : 0;  // positions that each row of the wave sees
-    Unit<Rows<T, kC>::kRoom> unit;
+    Unit unit;
 
     Blocks bl, bl_next;
     uint4 kr[kC], vr[2];
@@ -937,7 +964,7 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
         if (p.rows) {
             qh_launch((kv8_rows_kernel<T, kC>), dim3((unsigned)p.shares, (unsigned)c.n_kv), dim3(256), 0, s, c, a);
             qh_launch((kv8_join_kernel<T, kC>), dim3((unsigned)p.items, (unsigned)c.n_kv, (unsigned)p.join_rows), dim3(256), 0,
-                      s, c, a, kRowTile, 2);
+                      s, c, a);
         } else {
             constexpr size_t lds = 2 * 2 * (size_t)kTile * 64 * kC * 2;
             const dim3 grid((unsigned)c.n_kv * (unsigned)p.items, (unsigned)p.splits);
@@ -946,8 +973,9 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
             else
                 qh_launch((kv8_tile_kernel<T, kC, 1>), grid, dim3(256), lds, s, c, a);
             if (p.splits > 1)
-                qh_launch((kv8_join_kernel<T, kC>), dim3((unsigned)p.items, (unsigned)c.n_kv, (unsigned)p.join_rows),
-                          dim3(256), 0, s, c, a, p.tile, 1);
+                qh_launch((kv8_join_splits_kernel<T, kC>),
+                          dim3((unsigned)p.items, (unsigned)c.n_kv, (unsigned)(p.join_rows * kC / 16)), dim3(256), 0, s, c,
+                          a, p.tile);
         }
     };
     using std::integral_constant;

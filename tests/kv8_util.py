@@ -209,11 +209,11 @@ def attention_bound(dtype, out, spread, score, small, n, hd):
     relative error is the score's absolute one; twice, for the sum below the fraction too. A weight: exp2 and its product
     with the value scale, five roundings, and its own format: two f16 (2^-22) or one (2^-11). The sums over n positions
     round n times, in both parts of the fraction; joining partial results adds sixteen. The smallest weights end in f16's
-    subnormals: a weight (times its value scale, over a unit of at most twice the largest scale, times 2^14, in f16 calls
-    2^6) is off by at most half their step of 2^-24, so a position by 2^-25 / 2^14 * 2 * largest scale * |code| = 2^-38 of
-    them (2^-30 in f16 calls); the weights' sum is at least 1."""
+    subnormals: a weight (times its value scale, over a unit of at most twice the largest scale, times 2^6) is off by at
+    most half their step of 2^-24, so a position by 2^-25 / 2^6 * 2 * largest scale * |code| = 2^-30 of them; the weights'
+    sum is at least 1."""
     f32 = dtype == "f32"
     weight = 2 * score * (2.0 ** -22 + (hd + 8) * 2.0 ** -24)
     rel = weight + 10 * 2.0 ** -24 + (2.0 ** -22 if f32 else 2.0 ** -11) + 2 * (n + 16) * 2.0 ** -24
-    bound = spread * rel[..., None] + small * 2.0 ** (-38 if f32 else -30)
+    bound = spread * rel[..., None] + small * 2.0 ** -30
     return bound + (np.abs(out) * 2.0 ** -24 + 1e-37 if f32 else np.abs(out) * 2.0 ** -11 + 2.0 ** -25)
