@@ -142,17 +142,11 @@ struct Blocks {
         page = good ? page : 0;
     }
     __device__ __forceinline__ int page_of(int i) const { return __builtin_amdgcn_readlane(page, i); }
-    __device__ __forceinline__ float key(int i) const {
-        return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ck), i));
-    }
-    __device__ __forceinline__ float value(int i) const {
-        return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, cv), i));
-    }
 };
 
 // The running state of 16 query rows: the base that exponents are relative to, this lane's share of the sum, and the
 // output, transposed: lane 16 g + r holds row r, register [4 c + i][s] dimension 64 c + 16 g + 4 s + i.
-// The base is a maximum that the row has had, and no later score exceeds it by more than 2^kSlack: only then does it move
+// The base is a maximum that the row has had, and no later score exceeds it by more than kSlack: only then does it move
 // and the output with it (16 registers per 64 dimensions and row tile), so that most tiles need neither that nor the
 // maximum over the row's four lanes. Weights, up to 2^kSlack, stay clear of f16's largest number because their unit leaves
 // that much room; their smallest step is 2^-31 of the base's weight.
@@ -172,12 +166,29 @@ struct Rows {
         for (int i = 0; i < 4 * kC; ++i) o[i] = f4{0, 0, 0, 0};
     }
 
-    // x: a tile's products of codes and queries, [block][token 4 g + s], -inf where masked; x * f[b] is the score (log2).
-    // weight[b]: value scale of block b over the running unit, shrink: what that unit grew by (<= 1). Leaves the weights
-    // as operands w (and their low halves lo). masked: some x may be masked, and then counts nothing whatever its block's
-    // scales are.
-    __device__ __forceinline__ void step(const f4 (&x)[4], const float (&f)[4], const float (&weight)[4], float shrink,
-                                         bool masked, h8 (&w)[2], h8 (&lo)[2]) {
+    // A step over a tile: x its products of codes and queries, [block][token 4 g + s]; x * f[b] is the score (log2).
+    // The row sees the positions below vis; pos: this lane's first position in the tile, ok: bit b for a block that
+    // exists. A masked position gets the score -inf, and so the weight 0: f may not be 0 for that (scores that a larger f
+    // changes are below 2^-80).
+    __device__ __forceinline__ static void mask(f4 (&x)[4], float (&f)[4], int pos, int vis, uint32_t ok) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            f[b] = __builtin_fmaxf(f[b], 0x1p-126f);
+            const int end = (ok >> b) & 1u ? vis : 0;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) x[b][s] = pos + 16 * b + s >= end ? -__builtin_inff() : x[b][s];
+        }
+    }
+    // Blocks of a tile whose scales are NaN (bits of nan) make NaN of the rows that see any of their tokens.
+    __device__ __forceinline__ void poison(uint32_t nan, int pos0, int vis) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+            if ((nan >> b) & 1u) l = pos0 + 16 * b < vis ? __builtin_nanf("") : l;
+    }
+
+    // Moves the base where a score passes it by too much, and the output with it; shrink: what the value scales' unit asks
+    // for.
+    __device__ __forceinline__ void settle(const f4 (&x)[4], const float (&f)[4], float shrink) {
         float top = -__builtin_inff();
 #pragma unroll
         for (int b = 0; b < 4; ++b)
@@ -191,59 +202,69 @@ struct Rows {
 #pragma unroll
             for (int i = 0; i < 4 * kC; ++i) o[i] *= a;
         }
+    }
+
+    // The weights as operands w, two blocks to each (and their low halves lo).
+    __device__ __forceinline__ void weigh(const f4 (&x)[4], const float (&f)[4], const float (&weight)[4], h8 (&w)[2],
+                                          h8 (&lo)[2]) {
         // a row that has seen nothing yet: subtract 0, so that its weights are 2^-inf = 0 and not NaN
         const float base = m == -__builtin_inff() ? 0.0f : m;
-        float p[4][4], v[4][4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                p[b][s] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][s], f[b], -base));
-                v[b][s] = p[b][s] * weight[b];
-            }
-        if (masked) {
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const bool out = x[b][s] == -__builtin_inff();
-                    p[b][s] = out ? 0.0f : p[b][s];
-                    v[b][s] = out ? 0.0f : v[b][s];
-                }
-        }
-#pragma unroll
-        for (int b = 0; b < 4; ++b) l += (p[b][0] + p[b][1]) + (p[b][2] + p[b][3]);
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
+        for (int b = 0; b < 4; ++b) {
+            float p[4];
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                const _Float16 hi = (_Float16)v[b][s];
+                p[s] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][s], f[b], -base));
+                float v = p[s] * weight[b];
+                // the halves are of one number: without this the compiler may round the product straight to f16 for one
+                // use of hi and the f32 product for the other, which differ where the product is close to a tie
+                if constexpr (kSplit) asm("" : "+v"(v));
+                const _Float16 hi = (_Float16)v;
                 w[b >> 1][4 * (b & 1) + s] = hi;
-                if constexpr (kSplit) lo[b >> 1][4 * (b & 1) + s] = (_Float16)(v[b][s] - (float)hi);
+                if constexpr (kSplit) lo[b >> 1][4 * (b & 1) + s] = (_Float16)(v - (float)hi);
             }
+            l += (p[0] + p[1]) + (p[2] + p[3]);
+        }
     }
 };
 
+// A tile's scales, the same for every lane.
+struct Scales {
+    float key[4], weight[4];
+    float shrink;  // what the output so far is multiplied by, as the unit grew
+    uint32_t ok;   // bits of the blocks that exist
+    uint32_t nan;  // and of those with a NaN scale: they count as zeros here, see Rows::poison
+};
+
 // The value scales' running unit, a power of two above all of them so far and at least 2^-110, as its biased exponent (0:
-// none yet). All of it is scalar arithmetic: the scales of a tile are the same for every lane. Weights carry 2^kRoom more.
+// none yet). Weights are value scales over it, times 2^kRoom.
 struct Unit {
     int e = 0;
-    // The scales of a tile's blocks (first one: lane i0 of bl) as weights over the unit, grown where it has to be; returns
-    // by what factor the output so far shrinks. A NaN scale, which some rows may not see, leaves the unit alone.
-    __device__ __forceinline__ float weights(const Blocks& bl, int i0, float (&weight)[4]) {
+    // The scales of the tile whose first block is lane i0 of bl; the unit grows where it has to.
+    __device__ __forceinline__ Scales next(const Blocks& bl, int i0) {
+        Scales t;
         int v[4], top = 17 << 23;
+        t.ok = (uint32_t)(bl.ok >> i0) & 15u;
+        t.nan = 0;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
+            int k = __builtin_amdgcn_readlane(__builtin_bit_cast(int, bl.ck), i0 + b);
             v[b] = __builtin_amdgcn_readlane(__builtin_bit_cast(int, bl.cv), i0 + b);
-            top = max(top, v[b] < 0x7f800000 ? v[b] : 0);
+            const bool bad = max(k, v[b]) >= 0x7f800000;  // scales are never negative
+            t.nan |= bad ? 1u << b : 0u;
+            k = bad ? 0 : k;
+            v[b] = bad ? 0 : v[b];
+            t.key[b] = __builtin_bit_cast(float, k);
+            top = max(top, v[b]);
         }
         const int grown = max(e, min((top >> 23) + 1, 253));
-        const float shrink = __builtin_bit_cast(float, max(127 + e - grown, 0) << 23);
+        t.shrink = __builtin_bit_cast(float, max(127 + e - grown, 0) << 23);
         e = grown;
         const float inv = __builtin_bit_cast(float, (127 + kRoom + 127 - grown) << 23);
 #pragma unroll
-        for (int b = 0; b < 4; ++b) weight[b] = __builtin_bit_cast(float, v[b]) * inv;
-        return shrink;
+        for (int b = 0; b < 4; ++b)
+            t.weight[b] = __builtin_bit_cast(float, v[b]) * inv;
+        return t;
     }
     // What the output is multiplied by at the end.
     __device__ __forceinline__ float back() const { return e ? __builtin_bit_cast(float, (e - kRoom) << 23) : 0.0f; }
@@ -475,11 +496,7 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
 
         for (int j = 0; j < n_mine; ++j) {
             const int pos0 = (t0 + wave + 4 * j) * kTile, i0 = 4 * (j & 15);
-            float weight[4], key[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) key[k] = bl.key(i0 + k);
-            const float shrink = unit.weights(bl, i0, weight);
-            const uint32_t ok = (uint32_t)(bl.ok >> i0) & 15u;
+            const Scales sc = unit.next(bl, i0);
             f4 x[4];
             float f[4];
 #pragma unroll
@@ -491,7 +508,7 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
                     acc = q.dot(codes8_to_f16(kr[k][cc].z, kr[k][cc].w), cc, 1, acc);
                 }
                 x[k] = acc;
-                f[k] = key[k] * q.unit;
+                f[k] = sc.key[k] * q.unit;
             }
             // the next tile's keys are in flight from here on, its values from the end of the step
             __builtin_amdgcn_sched_barrier(0);
@@ -502,15 +519,10 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
             }
             __builtin_amdgcn_sched_barrier(0);
             h8 w[2], lo[2];
-            const bool masked = pos0 + kTile > all_see || ok != 15u;
-            if (masked) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-#pragma unroll
-                    for (int s = 0; s < 4; ++s)
-                        if (pos0 + 16 * k + 4 * g + s >= vis || !((ok >> k) & 1u)) x[k][s] = -__builtin_inff();
-            }
-            st.step(x, f, weight, shrink, masked, w, lo);
+            if (pos0 + kTile > all_see || sc.ok != 15u) st.mask(x, f, pos0 + 4 * g, vis, sc.ok);
+            if (sc.nan) st.poison(sc.nan, pos0, vis);
+            st.settle(x, f, sc.shrink);
+            st.weigh(x, f, sc.weight, w, lo);
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -676,16 +688,16 @@ __global__ __launch_bounds__(256) void kv8_join_splits_kernel(Kv8View c, AttnArg
 
 // ------------------------------------------------------------------------------------------------ many rows
 
-// Row tiles of 64 kCt (a prompt's tokens times the query heads of a KV head), bound by the matrix instructions and, next to
-// them, by the exponentials. Each of the four waves holds 16 kCt rows; a tile's codes become f16 once per workgroup, into
-// shared memory, in the order in which the waves read them as operands (1 KB a read, no bank conflicts), in two buffers:
-// one barrier a tile, the next tile's codes converted and the one after that in flight while one is computed. The KV head
-// is the fastest grid index, so that the workgroups of one head share an XCD's L2 where there are eight heads, and the
-// last row tiles (which see the most positions) start first. splits > 1: that many workgroups share a row tile's
-// positions and leave partials.
+// Row tiles of 16 kW kCt (a prompt's tokens times the query heads of a KV head), bound by instruction issue: the matrix
+// instructions and, next to them, the exponentials. Each of the kW waves holds 16 kCt rows; a tile's codes become f16 once
+// per workgroup, into shared memory, in the order in which the waves read them as operands (1 KB a read, no bank
+// conflicts), in two buffers: one barrier a tile, the next tile's codes converted between the matrix instructions of this
+// one and the one after that in flight. The KV head is the fastest grid index, so that the workgroups of one head share an
+// XCD's L2 where there are eight heads, and the last row tiles (which see the most positions) start first. splits > 1:
+// that many workgroups share a row tile's positions and leave partials.
 template <typename T, int kC, int kCt>
 __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a) {
-    constexpr int kHd = 64 * kC, kRows = 64 * kCt;
+    constexpr int kHd = 64 * kC, kW = 4, kRows = 16 * kW * kCt;
     constexpr int kUnits = 4 * kC * 2 * 64;  // 16-byte units of a tile's keys (and values) in f16
     extern __shared__ __align__(16) uint4 lds[];  // [buffer][keys, values][kUnits]
     const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4,
@@ -722,76 +734,84 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
     const int all_see = w0 <= last ? visible(e, a, w0) : 0;  // positions that each row of the wave sees
     Unit unit;
 
-    Blocks bl, bl_next;
-    uint4 kr[kC], vr[2];
-    // Wave w stages key block w and a quarter of the values: pair u = w / 2 of the blocks, dimensions by w % 2.
+    // Each wave stages kPer operands of the keys and of the values, of one block of keys and one pair of blocks of values.
+    constexpr int kPer = 8 * kC / kW;
+    const int k_op = wave * kPer, k_blk = k_op / (2 * kC), v_pair = k_op / (4 * kC), v_c = k_op / 4 % kC, v_i = k_op % 4;
+    Blocks bl, ahead;
+    uint32_t kr[2 * kPer], vr[2][kPer];
+    const int per = (1 << (c.page_shift - 4)) - 1;
     auto fetch = [&](int t) {
         const int j = (t - t0) & 15;
         if (j == 0) {
             const int tl = t + (lane >> 2);
-            bl_next.load(c, e.seq, kvh, tl, tl < t1, e.len);
+            ahead.load(c, e.seq, kvh, tl, tl < t1, e.len);
         }
-        const int per = (1 << (c.page_shift - 4)) - 1;
-        const uint4* kp =
-            reinterpret_cast<const uint4*>(kv8_codes(c, bl_next.page_of(4 * j + wave), 0, kvh, (t * 4 + wave) & per)) + lane;
+        const uint8_t* kp = kv8_codes(c, ahead.page_of(4 * j + k_blk), 0, kvh, (t * 4 + k_blk) & per);
+        if constexpr (kPer == 1) {
+            const uint2 x = reinterpret_cast<const uint2*>(kp)[2 * (64 * (k_op / 2 % kC) + lane) + k_op % 2];
+            kr[0] = x.x, kr[1] = x.y;
+        } else {
 #pragma unroll
-        for (int cc = 0; cc < kC; ++cc) kr[cc] = kp[64 * cc];
+            for (int n = 0; n < kPer / 2; ++n) {
+                const uint4 x = reinterpret_cast<const uint4*>(kp)[64 * ((k_op / 2 + n) % kC) + lane];
+                kr[4 * n] = x.x, kr[4 * n + 1] = x.y, kr[4 * n + 2] = x.z, kr[4 * n + 3] = x.w;
+            }
+        }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const int blk = 2 * (wave >> 1) + k;
-            const uint8_t* vp = kv8_codes(c, bl_next.page_of(4 * j + blk), 1, kvh, (t * 4 + blk) & per);
-            if constexpr (kC == 2) {
-                vr[k] = reinterpret_cast<const uint4*>(vp)[64 * (wave & 1) + lane];
+            const int blk = 2 * v_pair + k;
+            const uint32_t* vp = reinterpret_cast<const uint32_t*>(
+                                     kv8_codes(c, ahead.page_of(4 * j + blk), 1, kvh, (t * 4 + blk) & per)) +
+                                 4 * (64 * v_c + lane) + v_i;
+            if constexpr (kPer == 4) {
+                const uint4 x = *reinterpret_cast<const uint4*>(vp);
+                vr[k][0] = x.x, vr[k][1] = x.y, vr[k][2] = x.z, vr[k][3] = x.w;
+            } else if constexpr (kPer == 2) {
+                const uint2 x = *reinterpret_cast<const uint2*>(vp);
+                vr[k][0] = x.x, vr[k][1] = x.y;
             } else {
-                const uint2 h = reinterpret_cast<const uint2*>(vp)[2 * lane + (wave & 1)];
-                vr[k].x = h.x;
-                vr[k].y = h.y;
+                vr[k][0] = *vp;
             }
         }
     };
     auto stage = [&](int buf) {
-        uint4* ks = lds + (size_t)buf * 2 * kUnits;
+        uint4* ks = lds + (size_t)buf * 2 * kUnits + (size_t)k_op * 64 + lane;
         uint4* vs = ks + kUnits;
 #pragma unroll
-        for (int cc = 0; cc < kC; ++cc) {
-            ks[((wave * kC + cc) * 2 + 0) * 64 + lane] = __builtin_bit_cast(uint4, codes8_to_f16(kr[cc].x, kr[cc].y));
-            ks[((wave * kC + cc) * 2 + 1) * 64 + lane] = __builtin_bit_cast(uint4, codes8_to_f16(kr[cc].z, kr[cc].w));
-        }
-        const int u = wave >> 1;
-        const uint32_t a0[4] = {vr[0].x, vr[0].y, vr[0].z, vr[0].w}, a1[4] = {vr[1].x, vr[1].y, vr[1].z, vr[1].w};
-#pragma unroll
-        for (int i = 0; i < 2 * kC; ++i) {
-            const int at = kC == 2 ? (u * 2 + (wave & 1)) * 4 + i : u * 4 + 2 * (wave & 1) + i;
-            vs[at * 64 + lane] = __builtin_bit_cast(uint4, codes8_to_f16(a0[i], a1[i]));
+        for (int n = 0; n < kPer; ++n) {
+            ks[n * 64] = __builtin_bit_cast(uint4, codes8_to_f16(kr[2 * n], kr[2 * n + 1]));
+            vs[n * 64] = __builtin_bit_cast(uint4, codes8_to_f16(vr[0][n], vr[1][n]));
         }
     };
+
     // One tile from buffer buf, while the next tile's codes go into the other one. The matrix instructions run in the
     // background of a wave, four issue slots each: the conversion of the next tile fills them in the first product, and
-    // each operand is read from shared memory several matrix instructions before its use.
+    // each operand is read from shared memory kDeep reads before its use.
     constexpr int kMm = kCt * (Query<T, kC>::kSplit ? 2 : 1);  // matrix instructions to an operand read
-    h8 kk[4], vv[4];
+    constexpr int kOps = 8 * kC, kDeep = 4;
     auto compute = [&](int buf, int t) {
         const int pos0 = t * kTile, i0 = 4 * ((t - t0) & 15);
         const uint4* ks = lds + (size_t)buf * 2 * kUnits + lane;
         const uint4* vs = ks + kUnits;
+        h8 kk[kDeep], vv[kDeep];
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) kk[r] = __builtin_bit_cast(h8, ks[r * 64]);
+        for (int r = 0; r < kDeep; ++r) kk[r] = __builtin_bit_cast(h8, ks[r * 64]);
         f4 x[kCt][4];
 #pragma unroll
-        for (int r = 0; r < 8 * kC; ++r) {  // operand r: key block r / (2 kC), dimensions by r % (2 kC)
+        for (int r = 0; r < kOps; ++r) {  // operand r: key block r / (2 kC), dimensions by r % (2 kC)
             const int k = r / (2 * kC), cc = r / 2 % kC, h = r & 1;
 #pragma unroll
             for (int ct = 0; ct < kCt; ++ct) {
                 if (r % (2 * kC) == 0) x[ct][k] = f4{0, 0, 0, 0};
-                x[ct][k] = q[ct].dot(kk[r & 3], cc, h, x[ct][k]);
+                x[ct][k] = q[ct].dot(kk[r % kDeep], cc, h, x[ct][k]);
             }
-            if (r + 4 < 8 * kC) kk[r & 3] = __builtin_bit_cast(h8, ks[(r + 4) * 64]);
+            if (r + kDeep < kOps) kk[r % kDeep] = __builtin_bit_cast(h8, ks[(r + kDeep) * 64]);
         }
         stage(buf ^ 1);
-        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, kDeep, 0);
 #pragma unroll
-        for (int r = 0; r < 8 * kC; ++r) {
+        for (int r = 0; r < kOps; ++r) {
             __builtin_amdgcn_sched_group_barrier(0x008, kMm, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
@@ -800,45 +820,42 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
         __builtin_amdgcn_sched_barrier(0);
         if (t + 2 < t1) fetch(t + 2);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) vv[r] = __builtin_bit_cast(h8, vs[r * 64]);
+        for (int r = 0; r < kDeep; ++r) vv[r] = __builtin_bit_cast(h8, vs[r * 64]);
         __builtin_amdgcn_sched_barrier(0);
-        float weight[4], f[kCt][4];
-        const float shrink = unit.weights(bl, i0, weight);
-        const uint32_t ok = (uint32_t)(bl.ok >> i0) & 15u;
+        const Scales sc = unit.next(bl, i0);
+        float f[kCt][4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float key = bl.key(i0 + k);
+        for (int ct = 0; ct < kCt; ++ct)
 #pragma unroll
-            for (int ct = 0; ct < kCt; ++ct) f[ct][k] = key * q[ct].unit;
+            for (int k = 0; k < 4; ++k) f[ct][k] = sc.key[k] * q[ct].unit;
+        if (pos0 + kTile > all_see || sc.ok != 15u) {
+#pragma unroll
+            for (int ct = 0; ct < kCt; ++ct) st[ct].mask(x[ct], f[ct], pos0 + 4 * g, vis[ct], sc.ok);
+        }
+        if (sc.nan) {
+#pragma unroll
+            for (int ct = 0; ct < kCt; ++ct) st[ct].poison(sc.nan, pos0, vis[ct]);
         }
         h8 w[kCt][2], lo[kCt][2];
-        const bool masked = pos0 + kTile > all_see || ok != 15u;
 #pragma unroll
-        for (int ct = 0; ct < kCt; ++ct) {
-            if (masked) {
+        for (int ct = 0; ct < kCt; ++ct) st[ct].settle(x[ct], f[ct], sc.shrink);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-#pragma unroll
-                    for (int s = 0; s < 4; ++s)
-                        if (pos0 + 16 * k + 4 * g + s >= vis[ct] || !((ok >> k) & 1u)) x[ct][k][s] = -__builtin_inff();
-            }
-            st[ct].step(x[ct], f[ct], weight, shrink, masked, w[ct], lo[ct]);
-        }
+        for (int ct = 0; ct < kCt; ++ct) st[ct].weigh(x[ct], f[ct], sc.weight, w[ct], lo[ct]);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int r = 0; r < 8 * kC; ++r) {  // operand r: token pair of blocks r / (4 kC), dimensions by r % (4 kC)
+        for (int r = 0; r < kOps; ++r) {  // operand r: token pair of blocks r / (4 kC), dimensions by r % (4 kC)
             const int u = r / (4 * kC), i = r % (4 * kC);
 #pragma unroll
             for (int ct = 0; ct < kCt; ++ct) {
                 f4& o = st[ct].o[i];
-                o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv[r & 3], w[ct][u], o, 0, 0, 0);
+                o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv[r % kDeep], w[ct][u], o, 0, 0, 0);
                 if constexpr (Query<T, kC>::kSplit)
-                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv[r & 3], lo[ct][u], o, 0, 0, 0);
+                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv[r % kDeep], lo[ct][u], o, 0, 0, 0);
             }
-            if (r + 4 < 8 * kC) vv[r & 3] = __builtin_bit_cast(h8, vs[(r + 4) * 64]);
+            if (r + kDeep < kOps) vv[r % kDeep] = __builtin_bit_cast(h8, vs[(r + kDeep) * 64]);
         }
 #pragma unroll
-        for (int r = 0; r < 8 * kC; ++r) {
+        for (int r = 0; r < kOps; ++r) {
             __builtin_amdgcn_sched_group_barrier(0x008, kMm, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
@@ -847,12 +864,12 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
 
     if (t0 < t1) {
         fetch(t0);
-        bl = bl_next;
+        bl = ahead;
         stage(0);
         if (t0 + 1 < t1) fetch(t0 + 1);
         for (int t = t0; t < t1; ++t) {
             __syncthreads();  // tile t is staged, and tile t - 1 (whose buffer comes next) has been read
-            if (t > t0 && ((t - t0) & 15) == 0) bl = bl_next;
+            if (t > t0 && ((t - t0) & 15) == 0) bl = ahead;
             compute((t - t0) & 1, t);  // past the last tile it stages what it has once more, for nobody
         }
     }
@@ -898,7 +915,7 @@ struct Plan {
     }
 };
 // capacity: positions that a sequence can have.
-Plan plan_of(int group, int n_kv, int capacity, int n, int n_tok, bool single) {
+Plan plan_of(int group, int n_kv, int hd, int capacity, int n, int n_tok, bool single) {
     const long rows = (long)n_tok * group;
     const long few = single ? (long)n * ((group + kRowTile - 1) / kRowTile) : rows / kRowTile + n;
     const int cus = device_cus();
@@ -914,8 +931,10 @@ Plan plan_of(int group, int n_kv, int capacity, int n, int n_tok, bool single) {
         p.part_rows = 2 * (size_t)p.shares * kRowTile;
         return p;
     }
-    // 128 rows to a workgroup, or 64 where that leaves compute units idle
-    p.tile = rows / 128 * n_kv >= cus ? 128 : 64;
+    // 128 rows to a workgroup at head_dim 128 (4 x 2,000 tokens behind 6,000, 32 heads over 8, f16: 1,236 us, with 64 rows
+    // 1,611), but 64 where 128 would leave compute units idle, and at head_dim 64, where the longer loop is no faster
+    // (14 heads over 2: f32 579 and 534 us, f16 411 and 416; one prompt of 512: f32 20.9 and 17.2)
+    p.tile = hd == 128 && rows / 128 * n_kv >= cus ? 128 : 64;
     p.items = (int)(rows / p.tile + n);
     const long wgs = (long)p.items * n_kv;
     // splits for two workgroups to a compute unit, but none of fewer than four tiles
@@ -932,9 +951,9 @@ Plan plan_of(int group, int n_kv, int capacity, int n, int n_tok, bool single) {
 
 size_t kv8_attention_workspace_bytes(int n_heads, int n_kv, int hd, int capacity, int n, int n_tok) {
     const int group = n_heads / n_kv;
-    size_t b = plan_of(group, n_kv, capacity, n, n_tok, false).bytes(n_kv, hd);
+    size_t b = plan_of(group, n_kv, hd, capacity, n, n_tok, false).bytes(n_kv, hd);
     if (n == n_tok) {
-        const size_t single = plan_of(group, n_kv, capacity, n, n_tok, true).bytes(n_kv, hd);
+        const size_t single = plan_of(group, n_kv, hd, capacity, n, n_tok, true).bytes(n_kv, hd);
         b = b > single ? b : single;
     }
     return b;
@@ -952,7 +971,7 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
     a.group = n_heads / c.n_kv;
     a.causal = causal ? 1 : 0;
     a.scale_log2e = scale * 1.44269504088896340736f;
-    const Plan p = plan_of(a.group, c.n_kv, c.seq_pages << c.page_shift, n, n_tok, start == nullptr);
+    const Plan p = plan_of(a.group, c.n_kv, c.hd, c.seq_pages << c.page_shift, n, n_tok, start == nullptr);
     a.items = p.items;
     a.splits = p.splits;
     a.rec = static_cast<int4*>(ws);
@@ -968,10 +987,10 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
         } else {
             constexpr size_t lds = 2 * 2 * (size_t)kTile * 64 * kC * 2;
             const dim3 grid((unsigned)c.n_kv * (unsigned)p.items, (unsigned)p.splits);
-            if (p.tile == 128)
-                qh_launch((kv8_tile_kernel<T, kC, 2>), grid, dim3(256), lds, s, c, a);
-            else
-                qh_launch((kv8_tile_kernel<T, kC, 1>), grid, dim3(256), lds, s, c, a);
+            if constexpr (kC == 2) {
+                if (p.tile == 128) qh_launch((kv8_tile_kernel<T, kC, 2>), grid, dim3(256), lds, s, c, a);
+            }
+            if (p.tile == 64) qh_launch((kv8_tile_kernel<T, kC, 1>), grid, dim3(256), lds, s, c, a);
             if (p.splits > 1)
                 qh_launch((kv8_join_splits_kernel<T, kC>),
                           dim3((unsigned)p.items, (unsigned)c.n_kv, (unsigned)(p.join_rows * kC / 16)), dim3(256), 0, s, c,
