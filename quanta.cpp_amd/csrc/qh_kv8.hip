@@ -544,48 +544,70 @@ __global__ __launch_bounds__(kWg) void kv8_compact_kernel(Kv8View c, int32_t* __
     }
 }
 
-// Copies the listed pages in every layer, 16 KB to a workgroup and turn, 16 bytes to a lane and four of them in flight;
-// remap (compact): first the table entries take the pages' new numbers. Bound by memory.
-constexpr int kMoveBytes = 16384;
+// Copies the listed pages in every layer. All pages of all layers lie end to end as 16-byte words, and a workgroup takes
+// kPer of 256 of them at a time, wherever pages end, so that every lane has kPer loads in flight whatever a page's size
+// is; remap (compact): first the table entries take the pages' new numbers. Bound by memory (large lists) and by the two
+// dependent reads of the list (a page or two).
+template <int kPer>
 __global__ __launch_bounds__(256) void kv8_move_kernel(Kv8View c, int n_layers, int remap, void* ws) {
     const PagesWs w = pages_ws(ws, c.n_pages, c.n_seqs);
     const int n = *w.n_copy;
     if (n == 0) return;
     if (remap) {
         // the first copy's source is the lowest number that moves; `goes` holds every number from it on
+        const int first = w.copies[0].x;
         for (size_t e = (size_t)blockIdx.x * 256 + threadIdx.x; e < (size_t)c.n_seqs * c.seq_pages;
              e += (size_t)gridDim.x * 256) {
             const int page = c.table[e];
-            if (page >= w.copies[0].x && page < c.n_pages) c.table[e] = w.goes[page];
+            if (page >= first && page < c.n_pages) c.table[e] = w.goes[page];
         }
     }
-    const int chunks = (int)((c.page_bytes + kMoveBytes - 1) / kMoveBytes);
-    const long items = (long)n * n_layers * chunks;
-    for (long it = blockIdx.x; it < items; it += gridDim.x) {
-        const int chunk = (int)(it % chunks);
-        const long rest = it / chunks;
-        const int2 p = w.copies[rest / n_layers];
-        if (p.x < 0 || p.x >= c.n_pages) continue;
-        uint8_t* layer = c.pages + (size_t)(rest % n_layers) * c.n_pages * c.page_bytes;
-        const uint4* from = reinterpret_cast<const uint4*>(layer + (size_t)p.x * c.page_bytes + (size_t)chunk * kMoveBytes);
-        uint4* to = reinterpret_cast<uint4*>(layer + (size_t)p.y * c.page_bytes + (size_t)chunk * kMoveBytes);
-        const int words = (int)(min((size_t)kMoveBytes, c.page_bytes - (size_t)chunk * kMoveBytes) / 16);
-        uint4 r[4];
+    const uint32_t words = (uint32_t)(c.page_bytes / 16);
+    const uint64_t total = (uint64_t)n * n_layers * words;
+    for (uint64_t base = (uint64_t)blockIdx.x * (256 * kPer); base < total; base += (uint64_t)gridDim.x * (256 * kPer)) {
+        // the page of the first word, copy by copy with the layers in turn
+        const uint64_t item = base / words;
+        const uint32_t copy0 = (uint32_t)(item / (uint32_t)n_layers), layer0 = (uint32_t)(item % (uint32_t)n_layers);
+        const uint32_t off0 = (uint32_t)(base - item * words);
+        uint4 r[kPer];
+        uint4* to[kPer];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if ((int)threadIdx.x + 256 * j < words) r[j] = from[threadIdx.x + 256 * j];
+        for (int j = 0; j < kPer; ++j) {
+            uint32_t off = off0 + threadIdx.x + 256 * j, copy = copy0, layer = layer0;
+            while (off >= words) {
+                off -= words;
+                if (++layer == (uint32_t)n_layers) {
+                    layer = 0;
+                    ++copy;
+                }
+            }
+            to[j] = nullptr;
+            if (copy < (uint32_t)n) {
+                const int2 p = w.copies[copy];
+                if (p.x >= 0 && p.x < c.n_pages) {
+                    uint8_t* at = c.pages + (size_t)layer * c.n_pages * c.page_bytes;
+                    r[j] = reinterpret_cast<const uint4*>(at + (size_t)p.x * c.page_bytes)[off];
+                    to[j] = reinterpret_cast<uint4*>(at + (size_t)p.y * c.page_bytes) + off;
+                }
+            }
+        }
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if ((int)threadIdx.x + 256 * j < words) to[threadIdx.x + 256 * j] = r[j];
+        for (int j = 0; j < kPer; ++j)
+            if (to[j]) *to[j] = r[j];
     }
 }
 
 hipError_t launch_move(const Kv8View& c, int n_layers, long most_copies, bool remap, void* ws, hipStream_t s) {
-    const long chunks = (long)((c.page_bytes + kMoveBytes - 1) / kMoveBytes);
-    long items = most_copies * n_layers * chunks;
-    if (remap) items = items > 64 ? items : 64;
-    const unsigned grid = (unsigned)(items < 2048 ? items : 2048);
-    qh_launch(kv8_move_kernel, dim3(grid), dim3(256), 0, s, c, n_layers, remap ? 1 : 0, ws);
+    // one word to a lane up to 2,048 workgroups of them, else four
+    const uint64_t words = (uint64_t)most_copies * n_layers * (c.page_bytes / 16);
+    const bool few = words <= (uint64_t)2048 * 256;
+    uint64_t grid = (words + (few ? 255 : 1023)) / (few ? 256 : 1024);
+    if (remap && grid < 64) grid = 64;
+    if (grid > 2048) grid = 2048;
+    if (few)
+        qh_launch((kv8_move_kernel<1>), dim3((unsigned)grid), dim3(256), 0, s, c, n_layers, remap ? 1 : 0, ws);
+    else
+        qh_launch((kv8_move_kernel<4>), dim3((unsigned)grid), dim3(256), 0, s, c, n_layers, remap ? 1 : 0, ws);
     return hipGetLastError();
 }
 

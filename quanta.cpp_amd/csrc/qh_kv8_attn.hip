@@ -786,7 +786,9 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
 
     // One tile from buffer buf, while the next tile's codes go into the other one. The matrix instructions run in the
     // background of a wave, four issue slots each: the conversion of the next tile fills them in the first product, and
-    // each operand is read from shared memory kDeep reads before its use.
+    // each operand is read from shared memory kDeep reads before its use. A wave in one of its products goes before the
+    // other wave of its SIMD, which has exponentials to fill the slots that are left (4 x 2,000 tokens over 8,000, 32
+    // heads of 128 over 8, f16: 1,230 -> 1,165 us).
     constexpr int kMm = kCt * (Query<T, kC>::kSplit ? 2 : 1);  // matrix instructions to an operand read
     constexpr int kOps = 8 * kC, kDeep = 4;
     auto compute = [&](int buf, int t) {
@@ -795,6 +797,7 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
         const uint4* vs = ks + kUnits;
         h8 kk[kDeep], vv[kDeep];
         __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int r = 0; r < kDeep; ++r) kk[r] = __builtin_bit_cast(h8, ks[r * 64]);
         f4 x[kCt][4];
@@ -818,6 +821,7 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
             if (r & 1) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(0);
         if (t + 2 < t1) fetch(t + 2);
 #pragma unroll
         for (int r = 0; r < kDeep; ++r) vv[r] = __builtin_bit_cast(h8, vs[r * 64]);
@@ -841,6 +845,7 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
         for (int ct = 0; ct < kCt; ++ct) st[ct].settle(x[ct], f[ct], sc.shrink);
 #pragma unroll
         for (int ct = 0; ct < kCt; ++ct) st[ct].weigh(x[ct], f[ct], sc.weight, w[ct], lo[ct]);
+        __builtin_amdgcn_s_setprio(1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int r = 0; r < kOps; ++r) {  // operand r: token pair of blocks r / (4 kC), dimensions by r % (4 kC)
@@ -872,6 +877,7 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
             if (t > t0 && ((t - t0) & 15) == 0) bl = ahead;
             compute((t - t0) & 1, t);  // past the last tile it stages what it has once more, for nobody
         }
+        __builtin_amdgcn_s_setprio(0);
     }
 
     const float back = unit.back();
