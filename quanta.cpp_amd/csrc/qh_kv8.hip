@@ -10,47 +10,16 @@ namespace {
 
 constexpr uint32_t kBias = 0x80808080u;  // the 128 that stored codes carry, in each byte of a word
 
-// 16 consecutive values at p as f32.
-__device__ __forceinline__ void load_row16(const float* p, float* x) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float4 a = reinterpret_cast<const float4*>(p)[i];
-        x[4 * i] = a.x, x[4 * i + 1] = a.y, x[4 * i + 2] = a.z, x[4 * i + 3] = a.w;
-    }
-}
-__device__ __forceinline__ void load_row16(const _Float16* p, float* x) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-        const h8 a = reinterpret_cast<const h8*>(p)[i];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[8 * i + j] = (float)a[j];
-    }
-}
 __device__ __forceinline__ void load_row4(const float* p, float* x) {
-    const float4 a = *reinterpret_cast<const float4*>(p);
+    typedef float f4 __attribute__((ext_vector_type(4)));
+    const f4 a = __builtin_nontemporal_load(reinterpret_cast<const f4*>(p));
     x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
 }
 __device__ __forceinline__ void load_row4(const _Float16* p, float* x) {
     typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-    const h4 a = *reinterpret_cast<const h4*>(p);
+    const h4 a = __builtin_nontemporal_load(reinterpret_cast<const h4*>(p));
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] = (float)a[j];
-}
-__device__ __forceinline__ void store_row16(float* p, const float* x) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        reinterpret_cast<float4*>(p)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-}
-__device__ __forceinline__ void store_row16(_Float16* p, const float* x) {
-    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        h8 a;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) a[j] = (_Float16)x[8 * i + j];
-        reinterpret_cast<h8*>(p)[i] = a;
-    }
 }
 __device__ __forceinline__ void store_row4(float* p, const float* x) {
     *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
@@ -61,6 +30,23 @@ __device__ __forceinline__ void store_row4(_Float16* p, const float* x) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) a[j] = (_Float16)x[j];
     *reinterpret_cast<h4*>(p) = a;
+}
+
+// Lane q of each aligned group of four takes word q of the four lanes: w[j] becomes lane j's w[q].
+__device__ __forceinline__ void transpose_quad(uint32_t (&w)[4]) {
+    const bool odd = (threadIdx.x & 1) != 0, high = (threadIdx.x & 2) != 0;
+#pragma unroll
+    for (int k = 0; k < 4; k += 2) {
+        const uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)(odd ? w[k] : w[k + 1]), 0xB1, 0xF, 0xF, false);
+        w[k] = odd ? got : w[k];
+        w[k + 1] = odd ? w[k + 1] : got;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)(high ? w[k] : w[k + 2]), 0x4E, 0xF, 0xF, false);
+        w[k] = high ? got : w[k];
+        w[k + 2] = high ? w[k + 2] : got;
+    }
 }
 
 // The integer nearest to (a + e) / d, halves upwards, for 0 <= (a + e) / d < 127.6 and |e| at most half an ulp of a: the
@@ -79,18 +65,37 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     return wave_reduce32x2(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }
 
-// One wave stores the new tokens of one block: entry b's tokens are the positions [first, len) of its sequence, token at
-// position p in row row0 + p. Bound by the memory traffic of long batches (each value read once, its code written once)
-// and by the dependent loads (entry, length, page, scale, codes) of single tokens.
+// One wave stores the new tokens of one block: the positions [first, len) of a sequence are new, the one at position p in
+// row row0 + p. Bound by the memory traffic of long batches (each value read once, its code written once) and by the
+// dependent loads (entry, length, page, scale, codes) of single tokens.
+// Lane 16 g + j reads dims 4 j .. 4 j + 3 of tokens 4 g .. 4 g + 3, 16 lanes to a row, so that rows are read in one piece;
+// the values' codes are in place then, the keys' cross four lanes (rows read by the lanes that store them, 16 dims of one
+// token: 24,001 x 8 heads of 128, f32, 68 us; this 56).
 // The block's scale is max|x| / 127 over every token it has been given since its first one: a block that already holds
 // tokens (held > 0) keeps the larger of its scale and the new tokens', and its codes are rounded to the new scale where
 // that grew. Only the block's own wave touches it, so the update needs no atomics.
-template <typename T, int kC, bool kValues>
-__device__ __forceinline__ void append_block(const Kv8View& c, const T* __restrict__ x, int64_t ld, int h, int page,
-                                             int blk_in_page, int pos0, int first, int len, int row0) {
-    const int lane = (int)threadIdx.x & 63, g = lane >> 4, t = lane & 15;
+template <typename T, int kC>
+__device__ __forceinline__ void load_block(const T* __restrict__ x, int64_t ld, int pos0, int first, int len, int row0,
+                                           float (&v)[kC][4][4]) {
+    const int lane = (int)threadIdx.x & 63, g = lane >> 4, j = lane & 15;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int p = pos0 + 4 * g + r;
+        const bool there = p >= first && p < len;
+        const T* row = x + (int64_t)(row0 + (there ? p : first)) * ld + 4 * j;
+#pragma unroll
+        for (int k = 0; k < kC; ++k) load_row4(row + 64 * k, v[k][r]);
+    }
+}
+
+template <int kC, bool kValues>
+__device__ __forceinline__ void append_block(const Kv8View& c, float (&v)[kC][4][4], int h, int page, int blk_in_page, int pos0,
+                                             int first, int len) {
+    const int lane = (int)threadIdx.x & 63, g = lane >> 4, j = lane & 15;
     const int held = min(max(first - pos0, 0), kBlk);
-    uint4* codes = reinterpret_cast<uint4*>(kv8_codes(c, page, kValues ? 1 : 0, h, blk_in_page)) + lane;
+    // the 16 bytes that this lane stores: values where it reads them, keys of token 4 g + j % 4 and dims 16 (j / 4) ..
+    const int unit = kValues ? lane : 16 * (j >> 2) + 4 * g + (j & 3);
+    uint4* codes = reinterpret_cast<uint4*>(kv8_codes(c, page, kValues ? 1 : 0, h, blk_in_page)) + unit;
     float* scale = kv8_scale(c, page, kValues ? 1 : 0, h, blk_in_page);
     const float before = held ? *scale : 0.0f;
     uint4 old[kC];
@@ -98,33 +103,18 @@ __device__ __forceinline__ void append_block(const Kv8View& c, const T* __restri
 #pragma unroll
         for (int k = 0; k < kC; ++k) old[k] = codes[64 * k];
     }
-    // value e of the lane belongs to token t (keys: dims e) or 4 g + e % 4 (values: dim 4 t + e / 4)
-    auto token = [&](int e) { return kValues ? 4 * g + (e & 3) : t; };
-    float v[kC][16];
     uint32_t top = 0;
 #pragma unroll
-    for (int k = 0; k < kC; ++k) {
-        if (kValues) {
+    for (int r = 0; r < 4; ++r) {
+        const int p = pos0 + 4 * g + r;
+        const bool there = p >= first && p < len;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int p = pos0 + 4 * g + r;
-                float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                if (p >= first && p < len)
-                    load_row4(x + (int64_t)(row0 + p) * ld + (int64_t)h * c.hd + 64 * k + 4 * t, a);
+        for (int k = 0; k < kC; ++k)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[k][4 * i + r] = a[i];
+            for (int i = 0; i < 4; ++i) {
+                if (!there) v[k][r][i] = 0.0f;
+                top = max(top, __builtin_bit_cast(uint32_t, v[k][r][i]) & 0x7fffffffu);
             }
-        } else {
-            const int p = pos0 + t;
-            if (p >= first && p < len) {
-                load_row16(x + (int64_t)(row0 + p) * ld + (int64_t)h * c.hd + 64 * k + 16 * g, v[k]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) v[k][e] = 0.0f;
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = max(top, __builtin_bit_cast(uint32_t, v[k][e]) & 0x7fffffffu);
     }
     top = wave_max_u32(top);  // on the bits, so that a NaN is not lost
     float d = __builtin_bit_cast(float, top) / 127.0f;
@@ -136,39 +126,60 @@ __device__ __forceinline__ void append_block(const Kv8View& c, const T* __restri
     const float lift = d < 0x1p-100f ? 0x1p64f : 1.0f;
     const float ds = d * lift, inv = d > 0.0f ? 1.0f / ds : 0.0f;  // 0 for d = 0 and for NaN: every code 0
     const float db = before * lift;
+    // Codes from the rounded quotient, stored with their bias by the conversion itself. The quotient is off by at most
+    // 127 * 2^-23 < 2^-16, so a code is certain unless the quotient is that close to a half; a wave with such a value (one
+    // in twenty at 2,048 values) or a lifted scale takes every code again by the exact remainders.
+    uint32_t w[kC][4] = {};
+    float worst = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kC; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float t = v[k][r][i] * inv, q = __builtin_truncf(t + __builtin_copysignf(0.5f, t));
+                worst = __builtin_fmaxf(worst, __builtin_fabsf(t - q));
+                w[k][kValues ? i : r] = __builtin_amdgcn_cvt_pk_u8_f32(q + 128.0f, kValues ? r : i, w[k][kValues ? i : r]);
+            }
+    if (__any(!(worst <= 0.5f - 0x1p-16f)) || lift != 1.0f || !(inv > 0.0f)) {
+#pragma unroll
+        for (int k = 0; k < kC; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float q = 0.0f;
+                    if (inv > 0.0f) q = nearest_code(__builtin_fabsf(v[k][r][i] * lift), 0.0f, ds, inv);
+                    w[k][kValues ? i : r] = __builtin_amdgcn_cvt_pk_u8_f32(__builtin_copysignf(q, v[k][r][i]) + 128.0f,
+                                                                          kValues ? r : i, w[k][kValues ? i : r]);
+                }
+    }
 #pragma unroll
     for (int k = 0; k < kC; ++k) {
-        uint32_t w[4] = {0, 0, 0, 0};
-        if (inv > 0.0f) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float q = nearest_code(__builtin_fabsf(v[k][e] * lift), 0.0f, ds, inv);
-                w[e >> 2] |= ((uint32_t)(int)__builtin_copysignf(q, v[k][e]) & 0xffu) << (8 * (e & 3));
-            }
-        }
+        if (!kValues) transpose_quad(w[k]);
         if (held) {
             const uint32_t o[4] = {old[k].x ^ kBias, old[k].y ^ kBias, old[k].z ^ kBias, old[k].w ^ kBias};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t keep = o[j];
+            for (int i = 0; i < 4; ++i) {
+                uint32_t keep = o[i];
                 if (d != before) {
                     keep = 0;
                     if (inv > 0.0f) {
 #pragma unroll
                         for (int b = 0; b < 4; ++b) {
-                            const float f = (float)(int8_t)(o[j] >> (8 * b)), m = __builtin_fabsf(f);
+                            const float f = (float)(int8_t)(o[i] >> (8 * b)), m = __builtin_fabsf(f);
                             const float a = m * db, e = __builtin_fmaf(m, db, -a);
                             keep |= ((uint32_t)(int)__builtin_copysignf(nearest_code(a, e, ds, inv), f) & 0xffu) << (8 * b);
                         }
                     }
                 }
-                uint32_t mask = 0;  // the bytes of tokens the block held
+                uint32_t mask = 0;  // the bytes of tokens the block held: byte b of values is token 4 g + b
 #pragma unroll
-                for (int b = 0; b < 4; ++b) mask |= token(4 * j + b) < held ? 0xffu << (8 * b) : 0u;
-                w[j] = (keep & mask) | (w[j] & ~mask);
+                for (int b = 0; b < 4; ++b) mask |= 4 * g + (kValues ? b : j & 3) < held ? 0xffu << (8 * b) : 0u;
+                w[k][i] = ((keep ^ kBias) & mask) | (w[k][i] & ~mask);
             }
         }
-        codes[64 * k] = make_uint4(w[0] ^ kBias, w[1] ^ kBias, w[2] ^ kBias, w[3] ^ kBias);
+        codes[64 * k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
     }
     if (lane == 0) *scale = d;
 }
@@ -184,65 +195,71 @@ __device__ __forceinline__ Span span_of(const Kv8View& c, const Kv8Batch& q, int
     return {seq, max(p0, 0), len, s0 - p0};
 }
 
-// grid (items, ceil(2 n_kv / 4)), 4 waves: one wave per block of 16 positions, KV head, keys or values.
+// One wave per block of 16 positions, KV head, keys or values; the workgroups (4 waves) of one block follow each other, so
+// that a row's heads are read at about the same time.
 template <typename T, int kC>
 __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8View c, const T* __restrict__ k, const T* __restrict__ v,
                                                          int64_t ldk, int64_t ldv, Kv8Batch q) {
-    const int hw = (int)blockIdx.y * 4 + (int)(threadIdx.x >> 6);
-    int b = (int)blockIdx.x, from = b;
-    if (q.start) b = kv8_entry_of(q, (int)blockIdx.x, 1, kBlk, 2, &from);
+    const unsigned groups = (unsigned)(2 * c.n_kv + 3) / 4;
+    const int item = (int)(blockIdx.x / groups), hw = (int)(blockIdx.x % groups) * 4 + (int)(threadIdx.x >> 6);
+    int b = item, from = item;
+    if (q.start) b = kv8_entry_of(q, item, 1, kBlk, 2, &from);
     if (b < 0 || hw >= 2 * c.n_kv) return;
     const Span sp = span_of(c, q, b);
-    const int blk = sp.first / kBlk + ((int)blockIdx.x - from), pos0 = blk * kBlk;
+    const int blk = sp.first / kBlk + (item - from), pos0 = blk * kBlk;
     if (max(pos0, sp.first) >= sp.len) return;
+    const int h = hw >> 1;
+    const bool values = (hw & 1) != 0;
+    float x[kC][4][4];  // [.][token][dim]; in flight while the page is looked up
+    load_block<T, kC>((values ? v : k) + (int64_t)h * c.hd, values ? ldv : ldk, pos0, sp.first, sp.len, sp.row0, x);
     const int page = c.table[(size_t)sp.seq * c.seq_pages + (pos0 >> c.page_shift)];
     if (page < 0 || page >= c.n_pages) return;
     if (c.refs[page] > 1) {  // other sequences read this page
         if ((threadIdx.x & 63) == 0) atomicOr(c.status, QH_KV8_SHARED);
         return;
     }
-    const int bp = blk & ((1 << (c.page_shift - 4)) - 1), h = hw >> 1;
-    if (hw & 1)
-        append_block<T, kC, true>(c, v, ldv, h, page, bp, pos0, sp.first, sp.len, sp.row0);
+    const int bp = blk & ((1 << (c.page_shift - 4)) - 1);
+    if (values)
+        append_block<kC, true>(c, x, h, page, bp, pos0, sp.first, sp.len);
     else
-        append_block<T, kC, false>(c, k, ldk, h, page, bp, pos0, sp.first, sp.len, sp.row0);
+        append_block<kC, false>(c, x, h, page, bp, pos0, sp.first, sp.len);
 }
 
-// The same items: one wave writes the values of one block's tokens, code * scale rounded to f32, then to T.
+// The same items: one wave writes the values of one block's tokens, code * scale rounded to f32, then to T. Lanes as in
+// append_block.
 template <typename T, int kC>
 __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8View c, T* __restrict__ k, T* __restrict__ v, int64_t ldk,
                                                        int64_t ldv, Kv8Batch q) {
-    const int hw = (int)blockIdx.y * 4 + (int)(threadIdx.x >> 6), lane = (int)threadIdx.x & 63, g = lane >> 4, t = lane & 15;
-    int b = (int)blockIdx.x, from = b;
-    if (q.start) b = kv8_entry_of(q, (int)blockIdx.x, 1, kBlk, 2, &from);
+    const unsigned groups = (unsigned)(2 * c.n_kv + 3) / 4;
+    const int item = (int)(blockIdx.x / groups), hw = (int)(blockIdx.x % groups) * 4 + (int)(threadIdx.x >> 6);
+    const int lane = (int)threadIdx.x & 63, g = lane >> 4, j = lane & 15;
+    int b = item, from = item;
+    if (q.start) b = kv8_entry_of(q, item, 1, kBlk, 2, &from);
     if (b < 0 || hw >= 2 * c.n_kv) return;
     const Span sp = span_of(c, q, b);
-    const int blk = sp.first / kBlk + ((int)blockIdx.x - from), pos0 = blk * kBlk, h = hw >> 1;
+    const int blk = sp.first / kBlk + (item - from), pos0 = blk * kBlk, h = hw >> 1;
     if (max(pos0, sp.first) >= sp.len) return;
     const int page = c.table[(size_t)sp.seq * c.seq_pages + (pos0 >> c.page_shift)];
-    const bool ok = page >= 0 && page < c.n_pages;  // a missing page reads as zeros
+    const bool ok = page >= 0 && page < c.n_pages, values = (hw & 1) != 0;  // a missing page reads as zeros
     const int bp = blk & ((1 << (c.page_shift - 4)) - 1);
     const float d = ok ? *kv8_scale(c, page, hw & 1, h, bp) : 0.0f;
-    const uint4* codes = reinterpret_cast<const uint4*>(kv8_codes(c, ok ? page : 0, hw & 1, h, bp)) + lane;
+    const uint4* codes = reinterpret_cast<const uint4*>(kv8_codes(c, ok ? page : 0, hw & 1, h, bp)) +
+                         (values ? lane : 16 * (j >> 2) + 4 * g + (j & 3));
+    T* out = values ? v : k;
+    const int64_t ld = values ? ldv : ldk;
 #pragma unroll
     for (int kk = 0; kk < kC; ++kk) {
         const uint4 w4 = ok ? codes[64 * kk] : make_uint4(kBias, kBias, kBias, kBias);
-        const uint32_t w[4] = {w4.x ^ kBias, w4.y ^ kBias, w4.z ^ kBias, w4.w ^ kBias};
-        float x[16];
+        uint32_t w[4] = {w4.x ^ kBias, w4.y ^ kBias, w4.z ^ kBias, w4.w ^ kBias};
+        if (!values) transpose_quad(w);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = (float)(int8_t)(w[e >> 2] >> (8 * (e & 3))) * d;
-        if (hw & 1) {
+        for (int r = 0; r < 4; ++r) {
+            const int p = pos0 + 4 * g + r;
+            float x[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int p = pos0 + 4 * g + r;
-                const float a[4] = {x[r], x[4 + r], x[8 + r], x[12 + r]};
-                if (p >= sp.first && p < sp.len)
-                    store_row4(v + (int64_t)(sp.row0 + p) * ldv + (int64_t)h * c.hd + 64 * kk + 4 * t, a);
-            }
-        } else {
-            const int p = pos0 + t;
+            for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(values ? w[i] >> (8 * r) : w[r] >> (8 * i)) * d;
             if (p >= sp.first && p < sp.len)
-                store_row16(k + (int64_t)(sp.row0 + p) * ldk + (int64_t)h * c.hd + 64 * kk + 16 * g, x);
+                store_row4(out + (int64_t)(sp.row0 + p) * ld + (int64_t)h * c.hd + 64 * kk + 4 * j, x);
         }
     }
 }
@@ -632,7 +649,7 @@ unsigned block_items(const int32_t* start, int n, int n_tok) {
 
 hipError_t launch_kv8_append(const Kv8View& c, const void* k, const void* v, int dtype, int64_t ldk, int64_t ldv,
                              const int32_t* start, const int32_t* seqs, int n, int n_tok, hipStream_t s) {
-    const dim3 grid(block_items(start, n, n_tok), (unsigned)((2 * c.n_kv + 3) / 4));
+    const dim3 grid(block_items(start, n, n_tok) * (unsigned)((2 * c.n_kv + 3) / 4));
     return by_type(dtype, c.hd, [&](auto* t, auto kc) {
         using T = std::remove_pointer_t<decltype(t)>;
         qh_launch((kv8_append_kernel<T, decltype(kc)::value>), grid, dim3(256), 0, s, c, (const T*)k, (const T*)v, ldk,
@@ -642,7 +659,7 @@ hipError_t launch_kv8_append(const Kv8View& c, const void* k, const void* v, int
 
 hipError_t launch_kv8_read(const Kv8View& c, void* k, void* v, int dtype, int64_t ldk, int64_t ldv, const int32_t* start,
                            const int32_t* seqs, int n, int n_tok, hipStream_t s) {
-    const dim3 grid(block_items(start, n, n_tok), (unsigned)((2 * c.n_kv + 3) / 4));
+    const dim3 grid(block_items(start, n, n_tok) * (unsigned)((2 * c.n_kv + 3) / 4));
     return by_type(dtype, c.hd, [&](auto* t, auto kc) {
         using T = std::remove_pointer_t<decltype(t)>;
         qh_launch((kv8_read_kernel<T, decltype(kc)::value>), grid, dim3(256), 0, s, c, (T*)k, (T*)v, ldk, ldv,
