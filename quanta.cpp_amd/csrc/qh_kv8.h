@@ -36,6 +36,12 @@ __host__ __device__ __forceinline__ size_t kv8_page_bytes(int page_tokens, int n
 }
 
 #if defined(__HIPCC__)
+// A load of what is read once: it does not displace what others keep in the caches.
+__device__ __forceinline__ uint4 load_once(const uint4* p) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u4*>(p)));
+}
+
 // Tokens of a sequence, never more than its table row can hold.
 __device__ __forceinline__ int kv8_len(const Kv8View& c, int seq) {
     return min(max(c.lens[seq], 0), c.seq_pages << c.page_shift);

@@ -603,7 +603,7 @@ __global__ __launch_bounds__(256) void kv8_move_kernel(Kv8View c, int n_layers, 
                 const int2 p = w.copies[copy];
                 if (p.x >= 0 && p.x < c.n_pages) {
                     uint8_t* at = c.pages + (size_t)layer * c.n_pages * c.page_bytes;
-                    r[j] = reinterpret_cast<const uint4*>(at + (size_t)p.x * c.page_bytes)[off];
+                    r[j] = load_once(reinterpret_cast<const uint4*>(at + (size_t)p.x * c.page_bytes) + off);
                     to[j] = reinterpret_cast<uint4*>(at + (size_t)p.y * c.page_bytes) + off;
                 }
             }

@@ -29,6 +29,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 constexpr int kTile = 64;            // positions of one step
 constexpr int kRowTile = 16;         // query rows of a workgroup of the row kernel
 constexpr int kMaxItems = 1024;      // row tiles of one launch of the row kernel
+constexpr int kWhole = 1024;         // positions up to which the row kernel takes a sequence whole
 constexpr int kMaxParts = 1024;      // shares of the row kernel: partial results of a row
 
 // Four codes as f16: the stored bytes, code + 128, under the high byte 0x64 are the numbers 1024 + 128 + code.
@@ -283,6 +284,7 @@ struct AttnArgs {
     float* part_ml;
     int4* rec;       // [items] where an item's partials are: first slot, how many (0: none), first row, rows
     int items, splits;
+    int least;  // tiles of a share of the row kernel at least, a multiple of four
 };
 
 // Entry b's rows: global rows (token * group + head) from first on, and the positions its tokens see.
@@ -378,7 +380,7 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
     if (lane == 0) wave_sum[wave] = sum;
     __syncthreads();
     // a share is whole rounds of the four waves
-    const int share = max(4, ((wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3] + shares - 1) / shares + 3) & ~3);
+    const int share = max(a.least, ((wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3] + shares - 1) / shares + 3) & ~3);
     // items that begin on a share of their own where the shares suffice for that: no workgroup then has two items in turn
     int padded[kPer];
     sum = 0;
@@ -476,7 +478,7 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
                 const int page = bl.page_of(4 * (j & 15) + k), blk = (tile * 4 + k) & ((1 << (c.page_shift - 4)) - 1);
                 const uint4* p = reinterpret_cast<const uint4*>(kv8_codes(c, page, which, kvh, blk)) + lane;
 #pragma unroll
-                for (int cc = 0; cc < kC; ++cc) to[k][cc] = p[64 * cc];
+                for (int cc = 0; cc < kC; ++cc) to[k][cc] = load_once(p + 64 * cc);
             }
         };
         typename Query<T, kC>::Raw raw[kC][Query<T, kC>::kRaw];
@@ -914,7 +916,8 @@ struct Plan {
     bool rows;
     int items, shares, splits;
     int tile;          // rows of an item
-    int join_rows;     // rows of an item that can be used
+    int join_rows;     // rows of an item that can have partial results; 0: none
+    int least;
     size_t part_rows;  // rows of partial results (per KV head)
     size_t bytes(int n_kv, int hd) const {
         return sizeof(int4) * (size_t)items + sizeof(float) * part_rows * n_kv * (hd + 2);
@@ -929,10 +932,18 @@ Plan plan_of(int group, int n_kv, int hd, int capacity, int n, int n_tok, bool s
     if (few <= kMaxItems && rows <= 32l * n) {
         p.rows = true;
         p.items = (int)few;
-        p.shares = (2 * cus + n_kv - 1) / n_kv;
-        if (p.shares > kMaxParts) p.shares = kMaxParts;
         p.splits = 1;
         p.tile = kRowTile;
+        p.least = 4;
+        if (capacity <= kWhole) {
+            // every item fits one share: a workgroup each, and nothing to join (one token after 600, 14 heads over 2 of 64,
+            // f32: WHOLE_US us, split and joined 11.3; over 1,024 positions WHOLE2_US and 11.4)
+            p.shares = p.items;
+            p.least = (capacity / kTile + 4) & ~3;
+            return p;
+        }
+        p.shares = (2 * cus + n_kv - 1) / n_kv;
+        if (p.shares > kMaxParts) p.shares = kMaxParts;
         p.join_rows = single && group < kRowTile ? group : kRowTile;
         p.part_rows = 2 * (size_t)p.shares * kRowTile;
         return p;
@@ -948,7 +959,7 @@ Plan plan_of(int group, int n_kv, int hd, int capacity, int n, int n_tok, bool s
     const int most = capacity / (4 * kTile);
     if (p.splits > 16) p.splits = 16;
     if (p.splits > most) p.splits = most > 1 ? most : 1;
-    p.join_rows = p.tile;
+    p.join_rows = p.splits > 1 ? p.tile : 0;
     p.part_rows = p.splits > 1 ? (size_t)p.items * p.splits * p.tile : 0;
     return p;
 }
@@ -980,6 +991,7 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
     const Plan p = plan_of(a.group, c.n_kv, c.hd, c.seq_pages << c.page_shift, n, n_tok, start == nullptr);
     a.items = p.items;
     a.splits = p.splits;
+    a.least = p.least;
     a.rec = static_cast<int4*>(ws);
     a.part_o = reinterpret_cast<float*>(a.rec + p.items);
     a.part_ml = a.part_o + p.part_rows * c.n_kv * c.hd;
@@ -988,8 +1000,9 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
         constexpr int kC = decltype(kc)::value;
         if (p.rows) {
             qh_launch((kv8_rows_kernel<T, kC>), dim3((unsigned)p.shares, (unsigned)c.n_kv), dim3(256), 0, s, c, a);
-            qh_launch((kv8_join_kernel<T, kC>), dim3((unsigned)p.items, (unsigned)c.n_kv, (unsigned)p.join_rows), dim3(256), 0,
-                      s, c, a);
+            if (p.join_rows)
+                qh_launch((kv8_join_kernel<T, kC>), dim3((unsigned)p.items, (unsigned)c.n_kv, (unsigned)p.join_rows),
+                          dim3(256), 0, s, c, a);
         } else {
             constexpr size_t lds = 2 * 2 * (size_t)kTile * 64 * kC * 2;
             const dim3 grid((unsigned)c.n_kv * (unsigned)p.items, (unsigned)p.splits);
@@ -997,7 +1010,7 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
                 if (p.tile == 128) qh_launch((kv8_tile_kernel<T, kC, 2>), grid, dim3(256), lds, s, c, a);
             }
             if (p.tile == 64) qh_launch((kv8_tile_kernel<T, kC, 1>), grid, dim3(256), lds, s, c, a);
-            if (p.splits > 1)
+            if (p.join_rows)
                 qh_launch((kv8_join_splits_kernel<T, kC>),
                           dim3((unsigned)p.items, (unsigned)c.n_kv, (unsigned)(p.join_rows * kC / 16)), dim3(256), 0, s, c,
                           a, p.tile);
