@@ -399,7 +399,9 @@ typedef struct qh_decoder_state {
                                positions, each dimension's 8 values contiguous (position p, column c at
                                ((p / 8) * kv_dim + c) * 8 + p % 8 within its layer) */
     int32_t* status;        /* 0, or bit 0: a step ran at a position >= ctx_len (it wrote nothing to the cache);
-                               bit 1: a prompt token was outside [0, vocab). Cleared by qh_decoder_prefill. */
+                               bit 1: a prompt token was outside [0, vocab); bit 2: the cache that
+                               qh_decoder_bind_kv8 named had no place for a forward's tokens, which were not stored and
+                               attended to nothing. Cleared by qh_decoder_prefill. */
     int32_t* history;       /* [ctx_len + 1]: the token history (the session's history_, session.cpp:13-52): the
                                prompt ids of every prefill since position 0, then each chosen id */
     int32_t* history_len;   /* its length */
@@ -456,6 +458,20 @@ int qh_decoder_views(qh_decoder* d, qh_decoder_state* v);
  * is short, in more passes. On failure the previous stack stays.
  * Replaces: nothing (the reference's chunk is a compile-time constant); a scheduling choice of the GPU path. */
 int qh_decoder_set_prefill_stack(qh_decoder* d, int stack);
+
+/* Later prefill and step calls keep their keys and values in sequence `seq` of the 8-bit cache c (n_layers, n_kv_heads
+ * and head_dim of the model; its state arrays in order, its memory alive while it is bound) instead of the decoder's own
+ * cache, and attend to that sequence: results then carry the 8-bit rounding and are no longer the reference's bits. A
+ * prefill at pos0 (at most the sequence's length) first shortens the sequence to pos0; a step continues it, so its
+ * position has to be the sequence's length. Both take pages from the cache as the sequence grows, copying a last page that
+ * other sequences hold. So a prompt is read once and its continuations are forks: qh_kv8_fork, then for each fork this call
+ * and a prefill of the prompt's last token. Tokens that have no place (no free page, another position, past the context or
+ * the table row) set *status. Synchronises the device and allocates workspaces at the first call and where the cache's size
+ * changes (a failure leaves the decoder as it was); the sequence is read on the device, so a step captured in a HIP graph
+ * follows a later call that names another sequence of the same cache, and has to be captured again for another cache.
+ * c NULL: the decoder's own cache again (with what it held).
+ * No counterpart in the reference, whose Model owns one sequence. */
+int qh_decoder_bind_kv8(qh_decoder* d, const qh_kv8_cache* c, int seq);
 
 /* Stages of a decode step, as qh_decoder_step_timed names them: per layer l, id l * QH_STAGES_PER_LAYER + one of
  * QH_STAGE_QKV (rmsnorm + q/k/v projections), QH_STAGE_ATTENTION, QH_STAGE_O (o projection + residual),

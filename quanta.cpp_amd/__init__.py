@@ -96,7 +96,7 @@ EXPORTS = ("qh_last_error", "qh_version", "qh_init", "qh_quant_bytes", "qh_tenso
            "qh_decoder_create",
            "qh_decoder_destroy",
            "qh_decoder_prefill", "qh_decoder_begin", "qh_decoder_step", "qh_decoder_views",
-           "qh_decoder_set_prefill_stack", "qh_decoder_step_timed",
+           "qh_decoder_set_prefill_stack", "qh_decoder_bind_kv8", "qh_decoder_step_timed",
            "qh_decoder_set_query",
            "qh_decoder_set_sampler")
 
@@ -149,6 +149,7 @@ def _bind(lib):
         "qh_decoder_step": ([vp, i32, vp], i32),
         "qh_decoder_views": ([vp, C.POINTER(qh_decoder_state)], i32),
         "qh_decoder_set_prefill_stack": ([vp, i32], i32),
+        "qh_decoder_bind_kv8": ([vp, kv8, i32], i32),
         "qh_decoder_step_timed": ([vp, i32, vp, vp, vp, i32, vp], i32),
         "qh_sampler_state": ([C.c_uint64], C.c_uint64),
         "qh_sample": ([vp, i32, vp, vp, vp, i32, C.POINTER(qh_sampler_params), vp, vp, vp], i32),
@@ -633,6 +634,12 @@ class Decoder:
         _check(lib().qh_decoder_views(self.h, C.byref(st)))
         self.views = st
 
+    def bind_kv8(self, cache: KV8Cache | None, seq: int = 0):
+        """Later prefill and step calls keep their keys and values in sequence `seq` of an 8-bit cache and attend to it
+        (qh_decoder_bind_kv8); None: the decoder's own cache again."""
+        _check(lib().qh_decoder_bind_kv8(self.h, None if cache is None else cache._ref, seq))
+        self._kv8 = cache
+
     def prefill(self, tokens, pos0: int = 0, top_k: int = 1):
         torch = _torch()
         self.tokens = torch.as_tensor(np.ascontiguousarray(tokens, np.int32)).to(self.buf.device)
@@ -685,7 +692,8 @@ class Decoder:
         return int(_d2h(self.views.top1_full, 4, np.int32)[0])
 
     def status(self) -> int:
-        """0, or bit 0: a step ran past the context (nothing was written); bit 1: a prompt token was out of range."""
+        """0, or bit 0: a step ran past the context (nothing was written); bit 1: a prompt token was out of range; bit 2: a
+        bound 8-bit cache had no place for a forward's tokens."""
         return int(_d2h(self.views.status, 4, np.int32)[0])
 
     def kv(self, layer: int, n_pos: int):

@@ -749,6 +749,21 @@ int qh_decoder_set_prefill_stack(qh_decoder* d, int stack) {
     return check_hip(decoder_set_prefill_stack(reinterpret_cast<Decoder*>(d), stack), "qh_decoder_set_prefill_stack");
 }
 
+int qh_decoder_bind_kv8(qh_decoder* d, const qh_kv8_cache* c, int seq) {
+    const char* who = "qh_decoder_bind_kv8";
+    if (!d) return fail(QH_ERR_ARG, "%s: null decoder", who);
+    Decoder* dd = reinterpret_cast<Decoder*>(d);
+    if (!c) return check_hip(decoder_bind_kv8(dd, nullptr, 0), who);
+    if (int rc = validate_kv8(c, who)) return rc;
+    const qh_model_desc& hp = decoder_desc(dd);
+    if (c->n_layers != hp.n_layers || c->n_kv_heads != hp.n_kv_heads || c->head_dim != hp.head_dim)
+        return fail(QH_ERR_SHAPE, "%s: a cache of %d layers of %d KV heads of %d for a model of %d of %d of %d", who,
+                    c->n_layers, c->n_kv_heads, c->head_dim, hp.n_layers, hp.n_kv_heads, hp.head_dim);
+    if (seq < 0 || seq >= c->n_seqs) return fail(QH_ERR_ARG, "%s: sequence %d of %d", who, seq, c->n_seqs);
+    const Kv8View v = kv8_view(*c, 0);
+    return check_hip(decoder_bind_kv8(dd, &v, seq), who);
+}
+
 int qh_decoder_set_query(qh_decoder* d, const qh_sampler_params* p) {
     if (!d) return fail(QH_ERR_ARG, "qh_decoder_set_query: null decoder");
     if (p) {

@@ -38,6 +38,7 @@
 #include "qh_device.h"
 #include "qh_gemv.h"
 #include "qh_internal.h"
+#include "qh_kv8.h"
 #include "qh_math.h"
 
 namespace qh {
@@ -1256,6 +1257,59 @@ __global__ void set_subpos_kernel(int* p, int base, int n) {
     if (i < n) p[i] = base + kChunk * i;
 }
 
+// A bound 8-bit cache's state on the device (qh_decoder_bind_kv8): [kKv8Seq] the sequence, [kKv8Batch] the one that the
+// forward's rows belong to (-1: none, the cache has no place for them), [kKv8Want] the length asked for, [kKv8Ok] whether
+// the forward's positions are the sequence's next ones so far, [kKv8Start] the rows' range, {0, n}.
+enum { kKv8Seq, kKv8Batch, kKv8Want, kKv8Ok, kKv8Start, kKv8Ints = kKv8Start + 2 };
+
+// Before a forward of n tokens at pos0 (-1: one token at *pos): phase 0 asks for a length of pos0 (a prompt that starts
+// over inside the sequence), phase 1 for room for the tokens, phase 2 checks that it is there. A step continues its
+// sequence, so its position has to be the sequence's length.
+__global__ void kv8_room_kernel(Kv8View c, int* __restrict__ b, const int* __restrict__ pos, int pos0, int n, int phase, int ctx,
+                                int* __restrict__ status) {
+    const int len = c.lens[b[kKv8Seq]], p = pos0 >= 0 ? pos0 : *pos, most = min(ctx, c.seq_pages << c.page_shift);
+    if (phase == 2) {
+        const bool ok = b[kKv8Ok] && len == p + n;
+        b[kKv8Batch] = ok ? b[kKv8Seq] : -1;
+        if (!ok) *status |= p + n > ctx ? 1 : 4;
+        return;
+    }
+    const bool ok = p >= 0 && p + n <= most && (phase == 0 ? len >= p : len == p && (pos0 < 0 || b[kKv8Ok]));
+    b[kKv8Ok] = ok ? 1 : 0;
+    b[kKv8Want] = !ok ? len : phase == 0 ? p : p + n;
+    b[kKv8Start] = 0;
+    b[kKv8Start + 1] = n;
+}
+
+// Bias and RoPE of n tokens' projections in place, as kv_store_kernel and the attention kernels compute them (one
+// workgroup per token, positions *pos_dev + t).
+template <int HD>
+__global__ __launch_bounds__(256) void qkv_rope_kernel(float* __restrict__ q, float* __restrict__ k, float* __restrict__ v,
+                                                       const float* __restrict__ bq, const float* __restrict__ bk,
+                                                       const float* __restrict__ bv, const float* __restrict__ cs,
+                                                       const int* __restrict__ pos_dev, int ctx, int n_heads, int n_kv) {
+    constexpr int HALF = HD / 2;
+    const int t = blockIdx.x, tid = threadIdx.x, pos = *pos_dev + t;
+    if (pos >= ctx || pos < 0) return;
+    const float* crow = cs + (size_t)pos * HD;
+    for (int e = tid; e < (n_heads + n_kv) * HALF; e += 256) {
+        const int h = e / HALF, i = e % HALF;
+        const bool is_q = h < n_heads;
+        float* row = is_q ? q + ((size_t)t * n_heads + h) * HD : k + ((size_t)t * n_kv + h - n_heads) * HD;
+        const float* bias = is_q ? (bq ? bq + h * HD : nullptr) : (bk ? bk + (h - n_heads) * HD : nullptr);
+        float a = row[i], b = row[i + HALF];
+        if (bias) {
+            a = a + bias[i];
+            b = b + bias[i + HALF];
+        }
+        const float c = crow[2 * i], sn = crow[2 * i + 1];
+        row[i] = __builtin_fmaf(a, c, -(b * sn));
+        row[i + HALF] = __builtin_fmaf(b, c, a * sn);
+    }
+    if (bv)
+        for (int e = tid; e < n_kv * HD; e += 256) v[(size_t)t * n_kv * HD + e] += bv[e];
+}
+
 // The token a step chose: the sampler's pick when there is one, else the head's greedy top-1.
 struct Pick {
     const int32_t* sampled;
@@ -1337,6 +1391,11 @@ struct Decoder {
     size_t am_ws_bytes = 0;
     void* sample_ws = nullptr;  // the sampler's sorted path (more than QH_SAMPLE_MAX_TOPK survivors)
     int32_t* top1_full = nullptr;
+    // a bound 8-bit cache (qh_decoder_bind_kv8), its layer 0; state and workspaces are the decoder's
+    bool has_kv8 = false;
+    Kv8View kv8{};
+    int* kv8_state = nullptr;
+    void *kv8_pages_ws = nullptr, *kv8_attn_ws = nullptr;
     bool fuse = true;  // fused decode kernels (QH_DECODER_FUSE=0 at creation selects one launch per operation)
     std::vector<void*> allocs;
     // The stage the kernels launched since the previous mark belong to (qh_decoder_step_timed).
@@ -1729,8 +1788,45 @@ hipError_t attention_stack(Decoder* d, int l, int n, hipStream_t s) {
     return launch_attention_stack(a, hp.head_dim, d->aws, d->aws_bytes, s);
 }
 
+// Room in the bound 8-bit cache for a forward of n tokens at pos0 (-1: a step's token).
+hipError_t kv8_room(Decoder* d, int pos0, int n, hipStream_t s) {
+    const auto ask = [&](int phase) {
+        qh_launch(kv8_room_kernel, dim3(1), dim3(1), 0, s, d->kv8, d->kv8_state, d->pos, pos0, n, phase, d->hp.ctx_len,
+                  d->status);
+        return hipGetLastError();
+    };
+    for (int phase = pos0 >= 0 ? 0 : 1; phase < 2; ++phase) {
+        QH_TRY(ask(phase));
+        QH_TRY(launch_kv8_resize(d->kv8, d->hp.n_layers, d->kv8_state + kKv8Seq, d->kv8_state + kKv8Want, 1,
+                                 d->kv8_pages_ws, s));
+    }
+    return ask(2);
+}
+
+// Attention over the bound 8-bit cache: n tokens' keys and values stored, then their queries over the sequence.
+hipError_t attention_kv8(Decoder* d, int l, int n, hipStream_t s) {
+    const qh_model_desc& hp = d->hp;
+    const int64_t qd = (int64_t)hp.n_heads * hp.head_dim, kvd = (int64_t)hp.n_kv_heads * hp.head_dim;
+    Kv8View c = d->kv8;
+    c.pages += (size_t)l * c.n_pages * c.page_bytes;
+    if (hp.head_dim == 64)
+        qh_launch((qkv_rope_kernel<64>), dim3(n), dim3(256), 0, s, d->q, d->k, d->v, bias(d, l, L_BQ), bias(d, l, L_BK),
+                  bias(d, l, L_BV), d->cs, d->pos, hp.ctx_len, hp.n_heads, hp.n_kv_heads);
+    else
+        qh_launch((qkv_rope_kernel<128>), dim3(n), dim3(256), 0, s, d->q, d->k, d->v, bias(d, l, L_BQ), bias(d, l, L_BK),
+                  bias(d, l, L_BV), d->cs, d->pos, hp.ctx_len, hp.n_heads, hp.n_kv_heads);
+    QH_TRY(hipGetLastError());
+    const int32_t *start = n == 1 ? nullptr : d->kv8_state + kKv8Start, *seq = d->kv8_state + kKv8Batch;
+    QH_TRY(launch_kv8_append(c, d->k, d->v, QH_F32, kvd, kvd, start, seq, 1, n, s));
+    float* out = d->fb ? d->fb : d->o;  // unquantized matrices read it as it is
+    QH_TRY(launch_kv8_attention(c, d->q, out, QH_F32, hp.n_heads, qd, qd, start, seq, 1, n, true,
+                                1.0f / sqrtf((float)hp.head_dim), d->kv8_attn_ws, s));
+    return launch_quantize_q8(out, n, (int)qd, d->qb, d->db, s);
+}
+
 hipError_t attention(Decoder* d, int l, int n, hipStream_t s) {
     const qh_model_desc& hp = d->hp;
+    if (d->has_kv8) return attention_kv8(d, l, n, s);
     if (n > kChunk && stack_attention(d)) return attention_stack(d, l, n, s);
     if (n > kChunk) {  // a prefill stack without it: its 32-token sub-chunks in order (each reads the rows the ones before wrote)
         for (int i = 0; i * kChunk < n; ++i)
@@ -1753,6 +1849,7 @@ hipError_t attention(Decoder* d, int l, int n, hipStream_t s) {
 // in d->hidden and its quantization in qa / da for the head.
 hipError_t decode_layers(Decoder* d, hipStream_t s) {
     const qh_model_desc& hp = d->hp;
+    if (d->has_kv8) QH_TRY(kv8_room(d, -1, 1, s));
     for (int l = 0; l < hp.n_layers; ++l) {
         GemvPlan p;
         size_t lds = 0;
@@ -2067,6 +2164,7 @@ hipError_t decoder_prefill(Decoder* d, const int32_t* tokens, int n, int pos0, i
         qh_launch(set_int_kernel, dim3(1), dim3(1), 0, s, d->pos, pos0 + c0);
         QH_TRY(hipGetLastError());
         d->stack_end = pos0 + c0 + m;
+        if (d->has_kv8) QH_TRY(kv8_room(d, pos0 + c0, m, s));
         QH_TRY(embed(d, tokens + c0, m, s));
         QH_TRY(prefill_layers(d, m, s));
         last = m - 1;
@@ -2147,6 +2245,49 @@ hipError_t decoder_begin(Decoder* d, int top_k, int32_t* out, int out_cap, hipSt
 }
 
 int decoder_ctx(const Decoder* d) { return d->hp.ctx_len; }
+
+const qh_model_desc& decoder_desc(const Decoder* d) { return d->hp; }
+
+hipError_t decoder_bind_kv8(Decoder* d, const Kv8View* c, int seq) {
+    QH_TRY(hipDeviceSynchronize());  // nothing in flight uses what is replaced
+    if (!c) {
+        d->has_kv8 = false;
+        return hipSuccess;
+    }
+    const int capacity = c->seq_pages << c->page_shift;
+    // kept over an unbinding too: a captured step may still name them
+    const bool same = d->kv8_state && d->kv8.n_pages == c->n_pages && d->kv8.n_seqs == c->n_seqs &&
+                      d->kv8.seq_pages << d->kv8.page_shift == capacity;
+    if (!same) {
+        // all three anew, so that a failure leaves the binding as it was
+        void* fresh[3] = {};
+        size_t attn = 0;
+        for (int n = 1; n <= kMaxStack; ++n) {
+            const size_t b = kv8_attention_workspace_bytes(d->hp.n_heads, d->hp.n_kv_heads, d->hp.head_dim, capacity, 1, n);
+            attn = b > attn ? b : attn;
+        }
+        const size_t bytes[3] = {sizeof(int) * kKv8Ints, kv8_pages_workspace_bytes(c->n_pages, c->n_seqs), attn};
+        for (int i = 0; i < 3; ++i) {
+            const hipError_t e = dalloc(d, &fresh[i], bytes[i]);
+            if (e != hipSuccess) {
+                for (void* p : fresh) dfree(d, p);
+                (void)hipGetLastError();
+                return e;
+            }
+        }
+        dfree(d, d->kv8_state);
+        dfree(d, d->kv8_pages_ws);
+        dfree(d, d->kv8_attn_ws);
+        d->kv8_state = static_cast<int*>(fresh[0]);
+        d->kv8_pages_ws = fresh[1];
+        d->kv8_attn_ws = fresh[2];
+    }
+    const int state[kKv8Ints] = {seq, -1, 0, 0, 0, 0};
+    QH_TRY(hipMemcpy(d->kv8_state, state, sizeof state, hipMemcpyHostToDevice));
+    d->kv8 = *c;
+    d->has_kv8 = true;
+    return hipSuccess;
+}
 
 #if defined(QH_TIMELINE)
 extern "C" int qh_timeline_pa_read(uint64_t* host, int n) {

@@ -109,4 +109,9 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
                                 int64_t ldo, const int32_t* start, const int32_t* seqs, int n, int n_tok, bool causal,
                                 float scale, void* ws, hipStream_t s);
 
+// The decoder over a bound cache (qh_decoder.hip): c is its layer 0, null to unbind.
+struct Decoder;
+const qh_model_desc& decoder_desc(const Decoder* d);
+hipError_t decoder_bind_kv8(Decoder* d, const Kv8View* c, int seq);
+
 }  // namespace qh
