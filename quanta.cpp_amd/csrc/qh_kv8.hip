@@ -457,9 +457,12 @@ __global__ __launch_bounds__(kWg) void kv8_resize_kernel(Kv8View c, const int32_
 }
 
 // dst[i] becomes a fork of src[i]: dst's pages are given back, then (copy) it takes as many pages as src has, to be
-// filled by kv8_move_kernel, or shares src's (kv8_share_kernel).
+// filled by kv8_move_kernel, or shares src's: entry by entry here (mode kShareHere), or in kv8_share_kernel on the whole GPU
+// where the table rows are many.
+enum { kShareLater, kShareHere, kCopy };
+__device__ __forceinline__ void share_page(const Kv8View& c, int src, int dst, int j);
 __global__ __launch_bounds__(kWg) void kv8_fork_kernel(Kv8View c, const int32_t* __restrict__ src,
-                                                       const int32_t* __restrict__ dst, int n, int copy, void* ws) {
+                                                       const int32_t* __restrict__ dst, int n, int mode, void* ws) {
     __shared__ uint32_t seen[QH_KV8_MAX_SEQS / 32];
     const PagesWs w = pages_ws(ws, c.n_pages, c.n_seqs);
     const int tid = (int)threadIdx.x;
@@ -482,7 +485,9 @@ __global__ __launch_bounds__(kWg) void kv8_fork_kernel(Kv8View c, const int32_t*
     }
     for (int i = tid >> 6; i < n; i += kWg / 64) drop_pages(c, dst[i], 0, pages_of(c, kv8_len(c, dst[i])));
     __syncthreads();
-    if (!copy) {
+    if (mode != kCopy) {
+        if (mode == kShareHere)
+            for (int t = tid; t < n * c.seq_pages; t += kWg) share_page(c, src[t / c.seq_pages], dst[t / c.seq_pages], t % c.seq_pages);
         for (int i = tid; i < n; i += kWg) c.lens[dst[i]] = kv8_len(c, src[i]);
         if (tid == 0) *w.ok = 1;
         return;
@@ -513,15 +518,17 @@ __global__ __launch_bounds__(kWg) void kv8_fork_kernel(Kv8View c, const int32_t*
     }
 }
 
-// Shared forks: dst's table row is src's, and every page has one reference more. A thread per table entry.
+// Table entry j of a shared fork: src's page, which has one reference more then.
+__device__ __forceinline__ void share_page(const Kv8View& c, int src, int dst, int j) {
+    if (j >= pages_of(c, kv8_len(c, src))) return;
+    const int page = c.table[(size_t)src * c.seq_pages + j];
+    c.table[(size_t)dst * c.seq_pages + j] = page;
+    if (page >= 0 && page < c.n_pages) atomicAdd(&c.refs[page], 1);
+}
 __global__ __launch_bounds__(256) void kv8_share_kernel(Kv8View c, const int32_t* __restrict__ src,
                                                         const int32_t* __restrict__ dst, int n, void* ws) {
     if (*pages_ws(ws, c.n_pages, c.n_seqs).ok == 0) return;
-    const int i = (int)blockIdx.y, j = (int)(blockIdx.x * 256 + threadIdx.x);
-    if (j >= pages_of(c, kv8_len(c, src[i]))) return;
-    const int page = c.table[(size_t)src[i] * c.seq_pages + j];
-    c.table[(size_t)dst[i] * c.seq_pages + j] = page;
-    if (page >= 0 && page < c.n_pages) atomicAdd(&c.refs[page], 1);
+    share_page(c, src[blockIdx.y], dst[blockIdx.y], (int)(blockIdx.x * 256 + threadIdx.x));
 }
 
 // Which pages move: of L live pages those numbered L and above go, in order, to the free numbers below L, so sources and
@@ -687,9 +694,13 @@ hipError_t launch_kv8_resize(const Kv8View& c, int n_layers, const int32_t* seqs
 
 hipError_t launch_kv8_fork(const Kv8View& c, int n_layers, const int32_t* src, const int32_t* dst, int n, bool copy,
                            void* ws, hipStream_t s) {
-    qh_launch(kv8_fork_kernel, dim3(1), dim3(kWg), 0, s, c, src, dst, n, copy ? 1 : 0, ws);
+    // up to 2,048 table entries in the planning workgroup (16 forks of 128 pages: 5.9 us, with a second launch 6.8; of 256
+    // pages 8.8 and 7.5; 4 of 16: 3.5 and 5.4)
+    const int mode = copy ? kCopy : (int64_t)n * c.seq_pages <= 2048 ? kShareHere : kShareLater;
+    qh_launch(kv8_fork_kernel, dim3(1), dim3(kWg), 0, s, c, src, dst, n, mode, ws);
     if (hipError_t e = hipGetLastError()) return e;
     if (copy) return launch_move(c, n_layers, c.n_pages, false, ws, s);
+    if (mode == kShareHere) return hipSuccess;
     qh_launch(kv8_share_kernel, dim3((unsigned)((c.seq_pages + 255) / 256), (unsigned)n), dim3(256), 0, s, c, src, dst, n,
               ws);
     return hipGetLastError();

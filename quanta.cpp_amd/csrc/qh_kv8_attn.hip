@@ -936,8 +936,8 @@ Plan plan_of(int group, int n_kv, int hd, int capacity, int n, int n_tok, bool s
         p.tile = kRowTile;
         p.least = 4;
         if (capacity <= kWhole) {
-            // every item fits one share: a workgroup each, and nothing to join (one token after 600, 14 heads over 2 of 64,
-            // f32: WHOLE_US us, split and joined 11.3; over 1,024 positions WHOLE2_US and 11.4)
+            // every item fits one share: a workgroup each, and nothing to join (one token, 14 heads over 2 of 64, f32: over
+            // 300 positions 8.0 us, split and joined 10.9; 600 9.2 and 11.0; 1,024 10.6 and 10.9)
             p.shares = p.items;
             p.least = (capacity / kTile + 4) & ~3;
             return p;
