@@ -292,7 +292,7 @@ typedef struct qh_kv8_cache {
     int32_t* status; /* one: QH_KV8_* bits that calls on this cache have set (cleared by qh_kv8_reset or the caller) */
     int32_t n_layers, n_pages;
     int32_t page_tokens; /* a power of two, 16 to 256 */
-    int32_t n_kv_heads;
+    int32_t n_kv_heads; /* at most 256 */
     int32_t head_dim; /* 64 or 128 */
     int32_t n_seqs, seq_pages;
 } qh_kv8_cache;
@@ -341,8 +341,8 @@ int qh_kv8_compact(const qh_kv8_cache* c, int32_t* live, void* workspace, size_t
 /* Stores k and v, rows of [n_kv_heads][head_dim], into layer `layer`: per block d = max|x| / 127 (rounded to f32) and
  * the codes nearest to x / d, halves away from zero. A block that holds earlier tokens keeps the larger of its scale and
  * the new ones', and where that grows its codes are rounded to it. An infinite or NaN value makes its block's scale NaN,
- * so that all 16 tokens of that head read as NaN. Each sequence in one entry at most. Tokens in a page that other
- * sequences hold are left out (QH_KV8_SHARED). */
+ * so that all 16 tokens of that head read as NaN. Each sequence in one entry at most, and its tokens in order: a block's
+ * earlier tokens have to be there. Tokens in a page that other sequences hold are left out (QH_KV8_SHARED). */
 int qh_kv8_append(const qh_kv8_cache* c, int layer, const void* k, const void* v, int dtype, int64_t ldk, int64_t ldv,
                   const int32_t* start, const int32_t* seqs, int n, int n_tok, void* stream);
 
@@ -350,15 +350,16 @@ int qh_kv8_append(const qh_kv8_cache* c, int layer, const void* k, const void* v
 int qh_kv8_read(const qh_kv8_cache* c, int layer, void* k, void* v, int dtype, int64_t ldk, int64_t ldv,
                 const int32_t* start, const int32_t* seqs, int n, int n_tok, void* stream);
 
-/* Workspace bytes of qh_kv8_attention for up to n entries over n_tok rows (no initialisation). */
+/* Workspace bytes of a qh_kv8_attention call with n entries over n_tok rows (no initialisation; a smaller batch can need
+ * more, as it is split further). */
 size_t qh_kv8_attention_workspace_bytes(const qh_kv8_cache* c, int n_heads, int n, int n_tok);
 
 /* Attention of query rows q [n_heads][head_dim] over their sequences: out = sum_j p_j v_j with p = softmax(scale *
  * q . k_j) over the positions j that the row sees: up to its own (causal 1), or the whole sequence (causal 0, for states
  * that are not the queries' own: an entry may then have more rows than the sequence has tokens). Query head h reads KV
  * head h / (n_heads / n_kv_heads). A row that sees nothing (an empty sequence, or a position below 0) is 0. out may not
- * overlap q. Sums in f32; f32 queries and weights go through the matrix instructions as two f16 each, f16 calls' weights
- * as one. */
+ * overlap q. A row of q that is not finite gives NaN, and so does a visible token that reads as NaN. Sums in f32; f32
+ * queries and weights go through the matrix instructions as two f16 each, f16 calls' weights as one. */
 int qh_kv8_attention(const qh_kv8_cache* c, int layer, const void* q, void* out, int dtype, int n_heads, int64_t ldq,
                      int64_t ldo, const int32_t* start, const int32_t* seqs, int n, int n_tok, int causal, float scale,
                      void* workspace, size_t workspace_bytes, void* stream);

@@ -637,6 +637,8 @@ class Decoder:
     def bind_kv8(self, cache: KV8Cache | None, seq: int = 0):
         """Later prefill and step calls keep their keys and values in sequence `seq` of an 8-bit cache and attend to it
         (qh_decoder_bind_kv8); None: the decoder's own cache again."""
+        if cache is not None and cache.device != self.buf.device:
+            raise QHError(f"the cache is on {cache.device}, the decoder on {self.buf.device}")
         _check(lib().qh_decoder_bind_kv8(self.h, None if cache is None else cache._ref, seq))
         self._kv8 = cache
 

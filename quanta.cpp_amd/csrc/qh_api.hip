@@ -1,5 +1,6 @@
 // C-ABI layer: argument validation, error reporting and dispatch to the kernel launchers.
 // Every entry point returns a status and records a message for the calling thread on failure.
+#include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -97,7 +98,7 @@ int check_sampler(const qh_sampler_params& p, int n_valid, const char* who, bool
 
 // Supported page shapes of the 8-bit cache.
 bool kv8_shape_ok(int page_tokens, int n_kv, int hd) {
-    return page_tokens >= 16 && page_tokens <= 256 && (page_tokens & (page_tokens - 1)) == 0 && n_kv > 0 && n_kv <= 4096 &&
+    return page_tokens >= 16 && page_tokens <= 256 && (page_tokens & (page_tokens - 1)) == 0 && n_kv > 0 && n_kv <= 256 &&
            (hd == 64 || hd == 128);
 }
 
@@ -131,14 +132,19 @@ int validate_kv8_batch(const qh_kv8_cache& c, int layer, const int32_t* start, i
     if (layer < 0 || layer >= c.n_layers) return fail(QH_ERR_ARG, "%s: layer %d of %d", who, layer, c.n_layers);
     if (n < 0 || n_tok < 0 || n > (1 << 24)) return fail(QH_ERR_ARG, "%s: %d entries over %d rows", who, n, n_tok);
     if (!start && n != n_tok) return fail(QH_ERR_ARG, "%s: %d entries over %d rows without starts", who, n, n_tok);
+    // a launch has fewer than 2^24 workgroups of 256: blocks of 16 rows (two more to an entry), four heads' sides to one
+    if (((int64_t)n_tok / kBlk + 2 * (int64_t)n) * ((c.n_kv_heads + 1) / 2) >= 1 << 24)
+        return fail(QH_ERR_SHAPE, "%s: %d rows in %d entries are too many for one call", who, n_tok, n);
     return QH_OK;
 }
 
-int validate_kv8_heads(const qh_kv8_cache& c, int n_heads, int n_tok, const char* who) {
+int validate_kv8_heads(const qh_kv8_cache& c, int n_heads, int n, int n_tok, const char* who) {
     if (n_heads <= 0 || n_heads % c.n_kv_heads != 0)
         return fail(QH_ERR_SHAPE, "%s: %d query heads over %d KV heads", who, n_heads, c.n_kv_heads);
     if ((int64_t)n_heads / c.n_kv_heads * (n_tok > 0 ? n_tok : 0) > (1 << 30) || (int64_t)n_heads * c.head_dim > (1 << 24))
         return fail(QH_ERR_SHAPE, "%s: %d rows of %d heads", who, n_tok, n_heads);
+    if (((int64_t)n_heads / c.n_kv_heads * (n_tok > 0 ? n_tok : 0) / 64 + (n > 0 ? n : 0)) * c.n_kv_heads >= 1 << 24)
+        return fail(QH_ERR_SHAPE, "%s: %d rows of %d heads in %d entries are too many for one call", who, n_tok, n_heads, n);
     return QH_OK;
 }
 
@@ -600,7 +606,7 @@ int qh_kv8_read(const qh_kv8_cache* c, int layer, void* k, void* v, int dtype, i
 
 size_t qh_kv8_attention_workspace_bytes(const qh_kv8_cache* c, int n_heads, int n, int n_tok) {
     const char* who = "qh_kv8_attention_workspace_bytes";
-    if (validate_kv8(c, who) || validate_kv8_heads(*c, n_heads, n_tok, who)) return 0;
+    if (validate_kv8(c, who) || validate_kv8_heads(*c, n_heads, n, n_tok, who)) return 0;
     if (n <= 0 || n_tok <= 0) return 0;
     return kv8_attention_workspace_bytes(n_heads, c->n_kv_heads, c->head_dim, c->seq_pages * c->page_tokens, n, n_tok);
 }
@@ -610,14 +616,15 @@ int qh_kv8_attention(const qh_kv8_cache* c, int layer, const void* q, void* out,
                      void* workspace, size_t workspace_bytes, void* stream) {
     const char* who = "qh_kv8_attention";
     if (int rc = validate_kv8(c, who)) return rc;
-    if (int rc = validate_kv8_heads(*c, n_heads, n_tok, who)) return rc;
+    if (int rc = validate_kv8_heads(*c, n_heads, n, n_tok, who)) return rc;
     if (int rc = validate_kv8_batch(*c, layer, start, n, n_tok, who)) return rc;
     if (causal != 0 && causal != 1) return fail(QH_ERR_ARG, "%s: causal = %d", who, causal);
-    if (!(scale - scale == 0.0f)) return fail(QH_ERR_ARG, "%s: scale is not finite", who);
+    if (!(fabsf(scale) <= 1e38f)) return fail(QH_ERR_ARG, "%s: scale is not finite", who);
     if (n == 0 || n_tok == 0) return QH_OK;
     const int64_t width = (int64_t)n_heads * c->head_dim;
     if (int rc = validate_kv8_rows(q, dtype, ldq, width, who)) return rc;
     if (int rc = validate_kv8_rows(out, dtype, ldo, width, who)) return rc;
+    if (q == out) return fail(QH_ERR_ARG, "%s: out is q", who);
     const size_t need = kv8_attention_workspace_bytes(n_heads, c->n_kv_heads, c->head_dim, c->seq_pages * c->page_tokens, n, n_tok);
     if (!workspace || workspace_bytes < need)
         return fail(QH_ERR_NOMEM, "%s: workspace of %zu bytes, needs %zu", who, workspace ? workspace_bytes : 0, need);

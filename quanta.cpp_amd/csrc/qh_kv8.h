@@ -58,15 +58,15 @@ __device__ __forceinline__ float* kv8_scale(const Kv8View& c, int page, int whic
     return reinterpret_cast<float*>(s) + (which * c.n_kv + h) * per + blk;
 }
 
-// A ragged batch: entry b is the last rows [start[b], start[b + 1]) of sequence seqs[b] (null: b); start null: one row
-// each. Whatever the arrays hold, rows stay in [0, n_tok) and sequences outside the cache have none.
+// A ragged batch: entry b is the last rows [start[b], start[b + 1]) of sequence seqs[b] (null: seq0 + b); start null: one
+// row each. Whatever the arrays hold, rows stay in [0, n_tok) and sequences outside the cache have none.
 struct Kv8Batch {
     const int32_t *start, *seqs;
-    int n, n_tok;
+    int n, n_tok, seq0;
     __device__ __forceinline__ int at(int b) const {
         return start ? min(max(start[b], 0), n_tok) : min(b, n_tok);
     }
-    __device__ __forceinline__ int seq(int b) const { return seqs ? seqs[b] : b; }
+    __device__ __forceinline__ int seq(int b) const { return seqs ? seqs[b] : seq0 + b; }
 };
 
 // Work items of a ragged batch without a prefix sum: entry b's items begin at floor(start[b] * mul / unit) + pad * b,

@@ -69,8 +69,9 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 // row row0 + p. Bound by the memory traffic of long batches (each value read once, its code written once) and by the
 // dependent loads (entry, length, page, scale, codes) of single tokens.
 // Lane 16 g + j reads dims 4 j .. 4 j + 3 of tokens 4 g .. 4 g + 3, 16 lanes to a row, so that rows are read in one piece;
-// the values' codes are in place then, the keys' cross four lanes (rows read by the lanes that store them, 16 dims of one
-// token: 24,001 x 8 heads of 128, f32, 68 us; this 56).
+// the values' codes are in place then, the keys' cross four lanes. 24,001 x 8 heads of 128, f32: 62.6 us; with the rows read
+// by the lanes that store them, 16 dims of one token, 71. Codes from the rounded quotient (below) 60.8, and rows loaded past
+// the caches, which nothing reads again, 46.
 // The block's scale is max|x| / 127 over every token it has been given since its first one: a block that already holds
 // tokens (held > 0) keeps the larger of its scale and the new tokens', and its codes are rounded to the new scale where
 // that grew. Only the block's own wave touches it, so the update needs no atomics.
@@ -660,7 +661,7 @@ hipError_t launch_kv8_append(const Kv8View& c, const void* k, const void* v, int
     return by_type(dtype, c.hd, [&](auto* t, auto kc) {
         using T = std::remove_pointer_t<decltype(t)>;
         qh_launch((kv8_append_kernel<T, decltype(kc)::value>), grid, dim3(256), 0, s, c, (const T*)k, (const T*)v, ldk,
-                  ldv, Kv8Batch{start, seqs, n, n_tok});
+                  ldv, Kv8Batch{start, seqs, n, n_tok, 0});
     });
 }
 
@@ -670,7 +671,7 @@ hipError_t launch_kv8_read(const Kv8View& c, void* k, void* v, int dtype, int64_
     return by_type(dtype, c.hd, [&](auto* t, auto kc) {
         using T = std::remove_pointer_t<decltype(t)>;
         qh_launch((kv8_read_kernel<T, decltype(kc)::value>), grid, dim3(256), 0, s, c, (T*)k, (T*)v, ldk, ldv,
-                  Kv8Batch{start, seqs, n, n_tok});
+                  Kv8Batch{start, seqs, n, n_tok, 0});
     });
 }
 

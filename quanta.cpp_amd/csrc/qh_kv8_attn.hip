@@ -107,10 +107,20 @@ struct Query {
                     }
         } else {
             unit = __builtin_fabsf(scale_log2e);
+            float z = 0.0f;  // NaN for a row that is not finite, and then all of it becomes NaN
 #pragma unroll
             for (int c = 0; c < kC; ++c)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) hi[c][h] = valid ? (scale_log2e < 0.0f ? -r[c][h] : r[c][h]) : h8{};
+                for (int h = 0; h < 2; ++h) {
+                    hi[c][h] = valid ? (scale_log2e < 0.0f ? -r[c][h] : r[c][h]) : h8{};
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) z = __builtin_fmaf((float)hi[c][h][j], 0.0f, z);
+                }
+            z = over_groups(z, [](float p, float q) { return p + q; });
+            if (z != z) {
+#pragma unroll
+                for (int c = 0; c < kC; ++c) hi[c][0] = hi[c][1] = h8{} + (_Float16)__builtin_nanf("");
+            }
         }
     }
 
@@ -914,6 +924,7 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
 // How a call is split: few rows to an entry take the row kernel (shares over all lengths), many the tile kernel.
 struct Plan {
     bool rows;
+    int entries;  // of a launch (the row kernel)
     int items, shares, splits;
     int tile;          // rows of an item
     int join_rows;     // rows of an item that can have partial results; 0: none
@@ -929,9 +940,13 @@ Plan plan_of(int group, int n_kv, int hd, int capacity, int n, int n_tok, bool s
     const long few = single ? (long)n * ((group + kRowTile - 1) / kRowTile) : rows / kRowTile + n;
     const int cus = device_cus();
     Plan p{};
-    if (few <= kMaxItems && rows <= 32l * n) {
+    if ((single || few <= kMaxItems) && rows <= 32l * n) {
+        // single tokens in launches of as many entries as make kMaxItems row tiles (2,048 sequences of 2,000, 32 heads of
+        // 128 over 8, f16: 1,328 us, by the tile kernel 2,803; 14 heads of 64 over 2: 221 and 335)
         p.rows = true;
-        p.items = (int)few;
+        const int tiles = (group + kRowTile - 1) / kRowTile, most = kMaxItems / tiles;
+        p.entries = single && n > most ? most : n;
+        p.items = single ? p.entries * tiles : (int)few;
         p.splits = 1;
         p.tile = kRowTile;
         p.least = 4;
@@ -984,7 +999,7 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
     a.out = out;
     a.ldq = ldq;
     a.ldo = ldo;
-    a.batch = Kv8Batch{start, seqs, n, n_tok};
+    a.batch = Kv8Batch{start, seqs, n, n_tok, 0};
     a.group = n_heads / c.n_kv;
     a.causal = causal ? 1 : 0;
     a.scale_log2e = scale * 1.44269504088896340736f;
@@ -999,10 +1014,20 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
         using T = std::remove_pointer_t<decltype(t)>;
         constexpr int kC = decltype(kc)::value;
         if (p.rows) {
-            qh_launch((kv8_rows_kernel<T, kC>), dim3((unsigned)p.shares, (unsigned)c.n_kv), dim3(256), 0, s, c, a);
-            if (p.join_rows)
-                qh_launch((kv8_join_kernel<T, kC>), dim3((unsigned)p.items, (unsigned)c.n_kv, (unsigned)p.join_rows),
-                          dim3(256), 0, s, c, a);
+            const int tiles = p.items / p.entries;  // of a single token
+            for (int b = 0; b < n; b += p.entries) {
+                a.q = static_cast<const T*>(q) + (int64_t)b * ldq;  // only single tokens take more than one launch
+                a.out = static_cast<T*>(out) + (int64_t)b * ldo;
+                if (start == nullptr) {
+                    const int m = n - b < p.entries ? n - b : p.entries;
+                    a.batch = Kv8Batch{nullptr, seqs ? seqs + b : nullptr, m, m, b};
+                    a.items = m * tiles;
+                }
+                qh_launch((kv8_rows_kernel<T, kC>), dim3((unsigned)p.shares, (unsigned)c.n_kv), dim3(256), 0, s, c, a);
+                if (p.join_rows)
+                    qh_launch((kv8_join_kernel<T, kC>), dim3((unsigned)a.items, (unsigned)c.n_kv, (unsigned)p.join_rows),
+                              dim3(256), 0, s, c, a);
+            }
         } else {
             constexpr size_t lds = 2 * 2 * (size_t)kTile * 64 * kC * 2;
             const dim3 grid((unsigned)c.n_kv * (unsigned)p.items, (unsigned)p.splits);

@@ -318,12 +318,23 @@ def test_rows_that_see_no_poison_are_clean(qh):
     want, *sizes = c.plain.attention(0, [0], [160], q.cpu().numpy(), True, 0.125)
     got = out.cpu().double().numpy()[:112]
     assert (np.abs(got - want[:112]) <= attention_bound("f32", want, *sizes, 160, 64)[:112]).all()
-    # a query that is not finite is its own row's matter
-    q[5, 1, 0], q[6, 2, 7] = float("nan"), float("inf")
-    out2 = c.gpu.attention(0, q, start=starts([160]))
-    assert torch.isnan(out2[5, 1]).all() and torch.isnan(out2[6, 2]).all()
-    out2[5, 1], out2[6, 2] = out[5, 1], out[6, 2]
-    assert torch.equal(out2[:112], out[:112])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+def test_a_query_that_is_not_finite_is_its_own_row(qh, dtype):
+    import torch
+    rng = np.random.default_rng(SEED)
+    c = filled(qh, rng, [160], 2, 128, 16, dtype)
+    q = torch.from_numpy(rng.standard_normal((160, 4, 128)).astype(np.float32)).to("cuda").to(getattr(torch, dtype))
+    for rows in (160, 3):  # both kernels
+        x = q[-rows:].clone()
+        want = c.gpu.attention(0, x, start=starts([rows]))
+        x[0, 1, 0], x[1, 2, 100], x[2, 3, 7] = float("nan"), float("inf"), -float("inf")
+        got = c.gpu.attention(0, x, start=starts([rows]))
+        bad = torch.zeros(rows, 4, dtype=torch.bool, device="cuda")
+        bad[0, 1] = bad[1, 2] = bad[2, 3] = True
+        assert torch.isnan(got[bad]).all() and torch.isfinite(want).all()
+        assert torch.equal(got[~bad], want[~bad])
 
 
 def test_split_prompts_join(qh):
@@ -334,6 +345,39 @@ def test_split_prompts_join(qh):
         check_attention(c, rng, [0], [m], 8, "float16")
 
 
+def test_pools_and_rows_past_32_bit_offsets(qh):
+    """Pages behind more than 4 GiB of pool, rows more than 2^32 bytes apart: as in a small pool."""
+    import torch
+    rng = np.random.default_rng(SEED)
+    small = filled(qh, rng, [700, 300], 8, 128, 256, "float16").gpu
+    big = qh.KV8Cache(1, 12000, 256, 8, 128, 2, 3)  # 6.3 GB
+    big.refs[:11990] = 1  # in use by somebody: the sequences get the last pages
+    big.resize(ints([0, 1]), ints([700, 300]))
+    assert big.table[big.table >= 0].min() >= 11990
+    kv = small.read(0, 1000, start=starts([700, 300]), dtype=torch.float16)
+    big.append(0, kv[0], kv[1], start=starts([700, 300]))
+    small.resize(ints([0, 1]), ints([0, 0]))
+    small.resize(ints([0, 1]), ints([700, 300]))
+    small.append(0, kv[0], kv[1], start=starts([700, 300]))  # the values rounded twice, in both alike
+    for a, b in zip(*(c.read(0, 1000, start=starts([700, 300])) for c in (small, big))):
+        assert torch.equal(a, b)
+    q = torch.from_numpy(rng.standard_normal((9, 32, 128)).astype(np.float32)).to("cuda").half()
+    far = torch.empty((9, 1 << 28), dtype=torch.float16, device="cuda")
+    far[:, :32 * 128] = q.view(9, -1)
+    for counts in ([4, 5], [1, 8]):
+        want = small.attention(0, q, start=starts(counts)).view(9, -1)
+        assert torch.equal(want, big.attention(0, far[:, :32 * 128], start=starts(counts), out=far[:, 4096 * 2:4096 * 3]))
+    assert torch.equal(small.attention(0, q[7:]).view(2, -1), big.attention(0, far[7:, :4096]).view(2, -1))
+    far[:, :1024], far[:, 1024:2048] = kv[0][:9].view(9, -1), kv[1][:9].view(9, -1)
+    for c in (small, big):
+        c.resize(ints([1]), ints([0]))
+        c.resize(ints([1]), ints([9]))
+    small.append(0, kv[0][:9], kv[1][:9], start=starts([9]), seqs=ints([1]))
+    big.append(0, far[:, :1024], far[:, 1024:2048], start=starts([9]), seqs=ints([1]))
+    for a, b in zip(*(c.read(0, 9, start=starts([9]), seqs=ints([1])) for c in (small, big))):
+        assert torch.equal(a, b)
+
+
 def test_many_sequences(qh):
     """More entries than one launch of the few-row kernel takes."""
     rng = np.random.default_rng(SEED)
@@ -342,6 +386,18 @@ def test_many_sequences(qh):
     check_attention(c, rng, list(range(1100)), [1] * 1100, 2, "float32", single=True)
     check_attention(c, rng, list(range(1000)), [1] * 1000, 2, "float32", single=True)
     check_attention(c, rng, list(range(1000)), [1] * 1000, 2, "float32")
+
+
+def test_many_sequences_of_unlike_lengths(qh):
+    """The same where sequences are split and joined, with two row tiles to an entry, in and out of order."""
+    import torch
+    rng = np.random.default_rng(SEED)
+    lens = [int(x) for x in rng.integers(0, 20, 530)]
+    lens[3], lens[511], lens[512], lens[529] = 1100, 700, 1030, 65
+    c = filled(qh, rng, lens, 1, 64, 16, "float32")
+    check_attention(c, rng, [int(x) for x in rng.permutation(530)], [1] * 530, 17, "float32", single=True)
+    q = torch.from_numpy(rng.standard_normal((530, 17, 64)).astype(np.float32)).to("cuda")
+    assert torch.equal(c.gpu.attention(0, q), c.gpu.attention(0, q, seqs=ints(range(530))))
 
 
 # ------------------------------------------------------------------------------------------------ pages

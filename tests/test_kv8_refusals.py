@@ -21,8 +21,8 @@ def append(qh, c, layer=0, k=P, v=P, dtype=0, ldk=128, ldv=128, start=P, seqs=P,
     return qh.lib().qh_kv8_append(C.byref(c), layer, k, v, dtype, ldk, ldv, start, seqs, n, n_tok, None)
 
 
-def attend(qh, c, layer=0, q=P, out=P, dtype=0, heads=4, ldq=256, ldo=256, start=P, seqs=P, n=2, n_tok=5, causal=1,
-           scale=0.1, ws=P, ws_bytes=1 << 40):
+def attend(qh, c, layer=0, q=P, out=C.c_void_p(8192), dtype=0, heads=4, ldq=256, ldo=256, start=P, seqs=P, n=2, n_tok=5,
+           causal=1, scale=0.1, ws=P, ws_bytes=1 << 40):
     return qh.lib().qh_kv8_attention(C.byref(c), layer, q, out, dtype, heads, ldq, ldo, start, seqs, n, n_tok, causal,
                                      scale, ws, ws_bytes, None)
 
@@ -31,7 +31,7 @@ def test_page_bytes(qh):
     f = qh.lib().qh_kv8_page_bytes
     assert f(64, 2, 64) == 2 * 2 * 64 * 64 + 128  # codes, and 16 scales padded to a line
     assert f(256, 8, 128) == 2 * 8 * 256 * 128 + 2 * 8 * 16 * 4
-    for bad in ((8, 2, 64), (48, 2, 64), (512, 2, 64), (64, 0, 64), (64, 2, 96), (64, 2, 256), (64, 5000, 64)):
+    for bad in ((8, 2, 64), (48, 2, 64), (512, 2, 64), (64, 0, 64), (64, 2, 96), (64, 2, 256), (64, 257, 64)):
         assert f(*bad) == 0, bad
 
 
@@ -62,7 +62,7 @@ def test_null_cache(qh):
 @pytest.mark.parametrize("change,code", [
     ({"layer": -1}, 1), ({"layer": 2}, 1), ({"n": -1}, 1), ({"n_tok": -1}, 1), ({"start": None}, 1), ({"dtype": 2}, 2),
     ({"k": None}, 1), ({"v": None}, 1), ({"ldk": 127}, 1), ({"ldv": 64}, 1), ({"ldk": 130}, 4), ({"k": C.c_void_p(4100)}, 4),
-    ({"dtype": 1, "ldk": 132}, 4),
+    ({"dtype": 1, "ldk": 132}, 4), ({"n": 1 << 23}, 3), ({"n_tok": 1 << 29}, 3),
 ])
 def test_append_refusals(qh, change, code):
     assert append(qh, cache(qh), **change) == code
@@ -71,9 +71,9 @@ def test_append_refusals(qh, change, code):
 
 @pytest.mark.parametrize("change,code", [
     ({"layer": 2}, 1), ({"heads": 3}, 3), ({"heads": 0}, 3), ({"start": None}, 1), ({"causal": 2}, 1),
-    ({"scale": float("nan")}, 1), ({"scale": float("inf")}, 1), ({"dtype": 3}, 2), ({"q": None}, 1), ({"out": None}, 1),
+    ({"scale": float("nan")}, 1), ({"scale": float("inf")}, 1), ({"scale": -3e38}, 1), ({"dtype": 3}, 2), ({"q": None}, 1), ({"out": None}, 1),
     ({"ldq": 255}, 1), ({"ldo": 258}, 4), ({"out": C.c_void_p(4104)}, 4), ({"ws": None}, 6), ({"ws": C.c_void_p(4104)}, 4),
-    ({"n_tok": 1 << 30}, 3),
+    ({"n_tok": 1 << 30}, 3), ({"n": 1 << 24}, 3), ({"n_tok": 1 << 29, "n": 1}, 3), ({"out": P, "q": P}, 1),
 ])
 def test_attention_refusals(qh, change, code):
     assert attend(qh, cache(qh), **change) == code
@@ -118,3 +118,9 @@ def test_plain_model_rounds_as_the_definition_says():
     m.resize([0], [3])
     m.append(0, [0], [1], 2 * x[:1], x[:1])  # the scale doubles: 64 -> 32
     assert m.values(0, 0)[0][:, 0, 0].tolist() == [128.0, 64.0, 254.0]
+
+
+def test_decoder_refuses_a_cache_of_another_device(qh):
+    from types import SimpleNamespace as N
+    with pytest.raises(qh.QHError, match="decoder on cuda:0"):
+        qh.Decoder.bind_kv8(N(buf=N(device="cuda:0"), h=None), N(device="cuda:1"))
