@@ -71,21 +71,21 @@ struct Kv8Batch {
 
 // Work items of a ragged batch without a prefix sum: entry b's items begin at floor(start[b] * mul / unit) + pad * b,
 // which leaves every entry floor(rows * mul / unit) + pad of them at least. The entry of `item` (a wave calls it, all
-// lanes with one item; the start array is read 64 entries at a time): the last one that begins at or before it.
+// lanes with one item): the last one that begins at or before it, found 64 entries at a time, each round in the stretch
+// that the one before has left.
 __device__ __forceinline__ int kv8_entry_of(const Kv8Batch& q, int item, int mul, int unit, int pad, int* first) {
     const int lane = (int)threadIdx.x & 63;
-    int b = -1;
-    for (int base = 0; base < q.n; base += 64) {
-        const int i = base + lane;
-        const int key = i < q.n ? (int)((long)q.at(i) * mul / unit) + pad * i : 0x7fffffff;
+    for (int lo = 0, n = q.n;;) {
+        const int stride = (n + 63) >> 6, at = lane * stride, i = lo + at;
+        const int key = at < n ? (int)((long)q.at(i) * mul / unit) + pad * i : 0x7fffffff;
         const uint64_t m = __ballot(key <= item);
-        if (m == 0) break;
-        b = base + 63 - __builtin_clzll(m);
-        const int k = __builtin_amdgcn_readlane(key, b - base);
-        *first = k;
-        if (b < base + 63) break;
+        if (m == 0) return -1;
+        const int l = 63 - __builtin_clzll(m);
+        *first = __builtin_amdgcn_readlane(key, l);
+        if (stride <= 1) return lo + l;
+        lo += l * stride;
+        n = min(stride, n - l * stride);
     }
-    return __builtin_amdgcn_readfirstlane(b);
 }
 #endif
 

@@ -29,7 +29,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 constexpr int kTile = 64;            // positions of one step
 constexpr int kRowTile = 16;         // query rows of a workgroup of the row kernel
 constexpr int kMaxItems = 1024;      // row tiles of one launch of the row kernel
-constexpr int kWhole = 1024;         // positions up to which the row kernel takes a sequence whole
+constexpr int kWhole = 1024;         // positions up to which a workgroup takes a row tile's sequence whole
 constexpr int kMaxParts = 1024;      // shares of the row kernel: partial results of a row
 
 // Four codes as f16: the stored bytes, code + 128, under the high byte 0x64 are the numbers 1024 + 128 + code.
@@ -294,7 +294,6 @@ struct AttnArgs {
     float* part_ml;
     int4* rec;       // [items] where an item's partials are: first slot, how many (0: none), first row, rows
     int items, splits;
-    int least;  // tiles of a share of the row kernel at least, a multiple of four
 };
 
 // Entry b's rows: global rows (token * group + head) from first on, and the positions its tokens see.
@@ -342,23 +341,166 @@ __device__ __forceinline__ const T* q_row(const AttnArgs& a, const Kv8View& c, i
 
 // ------------------------------------------------------------------------------------------------ few rows
 
+// The waves of a workgroup meet here.
+template <int kC, int kW>
+struct RowsLds {
+    __align__(16) float so[kW][kRowTile][64 * kC + 4];
+    float sm[kW][kRowTile], sl[kW][kRowTile];
+};
+
+// The tiles [t0, t1) of one row tile, from row r0 of entry e, by a workgroup of kW waves: they take every kW-th tile, each
+// with its own running maximum, straight from global memory into registers (one contiguous KB a load, the next tile's
+// loads in flight while one is computed), and meet in shared memory at the end. whole: those are all tiles of the rows, and
+// the result goes to out, else into partial result `slot`.
+template <typename T, int kC, int kW>
+__device__ __forceinline__ void rows_tiles(const Kv8View& c, const AttnArgs& a, RowsLds<kC, kW>& sh, int kvh, const Entry& e,
+                                           int r0, int t0, int t1, bool whole, int slot) {
+    constexpr int kHd = 64 * kC;
+    const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4,
+              col = lane & 15;
+    const int r = r0 + col;
+    const bool valid = r < e.rows;
+    const int n_mine = t1 - t0 > wave ? (t1 - t0 - wave + kW - 1) / kW : 0;  // tiles t0 + wave + kW j
+    Blocks bl;
+    auto blocks = [&](int j) {
+        const int jl = j + (lane >> 2);
+        bl.load(c, e.seq, kvh, t0 + wave + kW * jl, jl < n_mine, e.len);
+    };
+    uint4 kr[4][kC], vr[4][kC];
+    auto fetch = [&](uint4 (&to)[4][kC], int which, int j) {
+        const int tile = t0 + wave + kW * j;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int page = bl.page_of(4 * (j & 15) + k), blk = (tile * 4 + k) & ((1 << (c.page_shift - 4)) - 1);
+            const uint4* p = reinterpret_cast<const uint4*>(kv8_codes(c, page, which, kvh, blk)) + lane;
+#pragma unroll
+            for (int cc = 0; cc < kC; ++cc) to[k][cc] = load_once(p + 64 * cc);
+        }
+    };
+    typename Query<T, kC>::Raw raw[kC][Query<T, kC>::kRaw];
+    blocks(0);
+    Query<T, kC>::fetch(raw, q_row<T>(a, c, e.row0 + (valid ? r : r0), kvh) + 16 * g);
+    if (n_mine > 0) {
+        fetch(kr, 0, 0);
+        fetch(vr, 1, 0);
+    }
+    const int vis = valid ? visible(e, a, r) : 0;
+    const int all_see = visible(e, a, r0);  // positions that every row sees: the first row's
+    Query<T, kC> q;
+    q.convert(raw, valid, a.scale_log2e);
+    Rows<T, kC> st;
+    st.clear();
+    Unit unit;
+
+    for (int j = 0; j < n_mine; ++j) {
+        const int pos0 = (t0 + wave + kW * j) * kTile, i0 = 4 * (j & 15);
+        const Scales sc = unit.next(bl, i0);
+        f4 x[4];
+        float f[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            f4 acc = {0, 0, 0, 0};
+#pragma unroll
+            for (int cc = 0; cc < kC; ++cc) {
+                acc = q.dot(codes8_to_f16(kr[k][cc].x, kr[k][cc].y), cc, 0, acc);
+                acc = q.dot(codes8_to_f16(kr[k][cc].z, kr[k][cc].w), cc, 1, acc);
+            }
+            x[k] = acc;
+            f[k] = sc.key[k] * q.unit;
+        }
+        // the next tile's keys are in flight from here on, its values from the end of the step
+        __builtin_amdgcn_sched_barrier(0);
+        const bool more = j + 1 < n_mine;
+        if (more) {
+            if (((j + 1) & 15) == 0) blocks(j + 1);
+            fetch(kr, 0, j + 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        h8 w[2], lo[2];
+        if (pos0 + kTile > all_see || sc.ok != 15u) st.mask(x, f, pos0 + 4 * g, vis, sc.ok);
+        if (sc.nan) st.poison(sc.nan, pos0, vis);
+        st.settle(x, f, sc.shrink);
+        st.weigh(x, f, sc.weight, w, lo);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int cc = 0; cc < kC; ++cc) {
+                const uint4 v0 = vr[2 * u][cc], v1 = vr[2 * u + 1][cc];
+                const uint32_t a0[4] = {v0.x, v0.y, v0.z, v0.w}, a1[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const h8 v = codes8_to_f16(a0[i], a1[i]);
+                    f4& o = st.o[4 * cc + i];
+                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[u], o, 0, 0, 0);
+                    if constexpr (Query<T, kC>::kSplit) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[u], o, 0, 0, 0);
+                }
+            }
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) fetch(vr, 1, j + 1);
+    }
+
+    // the waves' results of this item together
+    const float l = over_groups(st.l, [](float p, float q2) { return p + q2; });
+    const float back = unit.back();
+    if (g == 0) {
+        sh.sm[wave][col] = st.m;
+        sh.sl[wave][col] = l;
+    }
+#pragma unroll
+    for (int cc = 0; cc < kC; ++cc)
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            *reinterpret_cast<float4*>(&sh.so[wave][col][64 * cc + 16 * g + 4 * s]) =
+                make_float4(st.o[4 * cc][s] * back, st.o[4 * cc + 1][s] * back, st.o[4 * cc + 2][s] * back,
+                            st.o[4 * cc + 3][s] * back);
+    __syncthreads();
+    const int rr = (tid >> 4) & 15, d0 = 4 * (tid & 15);
+    if (r0 + rr < e.rows) {
+        float top = sh.sm[0][rr];
+#pragma unroll
+        for (int w2 = 1; w2 < kW; ++w2) top = __builtin_fmaxf(top, sh.sm[w2][rr]);
+        const float base = top == -__builtin_inff() ? 0.0f : top;
+        float f[kW], lsum = 0.0f;
+#pragma unroll
+        for (int w2 = 0; w2 < kW; ++w2) {
+            f[w2] = __builtin_amdgcn_exp2f(sh.sm[w2][rr] - base);
+            lsum = __builtin_fmaf(f[w2], sh.sl[w2][rr], lsum);
+        }
+        const size_t pr = ((size_t)slot * c.n_kv + kvh) * kRowTile + rr;
+        for (int cc = tid >> 8; cc < kC; cc += kW / 4) {
+            float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int w2 = 0; w2 < kW; ++w2) {
+                const float4 v = *reinterpret_cast<const float4*>(&sh.so[w2][rr][64 * cc + d0]);
+                o.x = __builtin_fmaf(f[w2], v.x, o.x);
+                o.y = __builtin_fmaf(f[w2], v.y, o.y);
+                o.z = __builtin_fmaf(f[w2], v.z, o.z);
+                o.w = __builtin_fmaf(f[w2], v.w, o.w);
+            }
+            if (whole)
+                store_out(out_row<T>(a, c, e.row0 + r0 + rr, kvh) + 64 * cc + d0, o, top, lsum);
+            else
+                *reinterpret_cast<float4*>(a.part_o + pr * kHd + 64 * cc + d0) = o;
+        }
+        if (!whole && tid < 256 && (tid & 15) == 0) {
+            a.part_ml[2 * pr] = top;
+            a.part_ml[2 * pr + 1] = lsum;
+        }
+    }
+}
+
 // Row tiles of 16 (single tokens: the query heads of one KV head) over long caches, bound by reading the codes. The
 // tiles of all items lie end to end, and each of the gridDim.x workgroups of a KV head takes an equal share of them,
 // whatever the lengths are: a share may end inside an item (the parts are joined by kv8_join_kernel) or span several.
-// Every workgroup finds its share from the lengths itself. Its four waves take every fourth tile of a share, each with
-// its own running maximum, straight from global memory into registers (one contiguous KB a load, the next tile's loads
-// in flight while one is computed), and meet in shared memory at the end of an item.
+// Every workgroup finds its share from the lengths itself.
 template <typename T, int kC>
 __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a) {
-    constexpr int kHd = 64 * kC, kPad = kHd + 4;
     __shared__ int pre[kMaxItems + 1];
     __shared__ uint16_t ent[kMaxItems];
     __shared__ Entry entries[kMaxItems];
     __shared__ int wave_sum[12];
-    __shared__ __align__(16) float so[4][kRowTile][kPad];
-    __shared__ float sm[4][kRowTile], sl[4][kRowTile];
-    const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4,
-              col = lane & 15;
+    __shared__ RowsLds<kC, 4> sh;
+    const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int kvh = (int)blockIdx.y, tiles_per_token = (a.group + kRowTile - 1) / kRowTile;
     auto first_item = [&](const Entry& e, int b) {
         return a.batch.start ? (int)((long)e.row0 / kRowTile) + b : b * tiles_per_token;
@@ -390,7 +532,7 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
     if (lane == 0) wave_sum[wave] = sum;
     __syncthreads();
     // a share is whole rounds of the four waves
-    const int share = max(a.least, ((wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3] + shares - 1) / shares + 3) & ~3);
+    const int share = max(4, ((wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3] + shares - 1) / shares + 3) & ~3);
     // items that begin on a share of their own where the shares suffice for that: no workgroup then has two items in turn
     int padded[kPer];
     sum = 0;
@@ -472,140 +614,26 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
         if (t0 >= t1) continue;  // only what pads the item
         const int b = __builtin_amdgcn_readfirstlane((int)ent[item]);
         const Entry e = uniform(entries[b]);
-        const int r0 = (item - first_item(e, b)) * kRowTile, r = r0 + col;
-        const bool valid = r < e.rows;
-        const int n_mine = t1 - t0 > wave ? (t1 - t0 - wave + 3) / 4 : 0;  // tiles t0 + wave + 4 j
-        Blocks bl;
-        auto blocks = [&](int j) {
-            const int jl = j + (lane >> 2);
-            bl.load(c, e.seq, kvh, t0 + wave + 4 * jl, jl < n_mine, e.len);
-        };
-        uint4 kr[4][kC], vr[4][kC];
-        auto fetch = [&](uint4 (&to)[4][kC], int which, int j) {
-            const int tile = t0 + wave + 4 * j;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int page = bl.page_of(4 * (j & 15) + k), blk = (tile * 4 + k) & ((1 << (c.page_shift - 4)) - 1);
-                const uint4* p = reinterpret_cast<const uint4*>(kv8_codes(c, page, which, kvh, blk)) + lane;
-#pragma unroll
-                for (int cc = 0; cc < kC; ++cc) to[k][cc] = load_once(p + 64 * cc);
-            }
-        };
-        typename Query<T, kC>::Raw raw[kC][Query<T, kC>::kRaw];
-        blocks(0);
-        Query<T, kC>::fetch(raw, q_row<T>(a, c, e.row0 + (valid ? r : r0), kvh) + 16 * g);
-        if (n_mine > 0) {
-            fetch(kr, 0, 0);
-            fetch(vr, 1, 0);
-        }
-        const int vis = valid ? visible(e, a, r) : 0;
-        const int all_see = visible(e, a, r0);  // positions that every row sees: the first row's
-        Query<T, kC> q;
-        q.convert(raw, valid, a.scale_log2e);
-        Rows<T, kC> st;
-        st.clear();
-        Unit unit;
-
-        for (int j = 0; j < n_mine; ++j) {
-            const int pos0 = (t0 + wave + 4 * j) * kTile, i0 = 4 * (j & 15);
-            const Scales sc = unit.next(bl, i0);
-            f4 x[4];
-            float f[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                f4 acc = {0, 0, 0, 0};
-#pragma unroll
-                for (int cc = 0; cc < kC; ++cc) {
-                    acc = q.dot(codes8_to_f16(kr[k][cc].x, kr[k][cc].y), cc, 0, acc);
-                    acc = q.dot(codes8_to_f16(kr[k][cc].z, kr[k][cc].w), cc, 1, acc);
-                }
-                x[k] = acc;
-                f[k] = sc.key[k] * q.unit;
-            }
-            // the next tile's keys are in flight from here on, its values from the end of the step
-            __builtin_amdgcn_sched_barrier(0);
-            const bool more = j + 1 < n_mine;
-            if (more) {
-                if (((j + 1) & 15) == 0) blocks(j + 1);
-                fetch(kr, 0, j + 1);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            h8 w[2], lo[2];
-            if (pos0 + kTile > all_see || sc.ok != 15u) st.mask(x, f, pos0 + 4 * g, vis, sc.ok);
-            if (sc.nan) st.poison(sc.nan, pos0, vis);
-            st.settle(x, f, sc.shrink);
-            st.weigh(x, f, sc.weight, w, lo);
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int cc = 0; cc < kC; ++cc) {
-                    const uint4 v0 = vr[2 * u][cc], v1 = vr[2 * u + 1][cc];
-                    const uint32_t a0[4] = {v0.x, v0.y, v0.z, v0.w}, a1[4] = {v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const h8 v = codes8_to_f16(a0[i], a1[i]);
-                        f4& o = st.o[4 * cc + i];
-                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[u], o, 0, 0, 0);
-                        if constexpr (Query<T, kC>::kSplit) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[u], o, 0, 0, 0);
-                    }
-                }
-            __builtin_amdgcn_sched_barrier(0);
-            if (more) fetch(vr, 1, j + 1);
-        }
-
-        // the four waves' results of this item together
-        const float l = over_groups(st.l, [](float p, float q2) { return p + q2; });
-        const float back = unit.back();
-        if (g == 0) {
-            sm[wave][col] = st.m;
-            sl[wave][col] = l;
-        }
-#pragma unroll
-        for (int cc = 0; cc < kC; ++cc)
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-                *reinterpret_cast<float4*>(&so[wave][col][64 * cc + 16 * g + 4 * s]) =
-                    make_float4(st.o[4 * cc][s] * back, st.o[4 * cc + 1][s] * back, st.o[4 * cc + 2][s] * back,
-                                st.o[4 * cc + 3][s] * back);
-        __syncthreads();
-        const int rr = tid >> 4, d0 = 4 * (tid & 15);
-        if (r0 + rr < e.rows) {
-            float top = sm[0][rr];
-#pragma unroll
-            for (int w2 = 1; w2 < 4; ++w2) top = __builtin_fmaxf(top, sm[w2][rr]);
-            const float base = top == -__builtin_inff() ? 0.0f : top;
-            float f[4], lsum = 0.0f;
-#pragma unroll
-            for (int w2 = 0; w2 < 4; ++w2) {
-                f[w2] = __builtin_amdgcn_exp2f(sm[w2][rr] - base);
-                lsum = __builtin_fmaf(f[w2], sl[w2][rr], lsum);
-            }
-            const bool whole = t0 == 0 && t1 == n_tiles;
-            const int slot = 2 * (int)blockIdx.x + (p0 + t0 > from ? 1 : 0);
-            const size_t pr = ((size_t)slot * c.n_kv + kvh) * kRowTile + rr;
-#pragma unroll
-            for (int cc = 0; cc < kC; ++cc) {
-                float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll
-                for (int w2 = 0; w2 < 4; ++w2) {
-                    const float4 v = *reinterpret_cast<const float4*>(&so[w2][rr][64 * cc + d0]);
-                    o.x = __builtin_fmaf(f[w2], v.x, o.x);
-                    o.y = __builtin_fmaf(f[w2], v.y, o.y);
-                    o.z = __builtin_fmaf(f[w2], v.z, o.z);
-                    o.w = __builtin_fmaf(f[w2], v.w, o.w);
-                }
-                if (whole)
-                    store_out(out_row<T>(a, c, e.row0 + r0 + rr, kvh) + 64 * cc + d0, o, top, lsum);
-                else
-                    *reinterpret_cast<float4*>(a.part_o + pr * kHd + 64 * cc + d0) = o;
-            }
-            if (!whole && (tid & 15) == 0) {
-                a.part_ml[2 * pr] = top;
-                a.part_ml[2 * pr + 1] = lsum;
-            }
-        }
+        rows_tiles<T, kC, 4>(c, a, sh, kvh, e, (item - first_item(e, b)) * kRowTile, t0, t1, t0 == 0 && t1 == n_tiles,
+                             2 * (int)blockIdx.x + (p0 + t0 > from ? 1 : 0));
         __syncthreads();
     }
+}
+
+// Row tiles over sequences of a few tiles: a workgroup each, with nothing to share out or to join. Bound by its dependent
+// loads: the entry, the length, pages, scales and then two or three tiles' codes (one token over 64 positions 4.5 us).
+template <typename T, int kC, int kW>
+__global__ __launch_bounds__(64 * kW, 2) void kv8_whole_kernel(Kv8View c, AttnArgs a) {
+    __shared__ RowsLds<kC, kW> sh;
+    const int kvh = (int)blockIdx.y, item = (int)blockIdx.x, tiles_per_token = (a.group + kRowTile - 1) / kRowTile;
+    int b = item / tiles_per_token, from = b * tiles_per_token;
+    if (a.batch.start) b = kv8_entry_of(a.batch, item, a.group, kRowTile, 1, &from);
+    if (b < 0) return;
+    const Entry e = uniform(entry_of(c, a, b));
+    const int r0 = (item - __builtin_amdgcn_readfirstlane(from)) * kRowTile;
+    if (r0 >= e.rows) return;
+    const int tiles = (visible(e, a, min(r0 + kRowTile, e.rows) - 1) + kTile - 1) / kTile;
+    rows_tiles<T, kC, kW>(c, a, sh, kvh, e, r0, 0, tiles, true, 0);
 }
 
 // Joins an item's partial results: one workgroup per item, KV head and row. First the partials' maxima, a thread to each,
@@ -924,37 +952,41 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
 // How a call is split: few rows to an entry take the row kernel (shares over all lengths), many the tile kernel.
 struct Plan {
     bool rows;
-    int entries;  // of a launch (the row kernel)
+    int entries;  // of a launch (single tokens)
     int items, shares, splits;
+    int waves;         // of the workgroup that takes a row tile's sequence whole; 0: shares
     int tile;          // rows of an item
     int join_rows;     // rows of an item that can have partial results; 0: none
-    int least;
     size_t part_rows;  // rows of partial results (per KV head)
     size_t bytes(int n_kv, int hd) const {
-        return sizeof(int4) * (size_t)items + sizeof(float) * part_rows * n_kv * (hd + 2);
+        return waves ? 0 : sizeof(int4) * (size_t)items + sizeof(float) * part_rows * n_kv * (hd + 2);
     }
 };
 // capacity: positions that a sequence can have.
 Plan plan_of(int group, int n_kv, int hd, int capacity, int n, int n_tok, bool single) {
     const long rows = (long)n_tok * group;
-    const long few = single ? (long)n * ((group + kRowTile - 1) / kRowTile) : rows / kRowTile + n;
+    const int tiles = (group + kRowTile - 1) / kRowTile;  // of a single token
+    const long few = single ? (long)n * tiles : rows / kRowTile + n;
     const int cus = device_cus();
+    // sequences whole up to 1,024 positions (one token, 14 heads of 64 over 2, f32: over 300 positions 6.1 us, in shares and
+    // joined 11.0; 1,024 7.9 and 11.1; 2,048 12.0 and 11.1; 32 heads of 128 over 8: 900 10.6 and 13.1, 2,048 16.4 and
+    // 13.2), and where their row tiles fill the GPU up to 2,048 (32 tokens of the latter, f16, over 2,048: 21.5 and 29.1;
+    // a batch of unlike lengths lasts as long as the longest one, and that no longer than the single one)
+    const bool whole = capacity <= kWhole || (capacity <= 2 * kWhole && few * n_kv >= cus);
+    const long most = whole ? (1 << 23) / n_kv : kMaxItems;  // row tiles of a launch
     Plan p{};
-    if ((single || few <= kMaxItems) && rows <= 32l * n) {
-        // single tokens in launches of as many entries as make kMaxItems row tiles (2,048 sequences of 2,000, 32 heads of
-        // 128 over 8, f16: 1,328 us, by the tile kernel 2,803; 14 heads of 64 over 2: 221 and 335)
+    if ((single || few <= most) && rows <= 32l * n) {
+        // single tokens in launches of as many entries as make that many row tiles (shares: 2,048 sequences of 2,000, 32
+        // heads of 128 over 8, f16: 1,328 us, by the tile kernel 2,803; 14 heads of 64 over 2: 221 and 335)
         p.rows = true;
-        const int tiles = (group + kRowTile - 1) / kRowTile, most = kMaxItems / tiles;
-        p.entries = single && n > most ? most : n;
+        p.entries = single && few > most ? (int)(most / tiles) : n;
         p.items = single ? p.entries * tiles : (int)few;
         p.splits = 1;
         p.tile = kRowTile;
-        p.least = 4;
-        if (capacity <= kWhole) {
-            // every item fits one share: a workgroup each, and nothing to join (one token, 14 heads over 2 of 64, f32: over
-            // 300 positions 8.0 us, split and joined 10.9; 600 9.2 and 11.0; 1,024 10.6 and 10.9)
-            p.shares = p.items;
-            p.least = (capacity / kTile + 4) & ~3;
+        if (whole) {
+            // 8 waves share a tile's sequence where there is a compute unit for each (32 tokens as above over 1,024: 11.8
+            // us, 4 waves 13.9; 64 tokens 24.6 and 21.9; 2,000 over 100 275 and 120)
+            p.waves = (long)p.items * n_kv <= cus ? 8 : 4;
             return p;
         }
         p.shares = (2 * cus + n_kv - 1) / n_kv;
@@ -971,9 +1003,9 @@ Plan plan_of(int group, int n_kv, int hd, int capacity, int n, int n_tok, bool s
     const long wgs = (long)p.items * n_kv;
     // splits for two workgroups to a compute unit, but none of fewer than four tiles
     p.splits = wgs >= cus ? 1 : (int)((2 * cus + wgs - 1) / wgs);
-    const int most = capacity / (4 * kTile);
+    const int most_splits = capacity / (4 * kTile);
     if (p.splits > 16) p.splits = 16;
-    if (p.splits > most) p.splits = most > 1 ? most : 1;
+    if (p.splits > most_splits) p.splits = most_splits > 1 ? most_splits : 1;
     p.join_rows = p.splits > 1 ? p.tile : 0;
     p.part_rows = p.splits > 1 ? (size_t)p.items * p.splits * p.tile : 0;
     return p;
@@ -988,7 +1020,7 @@ size_t kv8_attention_workspace_bytes(int n_heads, int n_kv, int hd, int capacity
         const size_t single = plan_of(group, n_kv, hd, capacity, n, n_tok, true).bytes(n_kv, hd);
         b = b > single ? b : single;
     }
-    return b;
+    return b > 16 ? b : 16;
 }
 
 hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int dtype, int n_heads, int64_t ldq,
@@ -1006,7 +1038,6 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
     const Plan p = plan_of(a.group, c.n_kv, c.hd, c.seq_pages << c.page_shift, n, n_tok, start == nullptr);
     a.items = p.items;
     a.splits = p.splits;
-    a.least = p.least;
     a.rec = static_cast<int4*>(ws);
     a.part_o = reinterpret_cast<float*>(a.rec + p.items);
     a.part_ml = a.part_o + p.part_rows * c.n_kv * c.hd;
@@ -1014,7 +1045,7 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
         using T = std::remove_pointer_t<decltype(t)>;
         constexpr int kC = decltype(kc)::value;
         if (p.rows) {
-            const int tiles = p.items / p.entries;  // of a single token
+            const int tiles = (a.group + kRowTile - 1) / kRowTile;
             for (int b = 0; b < n; b += p.entries) {
                 a.q = static_cast<const T*>(q) + (int64_t)b * ldq;  // only single tokens take more than one launch
                 a.out = static_cast<T*>(out) + (int64_t)b * ldo;
@@ -1023,7 +1054,12 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
                     a.batch = Kv8Batch{nullptr, seqs ? seqs + b : nullptr, m, m, b};
                     a.items = m * tiles;
                 }
-                qh_launch((kv8_rows_kernel<T, kC>), dim3((unsigned)p.shares, (unsigned)c.n_kv), dim3(256), 0, s, c, a);
+                if (p.waves == 8)
+                    qh_launch((kv8_whole_kernel<T, kC, 8>), dim3((unsigned)a.items, (unsigned)c.n_kv), dim3(512), 0, s, c, a);
+                else if (p.waves == 4)
+                    qh_launch((kv8_whole_kernel<T, kC, 4>), dim3((unsigned)a.items, (unsigned)c.n_kv), dim3(256), 0, s, c, a);
+                else
+                    qh_launch((kv8_rows_kernel<T, kC>), dim3((unsigned)p.shares, (unsigned)c.n_kv), dim3(256), 0, s, c, a);
                 if (p.join_rows)
                     qh_launch((kv8_join_kernel<T, kC>), dim3((unsigned)a.items, (unsigned)c.n_kv, (unsigned)p.join_rows),
                               dim3(256), 0, s, c, a);

@@ -388,12 +388,14 @@ def test_many_sequences(qh):
     check_attention(c, rng, list(range(1000)), [1] * 1000, 2, "float32")
 
 
-def test_many_sequences_of_unlike_lengths(qh):
-    """The same where sequences are split and joined, with two row tiles to an entry, in and out of order."""
+@pytest.mark.parametrize("longest", [1100, 2100])
+def test_many_sequences_of_unlike_lengths(qh, longest):
+    """The same for long sequences, whole and in shares that are joined, with two row tiles to an entry, in and out of
+    order."""
     import torch
     rng = np.random.default_rng(SEED)
     lens = [int(x) for x in rng.integers(0, 20, 530)]
-    lens[3], lens[511], lens[512], lens[529] = 1100, 700, 1030, 65
+    lens[3], lens[511], lens[512], lens[529] = longest, 700, 1030, 65
     c = filled(qh, rng, lens, 1, 64, 16, "float32")
     check_attention(c, rng, [int(x) for x in rng.permutation(530)], [1] * 530, 17, "float32", single=True)
     q = torch.from_numpy(rng.standard_normal((530, 17, 64)).astype(np.float32)).to("cuda")
