@@ -30,7 +30,8 @@ constexpr int kTile = 64;            // positions of one step
 constexpr int kRowTile = 16;         // query rows of a workgroup of the row kernel
 constexpr int kMaxItems = 1024;      // row tiles of one launch of the row kernel
 constexpr int kWhole = 1024;         // positions up to which a workgroup takes a row tile's sequence whole
-constexpr int kMaxParts = 1024;      // shares of the row kernel: partial results of a row
+constexpr int kSplitTiles = 5;       // positions of a split of the tile kernel, in tiles, at least
+constexpr int kMaxParts = 512;       // shares of the row kernel: partial results of a row
 
 // Four codes as f16: the stored bytes, code + 128, under the high byte 0x64 are the numbers 1024 + 128 + code.
 __device__ __forceinline__ void codes_to_f16(uint32_t x, uint32_t* out) {
@@ -493,23 +494,34 @@ __device__ __forceinline__ void rows_tiles(const Kv8View& c, const AttnArgs& a, 
 // tiles of all items lie end to end, and each of the gridDim.x workgroups of a KV head takes an equal share of them,
 // whatever the lengths are: a share may end inside an item (the parts are joined by kv8_join_kernel) or span several.
 // Every workgroup finds its share from the lengths itself.
-template <typename T, int kC>
-__global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a) {
-    __shared__ int pre[kMaxItems + 1];
-    __shared__ uint16_t ent[kMaxItems];
-    __shared__ Entry entries[kMaxItems];
-    __shared__ int wave_sum[12];
-    __shared__ RowsLds<kC, 4> sh;
+template <typename T, int kC, int kW>
+__global__ __launch_bounds__(64 * kW, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a) {
+    __shared__ int pre_all[kMaxItems + 1];
+    __shared__ uint16_t ent_all[kMaxItems];
+    __shared__ Entry entries_all[kMaxItems];
+    __shared__ int wave_sum[3 * kW];
+    __shared__ RowsLds<kC, kW> sh;
     const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int kvh = (int)blockIdx.y, tiles_per_token = (a.group + kRowTile - 1) / kRowTile;
+    const int kvh = (int)blockIdx.y, tiles_per_token = (a.group + kRowTile - 1) / kRowTile, shares = (int)gridDim.x;
     auto first_item = [&](const Entry& e, int b) {
         return a.batch.start ? (int)((long)e.row0 / kRowTile) + b : b * tiles_per_token;
     };
+    // up to 64 items each wave works the shares out for itself, without a barrier (one token over 100,000 positions, 12
+    // heads of 128 over 2, f32: 24.3 us, by the workgroup 25.3)
+    const bool alone = a.items <= 64;
+    int* pre = pre_all + (alone ? 65 * wave : 0);
+    uint16_t* ent = ent_all + (alone ? 64 * wave : 0);
+    Entry* entries = entries_all + (alone ? 64 * wave : 0);
+    const int me = alone ? lane : tid, width = alone ? 64 : 64 * kW;
+    auto meet = [&] {
+        if (alone) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        else __syncthreads();
+    };
 
     // the items' tile counts, then their prefix sums
-    for (int i = tid; i < a.items; i += 256) pre[i] = 0;
-    __syncthreads();
-    for (int b = tid; b < a.batch.n; b += 256) {
+    for (int i = me; i < a.items; i += width) pre[i] = 0;
+    meet();
+    for (int b = me; b < a.batch.n; b += width) {
         const Entry e = entry_of(c, a, b);
         entries[b] = e;
         const int at = first_item(e, b);
@@ -519,20 +531,28 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
             ent[at + t] = (uint16_t)b;
         }
     }
-    __syncthreads();
-    constexpr int kPer = kMaxItems / 256;
-    const int shares = (int)gridDim.x;
+    meet();
+    constexpr int kPer = kMaxItems / (64 * kW);
+    const int per = alone ? 1 : kPer;
     int mine[kPer], sum = 0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-        mine[j] = tid * kPer + j < a.items ? pre[tid * kPer + j] : 0;
+        mine[j] = j < per && me * per + j < a.items ? pre[me * per + j] : 0;
         sum += mine[j];
     }
-    sum = wave_sum_i32(sum);
-    if (lane == 0) wave_sum[wave] = sum;
-    __syncthreads();
-    // a share is whole rounds of the four waves
-    const int share = max(4, ((wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3] + shares - 1) / shares + 3) & ~3);
+    auto all_of = [&](int v, int* s) {  // the sum over the workgroup, or the wave that is alone
+        v = wave_sum_i32(v);
+        if (alone) return v;
+        if (lane == 0) s[wave] = v;
+        __syncthreads();
+        v = 0;
+#pragma unroll
+        for (int i = 0; i < kW; ++i) v += s[i];
+        return v;
+    };
+    // a tile to each wave at least, but no whole rounds of them (48 conversations of 2,500, 32 heads of 128 over 8, f16:
+    // 46.8 us, in whole rounds 48.2)
+    const int share = max(kW, (all_of(sum, wave_sum) + shares - 1) / shares);
     // items that begin on a share of their own where the shares suffice for that: no workgroup then has two items in turn
     int padded[kPer];
     sum = 0;
@@ -541,10 +561,7 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
         padded[j] = (mine[j] + share - 1) / share * share;
         sum += padded[j];
     }
-    sum = wave_sum_i32(sum);
-    if (lane == 0) wave_sum[4 + wave] = sum;
-    __syncthreads();
-    const bool apart = wave_sum[4] + wave_sum[5] + wave_sum[6] + wave_sum[7] <= shares * share;
+    const bool apart = all_of(sum, wave_sum + kW) <= shares * share;
     sum = 0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) sum += apart ? padded[j] : mine[j];
@@ -554,21 +571,24 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
         const int y = __shfl_up(incl, s);
         incl += lane >= s ? y : 0;
     }
-    if (lane == 63) wave_sum[8 + wave] = incl;
-    __syncthreads();
-    int at = incl - sum, total = 0;
+    int at = incl - sum, total = __builtin_amdgcn_readlane(incl, 63);
+    if (!alone) {
+        if (lane == 63) wave_sum[2 * kW + wave] = incl;
+        __syncthreads();
+        total = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        at += i < wave ? wave_sum[8 + i] : 0;
-        total += wave_sum[8 + i];
+        for (int i = 0; i < kW; ++i) {
+            at += i < wave ? wave_sum[2 * kW + i] : 0;
+            total += wave_sum[2 * kW + i];
+        }
     }
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-        if (tid * kPer + j < a.items) pre[tid * kPer + j] = at;
+        if (j < per && me * per + j < a.items) pre[me * per + j] = at;
         at += apart ? padded[j] : mine[j];
     }
-    if (tid == 0) pre[a.items] = total;
-    __syncthreads();
+    if (me == 0) pre[a.items] = total;
+    meet();
 
     // tiles of an item: its own, without what pads it
     auto tiles_of = [&](int i) {
@@ -577,12 +597,13 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
         return max(1, (visible(e, a, r1) + kTile - 1) / kTile);
     };
     if (blockIdx.x == 0 && kvh == 0) {
-        for (int i = tid; i < a.items; i += 256) {
+        for (int i = tid; i < a.items; i += 64 * kW) {
             int4 r = make_int4(0, 0, 0, 0);
             if (pre[i + 1] > pre[i]) {
                 const int b = ent[i];
                 const Entry e = entries[b];
-                const int t = i - first_item(e, b), w0 = pre[i] / share, w1 = (min(pre[i] + tiles_of(i), pre[i + 1]) - 1) / share;
+                const int t = i - first_item(e, b), end = min(pre[i] + tiles_of(i), pre[i + 1]);
+                const int w0 = pre[i] / share, w1 = (end - 1) / share;
                 r = make_int4(2 * w0 + (pre[i] > w0 * share ? 1 : 0), w1 > w0 ? w1 - w0 + 1 : 0, e.row0 + t * kRowTile,
                               min(kRowTile, e.rows - t * kRowTile));
             }
@@ -614,8 +635,8 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(Kv8View c, AttnArgs a)
         if (t0 >= t1) continue;  // only what pads the item
         const int b = __builtin_amdgcn_readfirstlane((int)ent[item]);
         const Entry e = uniform(entries[b]);
-        rows_tiles<T, kC, 4>(c, a, sh, kvh, e, (item - first_item(e, b)) * kRowTile, t0, t1, t0 == 0 && t1 == n_tiles,
-                             2 * (int)blockIdx.x + (p0 + t0 > from ? 1 : 0));
+        rows_tiles<T, kC, kW>(c, a, sh, kvh, e, (item - first_item(e, b)) * kRowTile, t0, t1, t0 == 0 && t1 == n_tiles,
+                              2 * (int)blockIdx.x + (p0 + t0 > from ? 1 : 0));
         __syncthreads();
     }
 }
@@ -734,7 +755,7 @@ __global__ __launch_bounds__(256) void kv8_join_splits_kernel(Kv8View c, AttnArg
 // conflicts), in two buffers: one barrier a tile, the next tile's codes converted between the matrix instructions of this
 // one and the one after that in flight. The KV head is the fastest grid index, so that the workgroups of one head share an
 // XCD's L2 where there are eight heads, and the last row tiles (which see the most positions) start first. splits > 1:
-// that many workgroups share a row tile's positions and leave partials.
+// up to that many workgroups share a row tile's positions and leave partials.
 template <typename T, int kC, int kCt>
 __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a) {
     constexpr int kHd = 64 * kC, kW = 4, kRows = 16 * kW * kCt;
@@ -749,13 +770,16 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
     Entry e{0, 0, 0, 0, 0};
     if (b >= 0) e = uniform(entry_of(c, a, b));
     const int r0 = b < 0 ? 0 : (item - __builtin_amdgcn_readfirstlane(from)) * kRows;
-    if (a.splits > 1 && split == 0 && kvh == 0 && tid == 0)
-        a.rec[item] = r0 < e.rows ? make_int4(item * a.splits, a.splits, e.row0 + r0, min(kRows, e.rows - r0))
-                                  : make_int4(0, 0, 0, 0);
-    if (r0 >= e.rows) return;
     const int last = min(r0 + kRows, e.rows) - 1;
-    const int tiles = (visible(e, a, last) + kTile - 1) / kTile;
-    const int t0 = (int)((long)tiles * split / a.splits), t1 = (int)((long)tiles * (split + 1) / a.splits);
+    const int tiles = r0 < e.rows ? (visible(e, a, last) + kTile - 1) / kTile : 0;
+    // The splits that this item takes, of at least five tiles: the join moves the rows' outputs twice in f32 (14 heads of
+    // 64 over 2, f32: a prompt of 512 whole 17.3 us, in two splits 17.8; 4 x 120 behind 580 21.7 and 18.3; 256 tokens of
+    // 32 heads of 128 over 8, f16, whole 12.1, a tile to a split 21.2)
+    const int splits = min(a.splits, max(tiles / kSplitTiles, 1));
+    if (a.splits > 1 && split == 0 && kvh == 0 && tid == 0)
+        a.rec[item] = splits > 1 ? make_int4(item * a.splits, splits, e.row0 + r0, last + 1 - r0) : make_int4(0, 0, 0, 0);
+    if (r0 >= e.rows || split >= splits) return;
+    const int t0 = tiles * split / splits, t1 = tiles * (split + 1) / splits;
 
     Query<T, kC> q[kCt];
     Rows<T, kC> st[kCt];
@@ -935,12 +959,12 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
                 const float4 o = make_float4(st[ct].o[4 * cc][s] * back, st[ct].o[4 * cc + 1][s] * back,
                                              st[ct].o[4 * cc + 2][s] * back, st[ct].o[4 * cc + 3][s] * back);
                 const int d = 64 * cc + 16 * g + 4 * s;
-                if (a.splits == 1)
+                if (splits == 1)
                     store_out(out + d, o, st[ct].m, l);
                 else
                     *reinterpret_cast<float4*>(a.part_o + pr * kHd + d) = o;
             }
-        if (a.splits > 1 && g == 0) {
+        if (splits > 1 && g == 0) {
             a.part_ml[2 * pr] = st[ct].m;
             a.part_ml[2 * pr + 1] = l;
         }
@@ -954,12 +978,13 @@ struct Plan {
     bool rows;
     int entries;  // of a launch (single tokens)
     int items, shares, splits;
-    int waves;         // of the workgroup that takes a row tile's sequence whole; 0: shares
+    bool whole;        // a workgroup to a row tile, else shares
+    int waves;         // of a workgroup of the row kernels
     int tile;          // rows of an item
     int join_rows;     // rows of an item that can have partial results; 0: none
     size_t part_rows;  // rows of partial results (per KV head)
     size_t bytes(int n_kv, int hd) const {
-        return waves ? 0 : sizeof(int4) * (size_t)items + sizeof(float) * part_rows * n_kv * (hd + 2);
+        return whole ? 0 : sizeof(int4) * (size_t)items + sizeof(float) * part_rows * n_kv * (hd + 2);
     }
 };
 // capacity: positions that a sequence can have.
@@ -969,9 +994,9 @@ Plan plan_of(int group, int n_kv, int hd, int capacity, int n, int n_tok, bool s
     const long few = single ? (long)n * tiles : rows / kRowTile + n;
     const int cus = device_cus();
     // sequences whole up to 1,024 positions (one token, 14 heads of 64 over 2, f32: over 300 positions 6.1 us, in shares and
-    // joined 11.0; 1,024 7.9 and 11.1; 2,048 12.0 and 11.1; 32 heads of 128 over 8: 900 10.6 and 13.1, 2,048 16.4 and
-    // 13.2), and where their row tiles fill the GPU up to 2,048 (32 tokens of the latter, f16, over 2,048: 21.5 and 29.1;
-    // a batch of unlike lengths lasts as long as the longest one, and that no longer than the single one)
+    // joined 9.2; 1,024 8.0 and 10.7; 2,048 12.1 and 10.7; 32 heads of 128 over 8: 900 10.9 and 13.0, 2,048 16.5 and
+    // 12.8), and where their row tiles fill the GPU up to 2,048 (32 tokens of the latter, f16, over 2,048: 22.0 and 25.8; a
+    // batch of unlike lengths lasts as long as its longest, and that no longer than the single one)
     const bool whole = capacity <= kWhole || (capacity <= 2 * kWhole && few * n_kv >= cus);
     const long most = whole ? (1 << 23) / n_kv : kMaxItems;  // row tiles of a launch
     Plan p{};
@@ -983,13 +1008,14 @@ Plan plan_of(int group, int n_kv, int hd, int capacity, int n, int n_tok, bool s
         p.items = single ? p.entries * tiles : (int)few;
         p.splits = 1;
         p.tile = kRowTile;
-        if (whole) {
-            // 8 waves share a tile's sequence where there is a compute unit for each (32 tokens as above over 1,024: 11.8
-            // us, 4 waves 13.9; 64 tokens 24.6 and 21.9; 2,000 over 100 275 and 120)
-            p.waves = (long)p.items * n_kv <= cus ? 8 : 4;
-            return p;
-        }
-        p.shares = (2 * cus + n_kv - 1) / n_kv;
+        // 8 waves to a workgroup while there is a compute unit for each row tile and KV head. Whole: 32 tokens as above over
+        // 1,024 11.8 us, by 4 waves 13.9; 64 tokens 24.6 and 21.9; 2,000 over 100 275 and 120. Shares (one workgroup to a
+        // compute unit, half the partial results): 32 over 4,096 46.8 and 51.4; 48 over 2,500 45.3 and 46.8; but 40 over up
+        // to 300 23.5 and 12.0, 500 over 100 75 and 53
+        p.waves = (long)p.items * n_kv <= cus ? 8 : 4;
+        p.whole = whole;
+        if (whole) return p;
+        p.shares = ((p.waves == 8 ? 1 : 2) * cus + n_kv - 1) / n_kv;
         if (p.shares > kMaxParts) p.shares = kMaxParts;
         p.join_rows = single && group < kRowTile ? group : kRowTile;
         p.part_rows = 2 * (size_t)p.shares * kRowTile;
@@ -1001,9 +1027,10 @@ Plan plan_of(int group, int n_kv, int hd, int capacity, int n, int n_tok, bool s
     p.tile = hd == 128 && rows / 128 * n_kv >= cus ? 128 : 64;
     p.items = (int)(rows / p.tile + n);
     const long wgs = (long)p.items * n_kv;
-    // splits for two workgroups to a compute unit, but none of fewer than four tiles
-    p.splits = wgs >= cus ? 1 : (int)((2 * cus + wgs - 1) / wgs);
-    const int most_splits = capacity / (4 * kTile);
+    // splits for two workgroups to a compute unit and no more, which would run after the others (100 tokens behind 8,000,
+    // 32 heads of 128 over 8, f16: 43.5 us, rounded up 57.9)
+    p.splits = wgs >= cus ? 1 : (int)(2 * cus / wgs);
+    const int most_splits = capacity / (kSplitTiles * kTile);
     if (p.splits > 16) p.splits = 16;
     if (p.splits > most_splits) p.splits = most_splits > 1 ? most_splits : 1;
     p.join_rows = p.splits > 1 ? p.tile : 0;
@@ -1054,12 +1081,11 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
                     a.batch = Kv8Batch{nullptr, seqs ? seqs + b : nullptr, m, m, b};
                     a.items = m * tiles;
                 }
-                if (p.waves == 8)
-                    qh_launch((kv8_whole_kernel<T, kC, 8>), dim3((unsigned)a.items, (unsigned)c.n_kv), dim3(512), 0, s, c, a);
-                else if (p.waves == 4)
-                    qh_launch((kv8_whole_kernel<T, kC, 4>), dim3((unsigned)a.items, (unsigned)c.n_kv), dim3(256), 0, s, c, a);
-                else
-                    qh_launch((kv8_rows_kernel<T, kC>), dim3((unsigned)p.shares, (unsigned)c.n_kv), dim3(256), 0, s, c, a);
+                const dim3 grid((unsigned)(p.whole ? a.items : p.shares), (unsigned)c.n_kv);
+                if (p.whole && p.waves == 8) qh_launch((kv8_whole_kernel<T, kC, 8>), grid, dim3(512), 0, s, c, a);
+                else if (p.whole) qh_launch((kv8_whole_kernel<T, kC, 4>), grid, dim3(256), 0, s, c, a);
+                else if (p.waves == 8) qh_launch((kv8_rows_kernel<T, kC, 8>), grid, dim3(512), 0, s, c, a);
+                else qh_launch((kv8_rows_kernel<T, kC, 4>), grid, dim3(256), 0, s, c, a);
                 if (p.join_rows)
                     qh_launch((kv8_join_kernel<T, kC>), dim3((unsigned)a.items, (unsigned)c.n_kv, (unsigned)p.join_rows),
                               dim3(256), 0, s, c, a);

@@ -125,6 +125,21 @@ def test_append_many_entries(qh, n_entries):
     c.check_values(0)
 
 
+def test_thousands_of_entries(qh):
+    """Entry lookup past 64 x 64 entries, some without rows, by append, read and attention."""
+    rng = np.random.default_rng(SEED)
+    n = 4200
+    counts = [int(x) for x in rng.choice([0, 1, 2, 17], n, p=[.3, .4, .29, .01])]
+    c = Pair(qh, 1, n + 60, 16, 1, 64, n, 2)
+    seqs = [int(x) for x in rng.permutation(n)]
+    c.resize(seqs, counts)
+    c.append(rng, 0, seqs, counts, "float32")
+    check_attention(c, rng, seqs, counts, 2, "float32")
+    c.check_values(0)
+    # few entries with rows among many without
+    check_attention(c, rng, seqs, [0] * (n - 3) + [100, 0, 40], 2, "float32", causal=False)
+
+
 def test_append_extreme_values(qh):
     """Zeros, the largest and the smallest numbers, halves between codes, infinities and NaN: the block of the head reads
     as NaN, the others are untouched by it."""
