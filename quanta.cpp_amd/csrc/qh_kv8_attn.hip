@@ -14,6 +14,7 @@
 //   f16 calls round each weight to f16 once, half an ulp of the result's own type, in errors that average out over the
 //   positions. A weight carries the value scale of its block divided by a running power of two at least as large as all
 //   of them, times 2^6, so that small weights stay clear of f16's subnormals and large ones of its infinity.
+#include <algorithm>
 #include <type_traits>
 
 #include "qh_device.h"
@@ -755,14 +756,16 @@ __global__ __launch_bounds__(256) void kv8_join_splits_kernel(Kv8View c, AttnArg
 // conflicts), in two buffers: one barrier a tile, the next tile's codes converted between the matrix instructions of this
 // one and the one after that in flight. The KV head is the fastest grid index, so that the workgroups of one head share an
 // XCD's L2 where there are eight heads, and the last row tiles (which see the most positions) start first. splits > 1:
-// up to that many workgroups share a row tile's positions and leave partials.
-template <typename T, int kC, int kCt>
-__global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a) {
+// up to that many workgroups share a row tile's positions and leave partials. kG groups of four waves share a workgroup's
+// positions, each with buffers of its own, and meet in shared memory at the end.
+template <typename T, int kC, int kCt, int kG>
+__global__ __launch_bounds__(256 * kG, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a) {
     constexpr int kHd = 64 * kC, kW = 4, kRows = 16 * kW * kCt;
     constexpr int kUnits = 4 * kC * 2 * 64;  // 16-byte units of a tile's keys (and values) in f16
-    extern __shared__ __align__(16) uint4 lds[];  // [buffer][keys, values][kUnits]
-    const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4,
-              col = lane & 15;
+    extern __shared__ __align__(16) uint4 lds_all[];  // [group][buffer][keys, values][kUnits]
+    const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3,
+              grp = __builtin_amdgcn_readfirstlane(tid >> 8), lane = tid & 63, g = lane >> 4, col = lane & 15;
+    uint4* lds = lds_all + grp * 4 * kUnits;
     const int kvh = (int)(blockIdx.x % (unsigned)c.n_kv), split = (int)blockIdx.y;
     const int item = a.items - 1 - (int)(blockIdx.x / (unsigned)c.n_kv);
     int from = 0, b = item;
@@ -779,7 +782,8 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
     if (a.splits > 1 && split == 0 && kvh == 0 && tid == 0)
         a.rec[item] = splits > 1 ? make_int4(item * a.splits, splits, e.row0 + r0, last + 1 - r0) : make_int4(0, 0, 0, 0);
     if (r0 >= e.rows || split >= splits) return;
-    const int t0 = tiles * split / splits, t1 = tiles * (split + 1) / splits;
+    const int first = tiles * split / splits, end = tiles * (split + 1) / splits;  // the workgroup's tiles
+    const int steps = (end - first + kG - 1) / kG, t0 = first + grp * steps, t1 = min(t0 + steps, end);  // the group's
 
     Query<T, kC> q[kCt];
     Rows<T, kC> st[kCt];
@@ -936,19 +940,49 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
         bl = ahead;
         stage(0);
         if (t0 + 1 < t1) fetch(t0 + 1);
-        for (int t = t0; t < t1; ++t) {
-            __syncthreads();  // tile t is staged, and tile t - 1 (whose buffer comes next) has been read
-            if (t > t0 && ((t - t0) & 15) == 0) bl = ahead;
-            compute((t - t0) & 1, t);  // past the last tile it stages what it has once more, for nobody
-        }
-        __builtin_amdgcn_s_setprio(0);
     }
+    for (int t = t0; t < t0 + steps; ++t) {
+        __syncthreads();  // tile t is staged, and tile t - 1 (whose buffer comes next) has been read
+        if (kG > 1 && t >= t1) continue;
+        if (t > t0 && ((t - t0) & 15) == 0) bl = ahead;
+        compute((t - t0) & 1, t);  // past the last tile it stages what it has once more, for nobody
+    }
+    __builtin_amdgcn_s_setprio(0);
 
-    const float back = unit.back();
+    float back = unit.back();
+#pragma unroll
+    for (int ct = 0; ct < kCt; ++ct) st[ct].l = over_groups(st[ct].l, [](float p, float q2) { return p + q2; });
+    if constexpr (kG == 2) {
+        // the second group's results to the first
+        f4* so = reinterpret_cast<f4*>(lds_all) + (tid & 255);
+        float* ml = reinterpret_cast<float*>(lds_all + kCt * 4 * kC * 256) + (tid & 255);
+        __syncthreads();
+        if (grp == 1) {
+#pragma unroll
+            for (int ct = 0; ct < kCt; ++ct) {
+#pragma unroll
+                for (int n = 0; n < 4 * kC; ++n) so[(ct * 4 * kC + n) * 256] = st[ct].o[n] * back;
+                ml[512 * ct] = st[ct].m;
+                ml[512 * ct + 256] = st[ct].l;
+            }
+        }
+        __syncthreads();
+        if (grp == 1) return;
+#pragma unroll
+        for (int ct = 0; ct < kCt; ++ct) {
+            const float m1 = ml[512 * ct], top = __builtin_fmaxf(st[ct].m, m1);
+            const float base = top == -__builtin_inff() ? 0.0f : top;
+            const float f0 = __builtin_amdgcn_exp2f(st[ct].m - base), f1 = __builtin_amdgcn_exp2f(m1 - base);
+            st[ct].l = f0 * st[ct].l + f1 * ml[512 * ct + 256];
+#pragma unroll
+            for (int n = 0; n < 4 * kC; ++n) st[ct].o[n] = st[ct].o[n] * (back * f0) + so[(ct * 4 * kC + n) * 256] * f1;
+            st[ct].m = top;
+        }
+        back = 1.0f;
+    }
 #pragma unroll
     for (int ct = 0; ct < kCt; ++ct) {
         const int rr = wave * (16 * kCt) + ct * 16 + col, r = r0 + rr;
-        const float l = over_groups(st[ct].l, [](float p, float q2) { return p + q2; });
         if (r >= e.rows) continue;
         const size_t pr = ((size_t)(item * a.splits + split) * c.n_kv + kvh) * kRows + rr;
         T* out = out_row<T>(a, c, e.row0 + r, kvh);
@@ -960,13 +994,13 @@ __global__ __launch_bounds__(256, 2) void kv8_tile_kernel(Kv8View c, AttnArgs a)
                                              st[ct].o[4 * cc + 2][s] * back, st[ct].o[4 * cc + 3][s] * back);
                 const int d = 64 * cc + 16 * g + 4 * s;
                 if (splits == 1)
-                    store_out(out + d, o, st[ct].m, l);
+                    store_out(out + d, o, st[ct].m, st[ct].l);
                 else
                     *reinterpret_cast<float4*>(a.part_o + pr * kHd + d) = o;
             }
         if (splits > 1 && g == 0) {
             a.part_ml[2 * pr] = st[ct].m;
-            a.part_ml[2 * pr + 1] = l;
+            a.part_ml[2 * pr + 1] = st[ct].l;
         }
     }
 }
@@ -981,6 +1015,7 @@ struct Plan {
     bool whole;        // a workgroup to a row tile, else shares
     int waves;         // of a workgroup of the row kernels
     int tile;          // rows of an item
+    int groups;        // of four waves to a workgroup of the tile kernel
     int join_rows;     // rows of an item that can have partial results; 0: none
     size_t part_rows;  // rows of partial results (per KV head)
     size_t bytes(int n_kv, int hd) const {
@@ -1027,12 +1062,18 @@ Plan plan_of(int group, int n_kv, int hd, int capacity, int n, int n_tok, bool s
     p.tile = hd == 128 && rows / 128 * n_kv >= cus ? 128 : 64;
     p.items = (int)(rows / p.tile + n);
     const long wgs = (long)p.items * n_kv;
-    // splits for two workgroups to a compute unit and no more, which would run after the others (100 tokens behind 8,000,
-    // 32 heads of 128 over 8, f16: 43.5 us, rounded up 57.9)
-    p.splits = wgs >= cus ? 1 : (int)(2 * cus / wgs);
-    const int most_splits = capacity / (kSplitTiles * kTile);
-    if (p.splits > 16) p.splits = 16;
-    if (p.splits > most_splits) p.splits = most_splits > 1 ? most_splits : 1;
+    // Splits for two workgroups of four waves to a compute unit, or one of eight, and no more, which would run after the
+    // others (100 tokens behind 8,000, 32 heads of 128 over 8, f16: 43.5 us, rounded up 57.9). Eight waves, whose halves
+    // share the positions without a join, where there is a compute unit to each workgroup (14 heads of 64 over 2, f32: a
+    // prompt of 512 13.7 us, by four waves 15.9; 64 tokens behind 30,000 45.7 and 55.6), but not where their splits leave
+    // a third of the GPU empty (620 tokens behind 4,380 76.2 and 57.2).
+    const long room = capacity / (kSplitTiles * kTile);
+    auto splits = [&](long places) {
+        const long k = std::min({places / wgs, room, 16l});
+        return (int)(k > 1 ? k : 1);
+    };
+    p.groups = wgs <= cus && 5 * 2 * splits(cus) >= 4 * splits(2 * cus) ? 2 : 1;
+    p.splits = wgs < cus ? splits(p.groups == 2 ? cus : 2 * cus) : 1;
     p.join_rows = p.splits > 1 ? p.tile : 0;
     p.part_rows = p.splits > 1 ? (size_t)p.items * p.splits * p.tile : 0;
     return p;
@@ -1094,9 +1135,10 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
             constexpr size_t lds = 2 * 2 * (size_t)kTile * 64 * kC * 2;
             const dim3 grid((unsigned)c.n_kv * (unsigned)p.items, (unsigned)p.splits);
             if constexpr (kC == 2) {
-                if (p.tile == 128) qh_launch((kv8_tile_kernel<T, kC, 2>), grid, dim3(256), lds, s, c, a);
+                if (p.tile == 128) qh_launch((kv8_tile_kernel<T, kC, 2, 1>), grid, dim3(256), lds, s, c, a);
             }
-            if (p.tile == 64) qh_launch((kv8_tile_kernel<T, kC, 1>), grid, dim3(256), lds, s, c, a);
+            if (p.tile == 64 && p.groups == 2) qh_launch((kv8_tile_kernel<T, kC, 1, 2>), grid, dim3(512), 2 * lds, s, c, a);
+            else if (p.tile == 64) qh_launch((kv8_tile_kernel<T, kC, 1, 1>), grid, dim3(256), lds, s, c, a);
             if (p.join_rows)
                 qh_launch((kv8_join_splits_kernel<T, kC>),
                           dim3((unsigned)p.items, (unsigned)c.n_kv, (unsigned)(p.join_rows * kC / 16)), dim3(256), 0, s, c,

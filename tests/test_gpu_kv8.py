@@ -360,6 +360,17 @@ def test_split_prompts_join(qh):
         check_attention(c, rng, [0], [m], 8, "float16")
 
 
+@pytest.mark.parametrize("dtype,kv,hd", [("float32", 2, 64), ("float16", 1, 128)])
+def test_prompts_on_part_of_the_gpu(qh, dtype, kv, hd):
+    """Few row tiles: halves of a workgroup share the positions, an odd and an even number of tiles, one and none."""
+    rng = np.random.default_rng(SEED)
+    lens = [470, 64, 65, 120, 300, 0, 129]
+    c = filled(qh, rng, lens, kv, hd, 16, dtype)
+    for counts in ([470, 64, 65, 120, 300, 0, 129], [40, 64, 1, 33, 200, 0, 100], [0, 0, 0, 0, 0, 40, 0]):
+        for causal in (True, False):
+            check_attention(c, rng, list(range(7)), counts, 6 * kv, dtype, causal=causal)
+
+
 def test_pools_and_rows_past_32_bit_offsets(qh):
     """Pages behind more than 4 GiB of pool, rows more than 2^32 bytes apart: as in a small pool."""
     import torch
