@@ -351,7 +351,7 @@ int qh_kv8_read(const qh_kv8_cache* c, int layer, void* k, void* v, int dtype, i
                 const int32_t* start, const int32_t* seqs, int n, int n_tok, void* stream);
 
 /* Workspace bytes of a qh_kv8_attention call with n entries over n_tok rows (no initialisation; a smaller batch can need
- * more, as it is split further). */
+ * more, as it is split further). 0 where it needs none: workspace may be NULL then. */
 size_t qh_kv8_attention_workspace_bytes(const qh_kv8_cache* c, int n_heads, int n, int n_tok);
 
 /* Attention of query rows q [n_heads][head_dim] over their sequences: out = sum_j p_j v_j with p = softmax(scale *

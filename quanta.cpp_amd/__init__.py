@@ -410,22 +410,28 @@ class KV8Cache:
         self._ref = C.byref(self.view)
         # what every call looks up, kept here: the calls on a small batch take a few microseconds
         self._index = self.device.index
-        self._int32, self._uint8, self._empty = torch.int32, torch.uint8, torch.empty
+        self._int32, self._uint8, self._empty, self._empty_like = torch.int32, torch.uint8, torch.empty, torch.empty_like
+        self._raw, self._float32 = torch._C, torch.float32
+        self._append, self._read, self._attend = lib().qh_kv8_append, lib().qh_kv8_read, lib().qh_kv8_attention
         self._dtypes = {torch.float32: F32, torch.float16: F16}
-        self._pages_ws = lib().qh_kv8_pages_workspace_bytes(self._ref)
+        self._pages_bytes = lib().qh_kv8_pages_workspace_bytes(self._ref)
+        # resize, fork and compact change the cache, so they are in order and can share a workspace
+        self._pages_ws = torch.empty(self._pages_bytes, dtype=torch.uint8, device=device)
+        self._pages_ptr = self._pages_ws.data_ptr()
         self._attention_ws = {}  # bytes by (heads, entries, rows)
+        self._scale = head_dim ** -0.5
         self.reset()
 
     def _here(self) -> int:
         """The current stream, on the cache's device."""
-        raw = _torch()._C
+        raw = self._raw
         device = raw._cuda_getDevice()
         if device != self._index:
             raise QHError(f"the cache is on {self.device}, the current device is cuda:{device}")
         return raw._cuda_getCurrentRawStream(device)
 
     def _ints(self, t, n, what):
-        if t.dtype is not self._int32 or t.device != self.device or t.dim() != 1 or not t.is_contiguous():
+        if t.dtype is not self._int32 or t.device != self.device or not t.is_contiguous() or t.dim() != 1:
             raise QHError(f"{what} must be a contiguous int32 vector on {self.device}")
         if t.shape[0] != n:
             raise QHError(f"{what} has {t.shape[0]} entries, expected {n}")
@@ -462,17 +468,12 @@ class KV8Cache:
             raise QHError(f"the heads of a row of {what} must be contiguous")
         return dtype, (stride[0] if shape[0] > 1 else heads * hd)
 
-    def _workspace(self, nbytes):
-        # a tensor for each call: nothing of one call (or captured graph) is shared with the next
-        return self._empty(max(nbytes, 16), dtype=self._uint8, device=self.device)
-
     def reset(self) -> None:
         """Every page free, every sequence empty, status 0."""
         _check(lib().qh_kv8_reset(self._ref, self._here()))
 
     def _pages_call(self, name, *args):
-        ws = self._workspace(self._pages_ws)
-        _check(getattr(lib(), name)(self._ref, *args, ws.data_ptr(), self._pages_ws, self._here()))
+        _check(getattr(lib(), name)(self._ref, *args, self._pages_ptr, self._pages_bytes, self._here()))
 
     def resize(self, seqs, lens) -> None:
         """Sequence seqs[i] gets length lens[i] (int32 device vectors): pages past it are given back, missing ones taken."""
@@ -498,18 +499,21 @@ class KV8Cache:
         if dtype != dtype_v or rows != v.shape[0]:
             raise QHError("k and v differ in dtype or rows")
         start, seqs, n = self._batch(rows, start, seqs)
-        _check(lib().qh_kv8_append(self._ref, layer, k.data_ptr(), v.data_ptr(), dtype, ldk, ldv, start, seqs, n, rows,
-                                   self._here()))
+        _check(self._append(self._ref, layer, k.data_ptr(), v.data_ptr(), dtype, ldk, ldv, start, seqs, n, rows,
+                            self._here()))
 
     def read(self, layer: int, n_tok: int, start=None, seqs=None, dtype=None):
         """The stored values (k, v) of the batch's tokens, [n_tok][n_kv_heads][head_dim] of dtype (float32). Rows outside
         the entries are undefined."""
-        out = self._empty((2, n_tok, self.n_kv_heads, self.head_dim), dtype=dtype or _torch().float32, device=self.device)
-        k, v = out[0], out[1]
-        code, ld = self._rows(k, self.n_kv_heads, "read")
+        heads, hd, dtype = self.n_kv_heads, self.head_dim, dtype or self._float32
+        code = self._dtypes.get(dtype)
+        if code is None:
+            raise QHError("read gives float32 or float16")
+        k = self._empty(n_tok, heads, hd, dtype=dtype, device=self.device)
+        v = self._empty(n_tok, heads, hd, dtype=dtype, device=self.device)
         start, seqs, n = self._batch(n_tok, start, seqs)
-        _check(lib().qh_kv8_read(self._ref, layer, k.data_ptr(), v.data_ptr(), code, ld, ld, start, seqs, n, n_tok,
-                                 self._here()))
+        _check(self._read(self._ref, layer, k.data_ptr(), v.data_ptr(), code, heads * hd, heads * hd, start, seqs, n, n_tok,
+                          self._here()))
         return k, v
 
     def attention(self, layer: int, q, start=None, seqs=None, causal: bool = True, scale: float | None = None, out=None):
@@ -520,7 +524,7 @@ class KV8Cache:
         heads = q.shape[1] if q.dim() == 3 else q.shape[-1] // self.head_dim
         dtype, ldq = self._rows(q, heads, "q")
         if out is None:
-            out = self._empty(q.shape, dtype=q.dtype, device=self.device)
+            out = self._empty_like(q) if q.is_contiguous() else self._empty(q.shape, dtype=q.dtype, device=self.device)
             ldo = heads * self.head_dim
         else:
             if out.shape != q.shape or out.dtype != q.dtype:
@@ -533,10 +537,11 @@ class KV8Cache:
             if len(self._attention_ws) > 4096:
                 self._attention_ws.clear()
             self._attention_ws[heads, n, rows] = need
-        ws = self._workspace(need)
-        _check(lib().qh_kv8_attention(self._ref, layer, q.data_ptr(), out.data_ptr(), dtype, heads, ldq, ldo, start, seqs, n,
-                                      rows, 1 if causal else 0, self.head_dim ** -0.5 if scale is None else scale,
-                                      ws.data_ptr(), need, self._here()))
+        # a tensor for each call: nothing of one call (or captured graph) is shared with the next
+        ws = self._empty(need, dtype=self._uint8, device=self.device) if need else None
+        _check(self._attend(self._ref, layer, q.data_ptr(), out.data_ptr(), dtype, heads, ldq, ldo, start, seqs, n, rows,
+                            1 if causal else 0, self._scale if scale is None else scale, ws.data_ptr() if need else None,
+                            need, self._here()))
         return out
 
 

@@ -626,7 +626,7 @@ int qh_kv8_attention(const qh_kv8_cache* c, int layer, const void* q, void* out,
     if (int rc = validate_kv8_rows(out, dtype, ldo, width, who)) return rc;
     if (q == out) return fail(QH_ERR_ARG, "%s: out is q", who);
     const size_t need = kv8_attention_workspace_bytes(n_heads, c->n_kv_heads, c->head_dim, c->seq_pages * c->page_tokens, n, n_tok);
-    if (!workspace || workspace_bytes < need)
+    if (need > (workspace ? workspace_bytes : 0))
         return fail(QH_ERR_NOMEM, "%s: workspace of %zu bytes, needs %zu", who, workspace ? workspace_bytes : 0, need);
     if (!aligned16(workspace)) return fail(QH_ERR_ALIGN, "%s: workspace not 16-byte aligned", who);
     return check_hip(launch_kv8_attention(kv8_view(*c, layer), q, out, dtype, n_heads, ldq, ldo, start, seqs, n, n_tok,

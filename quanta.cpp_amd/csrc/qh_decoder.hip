@@ -2266,7 +2266,7 @@ hipError_t decoder_bind_kv8(Decoder* d, const Kv8View* c, int seq) {
             const size_t b = kv8_attention_workspace_bytes(d->hp.n_heads, d->hp.n_kv_heads, d->hp.head_dim, capacity, 1, n);
             attn = b > attn ? b : attn;
         }
-        const size_t bytes[3] = {sizeof(int) * kKv8Ints, kv8_pages_workspace_bytes(c->n_pages, c->n_seqs), attn};
+        const size_t bytes[3] = {sizeof(int) * kKv8Ints, kv8_pages_workspace_bytes(c->n_pages, c->n_seqs), attn > 16 ? attn : 16};
         for (int i = 0; i < 3; ++i) {
             const hipError_t e = dalloc(d, &fresh[i], bytes[i]);
             if (e != hipSuccess) {

@@ -1016,10 +1016,10 @@ struct Plan {
     int waves;         // of a workgroup of the row kernels
     int tile;          // rows of an item
     int groups;        // of four waves to a workgroup of the tile kernel
-    int join_rows;     // rows of an item that can have partial results; 0: none
+    int join_rows;     // rows of an item that can have partial results; 0: none, and no workspace
     size_t part_rows;  // rows of partial results (per KV head)
     size_t bytes(int n_kv, int hd) const {
-        return whole ? 0 : sizeof(int4) * (size_t)items + sizeof(float) * part_rows * n_kv * (hd + 2);
+        return join_rows ? sizeof(int4) * (size_t)items + sizeof(float) * part_rows * n_kv * (hd + 2) : 0;
     }
 };
 // capacity: positions that a sequence can have.
@@ -1088,7 +1088,7 @@ size_t kv8_attention_workspace_bytes(int n_heads, int n_kv, int hd, int capacity
         const size_t single = plan_of(group, n_kv, hd, capacity, n, n_tok, true).bytes(n_kv, hd);
         b = b > single ? b : single;
     }
-    return b > 16 ? b : 16;
+    return b;
 }
 
 hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int dtype, int n_heads, int64_t ldq,

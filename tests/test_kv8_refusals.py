@@ -72,7 +72,7 @@ def test_append_refusals(qh, change, code):
 @pytest.mark.parametrize("change,code", [
     ({"layer": 2}, 1), ({"heads": 3}, 3), ({"heads": 0}, 3), ({"start": None}, 1), ({"causal": 2}, 1),
     ({"scale": float("nan")}, 1), ({"scale": float("inf")}, 1), ({"scale": -3e38}, 1), ({"dtype": 3}, 2), ({"q": None}, 1), ({"out": None}, 1),
-    ({"ldq": 255}, 1), ({"ldo": 258}, 4), ({"out": C.c_void_p(4104)}, 4), ({"ws": None}, 6), ({"ws": C.c_void_p(4104)}, 4),
+    ({"ldq": 255}, 1), ({"ldo": 258}, 4), ({"out": C.c_void_p(4104)}, 4), ({"ws": C.c_void_p(4104)}, 4),
     ({"n_tok": 1 << 30}, 3), ({"n": 1 << 24}, 3), ({"n_tok": 1 << 29, "n": 1}, 3), ({"out": P, "q": P}, 1),
 ])
 def test_attention_refusals(qh, change, code):
@@ -80,9 +80,9 @@ def test_attention_refusals(qh, change, code):
 
 
 def test_attention_workspace_is_checked(qh, monkeypatch):
-    c = cache(qh)
+    c = cache(qh, seq_pages=128)
     need = qh.lib().qh_kv8_attention_workspace_bytes(C.byref(c), 4, 2, 5)
-    assert need > 0 and attend(qh, c, ws_bytes=need - 1) == 6
+    assert need > 0 and attend(qh, c, ws_bytes=need - 1) == 6 and attend(qh, c, ws=None) == 6
     assert qh.lib().qh_kv8_attention_workspace_bytes(C.byref(c), 4, 0, 0) == 0
 
 
