@@ -163,7 +163,7 @@ struct Blocks {
 // and the output with it (16 registers per 64 dimensions and row tile), so that most tiles need neither that nor the
 // maximum over the row's four lanes. Weights, up to 2^kSlack, stay clear of f16's largest number because their unit leaves
 // that much room; their smallest step is 2^-31 of the base's weight.
-constexpr float kSlack = 8.0f;
+constexpr float kSlack = 8.0f, kMost = 0x1p8f;  // and 2^kSlack
 constexpr int kRoom = 6;  // weights are below 2^(kRoom + kSlack)
 
 template <typename T, int kC>
@@ -201,12 +201,12 @@ struct Rows {
 
     // Moves the base where a score passes it by too much, and the output with it; shrink: what the value scales' unit asks
     // for.
-    __device__ __forceinline__ void settle(const f4 (&x)[4], const float (&f)[4], float shrink) {
+    __device__ __forceinline__ void settle(const f4 (&x)[4], const float (&f)[4], float shrink, float slack) {
         float top = -__builtin_inff();
 #pragma unroll
         for (int b = 0; b < 4; ++b)
             top = __builtin_fmaxf(top, fmax2(fmax2(x[b][0], x[b][1]), fmax2(x[b][2], x[b][3])) * f[b]);
-        if (__any(top > m + kSlack) || shrink != 1.0f) {
+        if (__any(top > m + slack) || shrink != 1.0f) {
             const float was = m;
             m = __builtin_fmaxf(m, over_groups(top, fmax2));
             const float alpha = m == was ? 1.0f : __builtin_amdgcn_exp2f(was - m);
@@ -217,9 +217,10 @@ struct Rows {
         }
     }
 
-    // The weights as operands w, two blocks to each (and their low halves lo).
+    // The weights as operands w, two blocks to each (and their low halves lo); their sum, without the value scales, joins
+    // `sum`.
     __device__ __forceinline__ void weigh(const f4 (&x)[4], const float (&f)[4], const float (&weight)[4], h8 (&w)[2],
-                                          h8 (&lo)[2]) {
+                                          h8 (&lo)[2], float& sum) const {
         // a row that has seen nothing yet: subtract 0, so that its weights are 2^-inf = 0 and not NaN
         const float base = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
@@ -236,7 +237,7 @@ struct Rows {
                 w[b >> 1][4 * (b & 1) + s] = hi;
                 if constexpr (kSplit) lo[b >> 1][4 * (b & 1) + s] = (_Float16)(v - (float)hi);
             }
-            l += (p[0] + p[1]) + (p[2] + p[3]);
+            sum += (p[0] + p[1]) + (p[2] + p[3]);
         }
     }
 };
@@ -421,8 +422,8 @@ __device__ __forceinline__ void rows_tiles(const Kv8View& c, const AttnArgs& a, 
         h8 w[2], lo[2];
         if (pos0 + kTile > all_see || sc.ok != 15u) st.mask(x, f, pos0 + 4 * g, vis, sc.ok);
         if (sc.nan) st.poison(sc.nan, pos0, vis);
-        st.settle(x, f, sc.shrink);
-        st.weigh(x, f, sc.weight, w, lo);
+        st.settle(x, f, sc.shrink, kSlack);
+        st.weigh(x, f, sc.weight, w, lo, st.l);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -797,6 +798,7 @@ __global__ __launch_bounds__(256 * kG, 2) void kv8_tile_kernel(Kv8View c, AttnAr
         Query<T, kC>::fetch(raw, q_row<T>(a, c, e.row0 + (valid ? r : r0), kvh) + 16 * g);
         q[ct].convert(raw, valid, a.scale_log2e);
         st[ct].clear();
+        if (!valid) st[ct].m = 0.0f;  // a row that is not there asks for no base
     }
     const int w0 = r0 + wave * (16 * kCt);
     const int all_see = w0 <= last ? visible(e, a, w0) : 0;  // positions that each row of the wave sees
@@ -909,10 +911,34 @@ __global__ __launch_bounds__(256 * kG, 2) void kv8_tile_kernel(Kv8View c, AttnAr
             for (int ct = 0; ct < kCt; ++ct) st[ct].poison(sc.nan, pos0, vis[ct]);
         }
         h8 w[kCt][2], lo[kCt][2];
+        if constexpr (Query<T, kC>::kSplit) {
 #pragma unroll
-        for (int ct = 0; ct < kCt; ++ct) st[ct].settle(x[ct], f[ct], sc.shrink);
+            for (int ct = 0; ct < kCt; ++ct) st[ct].settle(x[ct], f[ct], sc.shrink, kSlack);
 #pragma unroll
-        for (int ct = 0; ct < kCt; ++ct) st[ct].weigh(x[ct], f[ct], sc.weight, w[ct], lo[ct]);
+            for (int ct = 0; ct < kCt; ++ct) st[ct].weigh(x[ct], f[ct], sc.weight, w[ct], lo[ct], st[ct].l);
+        } else {
+            // No maximum over the scores: the weights from the base as it is, and again from a new one where their sum says
+            // that one may be past the slack (2,000 of 8,000 tokens, f16: 14 heads of 64 over 2 398 -> 361 us, 32 of 128
+            // over 8 1,030 -> 1,001; f32, with more registers to keep, 32 of 128 over 8 1,402 and 1,543).
+            float sum[kCt];
+            bool move = sc.shrink != 1.0f;
+#pragma unroll
+            for (int ct = 0; ct < kCt; ++ct) {
+                sum[ct] = 0.0f;
+                st[ct].weigh(x[ct], f[ct], sc.weight, w[ct], lo[ct], sum[ct]);
+                move |= !(sum[ct] <= kMost) || st[ct].m == -__builtin_inff();
+            }
+            if (__any(move)) {
+#pragma unroll
+                for (int ct = 0; ct < kCt; ++ct) {
+                    st[ct].settle(x[ct], f[ct], sc.shrink, 0.0f);
+                    sum[ct] = 0.0f;
+                    st[ct].weigh(x[ct], f[ct], sc.weight, w[ct], lo[ct], sum[ct]);
+                }
+            }
+#pragma unroll
+            for (int ct = 0; ct < kCt; ++ct) st[ct].l += sum[ct];
+        }
         __builtin_amdgcn_s_setprio(1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll

@@ -290,6 +290,27 @@ def test_scores_far_apart(qh):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_scores_and_values_that_grow(qh, dtype, hd):
+    """Keys and values that grow along the sequence: the largest score and the values' unit move again and again."""
+    rng = np.random.default_rng(SEED)
+    c = Pair(qh, 1, 60, 16, 2, hd, 2, 48)
+    c.resize([0, 1], [700, 90])
+
+    def grow(k, v):
+        import torch
+        at = torch.cat([torch.arange(700), torch.arange(90)]).to("cuda").view(-1, 1, 1)
+        k.mul_((at / 40 + 0.05).to(k.dtype))
+        v.mul_(torch.exp2(at / 100 - 6).to(v.dtype))
+
+    c.append(rng, 0, [0, 1], [700, 90], dtype, edit=grow)
+    for q_scale in (0.1, 2.0):
+        check_attention(c, rng, [0, 1], [90, 90], 6, dtype, q_scale=q_scale)
+        check_attention(c, rng, [0, 1], [1, 1], 6, dtype, q_scale=q_scale)
+        check_attention(c, rng, [0, 1], [300, 5], 6, dtype, q_scale=q_scale, causal=False)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
 @pytest.mark.parametrize("heads,kv,hd,page", [(14, 2, 64, 64), (4, 2, 128, 16), (5, 5, 64, 32), (33, 1, 128, 128)])
 def test_ragged_prompts(qh, dtype, heads, kv, hd, page):
     """Entries of one row to hundreds, at the front of their sequences and far behind it, and one without rows."""
