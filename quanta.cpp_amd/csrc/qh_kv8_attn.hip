@@ -858,7 +858,7 @@ __global__ __launch_bounds__(256 * kG, 2) void kv8_tile_kernel(Kv8View c, AttnAr
     // background of a wave, four issue slots each: the conversion of the next tile fills them in the first product, and
     // each operand is read from shared memory kDeep reads before its use. A wave in one of its products goes before the
     // other wave of its SIMD, which has exponentials to fill the slots that are left (4 x 2,000 tokens over 8,000, 32
-    // heads of 128 over 8, f16: 1,230 -> 1,165 us).
+    // heads of 128 over 8, f16: 1,047 -> 996 us).
     constexpr int kMm = kCt * (Query<T, kC>::kSplit ? 2 : 1);  // matrix instructions to an operand read
     constexpr int kOps = 8 * kC, kDeep = 4;
     auto compute = [&](int buf, int t) {
@@ -1082,9 +1082,9 @@ Plan plan_of(int group, int n_kv, int hd, int capacity, int n, int n_tok, bool s
         p.part_rows = 2 * (size_t)p.shares * kRowTile;
         return p;
     }
-    // 128 rows to a workgroup at head_dim 128 (4 x 2,000 tokens behind 6,000, 32 heads over 8, f16: 1,236 us, with 64 rows
-    // 1,611), but 64 where 128 would leave compute units idle, and at head_dim 64, where the longer loop is no faster
-    // (14 heads over 2: f32 579 and 534 us, f16 411 and 416; one prompt of 512: f32 20.9 and 17.2)
+    // 128 rows to a workgroup at head_dim 128 (4 x 2,000 tokens behind 6,000, 32 heads over 8: f16 1,002 us, with 64 rows
+    // 1,372; f32 1,404 and 1,648), but 64 where 128 would leave compute units idle, and at head_dim 64, where the longer
+    // loop is no faster (14 heads over 2: f32 505 us, with 128 rows 541; f16 361 and 369)
     p.tile = hd == 128 && rows / 128 * n_kv >= cus ? 128 : 64;
     p.items = (int)(rows / p.tile + n);
     const long wgs = (long)p.items * n_kv;
