@@ -1809,19 +1809,23 @@ hipError_t attention_kv8(Decoder* d, int l, int n, hipStream_t s) {
     const int64_t qd = (int64_t)hp.n_heads * hp.head_dim, kvd = (int64_t)hp.n_kv_heads * hp.head_dim;
     Kv8View c = d->kv8;
     c.pages += (size_t)l * c.n_pages * c.page_bytes;
-    if (hp.head_dim == 64)
-        qh_launch((qkv_rope_kernel<64>), dim3(n), dim3(256), 0, s, d->q, d->k, d->v, bias(d, l, L_BQ), bias(d, l, L_BK),
-                  bias(d, l, L_BV), d->cs, d->pos, hp.ctx_len, hp.n_heads, hp.n_kv_heads);
-    else
-        qh_launch((qkv_rope_kernel<128>), dim3(n), dim3(256), 0, s, d->q, d->k, d->v, bias(d, l, L_BQ), bias(d, l, L_BK),
-                  bias(d, l, L_BV), d->cs, d->pos, hp.ctx_len, hp.n_heads, hp.n_kv_heads);
-    QH_TRY(hipGetLastError());
     const int32_t *start = n == 1 ? nullptr : d->kv8_state + kKv8Start, *seq = d->kv8_state + kKv8Batch;
-    QH_TRY(launch_kv8_append(c, d->k, d->v, QH_F32, kvd, kvd, start, seq, 1, n, s));
+    const float *bq = bias(d, l, L_BQ), *bk = bias(d, l, L_BK), *bv = bias(d, l, L_BV);
+    if (n == 1) {
+        QH_TRY(launch_kv8_append_token(c, {d->q, d->k, d->v, bq, bk, bv, d->cs, d->pos, hp.ctx_len, hp.n_heads}, seq, s));
+    } else {
+        if (hp.head_dim == 64)
+            qh_launch((qkv_rope_kernel<64>), dim3(n), dim3(256), 0, s, d->q, d->k, d->v, bq, bk, bv, d->cs, d->pos, hp.ctx_len,
+                      hp.n_heads, hp.n_kv_heads);
+        else
+            qh_launch((qkv_rope_kernel<128>), dim3(n), dim3(256), 0, s, d->q, d->k, d->v, bq, bk, bv, d->cs, d->pos, hp.ctx_len,
+                      hp.n_heads, hp.n_kv_heads);
+        QH_TRY(hipGetLastError());
+        QH_TRY(launch_kv8_append(c, d->k, d->v, QH_F32, kvd, kvd, start, seq, 1, n, s));
+    }
     float* out = d->fb ? d->fb : d->o;  // unquantized matrices read it as it is
-    QH_TRY(launch_kv8_attention(c, d->q, out, QH_F32, hp.n_heads, qd, qd, start, seq, 1, n, true,
-                                1.0f / sqrtf((float)hp.head_dim), d->kv8_attn_ws, s));
-    return launch_quantize_q8(out, n, (int)qd, d->qb, d->db, s);
+    return launch_kv8_attention(c, d->q, out, QH_F32, hp.n_heads, qd, qd, start, seq, 1, n, true,
+                                1.0f / sqrtf((float)hp.head_dim), d->kv8_attn_ws, s, d->qb, d->db);
 }
 
 hipError_t attention(Decoder* d, int l, int n, hipStream_t s) {

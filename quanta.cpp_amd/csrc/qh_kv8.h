@@ -94,6 +94,15 @@ hipError_t launch_kv8_append(const Kv8View& c, const void* k, const void* v, int
                              const int32_t* start, const int32_t* seqs, int n, int n_tok, hipStream_t s);
 hipError_t launch_kv8_read(const Kv8View& c, void* k, void* v, int dtype, int64_t ldk, int64_t ldv, const int32_t* start,
                            const int32_t* seqs, int n, int n_tok, hipStream_t s);
+// A decode step's token, one f32 row of q, k and v as projected: bias and RoPE at position *pos (in q in place), and k and v
+// stored as the last token of sequence *seq. cs: [ctx][head_dim / 2] cosines and sines; biases may be null.
+struct Kv8Token {
+    float* q;
+    const float *k, *v, *bq, *bk, *bv, *cs;
+    const int* pos;
+    int ctx, n_heads;
+};
+hipError_t launch_kv8_append_token(const Kv8View& c, const Kv8Token& t, const int32_t* seq, hipStream_t s);
 size_t kv8_pages_workspace_bytes(int n_pages, int n_seqs);
 // pages: the first layer's; n_layers of them lie layer_bytes apart.
 hipError_t launch_kv8_reset(const Kv8View& c, hipStream_t s);
@@ -103,11 +112,12 @@ hipError_t launch_kv8_fork(const Kv8View& c, int n_layers, const int32_t* src, c
                            void* ws, hipStream_t s);
 hipError_t launch_kv8_compact(const Kv8View& c, int n_layers, int32_t* live, void* ws, hipStream_t s);
 // qh_kv8_attn.hip
-// capacity: positions that a sequence can have.
+// capacity: positions that a sequence can have. oq, od: the f32 rows of out (without gaps) in 8 bits too, as
+// launch_quantize_q8 makes them.
 size_t kv8_attention_workspace_bytes(int n_heads, int n_kv, int hd, int capacity, int n, int n_tok);
 hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int dtype, int n_heads, int64_t ldq,
                                 int64_t ldo, const int32_t* start, const int32_t* seqs, int n, int n_tok, bool causal,
-                                float scale, void* ws, hipStream_t s);
+                                float scale, void* ws, hipStream_t s, int8_t* oq = nullptr, float* od = nullptr);
 
 // The decoder over a bound cache (qh_decoder.hip): c is its layer 0, null to unbind.
 struct Decoder;

@@ -226,6 +226,79 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8View c, const T* __r
         append_block<kC, false>(c, x, h, page, bp, pos0, sp.first, sp.len);
 }
 
+// A decode step's token: the waves of append, which first add the bias and rotate their key row, and behind them workgroups
+// that do so to the query heads in place: the decoder's rotation of many tokens in its order, with a launch less to a layer.
+template <int kC>
+__global__ __launch_bounds__(256) void kv8_append_token_kernel(Kv8View c, Kv8Token t, const int32_t* __restrict__ seqs) {
+    constexpr int kHd = 64 * kC, kHalf = kHd / 2;
+    const unsigned groups = (unsigned)(2 * c.n_kv + 3) / 4;
+    const int pos = *t.pos;
+    if (pos < 0 || pos >= t.ctx) return;
+    const float* cs = t.cs + (size_t)pos * kHd;
+    if (blockIdx.x >= groups) {
+        const int e = (int)(blockIdx.x - groups) * 256 + (int)threadIdx.x, h = e / kHalf, i = e % kHalf;
+        if (h >= t.n_heads) return;
+        float *row = t.q + (size_t)h * kHd, a = row[i], b = row[i + kHalf];
+        if (t.bq) {
+            a = a + t.bq[h * kHd + i];
+            b = b + t.bq[h * kHd + i + kHalf];
+        }
+        const float co = cs[2 * i], sn = cs[2 * i + 1];
+        row[i] = __builtin_fmaf(a, co, -(b * sn));
+        row[i + kHalf] = __builtin_fmaf(b, co, a * sn);
+        return;
+    }
+    const int hw = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6), h = hw >> 1, j = (int)threadIdx.x & 15;
+    if (hw >= 2 * c.n_kv) return;
+    const bool values = (hw & 1) != 0;
+    const float *row = (values ? t.v : t.k) + h * kHd + 4 * j, *bias = values ? t.bv : t.bk;
+    float x[kC][4];
+#pragma unroll
+    for (int k = 0; k < kC; ++k) {
+        const float4 r = *reinterpret_cast<const float4*>(row + 64 * k);
+        x[k][0] = r.x, x[k][1] = r.y, x[k][2] = r.z, x[k][3] = r.w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (bias) x[k][i] = x[k][i] + bias[h * kHd + 64 * k + 4 * j + i];
+    }
+    if (!values) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = (4 * j + i) % kHalf;
+            const float co = cs[2 * d], sn = cs[2 * d + 1];
+            if constexpr (kC == 2) {
+                const float a = x[0][i], b = x[1][i];
+                x[0][i] = __builtin_fmaf(a, co, -(b * sn));
+                x[1][i] = __builtin_fmaf(b, co, a * sn);
+            } else {  // the other half is eight lanes away
+                const float mine = x[0][i], other = __shfl_xor(mine, 8);
+                x[0][i] = j < 8 ? __builtin_fmaf(mine, co, -(other * sn)) : __builtin_fmaf(mine, co, other * sn);
+            }
+        }
+    }
+    const Span sp = span_of(c, Kv8Batch{nullptr, seqs, 1, 1, 0}, 0);
+    const int blk = sp.first / kBlk, pos0 = blk * kBlk;
+    if (sp.first >= sp.len) return;
+    const int page = c.table[(size_t)sp.seq * c.seq_pages + (pos0 >> c.page_shift)];
+    if (page < 0 || page >= c.n_pages) return;
+    if (c.refs[page] > 1) {
+        if ((threadIdx.x & 63) == 0) atomicOr(c.status, QH_KV8_SHARED);
+        return;
+    }
+    float rows[kC][4][4];  // append_block takes the one that is the new token's
+#pragma unroll
+    for (int k = 0; k < kC; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) rows[k][r][i] = x[k][i];
+    const int bp = blk & ((1 << (c.page_shift - 4)) - 1);
+    if (values)
+        append_block<kC, true>(c, rows, h, page, bp, pos0, sp.first, sp.len);
+    else
+        append_block<kC, false>(c, rows, h, page, bp, pos0, sp.first, sp.len);
+}
+
 // The same items: one wave writes the values of one block's tokens, code * scale rounded to f32, then to T. Lanes as in
 // append_block.
 template <typename T, int kC>
@@ -663,6 +736,13 @@ hipError_t launch_kv8_append(const Kv8View& c, const void* k, const void* v, int
         qh_launch((kv8_append_kernel<T, decltype(kc)::value>), grid, dim3(256), 0, s, c, (const T*)k, (const T*)v, ldk,
                   ldv, Kv8Batch{start, seqs, n, n_tok, 0});
     });
+}
+
+hipError_t launch_kv8_append_token(const Kv8View& c, const Kv8Token& t, const int32_t* seq, hipStream_t s) {
+    const dim3 grid((unsigned)(2 * c.n_kv + 3) / 4 + (unsigned)(t.n_heads * (c.hd / 2) + 255) / 256);
+    if (c.hd == 64) qh_launch((kv8_append_token_kernel<1>), grid, dim3(256), 0, s, c, t, seq);
+    else qh_launch((kv8_append_token_kernel<2>), grid, dim3(256), 0, s, c, t, seq);
+    return hipGetLastError();
 }
 
 hipError_t launch_kv8_read(const Kv8View& c, void* k, void* v, int dtype, int64_t ldk, int64_t ldv, const int32_t* start,

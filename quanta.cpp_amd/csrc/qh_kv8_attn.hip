@@ -297,6 +297,8 @@ struct AttnArgs {
     float* part_ml;
     int4* rec;       // [items] where an item's partials are: first slot, how many (0: none), first row, rows
     int items, splits;
+    int8_t* oq;  // the output in 8 bits as well, and its scales (f32 calls; null: not)
+    float* od;
 };
 
 // Entry b's rows: global rows (token * group + head) from first on, and the positions its tokens see.
@@ -319,12 +321,18 @@ __device__ __forceinline__ int visible(const Entry& e, const AttnArgs& a, int r)
     return a.causal ? min(max(e.len - e.tokens + r / a.group + 1, 0), e.len) : e.len;
 }
 
-// A row's share of the output, 4 values at dimension d: divided by the row's sum, zero where it saw nothing.
-template <typename T>
-__device__ __forceinline__ void store_out(T* out, float4 o, float m, float l) {
+// A row's share of the output, 4 values at dimension d: divided by the row's sum, zero where it saw nothing. kX8: 8 lanes
+// in a row hold 32 values of a row, and write them in 8 bits too where the call asks for that.
+template <typename T, bool kX8>
+__device__ __forceinline__ void store_out(const AttnArgs& a, T* out, float4 o, float m, float l) {
     const float inv = m == -__builtin_inff() ? 0.0f : 1.0f / l;
     if constexpr (std::is_same<T, float>::value) {
-        *reinterpret_cast<float4*>(out) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        const float4 v = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        *reinterpret_cast<float4*>(out) = v;
+        if (kX8 && a.oq) {
+            const int64_t at = (out - static_cast<float*>(a.out)) & ~31ll;
+            quant_block_x8(v, a.oq + at, a.od + at / 32);
+        }
     } else {
         typedef _Float16 h4 __attribute__((ext_vector_type(4)));
         *reinterpret_cast<h4*>(out) = h4{(_Float16)(o.x * inv), (_Float16)(o.y * inv), (_Float16)(o.z * inv),
@@ -481,7 +489,7 @@ __device__ __forceinline__ void rows_tiles(const Kv8View& c, const AttnArgs& a, 
                 o.w = __builtin_fmaf(f[w2], v.w, o.w);
             }
             if (whole)
-                store_out(out_row<T>(a, c, e.row0 + r0 + rr, kvh) + 64 * cc + d0, o, top, lsum);
+                store_out<T, true>(a, out_row<T>(a, c, e.row0 + r0 + rr, kvh) + 64 * cc + d0, o, top, lsum);
             else
                 *reinterpret_cast<float4*>(a.part_o + pr * kHd + 64 * cc + d0) = o;
         }
@@ -718,7 +726,7 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8View c, AttnArgs a) {
         const float4 v = *reinterpret_cast<const float4*>(&so[k][d]);
         o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
     }
-    store_out(out_row<T>(a, c, rec.z + row, kvh) + d, o, top, l);
+    store_out<T, true>(a, out_row<T>(a, c, rec.z + row, kvh) + d, o, top, l);
 }
 
 // The same for few partials (the splits of the tile kernel): every group of hd / 4 threads joins a row of its own.
@@ -746,7 +754,7 @@ __global__ __launch_bounds__(256) void kv8_join_splits_kernel(Kv8View c, AttnArg
         o.z = __builtin_fmaf(f, v.z, o.z);
         o.w = __builtin_fmaf(f, v.w, o.w);
     }
-    store_out(out_row<T>(a, c, rec.z + row, kvh) + d, o, top, l);
+    store_out<T, false>(a, out_row<T>(a, c, rec.z + row, kvh) + d, o, top, l);
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
@@ -1020,7 +1028,7 @@ __global__ __launch_bounds__(256 * kG, 2) void kv8_tile_kernel(Kv8View c, AttnAr
                                              st[ct].o[4 * cc + 2][s] * back, st[ct].o[4 * cc + 3][s] * back);
                 const int d = 64 * cc + 16 * g + 4 * s;
                 if (splits == 1)
-                    store_out(out + d, o, st[ct].m, st[ct].l);
+                    store_out<T, false>(a, out + d, o, st[ct].m, st[ct].l);
                 else
                     *reinterpret_cast<float4*>(a.part_o + pr * kHd + d) = o;
             }
@@ -1119,10 +1127,12 @@ size_t kv8_attention_workspace_bytes(int n_heads, int n_kv, int hd, int capacity
 
 hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int dtype, int n_heads, int64_t ldq,
                                 int64_t ldo, const int32_t* start, const int32_t* seqs, int n, int n_tok, bool causal,
-                                float scale, void* ws, hipStream_t s) {
+                                float scale, void* ws, hipStream_t s, int8_t* oq, float* od) {
     AttnArgs a{};
     a.q = q;
     a.out = out;
+    a.oq = oq;
+    a.od = od;
     a.ldq = ldq;
     a.ldo = ldo;
     a.batch = Kv8Batch{start, seqs, n, n_tok, 0};
@@ -1177,7 +1187,9 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
     else if (dtype == QH_F16 && c.hd == 64) go((_Float16*)nullptr, integral_constant<int, 1>{});
     else if (dtype == QH_F16 && c.hd == 128) go((_Float16*)nullptr, integral_constant<int, 2>{});
     else return hipErrorInvalidValue;
-    return hipGetLastError();
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !oq || p.rows) return e;
+    return launch_quantize_q8(static_cast<const float*>(out), n_tok, n_heads * c.hd, oq, od, s);
 }
 
 }  // namespace qh

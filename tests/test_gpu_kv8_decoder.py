@@ -26,6 +26,8 @@ def model(seed=3, **kw):
 NARROW = dict(vocab_size=1024, dim=256, n_heads=4, n_kv_heads=1, head_dim=64, ffn_dim=512)
 WIDE = dict(vocab_size=1024, dim=512, n_heads=4, n_kv_heads=2, head_dim=128, ffn_dim=512)
 
+MANY = dict(vocab_size=1024, dim=2560, n_heads=40, n_kv_heads=1, head_dim=64, ffn_dim=512)
+
 
 def cache_for(qh, hp, n_pages=40, page=32, seqs=4, seq_pages=10):
     c = qh.KV8Cache(hp.n_layers, n_pages, page, hp.n_kv_heads, hp.head_dim, seqs, seq_pages)
@@ -97,6 +99,26 @@ def test_hidden_states_agree_with_the_f32_cache(qh, gpu, shape, dtype):
     for m in (70, 1, 1, 40, 1, 17):
         for d in (dec, ref):
             d.prefill(ids[at:at + m], at, top_k=k)
+        at += m
+        a, b = dec.hidden().astype(np.float64), ref.hidden().astype(np.float64)
+        assert np.linalg.norm(a - b) <= 0.15 * np.linalg.norm(b), (at, np.linalg.norm(a - b) / np.linalg.norm(b))
+    assert dec.status() == 0
+    dec.close()
+    ref.close()
+
+
+@pytest.mark.parametrize("shape,pages", [(NARROW, 80), (WIDE, 80), (NARROW, 130), (MANY, 8), (MANY, 130)])
+def test_steps_agree_over_every_attention_kernel(qh, gpu, shape, pages):
+    """Tables of more than 1,024 and 2,048 positions, where a step's attention is joined from shares, and more query heads
+    to a KV head than its kernels take: the 8-bit outputs come from another place each. Bounds as above."""
+    hp, tens = model(5, **shape)
+    dec, ref = qh.Decoder(hp, tens, ctx_len=256), qh.Decoder(hp, tens, ctx_len=256, kv_f32=True)
+    dec.bind_kv8(cache_for(qh, hp, page=16, seq_pages=pages), 1)
+    ids = np.random.default_rng(2).integers(0, hp.vocab_size, 120).astype(np.int32)
+    at = 0
+    for m in (100, 1, 1, 1):
+        for d in (dec, ref):
+            d.prefill(ids[at:at + m], at)
         at += m
         a, b = dec.hidden().astype(np.float64), ref.hidden().astype(np.float64)
         assert np.linalg.norm(a - b) <= 0.15 * np.linalg.norm(b), (at, np.linalg.norm(a - b) / np.linalg.norm(b))
