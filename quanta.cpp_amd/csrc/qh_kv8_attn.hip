@@ -1153,6 +1153,7 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
             for (int b = 0; b < n; b += p.entries) {
                 a.q = static_cast<const T*>(q) + (int64_t)b * ldq;  // only single tokens take more than one launch
                 a.out = static_cast<T*>(out) + (int64_t)b * ldo;
+                if (oq) a.oq = oq + (int64_t)b * ldo, a.od = od + (int64_t)b * ldo / 32;
                 if (start == nullptr) {
                     const int m = n - b < p.entries ? n - b : p.entries;
                     a.batch = Kv8Batch{nullptr, seqs ? seqs + b : nullptr, m, m, b};
