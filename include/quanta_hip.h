@@ -359,7 +359,10 @@ size_t qh_kv8_attention_workspace_bytes(const qh_kv8_cache* c, int n_heads, int 
  * that are not the queries' own: an entry may then have more rows than the sequence has tokens). Query head h reads KV
  * head h / (n_heads / n_kv_heads). A row that sees nothing (an empty sequence, or a position below 0) is 0. out may not
  * overlap q. A row of q that is not finite gives NaN, and so does a visible token that reads as NaN. Sums in f32; f32
- * queries and weights go through the matrix instructions as two f16 each, f16 calls' weights as one. */
+ * queries and weights go through the matrix instructions as two f16 each, f16 calls' weights as one. A weight is also held
+ * to 2^-31 of the largest product of weight and value scale that its row sees (what storing that scale's block rounded off is
+ * 2^-1 of the product); blocks that a row does not see, or gives no weight to, take nothing from it, up to scales 2^80 times
+ * its own. */
 int qh_kv8_attention(const qh_kv8_cache* c, int layer, const void* q, void* out, int dtype, int n_heads, int64_t ldq,
                      int64_t ldo, const int32_t* start, const int32_t* seqs, int n, int n_tok, int causal, float scale,
                      void* workspace, size_t workspace_bytes, void* stream);

@@ -12,8 +12,10 @@
 //   f32 queries are split into two f16 (22 bits), scaled by a power of two so that the row's largest value has exponent
 //   13: what the split drops is below 2^-22 of each value, about what f32 sums round off. Weights likewise, in f32 calls;
 //   f16 calls round each weight to f16 once, half an ulp of the result's own type, in errors that average out over the
-//   positions. A weight carries the value scale of its block divided by a running power of two at least as large as all
-//   of them, times 2^6, so that small weights stay clear of f16's subnormals and large ones of its infinity.
+//   positions. A weight carries the value scale of its block over a unit, a power of two above all value scales so far, and
+//   the base that a row's exponentials are relative to follows the largest product of exponential and value scale that the
+//   row has seen, not the largest exponential: so the weights of every row reach 2^6, clear of f16's subnormals and of its
+//   infinity, whatever the scales of blocks are that the row does not see or gives no weight to.
 #include <algorithm>
 #include <type_traits>
 
@@ -159,12 +161,62 @@ struct Blocks {
 
 // The running state of 16 query rows: the base that exponents are relative to, this lane's share of the sum, and the
 // output, transposed: lane 16 g + r holds row r, register [4 c + i][s] dimension 64 c + 16 g + 4 s + i.
-// The base is a maximum that the row has had, and no later score exceeds it by more than kSlack: only then does it move
-// and the output with it (16 registers per 64 dimensions and row tile), so that most tiles need neither that nor the
-// maximum over the row's four lanes. Weights, up to 2^kSlack, stay clear of f16's largest number because their unit leaves
-// that much room; their smallest step is 2^-31 of the base's weight.
-constexpr float kSlack = 8.0f, kMost = 0x1p8f;  // and 2^kSlack
-constexpr int kRoom = 6;  // weights are below 2^(kRoom + kSlack)
+// The base is the largest x + level that the row has had, x a score (log2) and level the exponent of its block's value scale
+// over the unit (see Unit; below 0, and -kDepth at least), and no later one exceeds it by more than kSlack: only then does
+// it move and the output with it (16 registers per 64 dimensions and row tile), so that most tiles need neither that nor the
+// maximum over the row's four lanes. The weight at the base, with the value scale, is in [2^kRoom, 2^(kRoom + 1)), so that
+// weights stay below 2^15 and the smallest step of an f16, 2^-24, is 2^-30 of it. Without the value scale it is at most
+// 2^(kDepth + kSlack), far enough from f32's end for sums of them. A row whose value scales, weighted, are more than
+// 2^kDepth below the unit loses a bit of its weights for each power of two beyond.
+constexpr float kSlack = 8.0f;
+constexpr int kRoom = 6, kDepth = 80;
+constexpr float kMostWeight = 0x1p15f;                          // of a lane's weights of a tile together
+constexpr float kMostBare = kMostWeight / 0x1p88f;              // and of those without the value scale, 2^(kDepth + kSlack)
+
+// A tile's scales, the same for every lane.
+struct Scales {
+    float key[4], weight[4];
+    float level[4];  // exponents of the value scales over the unit
+    int grown;       // powers of two by which the unit grew
+    uint32_t ok;     // bits of the blocks that exist
+    uint32_t nan;    // and of those with a NaN scale: they count as zeros here, see Rows::poison
+};
+
+// The value scales' running unit, a power of two above all of them so far and at least 2^-110, as its biased exponent (0:
+// none yet). Weights are value scales over it, times 2^kRoom.
+struct Unit {
+    int e = 0;
+    // The scales of the tile whose first block is lane i0 of bl; the unit grows where it has to.
+    __device__ __forceinline__ Scales next(const Blocks& bl, int i0) {
+        Scales t;
+        int v[4], top = 17 << 23;
+        t.ok = (uint32_t)(bl.ok >> i0) & 15u;
+        t.nan = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            int k = __builtin_amdgcn_readlane(__builtin_bit_cast(int, bl.ck), i0 + b);
+            v[b] = __builtin_amdgcn_readlane(__builtin_bit_cast(int, bl.cv), i0 + b);
+            const bool bad = max(k, v[b]) >= 0x7f800000;  // scales are never negative
+            t.nan |= bad ? 1u << b : 0u;
+            k = bad ? 0 : k;
+            v[b] = bad ? 0 : v[b];
+            t.key[b] = __builtin_bit_cast(float, k);
+            top = max(top, v[b]);
+        }
+        const int unit = max(e, min((top >> 23) + 1, 253));
+        t.grown = e ? unit - e : 0;  // no row has an output before the first tile
+        e = unit;
+        const float inv = __builtin_bit_cast(float, (127 + kRoom + 127 - unit) << 23);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            t.weight[b] = __builtin_bit_cast(float, v[b]) * inv;
+            t.level[b] = (float)max((v[b] >> 23) - unit, -kDepth);
+        }
+        return t;
+    }
+    // What the output is multiplied by at the end.
+    __device__ __forceinline__ float back() const { return e ? __builtin_bit_cast(float, (e - kRoom) << 23) : 0.0f; }
+};
 
 template <typename T, int kC>
 struct Rows {
@@ -199,28 +251,32 @@ struct Rows {
             if ((nan >> b) & 1u) l = pos0 + 16 * b < vis ? __builtin_nanf("") : l;
     }
 
-    // Moves the base where a score passes it by too much, and the output with it; shrink: what the value scales' unit asks
-    // for.
-    __device__ __forceinline__ void settle(const f4 (&x)[4], const float (&f)[4], float shrink, float slack) {
+    // Moves the base where a score passes it by too much, and the output with it. Where the unit grew, the levels of the
+    // scores so far fall: the base falls with them, so that later weights reach 2^kRoom again, as far as the sum has room.
+    __device__ __forceinline__ void settle(const f4 (&x)[4], const float (&f)[4], const Scales& sc, float slack) {
         float top = -__builtin_inff();
 #pragma unroll
         for (int b = 0; b < 4; ++b)
-            top = __builtin_fmaxf(top, fmax2(fmax2(x[b][0], x[b][1]), fmax2(x[b][2], x[b][3])) * f[b]);
-        if (__any(top > m + slack) || shrink != 1.0f) {
+            top = __builtin_fmaxf(top, __builtin_fmaf(fmax2(fmax2(x[b][0], x[b][1]), fmax2(x[b][2], x[b][3])), f[b], sc.level[b]));
+        if (__any(top > m + slack) || sc.grown) {
             const float was = m;
+            if (sc.grown) {
+                const int most = (int)(__builtin_bit_cast(uint32_t, over_groups(l, fmax2)) >> 23) - 127;
+                m -= (float)min(sc.grown, max(kDepth - max(most, 0), 0));
+            }
             m = __builtin_fmaxf(m, over_groups(top, fmax2));
             const float alpha = m == was ? 1.0f : __builtin_amdgcn_exp2f(was - m);
             l *= alpha;
-            const float a = alpha * shrink;
+            const float a = __builtin_ldexpf(alpha, -sc.grown);
 #pragma unroll
             for (int i = 0; i < 4 * kC; ++i) o[i] *= a;
         }
     }
 
     // The weights as operands w, two blocks to each (and their low halves lo); their sum, without the value scales, joins
-    // `sum`.
-    __device__ __forceinline__ void weigh(const f4 (&x)[4], const float (&f)[4], const float (&weight)[4], h8 (&w)[2],
-                                          h8 (&lo)[2], float& sum) const {
+    // `sum`, and with them `load`.
+    __device__ __forceinline__ void weigh(const f4 (&x)[4], const float (&f)[4], const Scales& sc, h8 (&w)[2], h8 (&lo)[2],
+                                          float& sum, float& load) const {
         // a row that has seen nothing yet: subtract 0, so that its weights are 2^-inf = 0 and not NaN
         const float base = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
@@ -229,7 +285,7 @@ struct Rows {
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 p[s] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][s], f[b], -base));
-                float v = p[s] * weight[b];
+                float v = p[s] * sc.weight[b];
                 // the halves are of one number: without this the compiler may round the product straight to f16 for one
                 // use of hi and the f32 product for the other, which differ where the product is close to a tie
                 if constexpr (kSplit) asm("" : "+v"(v));
@@ -237,51 +293,11 @@ struct Rows {
                 w[b >> 1][4 * (b & 1) + s] = hi;
                 if constexpr (kSplit) lo[b >> 1][4 * (b & 1) + s] = (_Float16)(v - (float)hi);
             }
-            sum += (p[0] + p[1]) + (p[2] + p[3]);
+            const float of_block = (p[0] + p[1]) + (p[2] + p[3]);
+            sum += of_block;
+            load = __builtin_fmaf(of_block, sc.weight[b], load);
         }
     }
-};
-
-// A tile's scales, the same for every lane.
-struct Scales {
-    float key[4], weight[4];
-    float shrink;  // what the output so far is multiplied by, as the unit grew
-    uint32_t ok;   // bits of the blocks that exist
-    uint32_t nan;  // and of those with a NaN scale: they count as zeros here, see Rows::poison
-};
-
-// The value scales' running unit, a power of two above all of them so far and at least 2^-110, as its biased exponent (0:
-// none yet). Weights are value scales over it, times 2^kRoom.
-struct Unit {
-    int e = 0;
-    // The scales of the tile whose first block is lane i0 of bl; the unit grows where it has to.
-    __device__ __forceinline__ Scales next(const Blocks& bl, int i0) {
-        Scales t;
-        int v[4], top = 17 << 23;
-        t.ok = (uint32_t)(bl.ok >> i0) & 15u;
-        t.nan = 0;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            int k = __builtin_amdgcn_readlane(__builtin_bit_cast(int, bl.ck), i0 + b);
-            v[b] = __builtin_amdgcn_readlane(__builtin_bit_cast(int, bl.cv), i0 + b);
-            const bool bad = max(k, v[b]) >= 0x7f800000;  // scales are never negative
-            t.nan |= bad ? 1u << b : 0u;
-            k = bad ? 0 : k;
-            v[b] = bad ? 0 : v[b];
-            t.key[b] = __builtin_bit_cast(float, k);
-            top = max(top, v[b]);
-        }
-        const int grown = max(e, min((top >> 23) + 1, 253));
-        t.shrink = __builtin_bit_cast(float, max(127 + e - grown, 0) << 23);
-        e = grown;
-        const float inv = __builtin_bit_cast(float, (127 + kRoom + 127 - grown) << 23);
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-            t.weight[b] = __builtin_bit_cast(float, v[b]) * inv;
-        return t;
-    }
-    // What the output is multiplied by at the end.
-    __device__ __forceinline__ float back() const { return e ? __builtin_bit_cast(float, (e - kRoom) << 23) : 0.0f; }
 };
 
 // What a launch needs besides the cache.
@@ -430,8 +446,9 @@ __device__ __forceinline__ void rows_tiles(const Kv8View& c, const AttnArgs& a, 
         h8 w[2], lo[2];
         if (pos0 + kTile > all_see || sc.ok != 15u) st.mask(x, f, pos0 + 4 * g, vis, sc.ok);
         if (sc.nan) st.poison(sc.nan, pos0, vis);
-        st.settle(x, f, sc.shrink, kSlack);
-        st.weigh(x, f, sc.weight, w, lo, st.l);
+        st.settle(x, f, sc, kSlack);
+        float load = 0.0f;
+        st.weigh(x, f, sc, w, lo, st.l, load);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -921,27 +938,30 @@ __global__ __launch_bounds__(256 * kG, 2) void kv8_tile_kernel(Kv8View c, AttnAr
         h8 w[kCt][2], lo[kCt][2];
         if constexpr (Query<T, kC>::kSplit) {
 #pragma unroll
-            for (int ct = 0; ct < kCt; ++ct) st[ct].settle(x[ct], f[ct], sc.shrink, kSlack);
+            for (int ct = 0; ct < kCt; ++ct) st[ct].settle(x[ct], f[ct], sc, kSlack);
+            float load = 0.0f;
 #pragma unroll
-            for (int ct = 0; ct < kCt; ++ct) st[ct].weigh(x[ct], f[ct], sc.weight, w[ct], lo[ct], st[ct].l);
+            for (int ct = 0; ct < kCt; ++ct) st[ct].weigh(x[ct], f[ct], sc, w[ct], lo[ct], st[ct].l, load);
         } else {
-            // No maximum over the scores: the weights from the base as it is, and again from a new one where their sum says
-            // that one may be past the slack (2,000 of 8,000 tokens, f16: 14 heads of 64 over 2 398 -> 361 us, 32 of 128
+            // No maximum over the scores: the weights from the base as it is, and again from a new one where their sums, with
+            // and without the value scales, say that one may be too large (2,000 of 8,000 tokens, f16: 14 heads of 64 over 2 398 -> 361 us, 32 of 128
             // over 8 1,030 -> 1,001; f32, with more registers to keep, 32 of 128 over 8 1,402 and 1,543).
             float sum[kCt];
-            bool move = sc.shrink != 1.0f;
+            bool move = sc.grown != 0;
 #pragma unroll
             for (int ct = 0; ct < kCt; ++ct) {
                 sum[ct] = 0.0f;
-                st[ct].weigh(x[ct], f[ct], sc.weight, w[ct], lo[ct], sum[ct]);
-                move |= !(sum[ct] <= kMost) || st[ct].m == -__builtin_inff();
+                float load = 0.0f;
+                st[ct].weigh(x[ct], f[ct], sc, w[ct], lo[ct], sum[ct], load);
+                move |= !(__builtin_fmaf(sum[ct], kMostBare, load) <= kMostWeight) || st[ct].m == -__builtin_inff();
             }
             if (__any(move)) {
 #pragma unroll
                 for (int ct = 0; ct < kCt; ++ct) {
-                    st[ct].settle(x[ct], f[ct], sc.shrink, 0.0f);
+                    st[ct].settle(x[ct], f[ct], sc, 0.0f);
                     sum[ct] = 0.0f;
-                    st[ct].weigh(x[ct], f[ct], sc.weight, w[ct], lo[ct], sum[ct]);
+                    float load = 0.0f;
+                    st[ct].weigh(x[ct], f[ct], sc, w[ct], lo[ct], sum[ct], load);
                 }
             }
 #pragma unroll

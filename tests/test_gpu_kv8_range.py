@@ -1,0 +1,111 @@
+"""Attention over the 8-bit cache where value scales lie far apart: blocks that a row does not see, or gives no weight to, do
+not take bits from it. Bounds (kv8_bound) use only what a row sees."""
+import numpy as np
+import pytest
+
+from kv8_bound import exact_attention, worst
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _gpu(gpu):
+    return gpu
+
+
+def ints(x):
+    import torch
+    return torch.tensor(list(x), dtype=torch.int32, device="cuda")
+
+
+def starts(counts):
+    return ints(np.concatenate([[0], np.cumsum(counts)]))
+
+
+def filled(qh, k, v, lens, page=32, seq_pages=None):
+    """A cache that holds the rows k and v of sequences of these lengths."""
+    need = [-(-n // page) for n in lens]
+    c = qh.KV8Cache(1, sum(need) + 1, page, k.shape[1], k.shape[2], len(lens), seq_pages or max(need))
+    c.pages.fill_(0x7f)
+    c.resize(ints(range(len(lens))), ints(lens))
+    c.append(0, k, v, start=starts(lens))
+    return c
+
+
+def randn(seed, *shape):
+    import torch
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seed)
+    return torch.randn(*shape, device="cuda", generator=gen)
+
+
+def check(c, q, counts, seqs=None, single=False, causal=True):
+    import torch
+    seqs = list(range(len(counts))) if seqs is None else seqs
+    got = c.attention(0, q, start=None if single else starts(counts), seqs=ints(seqs), causal=causal)
+    want, bound = exact_attention(c, 0, q, seqs, counts, causal)
+    assert torch.isfinite(got).all()
+    ratio, at = worst(got, want, bound)
+    assert ratio <= 1, (ratio, at, float(got[at]), float(want[at]))
+
+
+# the largest values over the others: f16 rows reach no further than 2^26 (6e4 over 1e-3)
+RATIOS = [("float32", 2.0 ** 14), ("float32", 2.0 ** 22), ("float32", 1e10), ("float32", 1e20), ("float16", 2.0 ** 15)]
+
+
+@pytest.mark.parametrize("dtype,ratio", RATIOS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows,heads,seq_pages", [(3, 2, 40), (4, 2, 80), (70, 2, 40), (300, 2, 80), (300, 40, 40)])
+def test_a_large_value_behind_the_row(qh, dtype, ratio, hd, rows, heads, seq_pages):
+    """The last token holds a value `ratio` times the others: the rows before it do not see it. Tables on both sides of the
+    few-row kernels' and the splits' rules."""
+    import torch
+    n, t = 317, getattr(torch, dtype)
+    k, v = randn(1, n, 2, hd), randn(2, n, 2, hd) * (1.0 if dtype == "float32" else 2.0 ** -6)
+    v[-1] *= ratio
+    c = filled(qh, k.to(t), v.to(t), [n], seq_pages=seq_pages)
+    check(c, randn(3, rows, heads, hd).to(t), [rows])
+
+
+@pytest.mark.parametrize("dtype,ratio", RATIOS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows,seq_pages,at", [(1, 40, 5), (1, 90, 70), (6, 90, 40), (90, 40, 33), (300, 90, 130), (1, 40, 316)])
+def test_a_large_value_without_weight(qh, dtype, ratio, hd, rows, seq_pages, at):
+    """A visible block with a value `ratio` times the others and scores so low that it counts for nothing: first,
+    in the middle and last, with tiles of ordinary values behind it."""
+    import torch
+    n, t = 317, getattr(torch, dtype)
+    k, v = randn(1, n, 1, hd), randn(2, n, 1, hd) * (1.0 if dtype == "float32" else 2.0 ** -6)
+    q = randn(3, rows, 4, hd)
+    q[..., 0] = 8.0 * hd ** 0.5  # the first channel says: a score of 8 times the key's
+    k[..., 0] = 0.0
+    k[at // 16 * 16:at // 16 * 16 + 16, :, 0] = -25.0  # e^-200, for the block that the value gives its scale
+    v[at] *= ratio
+    c = filled(qh, k.to(t), v.to(t), [n], seq_pages=seq_pages)
+    check(c, q.to(t), [rows])
+    if rows == 1:
+        check(c, q.to(t), [1], single=True)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("rows,seq_pages", [(1, 40), (1, 90), (6, 90), (90, 40), (400, 90)])
+def test_values_of_every_size_in_any_order(qh, dtype, rows, seq_pages):
+    """Blocks of 16 tokens whose values are 2^-40 to 2^40 apart (2^-12 to 2^12 in f16), zeros among them, with scores that
+    prefer small ones, large ones or none."""
+    import torch
+    n, hd, t, far = 640, 64, getattr(torch, dtype), 40 if dtype == "float32" else 12
+    rng = np.random.default_rng(7)
+    for slope in (-1.0, -0.3, 0.0, 0.7):
+        size = rng.integers(-far, far + 1, n // 16)
+        k, v = randn(1, n, 2, hd), randn(2, n, 2, hd)
+        lift = torch.from_numpy(np.repeat(size, 16).astype(np.float32)).to("cuda").view(-1, 1)
+        v *= torch.exp2(lift).unsqueeze(-1)
+        v[16 * 7:16 * 8] = 0
+        v[:16] = 0
+        k[..., 0] = lift * slope * float(np.log(2.0))
+        k[16 * 7:16 * 8, :, 0] = 10.0  # zeros that nearly all the weight goes to in some rows
+        q = randn(3, rows, 4, hd)
+        q[..., 0] = hd ** 0.5
+        c = filled(qh, k.to(t), v.to(t), [n], seq_pages=seq_pages)
+        check(c, q.to(t), [rows])
+        check(c, q.to(t), [rows], causal=False)
