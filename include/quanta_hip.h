@@ -359,7 +359,9 @@ size_t qh_kv8_attention_workspace_bytes(const qh_kv8_cache* c, int n_heads, int 
  * that are not the queries' own: an entry may then have more rows than the sequence has tokens). Query head h reads KV
  * head h / (n_heads / n_kv_heads). A row that sees nothing (an empty sequence, or a position below 0) is 0. out may not
  * overlap q. A row of q that is not finite gives NaN, and so does a visible token that reads as NaN. Sums in f32; f32
- * queries and weights go through the matrix instructions as two f16 each, f16 calls' weights as one. A weight is also held
+ * queries and weights go through the matrix instructions as two f16 each, and so do the weights of f16 calls, but for
+ * prompts (more than 32 rows of a KV head's queries to an entry), whose weights are rounded to one f16: a caller who wants two
+ * there too passes the queries in f32. A weight is also held
  * to 2^-31 of the largest product of weight and value scale that its row sees (what storing that scale's block rounded off is
  * 2^-1 of the product); blocks that a row does not see, or gives no weight to, take nothing from it, up to scales 2^80 times
  * its own. */

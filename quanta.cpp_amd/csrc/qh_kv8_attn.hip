@@ -10,9 +10,12 @@
 // lane's weights are already the operand of the second product (values . weights, transposed too): no weight passes
 // through shared memory, and a row's maximum and sum belong to one lane column.
 //   f32 queries are split into two f16 (22 bits), scaled by a power of two so that the row's largest value has exponent
-//   13: what the split drops is below 2^-22 of each value, about what f32 sums round off. Weights likewise, in f32 calls;
-//   f16 calls round each weight to f16 once, half an ulp of the result's own type, in errors that average out over the
-//   positions. A weight carries the value scale of its block over a unit, a power of two above all value scales so far, and
+//   13: what the split drops is below 2^-22 of each value, about what f32 sums round off. Weights likewise, but for prompts
+//   in f16 calls, which round each weight to f16 once: half an ulp of the result's own type, for half of the second product
+//   (4 x 2,000 tokens over 8,000, 32 heads of 128 over 8: 392 us, with two halves 521; error against 64 bits 2.9e-4 and
+//   2.1e-4, which is the result's own rounding). Few rows wait for memory, and two halves cost them nothing (48 conversations
+//   of those heads 53.0 and 53.3 us).
+//   A weight carries the value scale of its block over a unit, a power of two above all value scales so far, and
 //   the base that a row's exponentials are relative to follows the largest product of exponential and value scale that the
 //   row has seen, not the largest exponential: so the weights of every row reach 2^6, clear of f16's subnormals and of its
 //   infinity, whatever the scales of blocks are that the row does not see or gives no weight to.
@@ -218,9 +221,9 @@ struct Unit {
     __device__ __forceinline__ float back() const { return e ? __builtin_bit_cast(float, (e - kRoom) << 23) : 0.0f; }
 };
 
-template <typename T, int kC>
+// kTwo: weights as two f16 each, else one.
+template <int kC, bool kTwo>
 struct Rows {
-    static constexpr bool kSplit = std::is_same<T, float>::value;
     float m = -__builtin_inff(), l = 0.0f;
     f4 o[4 * kC];
 
@@ -288,10 +291,10 @@ struct Rows {
                 float v = p[s] * sc.weight[b];
                 // the halves are of one number: without this the compiler may round the product straight to f16 for one
                 // use of hi and the f32 product for the other, which differ where the product is close to a tie
-                if constexpr (kSplit) asm("" : "+v"(v));
+                if constexpr (kTwo) asm("" : "+v"(v));
                 const _Float16 hi = (_Float16)v;
                 w[b >> 1][4 * (b & 1) + s] = hi;
-                if constexpr (kSplit) lo[b >> 1][4 * (b & 1) + s] = (_Float16)(v - (float)hi);
+                if constexpr (kTwo) lo[b >> 1][4 * (b & 1) + s] = (_Float16)(v - (float)hi);
             }
             const float of_block = (p[0] + p[1]) + (p[2] + p[3]);
             sum += of_block;
@@ -415,7 +418,7 @@ __device__ __forceinline__ void rows_tiles(const Kv8View& c, const AttnArgs& a, 
     const int all_see = visible(e, a, r0);  // positions that every row sees: the first row's
     Query<T, kC> q;
     q.convert(raw, valid, a.scale_log2e);
-    Rows<T, kC> st;
+    Rows<kC, true> st;
     st.clear();
     Unit unit;
 
@@ -460,7 +463,7 @@ __device__ __forceinline__ void rows_tiles(const Kv8View& c, const AttnArgs& a, 
                     const h8 v = codes8_to_f16(a0[i], a1[i]);
                     f4& o = st.o[4 * cc + i];
                     o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[u], o, 0, 0, 0);
-                    if constexpr (Query<T, kC>::kSplit) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[u], o, 0, 0, 0);
+                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[u], o, 0, 0, 0);
                 }
             }
         __builtin_amdgcn_sched_barrier(0);
@@ -812,7 +815,7 @@ __global__ __launch_bounds__(256 * kG, 2) void kv8_tile_kernel(Kv8View c, AttnAr
     const int steps = (end - first + kG - 1) / kG, t0 = first + grp * steps, t1 = min(t0 + steps, end);  // the group's
 
     Query<T, kC> q[kCt];
-    Rows<T, kC> st[kCt];
+    Rows<kC, Query<T, kC>::kSplit> st[kCt];
     int vis[kCt];
 #pragma unroll
     for (int ct = 0; ct < kCt; ++ct) {

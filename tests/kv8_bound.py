@@ -2,6 +2,7 @@
 and how far a result may be off: from the roundings of each step, of positions that the row sees and nothing else.
 
 The values read back are checked against the plain model (kv8_util) bit for bit elsewhere."""
+import numpy as np
 import torch
 
 HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11}  # half a step of the format, relative to a value
@@ -18,8 +19,9 @@ def value_scales(cache, layer, seq):
     return raw.view(-1, 2, kv, per)[:, 1].transpose(1, 2).reshape(-1, kv).double()
 
 
-def exact_attention(cache, layer, q, seqs, counts, causal=True, scale=None):
-    """(out, bound) of rows q [rows][heads][hd] in 64 bits. A row that sees nothing is 0.
+def exact_attention(cache, layer, q, seqs, counts, causal=True, scale=None, two=None):
+    """(out, bound) of rows q [rows][heads][hd] in 64 bits; two: weights as two f16 each (None: in f32 calls). A row that
+    sees nothing is 0.
 
     A score is off by dx: the f32 query in two f16 (2^-22 of each value and, in f16's subnormals, 2^-38 of the row's largest;
     an f16 query is exact), 2 hd products summed (hd for f16 queries), and 8 roundings of unit, scales and products. The
@@ -33,6 +35,7 @@ def exact_attention(cache, layer, q, seqs, counts, causal=True, scale=None):
     out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
     bound = torch.zeros_like(out)
     row, f32 = 0, q.dtype == torch.float32
+    two = f32 if two is None else two
     start = lambda n: torch.tensor([0, n], dtype=torch.int32, device=q.device)
     for s, m in zip(seqs, counts):
         n = int(cache.lens[s]) if 0 <= s < cache.n_seqs else 0
@@ -64,7 +67,7 @@ def exact_attention(cache, layer, q, seqs, counts, causal=True, scale=None):
                 dx = dx + 2.0 ** -38 * x.abs().amax(1) * far * abs(scale)
             else:
                 dx = size * (hd + 8) * 2.0 ** -24
-            rel = 2 * dx + 10 * 2.0 ** -24 + (2.0 ** -22 if f32 else 2.0 ** -11) + 2 * (seen + 32) * 2.0 ** -24
+            rel = 2 * dx + 10 * 2.0 ** -24 + (2.0 ** -22 if two else 2.0 ** -11) + 2 * (seen + 32) * 2.0 ** -24
             largest = (p * d[None, :, g]).amax(1)
             codes = (av / d[:, g, None].clamp(min=1e-300))
             codes = (~hidden).double() @ codes
@@ -82,3 +85,29 @@ def worst(got, want, bound):
     ratio = torch.where(torch.isnan(ratio), torch.full_like(ratio, 1e12), ratio)
     i = int(ratio.argmax())
     return float(ratio.flatten()[i]), tuple(int(t) for t in torch.unravel_index(torch.tensor(i), ratio.shape))
+
+
+# ---- caches and inputs of the tests
+
+def ints(x):
+    return torch.tensor(list(x), dtype=torch.int32, device="cuda")
+
+
+def starts(counts):
+    return ints(np.concatenate([[0], np.cumsum(counts)]))
+
+
+def filled(qh, k, v, lens, page=32, seq_pages=None):
+    """A cache that holds the rows k and v of sequences of these lengths."""
+    need = [-(-n // page) for n in lens]
+    c = qh.KV8Cache(1, sum(need) + 1, page, k.shape[1], k.shape[2], len(lens), seq_pages or max(need))
+    c.pages.fill_(0x7f)
+    c.resize(ints(range(len(lens))), ints(lens))
+    c.append(0, k, v, start=starts(lens))
+    return c
+
+
+def randn(seed, *shape):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seed)
+    return torch.randn(*shape, device="cuda", generator=gen)

@@ -3,7 +3,7 @@ not take bits from it. Bounds (kv8_bound) use only what a row sees."""
 import numpy as np
 import pytest
 
-from kv8_bound import exact_attention, worst
+from kv8_bound import exact_attention, filled, ints, randn, starts, worst
 
 pytestmark = pytest.mark.gpu
 
@@ -11,32 +11,6 @@ pytestmark = pytest.mark.gpu
 @pytest.fixture(autouse=True)
 def _gpu(gpu):
     return gpu
-
-
-def ints(x):
-    import torch
-    return torch.tensor(list(x), dtype=torch.int32, device="cuda")
-
-
-def starts(counts):
-    return ints(np.concatenate([[0], np.cumsum(counts)]))
-
-
-def filled(qh, k, v, lens, page=32, seq_pages=None):
-    """A cache that holds the rows k and v of sequences of these lengths."""
-    need = [-(-n // page) for n in lens]
-    c = qh.KV8Cache(1, sum(need) + 1, page, k.shape[1], k.shape[2], len(lens), seq_pages or max(need))
-    c.pages.fill_(0x7f)
-    c.resize(ints(range(len(lens))), ints(lens))
-    c.append(0, k, v, start=starts(lens))
-    return c
-
-
-def randn(seed, *shape):
-    import torch
-    gen = torch.Generator(device="cuda")
-    gen.manual_seed(seed)
-    return torch.randn(*shape, device="cuda", generator=gen)
 
 
 def check(c, q, counts, seqs=None, single=False, causal=True):
