@@ -312,7 +312,7 @@ struct AttnArgs {
     int group;  // query heads to a KV head; the rows of an entry are (token, head of the group)
     int causal;
     float scale_log2e;
-    float* part_o;   // partial outputs [slot][n_kv][rows][hd], with their maximum and sum [slot][n_kv][rows][2]
+    float* part_o;   // partial outputs, means [slot][n_kv][rows][hd], with their base and sum [slot][n_kv][rows][2]
     float* part_ml;
     int4* rec;       // [items] where an item's partials are: first slot, how many (0: none), first row, rows
     int items, splits;
@@ -340,13 +340,15 @@ __device__ __forceinline__ int visible(const Entry& e, const AttnArgs& a, int r)
     return a.causal ? min(max(e.len - e.tokens + r / a.group + 1, 0), e.len) : e.len;
 }
 
-// A row's share of the output, 4 values at dimension d: divided by the row's sum, zero where it saw nothing. kX8: 8 lanes
-// in a row hold 32 values of a row, and write them in 8 bits too where the call asks for that.
+// a over a row's sum of weights, zero where it saw nothing. Outputs are weighted means before they meet, never sums of values,
+// which may be past f32's largest number where no value is.
+__device__ __forceinline__ float over_sum(float a, float l) { return l == 0.0f ? 0.0f : a / l; }
+
+// 4 values of the output. kX8: 8 lanes in a row hold 32 values of a row, and write them in 8 bits too where the call asks for
+// that.
 template <typename T, bool kX8>
-__device__ __forceinline__ void store_out(const AttnArgs& a, T* out, float4 o, float m, float l) {
-    const float inv = m == -__builtin_inff() ? 0.0f : 1.0f / l;
+__device__ __forceinline__ void store_out(const AttnArgs& a, T* out, float4 v) {
     if constexpr (std::is_same<T, float>::value) {
-        const float4 v = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
         *reinterpret_cast<float4*>(out) = v;
         if (kX8 && a.oq) {
             const int64_t at = (out - static_cast<float*>(a.out)) & ~31ll;
@@ -354,8 +356,7 @@ __device__ __forceinline__ void store_out(const AttnArgs& a, T* out, float4 o, f
         }
     } else {
         typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-        *reinterpret_cast<h4*>(out) = h4{(_Float16)(o.x * inv), (_Float16)(o.y * inv), (_Float16)(o.z * inv),
-                                         (_Float16)(o.w * inv)};
+        *reinterpret_cast<h4*>(out) = h4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
     }
 }
 template <typename T>
@@ -472,7 +473,7 @@ __device__ __forceinline__ void rows_tiles(const Kv8View& c, const AttnArgs& a, 
 
     // the waves' results of this item together
     const float l = over_groups(st.l, [](float p, float q2) { return p + q2; });
-    const float back = unit.back();
+    const float mean = over_sum(unit.back(), l);
     if (g == 0) {
         sh.sm[wave][col] = st.m;
         sh.sl[wave][col] = l;
@@ -482,8 +483,8 @@ __device__ __forceinline__ void rows_tiles(const Kv8View& c, const AttnArgs& a, 
 #pragma unroll
         for (int s = 0; s < 4; ++s)
             *reinterpret_cast<float4*>(&sh.so[wave][col][64 * cc + 16 * g + 4 * s]) =
-                make_float4(st.o[4 * cc][s] * back, st.o[4 * cc + 1][s] * back, st.o[4 * cc + 2][s] * back,
-                            st.o[4 * cc + 3][s] * back);
+                make_float4(st.o[4 * cc][s] * mean, st.o[4 * cc + 1][s] * mean, st.o[4 * cc + 2][s] * mean,
+                            st.o[4 * cc + 3][s] * mean);
     __syncthreads();
     const int rr = (tid >> 4) & 15, d0 = 4 * (tid & 15);
     if (r0 + rr < e.rows) {
@@ -494,9 +495,12 @@ __device__ __forceinline__ void rows_tiles(const Kv8View& c, const AttnArgs& a, 
         float f[kW], lsum = 0.0f;
 #pragma unroll
         for (int w2 = 0; w2 < kW; ++w2) {
-            f[w2] = __builtin_amdgcn_exp2f(sh.sm[w2][rr] - base);
-            lsum = __builtin_fmaf(f[w2], sh.sl[w2][rr], lsum);
+            f[w2] = __builtin_amdgcn_exp2f(sh.sm[w2][rr] - base) * sh.sl[w2][rr];
+            lsum += f[w2];
         }
+        const float inv = over_sum(1.0f, lsum);
+#pragma unroll
+        for (int w2 = 0; w2 < kW; ++w2) f[w2] *= inv;
         const size_t pr = ((size_t)slot * c.n_kv + kvh) * kRowTile + rr;
         for (int cc = tid >> 8; cc < kC; cc += kW / 4) {
             float4 o = make_float4(0, 0, 0, 0);
@@ -509,7 +513,7 @@ __device__ __forceinline__ void rows_tiles(const Kv8View& c, const AttnArgs& a, 
                 o.w = __builtin_fmaf(f[w2], v.w, o.w);
             }
             if (whole)
-                store_out<T, true>(a, out_row<T>(a, c, e.row0 + r0 + rr, kvh) + 64 * cc + d0, o, top, lsum);
+                store_out<T, true>(a, out_row<T>(a, c, e.row0 + r0 + rr, kvh) + 64 * cc + d0, o);
             else
                 *reinterpret_cast<float4*>(a.part_o + pr * kHd + 64 * cc + d0) = o;
         }
@@ -687,14 +691,14 @@ __global__ __launch_bounds__(64 * kW, 2) void kv8_whole_kernel(Kv8View c, AttnAr
     rows_tiles<T, kC, kW>(c, a, sh, kvh, e, r0, 0, tiles, true, 0);
 }
 
-// Joins an item's partial results: one workgroup per item, KV head and row. First the partials' maxima, a thread to each,
-// and from them every partial's factor; then hd / 4 threads to a partial's row, the workgroup's groups of them taking
+// Joins an item's partial results: one workgroup per item, KV head and row. First the partials' bases, a thread to each,
+// and from them every partial's share; then hd / 4 threads to a partial's row, the workgroup's groups of them taking
 // turns, so that the loads are independent of each other. Partial k is slot first (k = 0) or the k-th even one after.
 template <typename T, int kC>
 __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8View c, AttnArgs a) {
     constexpr int kHd = 64 * kC, kThr = kHd / 4, kGroups = 256 / kThr;
     __shared__ __align__(16) float so[kGroups][kHd];
-    __shared__ float factor[kMaxParts], wave_top[4], wave_sum[4];
+    __shared__ float share[kMaxParts], wave_top[4], wave_sum[4];
     const int4 rec = a.rec[blockIdx.x];
     const int row = (int)blockIdx.z, kvh = (int)blockIdx.y, tid = (int)threadIdx.x, grp = tid / kThr, d = 4 * (tid % kThr);
     if (rec.y == 0 || row >= rec.w) return;
@@ -719,20 +723,20 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8View c, AttnArgs a) {
     for (int j = 0; j < kMaxParts / 256; ++j) {
         const int k = tid + 256 * j;
         if (k < rec.y) {
-            const float f = __builtin_amdgcn_exp2f(m[j] - base);
-            factor[k] = f;
-            l = __builtin_fmaf(f, a.part_ml[2 * at(k) + 1], l);
+            const float f = __builtin_amdgcn_exp2f(m[j] - base) * a.part_ml[2 * at(k) + 1];
+            share[k] = f;
+            l += f;
         }
     }
     l = wave_reduce32x2(l, [](float p, float q) { return p + q; });
     if ((tid & 63) == 0) wave_sum[tid >> 6] = l;
     __syncthreads();
-    l = (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]);
+    const float inv = over_sum(1.0f, (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]));
     float4 o = make_float4(0, 0, 0, 0);
 #pragma unroll 4
     for (int k = grp; k < rec.y; k += kGroups) {
         const float4 v = *reinterpret_cast<const float4*>(a.part_o + at(k) * kHd + d);
-        const float f = factor[k];
+        const float f = share[k] * inv;
         o.x = __builtin_fmaf(f, v.x, o.x);
         o.y = __builtin_fmaf(f, v.y, o.y);
         o.z = __builtin_fmaf(f, v.z, o.z);
@@ -746,7 +750,7 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8View c, AttnArgs a) {
         const float4 v = *reinterpret_cast<const float4*>(&so[k][d]);
         o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
     }
-    store_out<T, true>(a, out_row<T>(a, c, rec.z + row, kvh) + d, o, top, l);
+    store_out<T, true>(a, out_row<T>(a, c, rec.z + row, kvh) + d, o);
 }
 
 // The same for few partials (the splits of the tile kernel): every group of hd / 4 threads joins a row of its own.
@@ -762,19 +766,24 @@ __global__ __launch_bounds__(256) void kv8_join_splits_kernel(Kv8View c, AttnArg
     for (int k = 0; k < rec.y; ++k) top = __builtin_fmaxf(top, a.part_ml[2 * (first + k * next)]);
     const float base = top == -__builtin_inff() ? 0.0f : top;
     float l = 0.0f;
+    for (int k = 0; k < rec.y; ++k) {
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (first + k * next));
+        l = __builtin_fmaf(__builtin_amdgcn_exp2f(ml.x - base), ml.y, l);
+    }
+    const float inv = over_sum(1.0f, l);
     float4 o = make_float4(0, 0, 0, 0);
 #pragma unroll 4
     for (int k = 0; k < rec.y; ++k) {
         const size_t p = first + k * next;
-        const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * p] - base);
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * p);
+        const float f = __builtin_amdgcn_exp2f(ml.x - base) * ml.y * inv;
         const float4 v = *reinterpret_cast<const float4*>(a.part_o + p * kHd + d);
-        l = __builtin_fmaf(f, a.part_ml[2 * p + 1], l);
         o.x = __builtin_fmaf(f, v.x, o.x);
         o.y = __builtin_fmaf(f, v.y, o.y);
         o.z = __builtin_fmaf(f, v.z, o.z);
         o.w = __builtin_fmaf(f, v.w, o.w);
     }
-    store_out<T, false>(a, out_row<T>(a, c, rec.z + row, kvh) + d, o, top, l);
+    store_out<T, false>(a, out_row<T>(a, c, rec.z + row, kvh) + d, o);
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
@@ -1006,9 +1015,12 @@ __global__ __launch_bounds__(256 * kG, 2) void kv8_tile_kernel(Kv8View c, AttnAr
     }
     __builtin_amdgcn_s_setprio(0);
 
-    float back = unit.back();
+    float mean[kCt];  // what makes the output of a row its weighted mean
 #pragma unroll
-    for (int ct = 0; ct < kCt; ++ct) st[ct].l = over_groups(st[ct].l, [](float p, float q2) { return p + q2; });
+    for (int ct = 0; ct < kCt; ++ct) {
+        st[ct].l = over_groups(st[ct].l, [](float p, float q2) { return p + q2; });
+        mean[ct] = over_sum(unit.back(), st[ct].l);
+    }
     if constexpr (kG == 2) {
         // the second group's results to the first
         f4* so = reinterpret_cast<f4*>(lds_all) + (tid & 255);
@@ -1018,7 +1030,7 @@ __global__ __launch_bounds__(256 * kG, 2) void kv8_tile_kernel(Kv8View c, AttnAr
 #pragma unroll
             for (int ct = 0; ct < kCt; ++ct) {
 #pragma unroll
-                for (int n = 0; n < 4 * kC; ++n) so[(ct * 4 * kC + n) * 256] = st[ct].o[n] * back;
+                for (int n = 0; n < 4 * kC; ++n) so[(ct * 4 * kC + n) * 256] = st[ct].o[n] * mean[ct];
                 ml[512 * ct] = st[ct].m;
                 ml[512 * ct + 256] = st[ct].l;
             }
@@ -1029,13 +1041,16 @@ __global__ __launch_bounds__(256 * kG, 2) void kv8_tile_kernel(Kv8View c, AttnAr
         for (int ct = 0; ct < kCt; ++ct) {
             const float m1 = ml[512 * ct], top = __builtin_fmaxf(st[ct].m, m1);
             const float base = top == -__builtin_inff() ? 0.0f : top;
-            const float f0 = __builtin_amdgcn_exp2f(st[ct].m - base), f1 = __builtin_amdgcn_exp2f(m1 - base);
-            st[ct].l = f0 * st[ct].l + f1 * ml[512 * ct + 256];
-#pragma unroll
-            for (int n = 0; n < 4 * kC; ++n) st[ct].o[n] = st[ct].o[n] * (back * f0) + so[(ct * 4 * kC + n) * 256] * f1;
+            const float l0 = __builtin_amdgcn_exp2f(st[ct].m - base) * st[ct].l,
+                        l1 = __builtin_amdgcn_exp2f(m1 - base) * ml[512 * ct + 256];
             st[ct].m = top;
+            st[ct].l = l0 + l1;
+            const float f0 = over_sum(l0, st[ct].l), f1 = over_sum(l1, st[ct].l);
+#pragma unroll
+            for (int n = 0; n < 4 * kC; ++n)
+                st[ct].o[n] = st[ct].o[n] * mean[ct] * f0 + so[(ct * 4 * kC + n) * 256] * f1;
+            mean[ct] = 1.0f;
         }
-        back = 1.0f;
     }
 #pragma unroll
     for (int ct = 0; ct < kCt; ++ct) {
@@ -1047,11 +1062,11 @@ __global__ __launch_bounds__(256 * kG, 2) void kv8_tile_kernel(Kv8View c, AttnAr
         for (int cc = 0; cc < kC; ++cc)
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                const float4 o = make_float4(st[ct].o[4 * cc][s] * back, st[ct].o[4 * cc + 1][s] * back,
-                                             st[ct].o[4 * cc + 2][s] * back, st[ct].o[4 * cc + 3][s] * back);
+                const float4 o = make_float4(st[ct].o[4 * cc][s] * mean[ct], st[ct].o[4 * cc + 1][s] * mean[ct],
+                                             st[ct].o[4 * cc + 2][s] * mean[ct], st[ct].o[4 * cc + 3][s] * mean[ct]);
                 const int d = 64 * cc + 16 * g + 4 * s;
                 if (splits == 1)
-                    store_out<T, false>(a, out + d, o, st[ct].m, st[ct].l);
+                    store_out<T, false>(a, out + d, o);
                 else
                     *reinterpret_cast<float4*>(a.part_o + pr * kHd + d) = o;
             }

@@ -83,3 +83,19 @@ def test_values_of_every_size_in_any_order(qh, dtype, rows, seq_pages):
         c = filled(qh, k.to(t), v.to(t), [n], seq_pages=seq_pages)
         check(c, q.to(t), [rows])
         check(c, q.to(t), [rows], causal=False)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows,n,seq_pages", [(1, 300, 32), (4, 300, 32), (1, 2500, 90), (4, 2500, 90), (90, 300, 32), (90, 2500, 90),
+                                              (90, 2500, 32)])
+def test_values_near_the_end_of_the_range(qh, rows, n, seq_pages, hd):
+    """Values whose sum is past f32's largest number, and their weighted mean is not; in whole rows, shares, halves of a
+    workgroup and splits."""
+    import torch
+    k, v = randn(1, n, 2, hd) * 0.1, 2.9e38 * (1 - 0.2 * torch.sigmoid(randn(2, n, 2, hd)))
+    v[:, :, ::2] *= -1
+    c = filled(qh, k, v, [n], page=32 if n <= 32 * seq_pages else 128, seq_pages=seq_pages)
+    q = randn(3, rows, 6, hd)
+    check(c, q, [rows])
+    if rows == 1:
+        check(c, q, [1], single=True)
