@@ -38,6 +38,7 @@ constexpr int kMaxItems = 1024;      // row tiles of one launch of the row kerne
 constexpr int kWhole = 1024;         // positions up to which a workgroup takes a row tile's sequence whole
 constexpr int kSplitTiles = 5;       // positions of a split of the tile kernel, in tiles, at least
 constexpr int kMaxParts = 512;       // shares of the row kernel: partial results of a row
+constexpr long kMaxTiles = 1l << 30; // tiles of all items of one of its launches, so that counts and sums of them are ints
 
 // Four codes as f16: the stored bytes, code + 128, under the high byte 0x64 are the numbers 1024 + 128 + code.
 __device__ __forceinline__ void codes_to_f16(uint32_t x, uint32_t* out) {
@@ -588,17 +589,21 @@ __global__ __launch_bounds__(64 * kW, 2) void kv8_rows_kernel(Kv8View c, AttnArg
     // 46.8 us, in whole rounds 48.2)
     const int share = max(kW, (all_of(sum, wave_sum) + shares - 1) / shares);
     // items that begin on a share of their own where the shares suffice for that: no workgroup then has two items in turn
-    int padded[kPer];
+    // (counted in shares: in tiles, many short items would pass an int)
+    int own[kPer];
     sum = 0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-        padded[j] = (mine[j] + share - 1) / share * share;
-        sum += padded[j];
+        own[j] = (mine[j] + share - 1) / share;
+        sum += own[j];
     }
-    const bool apart = all_of(sum, wave_sum + kW) <= shares * share;
+    const bool apart = all_of(sum, wave_sum + kW) <= shares;
     sum = 0;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) sum += apart ? padded[j] : mine[j];
+    for (int j = 0; j < kPer; ++j) {
+        mine[j] = apart ? own[j] * share : mine[j];
+        sum += mine[j];
+    }
     int incl = sum;
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
@@ -619,7 +624,7 @@ __global__ __launch_bounds__(64 * kW, 2) void kv8_rows_kernel(Kv8View c, AttnArg
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
         if (j < per && me * per + j < a.items) pre[me * per + j] = at;
-        at += apart ? padded[j] : mine[j];
+        at += mine[j];
     }
     if (me == 0) pre[a.items] = total;
     meet();
@@ -1105,7 +1110,8 @@ Plan plan_of(int group, int n_kv, int hd, int capacity, int n, int n_tok, bool s
     // 12.8), and where their row tiles fill the GPU up to 2,048 (32 tokens of the latter, f16, over 2,048: 22.0 and 25.8; a
     // batch of unlike lengths lasts as long as its longest, and that no longer than the single one)
     const bool whole = capacity <= kWhole || (capacity <= 2 * kWhole && few * n_kv >= cus);
-    const long most = whole ? (1 << 23) / n_kv : kMaxItems;  // row tiles of a launch
+    // row tiles of a launch
+    const long most = whole ? (1 << 23) / n_kv : std::min<long>(kMaxItems, kMaxTiles / ((capacity + kTile - 1) / kTile));
     Plan p{};
     if ((single || few <= most) && rows <= 32l * n) {
         // single tokens in launches of as many entries as make that many row tiles (shares: 2,048 sequences of 2,000, 32
