@@ -112,7 +112,7 @@ hipError_t launch_kv8_fork(const Kv8View& c, int n_layers, const int32_t* src, c
                            void* ws, hipStream_t s);
 hipError_t launch_kv8_compact(const Kv8View& c, int n_layers, int32_t* live, void* ws, hipStream_t s);
 // qh_kv8_attn.hip
-// capacity: positions that a sequence can have. oq, od: the f32 rows of out (without gaps) in 8 bits too, as
+// capacity: positions that a sequence can have. oq, od (one entry): the f32 rows of out (without gaps) in 8 bits too, as
 // launch_quantize_q8 makes them.
 size_t kv8_attention_workspace_bytes(int n_heads, int n_kv, int hd, int capacity, int n, int n_tok);
 hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int dtype, int n_heads, int64_t ldq,

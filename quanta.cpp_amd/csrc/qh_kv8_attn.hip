@@ -848,6 +848,7 @@ __global__ __launch_bounds__(256 * kG, 2) void kv8_tile_kernel(Kv8View c, AttnAr
 
     // Each wave stages kPer operands of the keys and of the values, of one block of keys and one pair of blocks of values.
     constexpr int kPer = 8 * kC / kW;
+    static_assert(kPer == 2 || kPer == 4, "loads of whole uint4 of keys, uint2 or uint4 of values");
     const int k_op = wave * kPer, k_blk = k_op / (2 * kC), v_pair = k_op / (4 * kC), v_c = k_op / 4 % kC, v_i = k_op % 4;
     Blocks bl, ahead;
     uint32_t kr[2 * kPer], vr[2][kPer];
@@ -859,15 +860,10 @@ __global__ __launch_bounds__(256 * kG, 2) void kv8_tile_kernel(Kv8View c, AttnAr
             ahead.load(c, e.seq, kvh, tl, tl < t1, e.len);
         }
         const uint8_t* kp = kv8_codes(c, ahead.page_of(4 * j + k_blk), 0, kvh, (t * 4 + k_blk) & per);
-        if constexpr (kPer == 1) {
-            const uint2 x = reinterpret_cast<const uint2*>(kp)[2 * (64 * (k_op / 2 % kC) + lane) + k_op % 2];
-            kr[0] = x.x, kr[1] = x.y;
-        } else {
 #pragma unroll
-            for (int n = 0; n < kPer / 2; ++n) {
-                const uint4 x = reinterpret_cast<const uint4*>(kp)[64 * ((k_op / 2 + n) % kC) + lane];
-                kr[4 * n] = x.x, kr[4 * n + 1] = x.y, kr[4 * n + 2] = x.z, kr[4 * n + 3] = x.w;
-            }
+        for (int n = 0; n < kPer / 2; ++n) {
+            const uint4 x = reinterpret_cast<const uint4*>(kp)[64 * ((k_op / 2 + n) % kC) + lane];
+            kr[4 * n] = x.x, kr[4 * n + 1] = x.y, kr[4 * n + 2] = x.z, kr[4 * n + 3] = x.w;
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -878,11 +874,9 @@ __global__ __launch_bounds__(256 * kG, 2) void kv8_tile_kernel(Kv8View c, AttnAr
             if constexpr (kPer == 4) {
                 const uint4 x = *reinterpret_cast<const uint4*>(vp);
                 vr[k][0] = x.x, vr[k][1] = x.y, vr[k][2] = x.z, vr[k][3] = x.w;
-            } else if constexpr (kPer == 2) {
+            } else {
                 const uint2 x = *reinterpret_cast<const uint2*>(vp);
                 vr[k][0] = x.x, vr[k][1] = x.y;
-            } else {
-                vr[k][0] = *vp;
             }
         }
     };
@@ -1197,7 +1191,6 @@ hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int 
             for (int b = 0; b < n; b += p.entries) {
                 a.q = static_cast<const T*>(q) + (int64_t)b * ldq;  // only single tokens take more than one launch
                 a.out = static_cast<T*>(out) + (int64_t)b * ldo;
-                if (oq) a.oq = oq + (int64_t)b * ldo, a.od = od + (int64_t)b * ldo / 32;
                 if (start == nullptr) {
                     const int m = n - b < p.entries ? n - b : p.entries;
                     a.batch = Kv8Batch{nullptr, seqs ? seqs + b : nullptr, m, m, b};
