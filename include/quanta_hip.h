@@ -369,6 +369,22 @@ int qh_kv8_attention(const qh_kv8_cache* c, int layer, const void* q, void* out,
                      int64_t ldo, const int32_t* start, const int32_t* seqs, int n, int n_tok, int causal, float scale,
                      void* workspace, size_t workspace_bytes, void* stream);
 
+/* Which kernels a qh_kv8_attention call of this shape takes, by its sizes alone (single: start NULL); for profiles, and for
+ * tests that have to reach each of them. */
+enum {
+    QH_KV8_WHOLE = 0,  /* a workgroup takes a row tile's sequence whole */
+    QH_KV8_SHARES = 1, /* the tiles of all sequences in equal shares, which are joined */
+    QH_KV8_TILES = 2   /* many rows: a workgroup to a tile of them */
+};
+typedef struct qh_kv8_plan {
+    int32_t kernel;   /* QH_KV8_WHOLE, QH_KV8_SHARES or QH_KV8_TILES */
+    int32_t rows;     /* of a workgroup's row tile */
+    int32_t waves;    /* of a workgroup */
+    int32_t splits;   /* QH_KV8_SHARES: shares; QH_KV8_TILES: workgroups over a row tile's positions, at most; else 1 */
+    int32_t launches; /* of the kernel, over the batch's entries in turn */
+} qh_kv8_plan;
+int qh_kv8_attention_plan(const qh_kv8_cache* c, int n_heads, int n, int n_tok, int single, qh_kv8_plan* plan);
+
 /* ------------------------------------------------------------------ GPU-resident decoder */
 
 /* FLAG_HADAMARD_DOWN (reference engine/src/model_file.h:19-21): the down projection's input is rotated by the

@@ -80,6 +80,13 @@ class qh_kv8_cache(C.Structure):
         (n, C.c_int32) for n in ("n_layers", "n_pages", "page_tokens", "n_kv_heads", "head_dim", "n_seqs", "seq_pages")]
 
 
+KV8_WHOLE, KV8_SHARES, KV8_TILES = 0, 1, 2  # qh_kv8_plan.kernel
+
+
+class qh_kv8_plan(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("kernel", "rows", "waves", "splits", "launches")]
+
+
 STAGE_QKV, STAGE_ATTENTION, STAGE_O, STAGE_GATE_UP, STAGE_DOWN, STAGES_PER_LAYER = 0, 1, 2, 3, 4, 8
 STAGE_FINAL_NORM, STAGE_HEAD, STAGE_PICK = 1 << 20, (1 << 20) + 1, (1 << 20) + 2
 
@@ -93,6 +100,7 @@ EXPORTS = ("qh_last_error", "qh_version", "qh_init", "qh_quant_bytes", "qh_tenso
            "qh_sampler_state", "qh_sample", "qh_sample_workspace_bytes", "qh_sample_ws",
            "qh_kv8_page_bytes", "qh_kv8_reset", "qh_kv8_pages_workspace_bytes", "qh_kv8_resize", "qh_kv8_fork",
            "qh_kv8_compact", "qh_kv8_append", "qh_kv8_read", "qh_kv8_attention_workspace_bytes", "qh_kv8_attention",
+           "qh_kv8_attention_plan",
            "qh_decoder_create",
            "qh_decoder_destroy",
            "qh_decoder_prefill", "qh_decoder_begin", "qh_decoder_step", "qh_decoder_views",
@@ -142,6 +150,7 @@ def _bind(lib):
         "qh_kv8_attention_workspace_bytes": ([kv8, i32, i32, i32], sz),
         "qh_kv8_attention": ([kv8, i32, vp, vp, i32, i32, C.c_int64, C.c_int64, vp, vp, i32, i32, i32, C.c_float, vp, sz,
                               vp], i32),
+        "qh_kv8_attention_plan": ([kv8, i32, i32, i32, i32, C.POINTER(qh_kv8_plan)], i32),
         "qh_decoder_create": ([C.POINTER(qh_model_desc), C.POINTER(qh_tensor), i32, C.POINTER(vp)], i32),
         "qh_decoder_destroy": ([vp], i32),
         "qh_decoder_prefill": ([vp, vp, i32, i32, i32, vp], i32),
@@ -543,6 +552,12 @@ class KV8Cache:
                             1 if causal else 0, self._scale if scale is None else scale, ws.data_ptr() if need else None,
                             need, self._here()))
         return out
+
+    def attention_plan(self, heads: int, entries: int, rows: int, single: bool = False):
+        """Which kernels `attention` takes for a batch of this shape (qh_kv8_plan; single: without start)."""
+        plan = qh_kv8_plan()
+        _check(lib().qh_kv8_attention_plan(self._ref, heads, entries, rows, int(single), C.byref(plan)))
+        return plan
 
 
 # ------------------------------------------------------------------------------------------------ decoder

@@ -633,6 +633,16 @@ int qh_kv8_attention(const qh_kv8_cache* c, int layer, const void* q, void* out,
                                           causal != 0, scale, workspace, as_stream(stream)), who);
 }
 
+int qh_kv8_attention_plan(const qh_kv8_cache* c, int n_heads, int n, int n_tok, int single, qh_kv8_plan* plan) {
+    const char* who = "qh_kv8_attention_plan";
+    if (int rc = validate_kv8(c, who)) return rc;
+    if (int rc = validate_kv8_heads(*c, n_heads, n, n_tok, who)) return rc;
+    if (!plan || n <= 0 || n_tok <= 0 || (single && n != n_tok))
+        return fail(QH_ERR_ARG, "%s: %d entries over %d rows", who, n, n_tok);
+    *plan = kv8_attention_plan(n_heads, c->n_kv_heads, c->head_dim, c->seq_pages * c->page_tokens, n, n_tok, single != 0);
+    return QH_OK;
+}
+
 int qh_decoder_create(const qh_model_desc* hp, const qh_tensor* tensors, int n_tensors, qh_decoder** out) {
     if (!hp || !tensors || !out) return fail(QH_ERR_ARG, "qh_decoder_create: null argument");
     *out = nullptr;

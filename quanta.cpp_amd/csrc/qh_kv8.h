@@ -115,6 +115,7 @@ hipError_t launch_kv8_compact(const Kv8View& c, int n_layers, int32_t* live, voi
 // capacity: positions that a sequence can have. oq, od (one entry): the f32 rows of out (without gaps) in 8 bits too, as
 // launch_quantize_q8 makes them.
 size_t kv8_attention_workspace_bytes(int n_heads, int n_kv, int hd, int capacity, int n, int n_tok);
+qh_kv8_plan kv8_attention_plan(int n_heads, int n_kv, int hd, int capacity, int n, int n_tok, bool single);
 hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int dtype, int n_heads, int64_t ldq,
                                 int64_t ldo, const int32_t* start, const int32_t* seqs, int n, int n_tok, bool causal,
                                 float scale, void* ws, hipStream_t s, int8_t* oq = nullptr, float* od = nullptr);

@@ -1163,6 +1163,12 @@ size_t kv8_attention_workspace_bytes(int n_heads, int n_kv, int hd, int capacity
     return b;
 }
 
+qh_kv8_plan kv8_attention_plan(int n_heads, int n_kv, int hd, int capacity, int n, int n_tok, bool single) {
+    const Plan p = plan_of(n_heads / n_kv, n_kv, hd, capacity, n, n_tok, single);
+    if (!p.rows) return {QH_KV8_TILES, p.tile, 4 * (p.tile == 64 ? p.groups : 1), p.splits, 1};
+    return {p.whole ? QH_KV8_WHOLE : QH_KV8_SHARES, p.tile, p.waves, p.whole ? 1 : p.shares, (n + p.entries - 1) / p.entries};
+}
+
 hipError_t launch_kv8_attention(const Kv8View& c, const void* q, void* out, int dtype, int n_heads, int64_t ldq,
                                 int64_t ldo, const int32_t* start, const int32_t* seqs, int n, int n_tok, bool causal,
                                 float scale, void* ws, hipStream_t s, int8_t* oq, float* od) {
