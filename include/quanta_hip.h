@@ -310,7 +310,7 @@ size_t qh_kv8_page_bytes(int page_tokens, int n_kv_heads, int head_dim);
 /* Every page free, every sequence empty, status 0 (page contents are left). A new cache's state arrays need it. */
 int qh_kv8_reset(const qh_kv8_cache* c, void* stream);
 
-/* Workspace bytes of qh_kv8_resize, qh_kv8_fork and qh_kv8_compact (4-byte aligned, no initialisation). */
+/* Workspace bytes of qh_kv8_resize, qh_kv8_fork and qh_kv8_compact (16-byte aligned, no initialisation). */
 size_t qh_kv8_pages_workspace_bytes(const qh_kv8_cache* c);
 
 /* Sequence seqs[i] gets length lens[i] (DEVICE arrays of n; each sequence once), for every i of the list at once. First
@@ -350,8 +350,8 @@ int qh_kv8_append(const qh_kv8_cache* c, int layer, const void* k, const void* v
 int qh_kv8_read(const qh_kv8_cache* c, int layer, void* k, void* v, int dtype, int64_t ldk, int64_t ldv,
                 const int32_t* start, const int32_t* seqs, int n, int n_tok, void* stream);
 
-/* Workspace bytes of a qh_kv8_attention call with n entries over n_tok rows (no initialisation; a smaller batch can need
- * more, as it is split further). 0 where it needs none: workspace may be NULL then. */
+/* Workspace bytes of a qh_kv8_attention call with n entries over n_tok rows (16-byte aligned, no initialisation; a smaller
+ * batch can need more, as it is split further). 0 where it needs none: workspace may be NULL then. */
 size_t qh_kv8_attention_workspace_bytes(const qh_kv8_cache* c, int n_heads, int n, int n_tok);
 
 /* Attention of query rows q [n_heads][head_dim] over their sequences: out = sum_j p_j v_j with p = softmax(scale *

@@ -32,3 +32,20 @@ def test_a_launch_counts_its_tiles_in_an_int(qh, seq_pages, entries, launches):
     rc, p = plan(qh, c, heads=2, n=entries, n_tok=entries)
     assert rc == 0 and p.kernel == (qh.KV8_SHARES if entries + entries // 8 <= min(1024, (1 << 30) // (4 * seq_pages)) else
                                     qh.KV8_TILES)
+
+
+def test_workspaces_of_the_alignment_the_header_names(qh):
+    """16 bytes, for the page calls and for attention: every other address is refused, none of those with it is for that."""
+    import os
+    import re
+    from conftest import ROOT
+    from test_kv8_refusals import P, attend
+    text = open(os.path.join(ROOT, "include", "quanta_hip.h")).read()
+    names = re.findall(r"/\* Workspace bytes of (?:a )?(qh_kv8_\w+)[^*]*?\((\d+)-byte aligned", text.replace("\n *", ""))
+    assert names == [("qh_kv8_resize", "16"), ("qh_kv8_attention", "16")]
+    c = cache(qh, seq_pages=128)
+    L, r, need = qh.lib(), C.byref(c), qh.lib().qh_kv8_pages_workspace_bytes(C.byref(c))
+    for off in (4, 8, 12):
+        ws = C.c_void_p(4096 + off)
+        assert L.qh_kv8_resize(r, P, P, 1, ws, need, None) == 4 and L.qh_kv8_fork(r, P, P, 1, 0, ws, need, None) == 4
+        assert L.qh_kv8_compact(r, None, ws, need, None) == 4 and attend(qh, c, ws=ws) == 4
