@@ -341,12 +341,15 @@ int qh_kv8_compact(const qh_kv8_cache* c, int32_t* live, void* workspace, size_t
 /* Stores k and v, rows of [n_kv_heads][head_dim], into layer `layer`: per block d = max|x| / 127 (rounded to f32) and
  * the codes nearest to x / d, halves away from zero. A block that holds earlier tokens keeps the larger of its scale and
  * the new ones', and where that grows its codes are rounded to it. An infinite or NaN value makes its block's scale NaN,
- * so that all 16 tokens of that head read as NaN. Each sequence in one entry at most, and its tokens in order: a block's
+ * so that all 16 tokens of that head read as NaN. A scale never falls: where qh_kv8_resize has cut tokens off inside a block,
+ * the tokens that stay keep the rounding, or the NaN, that those brought, until the block is stored from its first token
+ * again. Each sequence in one entry at most, and its tokens in order: a block's
  * earlier tokens have to be there. Tokens in a page that other sequences hold are left out (QH_KV8_SHARED). */
 int qh_kv8_append(const qh_kv8_cache* c, int layer, const void* k, const void* v, int dtype, int64_t ldk, int64_t ldv,
                   const int32_t* start, const int32_t* seqs, int n, int n_tok, void* stream);
 
-/* The stored values of the entries' tokens: code * d rounded to f32, then to dtype. Tokens without a page read as 0. */
+/* The stored values of the entries' tokens: code * d rounded to f32, then to dtype. Tokens without a page read as 0; rows
+ * before a sequence's first position are left as they are. */
 int qh_kv8_read(const qh_kv8_cache* c, int layer, void* k, void* v, int dtype, int64_t ldk, int64_t ldv,
                 const int32_t* start, const int32_t* seqs, int n, int n_tok, void* stream);
 
@@ -357,7 +360,8 @@ size_t qh_kv8_attention_workspace_bytes(const qh_kv8_cache* c, int n_heads, int 
 /* Attention of query rows q [n_heads][head_dim] over their sequences: out = sum_j p_j v_j with p = softmax(scale *
  * q . k_j) over the positions j that the row sees: up to its own (causal 1), or the whole sequence (causal 0, for states
  * that are not the queries' own: an entry may then have more rows than the sequence has tokens). Query head h reads KV
- * head h / (n_heads / n_kv_heads). A row that sees nothing (an empty sequence, or a position below 0) is 0. out may not
+ * head h / (n_heads / n_kv_heads). Tokens without a page are left out. A row that sees nothing (an empty
+ * sequence, or a position below 0) is 0. out may not
  * overlap q. A row of q that is not finite gives NaN, and so does a visible token that reads as NaN. Sums in f32; f32
  * queries and weights go through the matrix instructions as two f16 each, and so do the weights of f16 calls, but for
  * prompts (more than 32 rows of a KV head's queries to an entry), whose weights are rounded to one f16: a caller who wants two
@@ -496,8 +500,8 @@ int qh_decoder_set_prefill_stack(qh_decoder* d, int stack);
 int qh_decoder_bind_kv8(qh_decoder* d, const qh_kv8_cache* c, int seq);
 
 /* Stages of a decode step, as qh_decoder_step_timed names them: per layer l, id l * QH_STAGES_PER_LAYER + one of
- * QH_STAGE_QKV (rmsnorm + q/k/v projections), QH_STAGE_ATTENTION, QH_STAGE_O (o projection + residual),
- * QH_STAGE_GATE_UP (rmsnorm + gate/up projections + SwiGLU), QH_STAGE_DOWN (down projection + residual); then
+ * QH_STAGE_QKV (rmsnorm + q/k/v projections; in layer 0 also what makes room in a bound 8-bit cache),
+ * QH_STAGE_ATTENTION, QH_STAGE_O (o projection + residual), QH_STAGE_GATE_UP (rmsnorm + gate/up projections + SwiGLU), QH_STAGE_DOWN (down projection + residual); then
  * QH_STAGE_FINAL_NORM, QH_STAGE_HEAD and, when a sampler picks the token, QH_STAGE_PICK. With the fused kernels (the
  * default) each per-layer stage is one kernel. */
 enum {

@@ -99,3 +99,34 @@ def test_values_near_the_end_of_the_range(qh, rows, n, seq_pages, hd):
     check(c, q, [rows])
     if rows == 1:
         check(c, q, [1], single=True)
+
+
+def test_tokens_that_are_cut_off_leave_their_scale(qh):
+    """A draft of large values and one of a NaN, cut off inside their blocks: the tokens that stay keep the scale (the NaN), as
+    the definition says, until the block is stored anew; other blocks are as if the draft had never been."""
+    import torch
+    hd = 64
+    k, v = randn(1, 40, 1, hd), randn(2, 40, 1, hd)
+    c = filled(qh, k[:20], v[:20], [20], seq_pages=4)
+    read = lambda m: c.read(0, m, start=ints([0, m]), seqs=ints([0]))[0]
+    before = read(20)
+    one, two = k[20:26] * 1000, k[20:26].clone()
+    two[1, 0, 5] = float("nan")
+
+    def draft(rows, keep):
+        c.resize(ints([0]), ints([26]))
+        c.append(0, rows, v[20:26], start=ints([0, 6]), seqs=ints([0]))
+        c.resize(ints([0]), ints([keep]))
+
+    draft(one, 20)
+    after = read(20)
+    assert torch.equal(after[:16], before[:16])
+    step = (one.abs().amax().double() / 127).float()
+    want = torch.trunc(before[16:].double() / step + torch.copysign(torch.tensor(0.5), before[16:])) * step
+    assert torch.allclose(after[16:].double(), want, rtol=2.0 ** -22, atol=0)
+    draft(two, 20)
+    assert torch.equal(read(20)[:16], before[:16]) and torch.isnan(read(20)[16:]).all()
+    c.resize(ints([0]), ints([16]))  # from the block's first token again
+    c.resize(ints([0]), ints([20]))
+    c.append(0, k[16:20], v[16:20], start=ints([0, 4]), seqs=ints([0]))
+    assert torch.equal(read(20), before)
