@@ -362,7 +362,8 @@ size_t qh_kv8_attention_workspace_bytes(const qh_kv8_cache* c, int n_heads, int 
  * that are not the queries' own: an entry may then have more rows than the sequence has tokens). Query head h reads KV
  * head h / (n_heads / n_kv_heads). Tokens without a page are left out. A row that sees nothing (an empty
  * sequence, or a position below 0) is 0. out may not
- * overlap q. A row of q that is not finite gives NaN, and so does a visible token that reads as NaN. Sums in f32; f32
+ * overlap q. One kind of kernel takes the whole batch, by its rows and entries together: prompts and single tokens are faster
+ * in a call each. A row of q that is not finite gives NaN, and so does a visible token that reads as NaN. Sums in f32; f32
  * queries and weights go through the matrix instructions as two f16 each, and so do the weights of f16 calls, but for
  * prompts (more than 32 rows of a KV head's queries to an entry), whose weights are rounded to one f16: a caller who wants two
  * there too passes the queries in f32. A weight is also held
@@ -501,9 +502,9 @@ int qh_decoder_bind_kv8(qh_decoder* d, const qh_kv8_cache* c, int seq);
 
 /* Stages of a decode step, as qh_decoder_step_timed names them: per layer l, id l * QH_STAGES_PER_LAYER + one of
  * QH_STAGE_QKV (rmsnorm + q/k/v projections; in layer 0 also what makes room in a bound 8-bit cache),
- * QH_STAGE_ATTENTION, QH_STAGE_O (o projection + residual), QH_STAGE_GATE_UP (rmsnorm + gate/up projections + SwiGLU), QH_STAGE_DOWN (down projection + residual); then
- * QH_STAGE_FINAL_NORM, QH_STAGE_HEAD and, when a sampler picks the token, QH_STAGE_PICK. With the fused kernels (the
- * default) each per-layer stage is one kernel. */
+ * QH_STAGE_ATTENTION, QH_STAGE_O (o projection + residual), QH_STAGE_GATE_UP (rmsnorm + gate/up projections + SwiGLU),
+ * QH_STAGE_DOWN (down projection + residual); then QH_STAGE_FINAL_NORM, QH_STAGE_HEAD and, when a sampler picks the token,
+ * QH_STAGE_PICK. With the fused kernels (the default) and the decoder's own cache each per-layer stage is one kernel. */
 enum {
     QH_STAGE_QKV = 0,
     QH_STAGE_ATTENTION = 1,

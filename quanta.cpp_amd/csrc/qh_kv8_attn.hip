@@ -1,8 +1,8 @@
 // Attention over the 8-bit paged key / value cache (layout in qh_kv8.h).
 //
-// For query row q of a head and the positions j it sees:  o = sum_j e_j d_j v_j / sum_j e_j,  e_j = 2^(x_j - max x),
+// For query row q of a head and the positions j it sees:  o = sum_j e_j d_j v_j / sum_j e_j,  e_j = 2^(x_j - base),
 // x_j = (q . k_j) c_j scale log2(e), with k_j, v_j the integer codes and c_j, d_j the scales of their blocks. One pass
-// over the cache with the running maximum and sum: 64 positions (a tile) at a time, in f32.
+// over the cache with a running base (the same in both sums) and sum: 64 positions (a tile) at a time, in f32.
 //
 // Both products run on the f16 matrix instructions (16 x 16 x 32): a code in [-127, 127] is exact in f16, so a tile's
 // codes become f16 operands (four instructions for four of them) and the block scales are applied to the scores and to
@@ -10,15 +10,15 @@
 // lane's weights are already the operand of the second product (values . weights, transposed too): no weight passes
 // through shared memory, and a row's maximum and sum belong to one lane column.
 //   f32 queries are split into two f16 (22 bits), scaled by a power of two so that the row's largest value has exponent
-//   13: what the split drops is below 2^-22 of each value, about what f32 sums round off. Weights likewise, but for prompts
-//   in f16 calls, which round each weight to f16 once: half an ulp of the result's own type, for half of the second product
-//   (4 x 2,000 tokens over 8,000, 32 heads of 128 over 8: 392 us, with two halves 521; error against 64 bits 2.9e-4 and
-//   2.1e-4, which is the result's own rounding). Few rows wait for memory, and two halves cost them nothing (48 conversations
-//   of those heads 53.0 and 53.3 us).
-//   A weight carries the value scale of its block over a unit, a power of two above all value scales so far, and
-//   the base that a row's exponentials are relative to follows the largest product of exponential and value scale that the
-//   row has seen, not the largest exponential: so the weights of every row reach 2^6, clear of f16's subnormals and of its
-//   infinity, whatever the scales of blocks are that the row does not see or gives no weight to.
+//   13: what the split drops is at most 2^-22 of a value or, in f16's subnormals, 2^-38 of the row's largest, about what f32
+//   sums round off. Weights are split too, but for prompts in f16 calls, which round each weight to f16 once: half an ulp of
+//   the result's own type, for half of the second product (4 x 2,000 tokens over 8,000, 32 heads of 128 over 8: 392 us, with
+//   two halves 521; error against 64 bits 2.9e-4 and 2.1e-4, which is the result's own rounding). Few rows wait for memory,
+//   and two halves cost them little (48 conversations of those heads 52.2 and 53.3 us).
+//   A weight carries the value scale of its block over a unit, a power of two above all value scales so far, and the base
+//   that a row's exponentials are relative to follows the largest product of exponential and value scale that the row has
+//   seen, not the largest exponential: so the weights of every row reach 2^6, clear of f16's subnormals and of its infinity,
+//   whatever the scales of blocks are that the row does not see or gives no weight to.
 #include <algorithm>
 #include <type_traits>
 
@@ -261,7 +261,7 @@ struct Rows {
         float top = -__builtin_inff();
 #pragma unroll
         for (int b = 0; b < 4; ++b)
-            top = __builtin_fmaxf(top, __builtin_fmaf(fmax2(fmax2(x[b][0], x[b][1]), fmax2(x[b][2], x[b][3])), f[b], sc.level[b]));
+            top = fmax2(top, __builtin_fmaf(fmax2(fmax2(x[b][0], x[b][1]), fmax2(x[b][2], x[b][3])), f[b], sc.level[b]));
         if (__any(top > m + slack) || sc.grown) {
             const float was = m;
             if (sc.grown) {
@@ -381,7 +381,7 @@ struct RowsLds {
 };
 
 // The tiles [t0, t1) of one row tile, from row r0 of entry e, by a workgroup of kW waves: they take every kW-th tile, each
-// with its own running maximum, straight from global memory into registers (one contiguous KB a load, the next tile's
+// with a base and sum of its own, straight from global memory into registers (one contiguous KB a load, the next tile's
 // loads in flight while one is computed), and meet in shared memory at the end. whole: those are all tiles of the rows, and
 // the result goes to out, else into partial result `slot`.
 template <typename T, int kC, int kW>
@@ -955,8 +955,9 @@ __global__ __launch_bounds__(256 * kG, 2) void kv8_tile_kernel(Kv8View c, AttnAr
             for (int ct = 0; ct < kCt; ++ct) st[ct].weigh(x[ct], f[ct], sc, w[ct], lo[ct], st[ct].l, load);
         } else {
             // No maximum over the scores: the weights from the base as it is, and again from a new one where their sums, with
-            // and without the value scales, say that one may be too large (2,000 of 8,000 tokens, f16: 14 heads of 64 over 2 398 -> 361 us, 32 of 128
-            // over 8 1,030 -> 1,001; f32, with more registers to keep, 32 of 128 over 8 1,402 and 1,543).
+            // and without the value scales, say that one may be too large (2,000 of 8,000 tokens, f16: 14 heads of 64 over 2
+            // 398 -> 361 us, 32 of 128 over 8 1,030 -> 1,001; f32, with more registers to keep, 32 of 128 over 8 1,402 and
+            // 1,543).
             float sum[kCt];
             bool move = sc.grown != 0;
 #pragma unroll
