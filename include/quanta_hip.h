@@ -367,9 +367,10 @@ size_t qh_kv8_attention_workspace_bytes(const qh_kv8_cache* c, int n_heads, int 
  * queries and weights go through the matrix instructions as two f16 each, and so do the weights of f16 calls, but for
  * prompts (more than 32 rows of a KV head's queries to an entry), whose weights are rounded to one f16: a caller who wants two
  * there too passes the queries in f32. A weight is also held
- * to 2^-31 of the largest product of weight and value scale that its row sees (what storing that scale's block rounded off is
- * 2^-1 of the product); blocks that a row does not see, or gives no weight to, take nothing from it, up to scales 2^80 times
- * its own. */
+ * to 2^-31 of the largest product of a token's weight and its block's value scale among the tokens that the row sees and whose
+ * stored values are not all zero (storing rounded off up to 2^-1 of that product). Tokens that a row does not see, or gives no
+ * weight to, take nothing from it, as long as that product is above 2^-80 of the sequence's largest value scale; below, as
+ * where zeros have all the weight, it loses bits. */
 int qh_kv8_attention(const qh_kv8_cache* c, int layer, const void* q, void* out, int dtype, int n_heads, int64_t ldq,
                      int64_t ldo, const int32_t* start, const int32_t* seqs, int n, int n_tok, int causal, float scale,
                      void* workspace, size_t workspace_bytes, void* stream);

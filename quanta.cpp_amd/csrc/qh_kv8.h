@@ -9,6 +9,9 @@
 //   keys    [head_dim / 64][4 groups][16 tokens][16 dims]: lane 16 g + t holds dims 64 c + 16 g .. + 15 of token t
 //   values  [head_dim / 64][4 groups][16][4 dims][4 tokens]: lane 16 g + j holds dims 64 c + 4 j .. + 3 of tokens
 //           4 g .. 4 g + 3, the tokens whose weights the same lane holds after the product of keys and queries
+// A value block's scale has its sign set where some of its tokens have only zeros for codes though the scale is not 0: next to
+// the token that gave the scale theirs were too small. Attention counts such tokens in the sum of weights alone, so that they
+// do not bring that scale to rows which give the large token no weight.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -20,6 +23,7 @@
 namespace qh {
 
 constexpr int kBlk = QH_KV8_BLOCK;
+constexpr uint32_t kBias = 0x80808080u;  // the 128 that stored codes carry, in each byte of a word
 
 // What the kernels need of a qh_kv8_cache for one layer.
 struct Kv8View {
@@ -45,6 +49,14 @@ __device__ __forceinline__ uint4 load_once(const uint4* p) {
 // Tokens of a sequence, never more than its table row can hold.
 __device__ __forceinline__ int kv8_len(const Kv8View& c, int seq) {
     return min(max(c.lens[seq], 0), c.seq_pages << c.page_shift);
+}
+
+// x combined by or over the 16 lanes of each row of the wave.
+__device__ __forceinline__ uint32_t or_row16(uint32_t x) {
+    x |= (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x128, 0xF, 0xF, false);
+    x |= (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x124, 0xF, 0xF, false);
+    x |= (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x122, 0xF, 0xF, false);
+    return x | (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x121, 0xF, 0xF, false);
 }
 
 // The codes of block `blk` (of the page) of KV head h, which = 0 keys, 1 values.

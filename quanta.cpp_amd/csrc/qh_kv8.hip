@@ -8,8 +8,6 @@ namespace {
 
 // ------------------------------------------------------------------------------------------- append and read back
 
-constexpr uint32_t kBias = 0x80808080u;  // the 128 that stored codes carry, in each byte of a word
-
 __device__ __forceinline__ void load_row4(const float* p, float* x) {
     typedef float f4 __attribute__((ext_vector_type(4)));
     const f4 a = __builtin_nontemporal_load(reinterpret_cast<const f4*>(p));
@@ -98,7 +96,7 @@ __device__ __forceinline__ void append_block(const Kv8View& c, float (&v)[kC][4]
     const int unit = kValues ? lane : 16 * (j >> 2) + 4 * g + (j & 3);
     uint4* codes = reinterpret_cast<uint4*>(kv8_codes(c, page, kValues ? 1 : 0, h, blk_in_page)) + unit;
     float* scale = kv8_scale(c, page, kValues ? 1 : 0, h, blk_in_page);
-    const float before = held ? *scale : 0.0f;
+    const float before = held ? __builtin_fabsf(*scale) : 0.0f;
     uint4 old[kC];
     if (held) {
 #pragma unroll
@@ -181,6 +179,18 @@ __device__ __forceinline__ void append_block(const Kv8View& c, float (&v)[kC][4]
             }
         }
         codes[64 * k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+    }
+    if constexpr (kValues) {  // the sign: a token of the block has only zeros
+        uint32_t any = 0;     // byte b: of token 4 g + b
+#pragma unroll
+        for (int k = 0; k < kC; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) any |= w[k][i] ^ kBias;
+        any = or_row16(any);
+        bool none = false;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) none |= pos0 + 4 * g + b < len && ((any >> (8 * b)) & 0xffu) == 0;
+        if (__any(none) && d > 0.0f) d = -d;
     }
     if (lane == 0) *scale = d;
 }
@@ -316,7 +326,7 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8View c, T* __restrict_
     const int page = c.table[(size_t)sp.seq * c.seq_pages + (pos0 >> c.page_shift)];
     const bool ok = page >= 0 && page < c.n_pages, values = (hw & 1) != 0;  // a missing page reads as zeros
     const int bp = blk & ((1 << (c.page_shift - 4)) - 1);
-    const float d = ok ? *kv8_scale(c, page, hw & 1, h, bp) : 0.0f;
+    const float d = ok ? __builtin_fabsf(*kv8_scale(c, page, hw & 1, h, bp)) : 0.0f;
     const uint4* codes = reinterpret_cast<const uint4*>(kv8_codes(c, ok ? page : 0, hw & 1, h, bp)) +
                          (values ? lane : 16 * (j >> 2) + 4 * g + (j & 3));
     T* out = values ? v : k;

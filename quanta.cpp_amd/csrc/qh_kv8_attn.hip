@@ -143,7 +143,8 @@ struct Query {
 struct Blocks {
     int page;
     float ck, cv;
-    uint64_t ok;  // lanes whose block exists
+    uint64_t ok;     // lanes whose block exists
+    uint64_t blank;  // lanes whose block has tokens with values of zero alone (the sign of its value scale)
 
     // tile: this lane's; blocks at or past len, or without a page, are left out.
     __device__ __forceinline__ void load(const Kv8View& c, int seq, int h, int tile, bool in_range, int len) {
@@ -158,6 +159,8 @@ struct Blocks {
             ck = *kv8_scale(c, page, 0, h, blk);
             cv = *kv8_scale(c, page, 1, h, blk);
         }
+        blank = __ballot(cv < 0.0f);
+        cv = __builtin_fabsf(cv);
         page = good ? page : 0;
     }
     __device__ __forceinline__ int page_of(int i) const { return __builtin_amdgcn_readlane(page, i); }
@@ -184,6 +187,7 @@ struct Scales {
     int grown;       // powers of two by which the unit grew
     uint32_t ok;     // bits of the blocks that exist
     uint32_t nan;    // and of those with a NaN scale: they count as zeros here, see Rows::poison
+    uint32_t blank;  // and of those with tokens whose values are all zero, see Rows::set_apart
 };
 
 // The value scales' running unit, a power of two above all of them so far and at least 2^-110, as its biased exponent (0:
@@ -195,12 +199,13 @@ struct Unit {
         Scales t;
         int v[4], top = 17 << 23;
         t.ok = (uint32_t)(bl.ok >> i0) & 15u;
+        t.blank = (uint32_t)(bl.blank >> i0) & 15u;
         t.nan = 0;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             int k = __builtin_amdgcn_readlane(__builtin_bit_cast(int, bl.ck), i0 + b);
             v[b] = __builtin_amdgcn_readlane(__builtin_bit_cast(int, bl.cv), i0 + b);
-            const bool bad = max(k, v[b]) >= 0x7f800000;  // scales are never negative
+            const bool bad = max(k, v[b]) >= 0x7f800000;  // scales of keys are never negative
             t.nan |= bad ? 1u << b : 0u;
             k = bad ? 0 : k;
             v[b] = bad ? 0 : v[b];
@@ -253,6 +258,43 @@ struct Rows {
 #pragma unroll
         for (int b = 0; b < 4; ++b)
             if ((nan >> b) & 1u) l = pos0 + 16 * b < vis ? __builtin_nanf("") : l;
+    }
+
+    // Tokens whose values are all zero (bit 4 b + s of blank for the scores x[b][s]) join the sum alone and are masked then:
+    // at the lowest level, as a block of zeros. The base moves where it has to for that. Selections by masks of whole words:
+    // conditions would take sixteen pairs of scalar registers from the loop around this.
+    __device__ __forceinline__ void set_apart(f4 (&x)[4], const float (&f)[4], uint32_t blank) {
+        const auto mask_of = [&](int n) { return (int)(blank << (31 - n)) >> 31; };
+        const auto pick = [](int mask, float a, float b) {
+            return __builtin_bit_cast(float, (__builtin_bit_cast(int, a) & mask) | (__builtin_bit_cast(int, b) & ~mask));
+        };
+        const float none = -__builtin_inff();
+        float top = none;
+        asm volatile("" : "+v"(blank));  // the masks are made here, not with those of the other row tiles
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                top = fmax2(top, pick(mask_of(4 * b + s), __builtin_fmaf(x[b][s], f[b], (float)-kDepth), none));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        const float was = m;
+        m = __builtin_fmaxf(m, over_groups(top, fmax2));
+        const float alpha = m == was ? 1.0f : __builtin_amdgcn_exp2f(was - m), base = m == none ? 0.0f : m;
+        l *= alpha;
+#pragma unroll
+        for (int i = 0; i < 4 * kC; ++i) o[i] *= alpha;
+        asm volatile("" : "+v"(blank));  // and made again, not kept
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int mask = mask_of(4 * b + s);
+                l += pick(mask, __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][s], f[b], -base)), 0.0f);
+                x[b][s] = pick(mask, none, x[b][s]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
 
     // Moves the base where a score passes it by too much, and the output with it. Where the unit grew, the levels of the
@@ -449,7 +491,24 @@ __device__ __forceinline__ void rows_tiles(const Kv8View& c, const AttnArgs& a, 
         }
         __builtin_amdgcn_sched_barrier(0);
         h8 w[2], lo[2];
-        if (pos0 + kTile > all_see || sc.ok != 15u) st.mask(x, f, pos0 + 4 * g, vis, sc.ok);
+        if (pos0 + kTile > all_see || sc.ok != 15u || sc.blank) {
+            st.mask(x, f, pos0 + 4 * g, vis, sc.ok);
+            if (sc.blank) {
+                uint32_t blank = 0;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    uint32_t any = 0;  // byte s: of token 4 g + s
+#pragma unroll
+                    for (int cc = 0; cc < kC; ++cc)
+                        any |= (vr[b][cc].x ^ kBias) | (vr[b][cc].y ^ kBias) | (vr[b][cc].z ^ kBias) | (vr[b][cc].w ^ kBias);
+                    any = or_row16(any);
+                    any = ~(any | ((any & 0x7f7f7f7fu) + 0x7f7f7f7fu)) & 0x80808080u;  // the top bits of bytes that are 0
+                    any = ((any >> 7) | (any >> 14) | (any >> 21) | (any >> 28)) & 15u;
+                    blank |= (sc.blank >> b) & 1u ? any << (4 * b) : 0u;
+                }
+                st.set_apart(x, f, blank);
+            }
+        }
         if (sc.nan) st.poison(sc.nan, pos0, vis);
         st.settle(x, f, sc, kSlack);
         float load = 0.0f;
@@ -929,23 +988,50 @@ __global__ __launch_bounds__(256 * kG, 2) void kv8_tile_kernel(Kv8View c, AttnAr
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_setprio(0);
         if (t + 2 < t1) fetch(t + 2);
+        // (before the scales; with two f32 row tiles behind the masks, where fewer registers are in use: 843 and 890 us)
+        const auto values_ahead = [&] {
 #pragma unroll
-        for (int r = 0; r < kDeep; ++r) vv[r] = __builtin_bit_cast(h8, vs[r * 64]);
-        __builtin_amdgcn_sched_barrier(0);
+            for (int r = 0; r < kDeep; ++r) vv[r] = __builtin_bit_cast(h8, vs[r * 64]);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        if constexpr (kMm < 4) values_ahead();
         const Scales sc = unit.next(bl, i0);
         float f[kCt][4];
 #pragma unroll
         for (int ct = 0; ct < kCt; ++ct)
 #pragma unroll
             for (int k = 0; k < 4; ++k) f[ct][k] = sc.key[k] * q[ct].unit;
-        if (pos0 + kTile > all_see || sc.ok != 15u) {
+        if (pos0 + kTile > all_see || sc.ok != 15u || sc.blank) {
 #pragma unroll
             for (int ct = 0; ct < kCt; ++ct) st[ct].mask(x[ct], f[ct], pos0 + 4 * g, vis[ct], sc.ok);
+            if (sc.blank) {
+                uint32_t blank = 0;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    uint32_t any[4] = {};  // tokens 0 1 and 2 3 of blocks 2 u and 2 u + 1, as the operands' f16
+#pragma unroll
+                    for (int i = 0; i < 4 * kC; ++i) {
+                        const uint4 v = vs[(u * 4 * kC + i) * 64];
+                        any[0] |= v.x, any[1] |= v.y, any[2] |= v.z, any[3] |= v.w;
+                    }
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        const int b = 2 * u + (n >> 1), s = 2 * (n & 1);
+                        uint32_t w = or_row16(any[n]);
+                        w = ~((w & 0x7fff7fffu) + 0x7fff7fffu) & 0x80008000u;  // the top bits of halves that are 0 or -0
+                        w = ((w >> 15) | (w >> 30)) & 3u;
+                        blank |= (sc.blank >> b) & 1u ? w << (4 * b + s) : 0u;
+                    }
+                }
+#pragma unroll
+                for (int ct = 0; ct < kCt; ++ct) st[ct].set_apart(x[ct], f[ct], blank);
+            }
         }
         if (sc.nan) {
 #pragma unroll
             for (int ct = 0; ct < kCt; ++ct) st[ct].poison(sc.nan, pos0, vis[ct]);
         }
+        if constexpr (kMm == 4) values_ahead();
         h8 w[kCt][2], lo[kCt][2];
         if constexpr (Query<T, kC>::kSplit) {
 #pragma unroll

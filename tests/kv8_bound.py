@@ -10,13 +10,13 @@ HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11}  # half a step of 
 
 def value_scales(cache, layer, seq):
     """Scales of a sequence's value blocks, [blocks][kv], 64 bits (pages: codes of keys and values, then the scales f32
-    [keys, values][kv][blocks of a page])."""
+    [keys, values][kv][blocks of a page]; the sign is a mark of its own)."""
     per, kv = cache.page_tokens // 16, cache.n_kv_heads
     at, n = 2 * kv * cache.page_tokens * cache.head_dim, 2 * kv * per
     length = int(cache.lens[seq])
     pages = cache.table[seq, :-(-length // cache.page_tokens)].long()
     raw = cache.pages[layer, pages, at:at + 4 * n].contiguous().view(torch.float32)
-    return raw.view(-1, 2, kv, per)[:, 1].transpose(1, 2).reshape(-1, kv).double()
+    return raw.view(-1, 2, kv, per)[:, 1].transpose(1, 2).reshape(-1, kv).abs().double()
 
 
 def exact_attention(cache, layer, q, seqs, counts, causal=True, scale=None, two=None):
@@ -27,7 +27,8 @@ def exact_attention(cache, layer, q, seqs, counts, causal=True, scale=None, two=
     an f16 query is exact), 2 hd products summed (hd for f16 queries), and 8 roundings of unit, scales and products. The
     weight's relative error is dx, once above and once below the fraction. A weight itself: its exponential and products, 10
     roundings; its format, two f16 (2^-22) or one (2^-11); and in f16's subnormals half of 2^-24, where the row's largest
-    weight times value scale stands at 2^6 at least, so 2^-31 of that for each code. Sums over the n positions that the
+    weight times value scale stands at 2^6 at least, so 2^-31 of that for each code (the largest of tokens whose values are
+    not all zero: the others count in the sum of weights alone). Sums over the n positions that the
     row sees: n roundings above and below, and 32 of joins."""
     hd, heads = cache.head_dim, q.shape[1]
     group = heads // cache.n_kv_heads
@@ -68,7 +69,7 @@ def exact_attention(cache, layer, q, seqs, counts, causal=True, scale=None, two=
             else:
                 dx = size * (hd + 8) * 2.0 ** -24
             rel = 2 * dx + 10 * 2.0 ** -24 + (2.0 ** -22 if two else 2.0 ** -11) + 2 * (seen + 32) * 2.0 ** -24
-            largest = (p * d[None, :, g]).amax(1)
+            largest = (p * (d[:, g] * (av.amax(1) > 0))[None]).amax(1)
             codes = (av / d[:, g, None].clamp(min=1e-300))
             codes = (~hidden).double() @ codes
             off = rel[:, None] * (p @ av) + 2.0 ** -31 * largest[:, None] * codes

@@ -83,3 +83,31 @@ def test_kernel_with_value_scales_far_apart(qh, gpu, case, dtype):
         want, bound = exact_attention(c, 0, q, range(len(lens)), counts, causal, two=kernel[0] != TILES or dtype == "float32")
         ratio, at_ = worst(got, want, bound)
         assert ratio <= 1, (causal, ratio, at_, float(got[at_]), float(want[at_]))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("case", [(c[0], hd) + c[2:] for c in CASES for hd in c[1]], ids=lambda c: f"{c[0]}, {c[1]}")
+def test_kernel_with_single_large_values(qh, gpu, case, dtype):
+    """Single tokens whose values are so large that the others of their blocks have only zeros for codes, and whose scores are so
+    low that they count for nothing (every seventh has a score like the others'): the zeros beside them have their share of the
+    weights, and ordinary values elsewhere keep all their bits."""
+    import torch
+    _, hd, heads, kv, lens, counts, kernel = case
+    t, n = getattr(torch, dtype), sum(lens)
+    k, v = randn(1, n, kv, hd), randn(2, n, kv, hd) * (1 if dtype == "float32" else 2.0 ** -9)
+    k[..., 0] = 0.0
+    at = torch.cat([torch.arange(m, device="cuda") for m in lens])
+    large = at % 97 == 5
+    v[large] *= 1e12 if dtype == "float32" else 2.0 ** 16
+    k[large & (at % 7 != 0), :, 0] = -25.0
+    c = filled(qh, k.to(t), v.to(t), lens)
+    single = counts is None
+    counts = [1] * len(lens) if single else counts
+    q = randn(3, sum(counts), heads, hd)
+    q[..., 0] = 8.0 * hd ** 0.5
+    q = q.to(t)
+    for causal in (True, False):
+        got = c.attention(0, q, start=None if single else starts(counts), seqs=ints(range(len(lens))), causal=causal)
+        want, bound = exact_attention(c, 0, q, range(len(lens)), counts, causal, two=kernel[0] != TILES or dtype == "float32")
+        ratio, at_ = worst(got, want, bound)
+        assert ratio <= 1, (causal, ratio, at_, float(got[at_]), float(want[at_]))

@@ -130,3 +130,50 @@ def test_tokens_that_are_cut_off_leave_their_scale(qh):
     c.resize(ints([0]), ints([20]))
     c.append(0, k[16:20], v[16:20], start=ints([0, 4]), seqs=ints([0]))
     assert torch.equal(read(20), before)
+
+
+@pytest.mark.parametrize("rows,seq_pages", [(1, 40), (1, 90), (6, 40), (90, 40)])
+@pytest.mark.parametrize("at", [3, 15, 40, 63, 64, 300])
+def test_a_large_value_of_one_token(qh, rows, seq_pages, at):
+    """One token's value 1e10 times the others' and its score too low to count, wherever it lies; stored with the prompt, or
+    token by token, so that earlier codes of its block are rounded to zero and later ones are zero from the start; read from a
+    copy; and gone again with the tokens from it on."""
+    import torch
+    n, hd = 317, 64
+    k, v, q = randn(1, n, 2, hd), randn(2, n, 2, hd), randn(3, rows, 6, hd)
+    k[..., 0], q[..., 0] = 0.0, 8.0 * hd ** 0.5
+    k[at, :, 0] = -25.0
+    v[at] *= 1e10
+    whole = filled(qh, k, v, [n], seq_pages=seq_pages)
+    check(whole, q, [rows])
+    c = qh.KV8Cache(1, 40, 32, 2, hd, 3, seq_pages)
+    c.pages.fill_(0x7f)
+    first = max(0, at - 9)
+    for a, b in [(0, first)] * (first > 0) + [(i, i + 1) for i in range(first, min(n, at + 20))] + [(min(n, at + 20), n)] * (at + 20 < n):
+        c.resize(ints([0]), ints([b]))
+        c.append(0, k[a:b], v[a:b], start=ints([0, b - a]), seqs=ints([0]))
+    check(c, q, [rows], seqs=[0])
+    c.fork(ints([0, 0]), ints([1, 2]), copy=True)
+    check(c, q, [rows], seqs=[2])
+    if at >= 15 and at % 16:
+        c.resize(ints([1]), ints([at]))  # the block of the cut keeps the scale, and only zeros
+        m = min(rows, at)
+        check(c, q[:m], [m], seqs=[1])
+
+
+def test_reads_do_not_see_the_mark(qh):
+    """The values read back beside a large one: zeros, not zeros of another sign of scale; and a block that grows again from
+    them takes its scale's size."""
+    import torch
+    k = torch.zeros(20, 1, 64, device="cuda")
+    k[:, 0, 0] = 1.0
+    v = k.clone()
+    v[3] *= 1e6
+    c = filled(qh, k[:17], v[:17], [17], seq_pages=2)
+    got = c.read(0, 17, start=ints([0, 17]))[1]
+    assert (got[:16] >= 0).all() and float(got[3, 0, 0]) == 1e6 and float(got[:16].sum()) == 1e6 and float(got[16, 0, 0]) == 1.0
+    c.resize(ints([0]), ints([10]))
+    c.resize(ints([0]), ints([12]))
+    c.append(0, k[10:12], -v[10:12], start=ints([0, 2]))
+    got = c.read(0, 12, start=ints([0, 12]))[1]
+    assert float(got[3, 0, 0]) == 1e6 and float(got.abs().sum()) == 1e6
