@@ -1,10 +1,12 @@
-"""What a step of many sequences does around the 8-bit paged cache's attention: its cost over the range it is used in.
+"""What a step of many sequences does around the 8-bit paged cache: its cost over the range it is used in.
 
-Four kinds of pass:
+Five kinds of pass:
 
 * norm: root-mean-square norm of rows, with the residual's addition before it, into rows of the same type or into 8-bit
   blocks of 32 with a scale each, as the quantized matmuls take them;
 * rope: rotary positions of the query and key heads, as a fused projection leaves them in one row;
+* attend: causal attention of whole prompts, packed end to end, over their own keys and values before those are rounded to
+  8 bits (or of new rows behind kept ones, or over states that are not their own);
 * beam: the best continuations of each prompt's beams over beams and vocabulary;
 * reorder: the cache's sequences become those beams' sequences, and room for each beam's next token.
 
@@ -51,6 +53,11 @@ def _rope(name, tokens, heads, kv, hd, rot, interleaved, scaling, last, dtype):
             "interleaved": interleaved, "scaling": scaling, "last": last, "dtype": dtype}
 
 
+def _attend(name, seqs, new, behind, heads, kv, hd, causal, dtype):
+    return {"name": name, "kind": "attend", "seqs": seqs, "new": new, "behind": behind, "heads": heads, "kv": kv, "hd": hd,
+            "causal": causal, "dtype": dtype}
+
+
 def _beam(name, prompts, beams, vocab, k, dtype):
     return {"name": name, "kind": "beam", "prompts": prompts, "beams": beams, "vocab": vocab, "k": k, "dtype": dtype}
 
@@ -68,20 +75,20 @@ def listed():
         _norm("norm_prompts", 4001, 5120, "f32", True, "q8"),
         # The same for unquantized projections, in f16: the largest norm.
         _norm("norm_rows", 16000, 4096, "f16", True, "rows"),
-        # The norm of a width that no vector divides, first in a model, where there is no residual yet.
-        _norm("norm_odd", 777, 1001, "f16", False, "rows"),
         # A server's decode step: one token each of conversations of mixed lengths, the benchmark's heads.
         _rope("rope_step", 48, 14, 2, 64, 64, False, "none", 5000, "f32"),
         # Long prompts in contexts stretched past the trained length.
         _rope("rope_prompts", 8000, 32, 8, 128, 128, False, "parts", 130000, "f16"),
-        # Neighbouring dimensions paired, and only a part of each head turned.
-        _rope("rope_partial", 3001, 16, 1, 128, 48, True, "linear", 9000, "f32"),
+        # The benchmark's 512-token prompt, in the type that the quantized projections give.
+        _attend("attend_prompt", 1, 512, 0, 14, 2, 64, True, "f32"),
+        # A batch of prompts of mixed lengths, packed.
+        _attend("attend_packed", 16, 2000, 0, 14, 2, 64, True, "f32"),
+        # A long document on the heads of a larger model.
+        _attend("attend_long", 1, 12001, 0, 32, 8, 128, True, "f16"),
         # Four beams of one prompt over the benchmark's vocabulary.
         _beam("beam_step", 1, 4, 151936, 8, "f32"),
         # A batch of prompts.
         _beam("beam_batch", 24, 8, 151936, 16, "f32"),
-        # Many beams over a smaller vocabulary whose rows begin anywhere, in f16, where logits are often equal.
-        _beam("beam_wide", 16, 32, 50257, 64, "f16"),
         # The four beams' sequences in the cache.
         _reorder("reorder_step", 1, 4, 600, 24, 2, 64, 64),
         # A batch's, in small pages.
@@ -97,7 +104,7 @@ _HEADS = [(14, 2, 64), (12, 2, 128), (32, 8, 128), (8, 8, 64), (4, 4, 128), (16,
 
 
 def draw(rng):
-    kind = rng.choice(["norm", "norm", "rope", "rope", "beam", "beam", "beam", "reorder"])
+    kind = rng.choice(["norm", "norm", "rope", "rope", "attend", "attend", "attend", "beam", "beam", "reorder"])
     dtype = rng.choice(["f32", "f16"])
     heads, kv, hd = rng.choice(_HEADS)
     if kind == "norm":
@@ -108,6 +115,11 @@ def draw(rng):
         rot = rng.choice([hd, hd, 2 * rng.randint(1, hd // 2)])
         return _rope(None, min(_log(rng, 1, 8000), 32000000 // ((heads + kv) * hd)), heads, kv, hd, rot,
                      rng.random() < 0.4, rng.choice(["none", "linear", "base", "parts"]), _log(rng, 100, 1000000), dtype)
+    if kind == "attend":
+        hd = 64 if hd == 64 else 128
+        new, behind = _log(rng, 1, 6000), rng.choice([0, 0, _log(rng, 1, 4000)])
+        seqs = max(1, min(_log(rng, 1, 64), 500000000 // (heads * new * (new + behind))))
+        return _attend(None, seqs, new, behind, heads, kv, hd, rng.random() < 0.8, dtype)
     if kind == "beam":
         beams, vocab = _log(rng, 1, 40), _log(rng, 40, 200000)
         k = min(rng.choice([1, beams, 2 * beams, _log(rng, 1, 256)]), beams * vocab, 256)
@@ -128,6 +140,13 @@ def _ceil(a, b):
 def _page_bytes(case):
     raw = 2 * case["kv"] * case["page"] * case["hd"] + 8 * case["kv"] * (case["page"] // 16)
     return _ceil(raw, 128) * 128
+
+
+def _lengths(case):
+    """Rows and keys of each sequence of an attend case, the same for every seed: the longest has the case's sizes."""
+    rng = random.Random("%s" % sorted((k, v) for k, v in case.items() if k != "name"))
+    new = [case["new"]] + [max(1, int(case["new"] * rng.uniform(0.1, 1))) for _ in range(case["seqs"] - 1)]
+    return new, [m + int(case["behind"] * (rng.uniform(0, 1) if i else 1)) for i, m in enumerate(new)]
 
 
 def _plan(case):
@@ -165,6 +184,11 @@ def work(case):
         heads = case["heads"] + case["kv"]
         return {"bytes": case["tokens"] * (2 * size * heads * case["hd"] + 4) + 4 * case["rot"],
                 "flops": 3 * case["tokens"] * heads * case["rot"]}
+    if case["kind"] == "attend":
+        new, keys = _lengths(case)
+        seen = sum(m * (l - m) + m * (m + 1) // 2 if case["causal"] else m * l for m, l in zip(new, keys))
+        return {"bytes": 2 * size * case["hd"] * (sum(new) * case["heads"] + sum(keys) * case["kv"]),
+                "flops": 4 * case["hd"] * case["heads"] * seen}
     if case["kind"] == "beam":
         rows = case["prompts"] * case["beams"]
         return {"bytes": rows * (size * case["vocab"] + 4) + 12 * case["prompts"] * case["k"],
@@ -253,6 +277,31 @@ def _prepare_rope(case, seed):
     return st
 
 
+def _starts(counts):
+    out = [0]
+    for c in counts:
+        out.append(out[-1] + c)
+    return out
+
+
+def _attend_inputs(case, seed):
+    gen, (new, keys) = _gen(seed), _lengths(case)
+    heads, kv, hd = case["heads"], case["kv"], case["hd"]
+    q = torch.randn(sum(new), heads, hd, generator=gen, device=DEVICE)
+    # keys with a few channels wider than the others, as rotated keys have; keys and values side by side in one row
+    row = torch.randn(sum(keys), 2 * kv, hd, generator=gen, device=DEVICE)
+    row[:, :kv] *= 1.0 + 3.0 * (torch.arange(hd, device=DEVICE) % 16 == 3)
+    row = row.to(_dtype(case))
+    return q.to(_dtype(case)), row[:, :kv], row[:, kv:]
+
+
+def _prepare_attend(case, seed):
+    new, keys = _lengths(case)
+    q, k, v = _attend_inputs(case, seed)
+    return {"case": case, "q": q, "k": k, "v": v, "start": _ints(_starts(new)), "longest": max(new), "most": max(keys),
+            "kstart": _ints(_starts(keys)) if case["behind"] else None}
+
+
 def _prepare_beam(case, seed):
     gen, rows = _gen(seed), case["prompts"] * case["beams"]
     # logits as a model's head gives them: a wide bulk, and a few ids well above it
@@ -291,7 +340,7 @@ def _prepare_reorder(case, seed):
 
 
 def prepare(case, seed):
-    return {"norm": _prepare_norm, "rope": _prepare_rope, "beam": _prepare_beam,
+    return {"norm": _prepare_norm, "rope": _prepare_rope, "attend": _prepare_attend, "beam": _prepare_beam,
             "reorder": _prepare_reorder}[case["kind"]](case, seed)
 
 
@@ -303,6 +352,8 @@ def run(state):
         return _own_norm(state) if own else _plain_norm(state)
     if kind == "rope":
         return _own_rope(state) if own else _plain_rope(state)
+    if kind == "attend":
+        return _own_attend(state) if own else _plain_attend(state)
     if kind == "beam":
         return _own_beam(state) if own else _plain_beam(state)
     # the state before, so that every pass has the same beams to reorder
@@ -330,6 +381,10 @@ def _own_norm(st):
 
 def _own_rope(st):
     return st["rope"](st["q"], st["k"], pos=st["pos"])
+
+
+def _own_attend(st):
+    return _package().attention(st["q"], st["k"], st["v"], st["start"], kstart=st["kstart"], causal=st["case"]["causal"])
 
 
 def _own_beam(st):
@@ -382,6 +437,34 @@ def _plain_turn(x, c, s, rot, interleaved):
         a, b = wide[..., :rot // 2], wide[..., rot // 2:rot]
         turned = torch.cat((a * c - b * s, a * s + b * c), dim=-1)
     return torch.cat((turned, wide[..., rot:]), dim=-1).to(x.dtype)
+
+
+def _padded(x, start, length):
+    """Packed rows as [sequences][heads][length][head_dim] in 32 bits, and which of them are there."""
+    place = start[:-1].long().view(-1, 1) + torch.arange(length, device=DEVICE)
+    there = place < start[1:].long().view(-1, 1)
+    return x[place.clamp(max=x.shape[0] - 1)].float().transpose(1, 2).contiguous(), there
+
+
+def _plain_attend(st):
+    case, start = st["case"], st["start"]
+    kstart = start if st["kstart"] is None else st["kstart"]
+    q, rows = _padded(st["q"], start, st["longest"])
+    k, cols = _padded(st["k"], kstart, st["most"])
+    v, _ = _padded(st["v"], kstart, st["most"])
+    n, kv, most, hd = k.shape
+    q = q.view(n * kv, -1, hd)
+    scores = torch.matmul(q, k.view(n * kv, most, hd).transpose(1, 2).contiguous()).view(n, kv, -1, st["longest"], most)
+    hidden = ~cols.view(n, 1, most)
+    if case["causal"]:
+        # a sequence's rows are its last ones
+        at = torch.arange(st["longest"], device=DEVICE) + (cols.sum(1) - rows.sum(1)).view(n, 1)
+        hidden = hidden | (torch.arange(most, device=DEVICE) > at.unsqueeze(-1))
+    scores = (scores * (1.0 / math.sqrt(hd))).masked_fill_(hidden.view(n, 1, 1, -1, most), -math.inf)
+    e = torch.exp(scores - scores.amax(-1, keepdim=True))
+    e = e / e.sum(-1, keepdim=True)
+    out = torch.matmul(e.view(n * kv, -1, most), v.view(n * kv, most, hd)).view(n, -1, st["longest"], hd)
+    return out.transpose(1, 2)[rows].to(st["q"].dtype)
 
 
 def _plain_beam(st):
@@ -471,6 +554,21 @@ def _exact_rope(case, seed):
     return tuple(out)
 
 
+def _exact_attend(case, seed):
+    q, k, v = _attend_inputs(case, seed)
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    group, a, b = case["heads"] // case["kv"], 0, 0
+    for m, l in zip(*_lengths(case)):
+        limit = torch.arange(l - m, l, device=q.device).unsqueeze(1)
+        for h in range(case["heads"]):
+            s = q[a:a + m, h].double() @ k[b:b + l, h // group].double().t().contiguous() / case["hd"] ** 0.5
+            if case["causal"]:
+                s = torch.where(torch.arange(l, device=q.device) <= limit, s, -math.inf)
+            out[a:a + m, h] = torch.softmax(s, dim=1) @ v[b:b + l, h // group].double()
+        a, b = a + m, b + l
+    return out
+
+
 def _exact_beam(case, seed):
     st = _prepare_beam(case, seed)
     logp = torch.log_softmax(st["logits"].double(), dim=-1) + st["scores"].double().unsqueeze(1)
@@ -481,4 +579,4 @@ def _exact_beam(case, seed):
 def exact(case, seed):
     if case["kind"] == "reorder":
         return None  # whole numbers only
-    return {"norm": _exact_norm, "rope": _exact_rope, "beam": _exact_beam}[case["kind"]](case, seed)
+    return {"norm": _exact_norm, "rope": _exact_rope, "attend": _exact_attend, "beam": _exact_beam}[case["kind"]](case, seed)
