@@ -391,6 +391,61 @@ typedef struct qh_kv8_plan {
 } qh_kv8_plan;
 int qh_kv8_attention_plan(const qh_kv8_cache* c, int n_heads, int n, int n_tok, int single, qh_kv8_plan* plan);
 
+/* ------------------------------------------------------------------ rows of a step of many sequences */
+
+/* Root-mean-square norm of n_tok rows of n, with a residual's addition before it: h = x + res, rounded to dtype (QH_F32 or
+ * QH_F16; res NULL: h = x), goes to sum (NULL: nowhere), and h / sqrt(mean(h^2) + eps) * w to the outputs that are given:
+ * y, rows of dtype, and / or q [n_tok][n] with d [n_tok][n / 32], the blocks that qh_quantize_q8 makes of the result in f32
+ * (n a multiple of 32 then). w is f32 [n]. Squares are summed in 64 bits and the result is rounded once. Rows are ld elements
+ * apart, on any alignment of their type (q: 16 bytes). sum may be x or res, with its row stride; the outputs overlap nothing
+ * else. n at most QH_NORM_MAX. A NaN makes its row NaN; an infinity makes its own place NaN and the rest of the row 0 (in
+ * blocks: as qh_quantize_q8 takes those).
+ * No counterpart among the reference's kernels by itself: its rmsnorm (ops_ref.cpp:194-199) sums in f32 in order, which the
+ * decoder's own kernels keep to the bit. */
+#define QH_NORM_MAX 32768
+int qh_rmsnorm(const void* x, const void* res, const float* w, int dtype, int64_t ldx, int64_t ldr, int n_tok, int n,
+               double eps, void* sum, int64_t lds, void* y, int64_t ldy, int8_t* q, float* d, void* stream);
+
+/* How far a rotary position turns the pairs of a head: pair i of rot_dim / 2 by theta^(-2 i / rot_dim) radians a position,
+ * changed by `scaling` for contexts longer than the trained one:
+ *   QH_ROPE_PLAIN  as it is
+ *   QH_ROPE_LINEAR all divided by factor
+ *   QH_ROPE_BASE   theta * factor^(rot_dim / (rot_dim - 2)) in theta's place: the slowest pair is divided by factor, the first
+ *                  by nothing (rot_dim 2: as it is)
+ *   QH_ROPE_PARTS  by parts: pairs that turn at most `low` times over `context` positions are divided by factor, those that
+ *                  turn `high` times or more are left, with a ramp linear in the turns between them */
+enum { QH_ROPE_PLAIN = 0, QH_ROPE_LINEAR = 1, QH_ROPE_BASE = 2, QH_ROPE_PARTS = 3 };
+typedef struct qh_rope_desc {
+    double theta;
+    int32_t rot_dim; /* even, 2 to QH_ROPE_MAX_DIM */
+    int32_t scaling; /* QH_ROPE_* */
+    double factor, context, low, high; /* factor > 0; by parts: context > 0, 0 <= low < high */
+} qh_rope_desc;
+#define QH_ROPE_MAX_DIM 256
+
+/* The pairs' turns (of 2 pi) per position in 64 bits: rot_dim / 2 of them into turns_host, which the caller uploads once.
+ * Host only. Another schedule is as good: qh_rope takes any table. */
+int qh_rope_turns(const qh_rope_desc* r, double* turns_host);
+
+/* The rows' side of qh_rope: n_heads heads of head_dim one after the other, rows ld (out: ldo) elements apart. out may be x
+ * (then ldo is ld); they do not overlap otherwise. */
+typedef struct qh_rope_rows {
+    const void* x;
+    void* out;
+    int64_t ld, ldo;
+    int32_t n_heads;
+} qh_rope_rows;
+
+/* Rotary positions: every head of q's and k's rows (k NULL: q alone) has its first rot_dim dims turned in pairs (a, b) ->
+ * (a cos - b sin, a sin + b cos) by the angle 2 pi pos[t] turns[i], cos and sin times `magnitude`; the others are copied. A
+ * pair is the dims i and i + rot_dim / 2, or (interleaved 1) 2 i and 2 i + 1. pos: DEVICE int32 [n_tok], of either sign;
+ * turns: DEVICE [rot_dim / 2]. Angles are taken in 64 bits less their whole turns, so that far positions lose nothing. Rows
+ * of dtype QH_F32 or QH_F16 on any alignment of their type; head_dim at most QH_ROPE_MAX_DIM.
+ * Replaces: the rotation in Model::forward (reference model.cpp:187-196), for many sequences' tokens; the decoder's own
+ * kernels keep the reference's f32 table to the bit. */
+int qh_rope(const double* turns, int rot_dim, int interleaved, float magnitude, int head_dim, const qh_rope_rows* q,
+            const qh_rope_rows* k, int dtype, const int32_t* pos, int n_tok, void* stream);
+
 /* ------------------------------------------------------------------ GPU-resident decoder */
 
 /* FLAG_HADAMARD_DOWN (reference engine/src/model_file.h:19-21): the down projection's input is rotated by the

@@ -87,6 +87,18 @@ class qh_kv8_plan(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("kernel", "rows", "waves", "splits", "launches")]
 
 
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = range(4)  # qh_rope_desc.scaling
+
+
+class qh_rope_desc(C.Structure):
+    _fields_ = [("theta", C.c_double), ("rot_dim", C.c_int32), ("scaling", C.c_int32)] + [
+        (n, C.c_double) for n in ("factor", "context", "low", "high")]
+
+
+class qh_rope_rows(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("ld", C.c_int64), ("ldo", C.c_int64), ("n_heads", C.c_int32)]
+
+
 STAGE_QKV, STAGE_ATTENTION, STAGE_O, STAGE_GATE_UP, STAGE_DOWN, STAGES_PER_LAYER = 0, 1, 2, 3, 4, 8
 STAGE_FINAL_NORM, STAGE_HEAD, STAGE_PICK = 1 << 20, (1 << 20) + 1, (1 << 20) + 2
 
@@ -101,6 +113,7 @@ EXPORTS = ("qh_last_error", "qh_version", "qh_init", "qh_quant_bytes", "qh_tenso
            "qh_kv8_page_bytes", "qh_kv8_reset", "qh_kv8_pages_workspace_bytes", "qh_kv8_resize", "qh_kv8_fork",
            "qh_kv8_compact", "qh_kv8_append", "qh_kv8_read", "qh_kv8_attention_workspace_bytes", "qh_kv8_attention",
            "qh_kv8_attention_plan",
+           "qh_rmsnorm", "qh_rope_turns", "qh_rope",
            "qh_decoder_create",
            "qh_decoder_destroy",
            "qh_decoder_prefill", "qh_decoder_begin", "qh_decoder_step", "qh_decoder_views",
@@ -151,6 +164,10 @@ def _bind(lib):
         "qh_kv8_attention": ([kv8, i32, vp, vp, i32, i32, C.c_int64, C.c_int64, vp, vp, i32, i32, i32, C.c_float, vp, sz,
                               vp], i32),
         "qh_kv8_attention_plan": ([kv8, i32, i32, i32, i32, C.POINTER(qh_kv8_plan)], i32),
+        "qh_rmsnorm": ([vp, vp, vp, i32, C.c_int64, C.c_int64, i32, i32, C.c_double, vp, C.c_int64, vp, C.c_int64, vp, vp, vp],
+                       i32),
+        "qh_rope_turns": ([C.POINTER(qh_rope_desc), vp], i32),
+        "qh_rope": ([vp, i32, i32, C.c_float, i32, C.POINTER(qh_rope_rows), C.POINTER(qh_rope_rows), i32, vp, i32, vp], i32),
         "qh_decoder_create": ([C.POINTER(qh_model_desc), C.POINTER(qh_tensor), i32, C.POINTER(vp)], i32),
         "qh_decoder_destroy": ([vp], i32),
         "qh_decoder_prefill": ([vp, vp, i32, i32, i32, vp], i32),
@@ -558,6 +575,144 @@ class KV8Cache:
         plan = qh_kv8_plan()
         _check(lib().qh_kv8_attention_plan(self._ref, heads, entries, rows, int(single), C.byref(plan)))
         return plan
+
+
+# ------------------------------------------------------------------------------- rows of a step of many sequences
+
+def _here(device) -> int:
+    """The current stream, on `device` (that of a call's tensors), which has to be the current one."""
+    torch = _torch()
+    if device.type != "cuda" or device.index != torch._C._cuda_getDevice():
+        raise QHError(f"the tensors are on {device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _dtype_of(t, what) -> int:
+    torch = _torch()
+    if t.dtype is torch.float32:
+        return F32
+    if t.dtype is torch.float16:
+        return F16
+    raise QHError(f"{what} is {t.dtype}, expected float32 or float16")
+
+
+def _like(t, shape, other, what):
+    """Checks that a tensor has this shape and another's dtype and device."""
+    if tuple(t.shape) != tuple(shape) or t.dtype is not other.dtype or t.device != other.device:
+        raise QHError(f"{what} is {tuple(t.shape)} {t.dtype} on {t.device}, expected {tuple(shape)} {other.dtype} on "
+                      f"{other.device}")
+
+
+def _row_stride(t, what) -> int:
+    """Elements from row to row of a matrix with contiguous rows."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise QHError(f"{what} must be a matrix with contiguous rows")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _rmsnorm(x, w, eps, residual, sum, out, q, d):
+    torch = _torch()
+    dtype, ldx = _dtype_of(x, "x"), _row_stride(x, "x")
+    rows, n = x.shape
+    if w.dtype is not torch.float32 or tuple(w.shape) != (n,) or w.device != x.device or not w.is_contiguous():
+        raise QHError(f"w must be a contiguous float32 vector of {n} on {x.device}")
+    ldr = lds = ldy = n
+    if residual is not None:
+        _like(residual, x.shape, x, "residual")
+        ldr = _row_stride(residual, "residual")
+    if sum is not None:
+        _like(sum, x.shape, x, "sum")
+        lds = _row_stride(sum, "sum")
+    if out is not None:
+        _like(out, x.shape, x, "out")
+        ldy = _row_stride(out, "out")
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    _check(lib().qh_rmsnorm(ptr(x), ptr(residual), ptr(w), dtype, ldx, ldr, rows, n, eps, ptr(sum), lds, ptr(out), ldy,
+                            ptr(q), ptr(d), _here(x.device)))
+
+
+def rmsnorm(x, w, eps: float = 1e-6, residual=None, sum=None, out=None):
+    """Root-mean-square norm of the rows x [rows][n] (float32 or float16; views of wider rows are fine) with weight w
+    (float32 [n]) -> out. With residual: (sum, out), where sum = x + residual is what is normalized; sum may be x or
+    residual itself (in place). See qh_rmsnorm."""
+    torch = _torch()
+    if residual is not None and sum is None:
+        sum = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _rmsnorm(x, w, eps, residual, sum, out, None, None)
+    return out if residual is None else (sum, out)
+
+
+def rmsnorm_q8(x, w, eps: float = 1e-6, residual=None, sum=None):
+    """The same into the 8-bit blocks that the quantized matmuls take: (q, d), as quantize_q8 makes them of the normalized
+    rows in float32; with residual (sum, q, d). n is a multiple of 32."""
+    torch = _torch()
+    if x.dim() != 2 or x.shape[1] % QK:
+        raise QHError(f"x is {tuple(x.shape)}, expected [rows][a multiple of {QK}]")
+    if residual is not None and sum is None:
+        sum = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    d = torch.empty((x.shape[0], x.shape[1] // QK), dtype=torch.float32, device=x.device)
+    _rmsnorm(x, w, eps, residual, sum, None, q, d)
+    return (q, d) if residual is None else (sum, q, d)
+
+
+class Rope:
+    """Rotary positions of heads of head_dim, the first rot_dim dims of each (all by default) in pairs (i, i + rot_dim / 2),
+    or (2 i, 2 i + 1) when interleaved. scaling: None, "linear", "base" or "parts" (qh_rope_desc), with factor and, by
+    parts, context, low and high; magnitude: what cosines and sines are multiplied by. turns: a table of one's own in
+    place of those (float64 [rot_dim / 2]: turns of 2 pi per position)."""
+
+    def __init__(self, head_dim: int, rot_dim: int | None = None, interleaved: bool = False, theta: float = 1e6,
+                 scaling: str | None = None, factor: float = 1.0, context: float = 0.0, low: float = 1.0, high: float = 32.0,
+                 magnitude: float = 1.0, turns=None, device="cuda"):
+        torch = _torch()
+        self.head_dim, self.rot_dim = head_dim, head_dim if rot_dim is None else rot_dim
+        self.interleaved, self.magnitude = int(bool(interleaved)), float(magnitude)
+        if turns is None:
+            kinds = {None: ROPE_PLAIN, "linear": ROPE_LINEAR, "base": ROPE_BASE, "parts": ROPE_PARTS}
+            if scaling not in kinds:
+                raise QHError(f"scaling {scaling!r} is none of {list(kinds)}")
+            desc = qh_rope_desc(theta, self.rot_dim, kinds[scaling], factor, context, low, high)
+            host = np.empty(max(self.rot_dim // 2, 1), np.float64)
+            _check(lib().qh_rope_turns(C.byref(desc), host.ctypes.data))
+            turns = torch.from_numpy(host)
+        if turns.dtype is not torch.float64 or turns.numel() != self.rot_dim // 2:
+            raise QHError(f"turns must be {self.rot_dim // 2} float64 values")
+        self.turns = turns.reshape(-1).to(device).contiguous()
+
+    def _rows(self, x, out, what):
+        if x.dim() != 3 or x.shape[2] != self.head_dim or x.device != self.turns.device:
+            raise QHError(f"{what} is {tuple(x.shape)} on {x.device}, expected [rows][heads][{self.head_dim}] on "
+                          f"{self.turns.device}")
+        strides = []
+        for t, name in ((x, what), (out, f"{what}_out")):
+            _like(t, x.shape, x, name)
+            if x.numel() and ((self.head_dim > 1 and t.stride(2) != 1) or (t.shape[1] > 1 and t.stride(1) != self.head_dim)):
+                raise QHError(f"the heads of a row of {name} must be contiguous")
+            strides.append(t.stride(0) if t.shape[0] > 1 else t.shape[1] * self.head_dim)
+        return qh_rope_rows(x.data_ptr(), out.data_ptr(), strides[0], strides[1], x.shape[1])
+
+    def __call__(self, q, k=None, *, pos, q_out=None, k_out=None):
+        """The rows q and k ([rows][heads][head_dim], float32 or float16; views of one wider row are fine) turned by the
+        positions pos (int32 [rows], on the device) -> (q', k'), or q' without k. q_out / k_out may be q / k (in place)."""
+        torch = _torch()
+        rows = q.shape[0]
+        if pos.dtype is not torch.int32 or tuple(pos.shape) != (rows,) or pos.device != q.device or not pos.is_contiguous():
+            raise QHError(f"pos must be a contiguous int32 vector of {rows} on {q.device}")
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        a, b, dtype = self._rows(q, q_out, "q"), None, _dtype_of(q, "q")
+        if k is not None:
+            if k.shape[0] != rows or k.dtype is not q.dtype:
+                raise QHError("q and k differ in rows or dtype")
+            if k_out is None:
+                k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+            b = C.byref(self._rows(k, k_out, "k"))
+        _check(lib().qh_rope(self.turns.data_ptr(), self.rot_dim, self.interleaved, self.magnitude, self.head_dim,
+                             C.byref(a), b, dtype, pos.data_ptr(), rows, _here(q.device)))
+        return q_out if k is None else (q_out, k_out)
 
 
 # ------------------------------------------------------------------------------------------------ decoder

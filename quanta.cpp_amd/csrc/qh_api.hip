@@ -10,6 +10,7 @@
 
 #include "qh_internal.h"
 #include "qh_kv8.h"
+#include "qh_rows.h"
 
 namespace qh {
 
@@ -174,6 +175,23 @@ Kv8View kv8_view(const qh_kv8_cache& c, int layer) {
     v.seq_pages = c.seq_pages;
     v.page_shift = __builtin_ctz((unsigned)c.page_tokens);
     return v;
+}
+
+// Rows of `width` elements of f32 or f16, ld apart, on their type's alignment.
+int validate_rows(const void* p, int dtype, int64_t ld, int64_t width, const char* what, const char* who) {
+    if (!p) return fail(QH_ERR_ARG, "%s: null %s", who, what);
+    if (ld < width || ld > (int64_t)1 << 32)
+        return fail(QH_ERR_ARG, "%s: rows of %s %lld apart, %lld wide", who, what, (long long)ld, (long long)width);
+    if ((reinterpret_cast<uintptr_t>(p) & (dtype == QH_F32 ? 3u : 1u)) != 0)
+        return fail(QH_ERR_ALIGN, "%s: %s is not aligned to its type", who, what);
+    return QH_OK;
+}
+
+int validate_row_type(int dtype, int n_tok, const char* who) {
+    if (dtype != QH_F32 && dtype != QH_F16) return fail(QH_ERR_DTYPE, "%s: dtype %d is not f32 (0) or f16 (1)", who, dtype);
+    // a launch has fewer than 2^24 workgroups of 256
+    if (n_tok < 0 || n_tok >= 1 << 24) return fail(QH_ERR_SHAPE, "%s: %d rows", who, n_tok);
+    return QH_OK;
 }
 
 // Device checks of qh_init for the current device (gfx950), once per device.
@@ -536,6 +554,90 @@ int qh_shortlist_head_noalloc(const qh_tensor* head8, const qh_tensor* head4, co
     must.n = query->n_must;
     return check_hip(launch_shortlist_head(*head8, *head4, *err, xq, xd, *query, must, *out, ws, as_stream(stream)),
                      "qh_shortlist_head_noalloc launch");
+}
+
+int qh_rmsnorm(const void* x, const void* res, const float* w, int dtype, int64_t ldx, int64_t ldr, int n_tok, int n,
+               double eps, void* sum, int64_t lds, void* y, int64_t ldy, int8_t* q, float* d, void* stream) {
+    const char* who = "qh_rmsnorm";
+    if (int rc = validate_row_type(dtype, n_tok, who)) return rc;
+    if (n <= 0 || n > QH_NORM_MAX) return fail(QH_ERR_SHAPE, "%s: rows of %d, at most %d", who, n, QH_NORM_MAX);
+    if (!(eps >= 0.0 && eps <= 1e38)) return fail(QH_ERR_ARG, "%s: eps is negative or not finite", who);
+    if (q && n % QH_QK != 0) return fail(QH_ERR_SHAPE, "%s: 8-bit blocks of rows of %d (not a multiple of 32)", who, n);
+    if (n_tok == 0) return QH_OK;
+    if (!y && !q) return fail(QH_ERR_ARG, "%s: neither y nor q", who);
+    if ((q == nullptr) != (d == nullptr)) return fail(QH_ERR_ARG, "%s: codes without scales, or scales without codes", who);
+    if (int rc = validate_rows(x, dtype, ldx, n, "x", who)) return rc;
+    if (int rc = validate_rows(w, QH_F32, n, n, "w", who)) return rc;
+    if (res)
+        if (int rc = validate_rows(res, dtype, ldr, n, "res", who)) return rc;
+    if (sum)
+        if (int rc = validate_rows(sum, dtype, lds, n, "sum", who)) return rc;
+    if (y)
+        if (int rc = validate_rows(y, dtype, ldy, n, "y", who)) return rc;
+    if (q && (!aligned16(q) || (reinterpret_cast<uintptr_t>(d) & 3u) != 0))
+        return fail(QH_ERR_ALIGN, "%s: codes not 16-byte aligned, or scales not 4-byte aligned", who);
+    if (y && (y == x || y == res || y == sum)) return fail(QH_ERR_ARG, "%s: y is x, res or sum", who);
+    if (n_tok > 1 && ((sum && sum == x && lds != ldx) || (sum && sum == res && lds != ldr)))
+        return fail(QH_ERR_ARG, "%s: sum in place with another row stride", who);
+    const NormArgs a{x, res, w, sum, y, q, d, ldx, ldr, lds, ldy, n_tok, n, eps};
+    return check_hip(launch_rmsnorm(a, dtype, as_stream(stream)), who);
+}
+
+int qh_rope_turns(const qh_rope_desc* r, double* turns_host) {
+    const char* who = "qh_rope_turns";
+    if (!r || !turns_host) return fail(QH_ERR_ARG, "%s: null argument", who);
+    if (r->rot_dim < 2 || r->rot_dim > QH_ROPE_MAX_DIM || r->rot_dim % 2 != 0)
+        return fail(QH_ERR_SHAPE, "%s: rot_dim %d (even, 2 to %d)", who, r->rot_dim, QH_ROPE_MAX_DIM);
+    if (r->scaling < QH_ROPE_PLAIN || r->scaling > QH_ROPE_PARTS) return fail(QH_ERR_ARG, "%s: scaling %d", who, r->scaling);
+    if (!(r->theta > 0.0 && r->theta <= 1e300)) return fail(QH_ERR_ARG, "%s: theta is not a positive number", who);
+    if (r->scaling != QH_ROPE_PLAIN && !(r->factor > 0.0 && r->factor <= 1e100))
+        return fail(QH_ERR_ARG, "%s: factor is not a positive number", who);
+    if (r->scaling == QH_ROPE_PARTS &&
+        !(r->context > 0.0 && r->context <= 1e100 && r->low >= 0.0 && r->high > r->low && r->high <= 1e100))
+        return fail(QH_ERR_ARG, "%s: by parts needs context > 0 and 0 <= low < high", who);
+    double theta = r->theta;
+    if (r->scaling == QH_ROPE_BASE && r->rot_dim > 2)
+        theta *= pow(r->factor, (double)r->rot_dim / (double)(r->rot_dim - 2));
+    for (int i = 0; i < r->rot_dim / 2; ++i) {
+        double f = pow(theta, -2.0 * i / r->rot_dim) / (2.0 * M_PI);
+        if (r->scaling == QH_ROPE_LINEAR) f /= r->factor;
+        if (r->scaling == QH_ROPE_PARTS) {
+            const double keep = fmin(fmax((r->context * f - r->low) / (r->high - r->low), 0.0), 1.0);
+            f *= keep + (1.0 - keep) / r->factor;
+        }
+        turns_host[i] = f;
+    }
+    return QH_OK;
+}
+
+int qh_rope(const double* turns, int rot_dim, int interleaved, float magnitude, int head_dim, const qh_rope_rows* q,
+            const qh_rope_rows* k, int dtype, const int32_t* pos, int n_tok, void* stream) {
+    const char* who = "qh_rope";
+    if (int rc = validate_row_type(dtype, n_tok, who)) return rc;
+    if (!turns || !q) return fail(QH_ERR_ARG, "%s: null turns or q", who);
+    if ((reinterpret_cast<uintptr_t>(turns) & 7u) != 0) return fail(QH_ERR_ALIGN, "%s: turns not 8-byte aligned", who);
+    if (rot_dim < 2 || rot_dim % 2 != 0 || head_dim < rot_dim || head_dim > QH_ROPE_MAX_DIM)
+        return fail(QH_ERR_SHAPE, "%s: %d of %d dims (even, 2 to %d)", who, rot_dim, head_dim, QH_ROPE_MAX_DIM);
+    if (interleaved != 0 && interleaved != 1) return fail(QH_ERR_ARG, "%s: interleaved = %d", who, interleaved);
+    if (!(fabsf(magnitude) <= 1e38f)) return fail(QH_ERR_ARG, "%s: magnitude is not finite", who);
+    const qh_rope_rows* both[2] = {q, k};
+    for (const qh_rope_rows* r : both) {
+        if (!r) continue;
+        if (r->n_heads < 1 || r->n_heads > 4096) return fail(QH_ERR_SHAPE, "%s: %d heads", who, r->n_heads);
+        if (n_tok == 0) continue;
+        const int64_t width = (int64_t)r->n_heads * head_dim;
+        if (int rc = validate_rows(r->x, dtype, r->ld, width, r == q ? "q" : "k", who)) return rc;
+        if (int rc = validate_rows(r->out, dtype, r->ldo, width, r == q ? "q's result" : "k's result", who)) return rc;
+        if (r->x == r->out && n_tok > 1 && r->ld != r->ldo)
+            return fail(QH_ERR_ARG, "%s: in place with another row stride", who);
+    }
+    if (n_tok == 0) return QH_OK;
+    if (k && (q->out == k->out || q->out == k->x || k->out == q->x)) return fail(QH_ERR_ARG, "%s: q's rows are k's", who);
+    if (!pos || (reinterpret_cast<uintptr_t>(pos) & 3u) != 0) return fail(QH_ERR_ARG, "%s: no positions", who);
+    const RopeRows rq{q->x, q->out, q->ld, q->ldo, q->n_heads};
+    const RopeRows rk = k ? RopeRows{k->x, k->out, k->ld, k->ldo, k->n_heads} : RopeRows{nullptr, nullptr, 0, 0, 0};
+    const RopeArgs a{turns, pos, rq, rk, magnitude, head_dim, rot_dim, n_tok};
+    return check_hip(launch_rope(a, dtype, interleaved != 0, as_stream(stream)), who);
 }
 
 size_t qh_kv8_page_bytes(int page_tokens, int n_kv_heads, int head_dim) {

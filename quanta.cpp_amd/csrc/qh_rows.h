@@ -1,0 +1,40 @@
+// Row operators between the matmuls of a step of many sequences: norm with residual, and rotary positions.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "qh_internal.h"
+
+namespace qh {
+
+// Rows ld elements apart; what a call does not use is null. Any alignment of the type's own size.
+struct NormArgs {
+    const void *x, *res;  // [n_tok][n]
+    const float* w;
+    void *sum, *y;
+    int8_t* q;  // [n_tok][n], d [n_tok][n / 32]
+    float* d;
+    int64_t ldx, ldr, lds, ldy;
+    int n_tok, n;
+    double eps;
+};
+constexpr int kMaxNorm = 32768;  // elements of a row: what a workgroup of 1,024 threads holds in registers
+hipError_t launch_rmsnorm(const NormArgs& a, int dtype, hipStream_t s);
+
+struct RopeRows {
+    const void* x;
+    void* out;
+    int64_t ld, ldo;
+    int heads;
+};
+struct RopeArgs {
+    const double* turns;  // [rot / 2] turns per position
+    const int32_t* pos;   // [n_tok]
+    RopeRows q, k;        // k.heads 0: none
+    float magnitude;
+    int hd, rot, n_tok;
+};
+hipError_t launch_rope(const RopeArgs& a, int dtype, bool interleaved, hipStream_t s);
+
+}  // namespace qh

@@ -1,0 +1,272 @@
+// Rows between the matmuls of a step of many sequences: root-mean-square norm with the residual's addition (into rows or
+// into the matmuls' 8-bit blocks), and rotary positions. Both read and write every element once and are bound by memory;
+// calls of a few rows by the launch and one round of loads.
+#include "qh_device.h"
+#include "qh_rows.h"
+
+namespace qh {
+namespace {
+
+// E elements at any address of the type's alignment: the hardware takes 16-byte accesses at any of them, so odd widths and
+// strides need no second kernel.
+template <typename T>
+constexpr int kE = 16 / (int)sizeof(T);
+template <typename T>
+struct Vec {
+    typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+};
+
+// Elements [0, n) of the E at p into f32 (the others 0), n uniform over most lanes.
+template <typename T>
+__device__ __forceinline__ void load_e(const T* p, int n, float (&x)[kE<T>]) {
+    if (n >= kE<T>) {
+        const auto v = *reinterpret_cast<const typename Vec<T>::type*>(p);
+#pragma unroll
+        for (int i = 0; i < kE<T>; ++i) x[i] = (float)v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < kE<T>; ++i) x[i] = i < n ? (float)p[i] : 0.0f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store_e(T* p, int n, const float (&x)[kE<T>]) {
+    if (n >= kE<T>) {
+        typename Vec<T>::type v;
+#pragma unroll
+        for (int i = 0; i < kE<T>; ++i) v[i] = (T)x[i];
+        *reinterpret_cast<typename Vec<T>::type*>(p) = v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < kE<T>; ++i)
+            if (i < n) p[i] = (T)x[i];
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------- norm
+
+// The 8-bit block of which this lane holds E consecutive values and the 32 / E lanes of its aligned group the others:
+// quantize_q8's codes and scale.
+__device__ __forceinline__ void quant_lanes(const float (&v)[4], int8_t* q, float* d) {
+    quant_block_x8(make_float4(v[0], v[1], v[2], v[3]), q, d);
+}
+__device__ __forceinline__ void quant_lanes(const float (&v)[8], int8_t* q, float* d) {
+    float a = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a = __builtin_fmaxf(a, __builtin_fabsf(v[i]));
+    a = dpp_max<0xB1>(a);
+    a = dpp_max<0x4E>(a);
+    const float sc = a / 127.0f, inv = sc > 0.0f ? 1.0f / sc : 0.0f;
+    uint32_t c[2] = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i >> 2] |= (uint32_t)(uint8_t)(int8_t)(int)round_half_away(v[i] * inv) << (8 * (i & 3));
+    const int j = (int)threadIdx.x & 3;
+    *reinterpret_cast<uint2*>(q + 8 * j) = make_uint2(c[0], c[1]);
+    if (j == 0) *d = sc;
+}
+
+// kWaves waves to a row, kVec vectors of E elements to a lane, 4 / kWaves rows to a workgroup of at least 4 waves. The sum
+// of squares and the scaled products are 64-bit (as fast as 32-bit ones here, and far from the memory's time): no square
+// overflows, the order of the sum does not show, and y is rounded once.
+template <typename T, int kWaves, int kVec>
+__global__ __launch_bounds__(kWaves < 4 ? 256 : 64 * kWaves) void rmsnorm_kernel(NormArgs a) {
+    constexpr int E = kE<T>, kRows = kWaves < 4 ? 4 / kWaves : 1;
+    const int tid = (int)threadIdx.x % (64 * kWaves);
+    const int row = (int)blockIdx.x * kRows + (int)threadIdx.x / (64 * kWaves);
+    __shared__ double part[kWaves < 4 ? 4 : kWaves];
+    if (kWaves == 1 && row >= a.n_tok) return;
+    const bool there = row < a.n_tok;
+    float h[kVec][E];
+    double ss = 0.0;
+    if (there) {
+        const T* x = static_cast<const T*>(a.x) + (int64_t)row * a.ldx;
+        const T* res = static_cast<const T*>(a.res) + (int64_t)row * a.ldr;
+        T* sum = static_cast<T*>(a.sum) + (int64_t)row * a.lds;
+        float r[kVec][E];
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) {
+            const int i = (c * 64 * kWaves + tid) * E;
+            load_e(x + i, a.n - i, h[c]);
+            if (a.res) load_e(res + i, a.n - i, r[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) {
+            const int i = (c * 64 * kWaves + tid) * E;
+            if (a.res) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) h[c][e] = (float)(T)(h[c][e] + r[c][e]);
+            }
+            if (a.sum) store_e(sum + i, a.n - i, h[c]);
+#pragma unroll
+            for (int e = 0; e < E; ++e) ss = __builtin_fma((double)h[c][e], (double)h[c][e], ss);
+        }
+    }
+    ss = wave_reduce32x2(ss, [](double p, double q) { return p + q; });
+    if (kWaves > 1) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = ss;
+        __syncthreads();
+        const int first = (int)threadIdx.x / (64 * kWaves) * kWaves;
+        ss = 0.0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) ss += part[first + w];
+    }
+    if (!there) return;
+    const double scale = 1.0 / __builtin_sqrt(ss / (double)a.n + a.eps);
+#pragma unroll
+    for (int c = 0; c < kVec; ++c) {
+        const int i = (c * 64 * kWaves + tid) * E;
+        if (i >= a.n) break;
+        float w[kE<T>];
+#pragma unroll
+        for (int v = 0; v < E / 4; ++v) {
+            float w4[4];
+            load_e(a.w + i + 4 * v, a.n - i - 4 * v, w4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[4 * v + e] = w4[e];
+        }
+        float y[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = (float)((double)h[c][e] * scale * (double)w[e]);
+        if (a.y) store_e(static_cast<T*>(a.y) + (int64_t)row * a.ldy + i, a.n - i, y);
+        if (a.q) quant_lanes(y, a.q + (int64_t)row * a.n + i / 32 * 32, a.d + (int64_t)row * (a.n / 32) + i / 32);
+    }
+}
+
+template <typename T>
+hipError_t rmsnorm_of(const NormArgs& a, hipStream_t s) {
+    const int vecs = (a.n + kE<T> - 1) / kE<T>;
+    auto run = [&](auto waves, auto vec) {
+        constexpr int kWaves = decltype(waves)::value, kRows = kWaves < 4 ? 4 / kWaves : 1;
+        qh_launch((rmsnorm_kernel<T, kWaves, decltype(vec)::value>), dim3((unsigned)((a.n_tok + kRows - 1) / kRows)),
+                  dim3(kWaves < 4 ? 256 : 64 * kWaves), 0, s, a);
+    };
+    using std::integral_constant;
+    if (vecs <= 64) run(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+    else if (vecs <= 256) run(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+    else if (vecs <= 512) run(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+    else if (vecs <= 1024) run(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+    else if (vecs <= 2048) run(integral_constant<int, 4>{}, integral_constant<int, 8>{});
+    else if (vecs <= 4096) run(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+    else run(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+    return hipGetLastError();
+}
+
+// ------------------------------------------------------------------------------------------------------- rope
+
+// cos and sin of 2 pi t, |t| <= 1/2. t is brought within an eighth of a turn of a multiple of a quarter, exactly; there the
+// power series to x^9 and x^8 are off by less than 2^-27.
+__device__ __forceinline__ float2 turn(double t) {
+    const double k = __builtin_rint(4.0 * t);
+    const float x = (float)((4.0 * t - k) * 1.5707963267948966), z = x * x;
+    float s = __builtin_fmaf(z, 1.0f / 362880, -1.0f / 5040);
+    s = __builtin_fmaf(z, s, 1.0f / 120);
+    s = __builtin_fmaf(z, s, -1.0f / 6);
+    s = __builtin_fmaf(z * x, s, x);
+    float c = __builtin_fmaf(z, -1.0f / 3628800, 1.0f / 40320);
+    c = __builtin_fmaf(z, c, -1.0f / 720);
+    c = __builtin_fmaf(z, c, 1.0f / 24);
+    c = __builtin_fmaf(z, c, -0.5f);
+    c = __builtin_fmaf(z, c, 1.0f);
+    const int quarter = (int)k & 3;
+    const float co = (quarter & 1) ? s : c, si = (quarter & 1) ? c : s;
+    return make_float2(quarter == 1 || quarter == 2 ? -co : co, quarter >= 2 ? -si : si);
+}
+
+// floor(g / d) with d's number from magic_of.
+__device__ __forceinline__ uint32_t div_below(uint32_t g, uint32_t magic) { return magic ? div_magic(g, magic) : g; }
+
+constexpr int kRopeThreads = 256;
+constexpr int kRopePairs = 512;  // cosines and sines that a workgroup keeps
+
+// A workgroup takes `per` tokens: their cosines and sines once into LDS (angles in 64 bits: position times turns per
+// position, less its whole turns), then every head's pairs, E of them to an item, and after them the dims past rot, E to an
+// item, where the result is not written in place. Consecutive lanes take consecutive items of a head, so rows move in one
+// piece.
+template <typename T, bool kInterleaved>
+__global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a, int per, int units, int rest, uint32_t unit_magic,
+                                                            uint32_t head_magic) {
+    constexpr int E = kE<T>;
+    __shared__ float2 cs[kRopePairs];
+    const int half = a.rot >> 1, t0 = (int)blockIdx.x * per, n = min(per, a.n_tok - t0), tid = (int)threadIdx.x;
+    for (int i = tid; i < n * half; i += kRopeThreads) {
+        const int t = i / half;
+        const double turns = (double)a.pos[t0 + t] * a.turns[i - t * half];
+        const float2 v = turn(turns - __builtin_rint(turns));
+        cs[i] = make_float2(v.x * a.magnitude, v.y * a.magnitude);
+    }
+    __syncthreads();
+    const int each = units + rest, heads = a.q.heads + a.k.heads;
+    for (int item = tid; item < n * heads * each; item += kRopeThreads) {
+        const int th = (int)div_below((uint32_t)item, unit_magic), u = item - th * each;
+        const int t = (int)div_below((uint32_t)th, head_magic), h = th - t * heads;
+        const bool of_q = h < a.q.heads;
+        const int at = (of_q ? h : h - a.q.heads) * a.hd;
+        const T* x = static_cast<const T*>(of_q ? a.q.x : a.k.x) + (int64_t)(t0 + t) * (of_q ? a.q.ld : a.k.ld) + at;
+        T* out = static_cast<T*>(of_q ? a.q.out : a.k.out) + (int64_t)(t0 + t) * (of_q ? a.q.ldo : a.k.ldo) + at;
+        if (u >= units) {
+            const int i = a.rot + (u - units) * E;
+            float v[E];
+            load_e(x + i, a.hd - i, v);
+            store_e(out + i, a.hd - i, v);
+            continue;
+        }
+        const int p = u * E, m = half - p;
+        const float2* c = cs + t * half + p;
+        float f[E], g[E];  // firsts and seconds of the pairs (half), or the pairs in order (interleaved)
+        if (kInterleaved) {
+            load_e(x + 2 * p, 2 * m, f);
+            load_e(x + 2 * p + E, 2 * m - E, g);
+            float o[2][E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const float2 w = c[i < m ? i : 0];
+                const float lo = 2 * i < E ? f[2 * i % E] : g[2 * i % E], hi = 2 * i < E ? f[2 * i % E + 1] : g[2 * i % E + 1];
+                o[2 * i / E][2 * i % E] = __builtin_fmaf(lo, w.x, -(hi * w.y));
+                o[2 * i / E][2 * i % E + 1] = __builtin_fmaf(hi, w.x, lo * w.y);
+            }
+            store_e(out + 2 * p, 2 * m, o[0]);
+            store_e(out + 2 * p + E, 2 * m - E, o[1]);
+        } else {
+            load_e(x + p, m, f);
+            load_e(x + half + p, m, g);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const float2 w = c[i < m ? i : 0];
+                const float lo = f[i], hi = g[i];
+                f[i] = __builtin_fmaf(lo, w.x, -(hi * w.y));
+                g[i] = __builtin_fmaf(hi, w.x, lo * w.y);
+            }
+            store_e(out + p, m, f);
+            store_e(out + half + p, m, g);
+        }
+    }
+}
+
+// Exact floor(g / d) by div_below with this number, for g * d < 2^32.
+uint32_t magic_of(int d) { return d == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + (uint32_t)d - 1) / (uint32_t)d); }
+
+template <typename T>
+hipError_t rope_of(const RopeArgs& a, bool interleaved, hipStream_t s) {
+    constexpr int E = kE<T>;
+    const int half = a.rot / 2, units = (half + E - 1) / E, heads = a.q.heads + a.k.heads;
+    const bool copies = a.q.x != a.q.out || (a.k.heads > 0 && a.k.x != a.k.out);
+    const int rest = copies ? (a.hd - a.rot + E - 1) / E : 0;
+    int per = a.n_tok / 2048;
+    per = per < 1 ? 1 : per < kRopePairs / half ? per : kRopePairs / half;
+    const dim3 grid((unsigned)((a.n_tok + per - 1) / per));
+    const uint32_t um = magic_of(units + rest), hm = magic_of(heads);
+    if (interleaved) qh_launch((rope_kernel<T, true>), grid, dim3(kRopeThreads), 0, s, a, per, units, rest, um, hm);
+    else qh_launch((rope_kernel<T, false>), grid, dim3(kRopeThreads), 0, s, a, per, units, rest, um, hm);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_rmsnorm(const NormArgs& a, int dtype, hipStream_t s) {
+    return dtype == QH_F32 ? rmsnorm_of<float>(a, s) : rmsnorm_of<_Float16>(a, s);
+}
+
+hipError_t launch_rope(const RopeArgs& a, int dtype, bool interleaved, hipStream_t s) {
+    return dtype == QH_F32 ? rope_of<float>(a, interleaved, s) : rope_of<_Float16>(a, interleaved, s);
+}
+
+}  // namespace qh
