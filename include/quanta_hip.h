@@ -328,6 +328,15 @@ int qh_kv8_resize(const qh_kv8_cache* c, const int32_t* seqs, const int32_t* len
 int qh_kv8_fork(const qh_kv8_cache* c, const int32_t* src, const int32_t* dst, int n, int copy, void* workspace,
                 size_t workspace_bytes, void* stream);
 
+/* Sequence dst[i] takes what src[i] held before the call, for every i of the list at once (DEVICE arrays of n; each dst once;
+ * dst NULL: sequence i): a beam search's sequences become those of the beams that are continued. src may name sequences of
+ * dst, any number of times, and -1 leaves its dst empty. Pages are shared; pages that no sequence holds afterwards are free.
+ * qh_kv8_resize then gives each sequence room for its next token, with a copy of a partly filled last page that others hold.
+ * Workspace: 16-byte aligned, no initialisation; NULL where the size is 0. */
+size_t qh_kv8_reorder_workspace_bytes(const qh_kv8_cache* c);
+int qh_kv8_reorder(const qh_kv8_cache* c, const int32_t* src, const int32_t* dst, int n, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
 /* Moves the pages in use to the front: with L of them, those numbered L and above move, in order, to the free numbers
  * below L, in every layer, and the tables follow. *live (DEVICE, may be NULL) = L: the pages from L on are free. */
 int qh_kv8_compact(const qh_kv8_cache* c, int32_t* live, void* workspace, size_t workspace_bytes, void* stream);
@@ -445,6 +454,24 @@ typedef struct qh_rope_rows {
  * kernels keep the reference's f32 table to the bit. */
 int qh_rope(const double* turns, int rot_dim, int interleaved, float magnitude, int head_dim, const qh_rope_rows* q,
             const qh_rope_rows* k, int dtype, const int32_t* pos, int n_tok, void* stream);
+
+/* Beam search's selection. logits: DEVICE rows [n_prompts * beams][n_valid] of dtype QH_F32 or QH_F16, ld elements apart, on
+ * any alignment of their type; scores: DEVICE f32 [n_prompts * beams], what each beam has so far (NULL: 0). A candidate is a
+ * beam b of a prompt and an id v, with the score scores[b] + logits[b][v] - log sum_u exp(logits[b][u]); sums, exponentials
+ * and the comparison of candidates are 64-bit, and equal ones go to the lower b, then the lower v. For each prompt its k best
+ * candidates, best first, into DEVICE arrays [n_prompts][k]: parent (the row, prompt * beams + b), token and score (f32). A
+ * logit of -infinity is no candidate, and neither is any of a row whose score is not finite or whose logits hold a NaN or
+ * +infinity or are all -infinity (a beam that ended gets the score -infinity); where there are fewer than k, the places
+ * behind them have parent and token -1 and the score -infinity (which is also what a score past f32's range rounds to). beams
+ * at most QH_BEAM_MAX_BEAMS, k at most QH_BEAM_MAX_K, n_valid at most QH_SAMPLE_MAX_VOCAB. The workspace is 16-byte aligned and needs no initialisation; calls that overlap must
+ * not share one.
+ * No counterpart in the reference, which samples one sequence (Sampler::sample, sampler.cpp:22-85). */
+#define QH_BEAM_MAX_BEAMS 256
+#define QH_BEAM_MAX_K 256
+size_t qh_beam_workspace_bytes(int dtype, int n_prompts, int beams, int n_valid);
+int qh_beam_select(const void* logits, int dtype, int64_t ld, const float* scores, int n_prompts, int beams, int n_valid,
+                   int k, int32_t* parent, int32_t* token, float* score, void* workspace, size_t workspace_bytes,
+                   void* stream);
 
 /* ------------------------------------------------------------------ GPU-resident decoder */
 

@@ -71,6 +71,7 @@ def sampler_params(temperature=0.7, top_k=20, top_p=0.8, min_p=0.0, repeat_penal
     return qh_sampler_params(temperature, top_k, top_p, min_p, repeat_penalty, repeat_window)
 
 
+BEAM_MAX_BEAMS, BEAM_MAX_K = 256, 256  # QH_BEAM_MAX_*
 KV8_BLOCK = 16  # QH_KV8_BLOCK: tokens that share a scale
 KV8_NO_PAGES, KV8_BAD_LIST, KV8_SHARED = 1, 2, 4  # bits of KV8Cache.status
 
@@ -111,9 +112,10 @@ EXPORTS = ("qh_last_error", "qh_version", "qh_init", "qh_quant_bytes", "qh_tenso
            "qh_head_planes", "qh_shortlist_planes",
            "qh_sampler_state", "qh_sample", "qh_sample_workspace_bytes", "qh_sample_ws",
            "qh_kv8_page_bytes", "qh_kv8_reset", "qh_kv8_pages_workspace_bytes", "qh_kv8_resize", "qh_kv8_fork",
+           "qh_kv8_reorder_workspace_bytes", "qh_kv8_reorder",
            "qh_kv8_compact", "qh_kv8_append", "qh_kv8_read", "qh_kv8_attention_workspace_bytes", "qh_kv8_attention",
            "qh_kv8_attention_plan",
-           "qh_rmsnorm", "qh_rope_turns", "qh_rope",
+           "qh_rmsnorm", "qh_rope_turns", "qh_rope", "qh_beam_workspace_bytes", "qh_beam_select",
            "qh_decoder_create",
            "qh_decoder_destroy",
            "qh_decoder_prefill", "qh_decoder_begin", "qh_decoder_step", "qh_decoder_views",
@@ -157,6 +159,8 @@ def _bind(lib):
         "qh_kv8_pages_workspace_bytes": ([kv8], sz),
         "qh_kv8_resize": ([kv8, vp, vp, i32, vp, sz, vp], i32),
         "qh_kv8_fork": ([kv8, vp, vp, i32, i32, vp, sz, vp], i32),
+        "qh_kv8_reorder_workspace_bytes": ([kv8], sz),
+        "qh_kv8_reorder": ([kv8, vp, vp, i32, vp, sz, vp], i32),
         "qh_kv8_compact": ([kv8, vp, vp, sz, vp], i32),
         "qh_kv8_append": ([kv8, i32, vp, vp, i32, C.c_int64, C.c_int64, vp, vp, i32, i32, vp], i32),
         "qh_kv8_read": ([kv8, i32, vp, vp, i32, C.c_int64, C.c_int64, vp, vp, i32, i32, vp], i32),
@@ -168,6 +172,8 @@ def _bind(lib):
                        i32),
         "qh_rope_turns": ([C.POINTER(qh_rope_desc), vp], i32),
         "qh_rope": ([vp, i32, i32, C.c_float, i32, C.POINTER(qh_rope_rows), C.POINTER(qh_rope_rows), i32, vp, i32, vp], i32),
+        "qh_beam_workspace_bytes": ([i32, i32, i32, i32], sz),
+        "qh_beam_select": ([vp, i32, C.c_int64, vp, i32, i32, i32, i32, vp, vp, vp, vp, sz, vp], i32),
         "qh_decoder_create": ([C.POINTER(qh_model_desc), C.POINTER(qh_tensor), i32, C.POINTER(vp)], i32),
         "qh_decoder_destroy": ([vp], i32),
         "qh_decoder_prefill": ([vp, vp, i32, i32, i32, vp], i32),
@@ -444,6 +450,8 @@ class KV8Cache:
         # resize, fork and compact change the cache, so they are in order and can share a workspace
         self._pages_ws = torch.empty(self._pages_bytes, dtype=torch.uint8, device=device)
         self._pages_ptr = self._pages_ws.data_ptr()
+        self._reorder_bytes = lib().qh_kv8_reorder_workspace_bytes(self._ref)
+        self._reorder_ws = torch.empty(self._reorder_bytes, dtype=torch.uint8, device=device)
         self._attention_ws = {}  # bytes by (heads, entries, rows)
         self._scale = head_dim ** -0.5
         self.reset()
@@ -510,6 +518,14 @@ class KV8Cache:
         """Sequence dst[i] becomes a fork of src[i]: it shares its pages, or (copy) holds copies of them."""
         n = src.numel()
         self._pages_call("qh_kv8_fork", self._ints(src, n, "src"), self._ints(dst, n, "dst"), n, int(copy))
+
+    def reorder(self, src, dst=None) -> None:
+        """Sequence dst[i] (i itself without dst) takes what src[i] held before the call, all at once: src may name the same
+        sequences, any number of times, and -1 leaves its dst empty. Pages are shared; `resize` then makes room."""
+        n = src.numel()
+        _check(lib().qh_kv8_reorder(self._ref, self._ints(src, n, "src"), None if dst is None else self._ints(dst, n, "dst"),
+                                    n, self._reorder_ws.data_ptr() if self._reorder_bytes else None, self._reorder_bytes,
+                                    self._here()))
 
     def compact(self):
         """Moves the pages in use to the front of the pool; returns how many there are (int32 device tensor [1])."""
@@ -713,6 +729,32 @@ class Rope:
         _check(lib().qh_rope(self.turns.data_ptr(), self.rot_dim, self.interleaved, self.magnitude, self.head_dim,
                              C.byref(a), b, dtype, pos.data_ptr(), rows, _here(q.device)))
         return q_out if k is None else (q_out, k_out)
+
+
+def beam_select(logits, scores, beams: int, k: int, n_valid: int | None = None):
+    """The k best continuations of each prompt's beams: logits [prompts * beams][vocabulary] (float32 or float16; views of
+    wider rows are fine), scores float32 [prompts * beams] or None (0), n_valid: ids from it on do not count. Returns
+    (parent, token, score), each [prompts][k], best first: the row that is continued, the id (both int32) and
+    score + log-softmax (float32); -1, -1 and -inf where there are fewer candidates. See qh_beam_select."""
+    torch = _torch()
+    dtype, ld = _dtype_of(logits, "logits"), _row_stride(logits, "logits")
+    rows, n = logits.shape
+    n_valid = n if n_valid is None else n_valid
+    if beams < 1 or rows % beams or not 1 <= n_valid <= n:
+        raise QHError(f"{rows} rows of {beams} beams, {n_valid} of {n} ids")
+    if scores is not None and (scores.dtype is not torch.float32 or tuple(scores.shape) != (rows,) or
+                               scores.device != logits.device or not scores.is_contiguous()):
+        raise QHError(f"scores must be a contiguous float32 vector of {rows} on {logits.device}")
+    prompts, dev = rows // beams, logits.device
+    parent = torch.empty((prompts, k), dtype=torch.int32, device=dev)
+    token = torch.empty((prompts, k), dtype=torch.int32, device=dev)
+    score = torch.empty((prompts, k), dtype=torch.float32, device=dev)
+    # a tensor for each call: nothing of one call (or captured graph) is shared with the next
+    ws = torch.empty(lib().qh_beam_workspace_bytes(dtype, prompts, beams, n_valid), dtype=torch.uint8, device=dev)
+    _check(lib().qh_beam_select(logits.data_ptr(), dtype, ld, None if scores is None else scores.data_ptr(), prompts, beams,
+                                n_valid, k, parent.data_ptr(), token.data_ptr(), score.data_ptr(), ws.data_ptr(), ws.numel(),
+                                _here(dev)))
+    return parent, token, score
 
 
 # ------------------------------------------------------------------------------------------------ decoder

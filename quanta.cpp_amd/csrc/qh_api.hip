@@ -640,6 +640,44 @@ int qh_rope(const double* turns, int rot_dim, int interleaved, float magnitude, 
     return check_hip(launch_rope(a, dtype, interleaved != 0, as_stream(stream)), who);
 }
 
+namespace {
+// The shape of a beam selection; up to 2^17 rows, so that its work items are told apart in 32 bits.
+int validate_beams(int dtype, int n_prompts, int beams, int n_valid, const char* who) {
+    if (dtype != QH_F32 && dtype != QH_F16) return fail(QH_ERR_DTYPE, "%s: dtype %d is not f32 (0) or f16 (1)", who, dtype);
+    if (beams < 1 || beams > QH_BEAM_MAX_BEAMS || n_valid < 1 || n_valid > QH_SAMPLE_MAX_VOCAB || n_prompts < 0 ||
+        (int64_t)n_prompts * beams > 1 << 17)
+        return fail(QH_ERR_SHAPE, "%s: %d prompts of %d beams over %d ids", who, n_prompts, beams, n_valid);
+    return QH_OK;
+}
+}  // namespace
+
+size_t qh_beam_workspace_bytes(int dtype, int n_prompts, int beams, int n_valid) {
+    return validate_beams(dtype, n_prompts, beams, n_valid, "qh_beam_workspace_bytes")
+               ? 0
+               : beam_workspace_bytes(dtype, n_prompts, beams, n_valid);
+}
+
+int qh_beam_select(const void* logits, int dtype, int64_t ld, const float* scores, int n_prompts, int beams, int n_valid,
+                   int k, int32_t* parent, int32_t* token, float* score, void* workspace, size_t workspace_bytes,
+                   void* stream) {
+    const char* who = "qh_beam_select";
+    if (int rc = validate_beams(dtype, n_prompts, beams, n_valid, who)) return rc;
+    if (k < 1 || k > QH_BEAM_MAX_K) return fail(QH_ERR_UNSUPPORTED, "%s: k %d outside [1, %d]", who, k, QH_BEAM_MAX_K);
+    if (n_prompts == 0) return QH_OK;
+    if (int rc = validate_rows(logits, dtype, ld, n_valid, "logits", who)) return rc;
+    if (!parent || !token || !score) return fail(QH_ERR_ARG, "%s: null output", who);
+    if (((reinterpret_cast<uintptr_t>(scores) | reinterpret_cast<uintptr_t>(parent) | reinterpret_cast<uintptr_t>(token) |
+          reinterpret_cast<uintptr_t>(score)) & 3u) != 0)
+        return fail(QH_ERR_ALIGN, "%s: scores or outputs not 4-byte aligned", who);
+    if (score == scores) return fail(QH_ERR_ARG, "%s: score is scores", who);
+    const size_t need = beam_workspace_bytes(dtype, n_prompts, beams, n_valid);
+    if (!workspace || workspace_bytes < need)
+        return fail(QH_ERR_NOMEM, "%s: workspace of %zu bytes, needs %zu", who, workspace ? workspace_bytes : 0, need);
+    if (!aligned16(workspace)) return fail(QH_ERR_ALIGN, "%s: workspace not 16-byte aligned", who);
+    const BeamArgs a{logits, scores, parent, token, score, workspace, ld, n_prompts, beams, n_valid, k};
+    return check_hip(launch_beam_select(a, dtype, as_stream(stream)), who);
+}
+
 size_t qh_kv8_page_bytes(int page_tokens, int n_kv_heads, int head_dim) {
     return kv8_shape_ok(page_tokens, n_kv_heads, head_dim) ? kv8_page_bytes(page_tokens, n_kv_heads, head_dim) : 0;
 }
@@ -671,6 +709,23 @@ int qh_kv8_fork(const qh_kv8_cache* c, const int32_t* src, const int32_t* dst, i
     if (copy != 0 && copy != 1) return fail(QH_ERR_ARG, "%s: copy = %d", who, copy);
     return check_hip(launch_kv8_fork(kv8_view(*c, 0), c->n_layers, src, dst, n, copy != 0, workspace, as_stream(stream)),
                      who);
+}
+
+size_t qh_kv8_reorder_workspace_bytes(const qh_kv8_cache* c) {
+    return validate_kv8(c, "qh_kv8_reorder_workspace_bytes") ? 0 : kv8_reorder_workspace_bytes(c->n_seqs, c->seq_pages);
+}
+
+int qh_kv8_reorder(const qh_kv8_cache* c, const int32_t* src, const int32_t* dst, int n, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+    const char* who = "qh_kv8_reorder";
+    if (int rc = validate_kv8(c, who)) return rc;
+    if (n == 0) return QH_OK;
+    if (n < 0 || n > c->n_seqs || !src) return fail(QH_ERR_ARG, "%s: a list of %d of %d sequences", who, n, c->n_seqs);
+    const size_t need = kv8_reorder_workspace_bytes(c->n_seqs, c->seq_pages);
+    if (need > (workspace ? workspace_bytes : 0))
+        return fail(QH_ERR_NOMEM, "%s: workspace of %zu bytes, needs %zu", who, workspace ? workspace_bytes : 0, need);
+    if (!aligned16(workspace)) return fail(QH_ERR_ALIGN, "%s: workspace not 16-byte aligned", who);
+    return check_hip(launch_kv8_reorder(kv8_view(*c, 0), src, dst, n, workspace, as_stream(stream)), who);
 }
 
 int qh_kv8_compact(const qh_kv8_cache* c, int32_t* live, void* workspace, size_t workspace_bytes, void* stream) {

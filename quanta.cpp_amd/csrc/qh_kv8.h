@@ -122,6 +122,8 @@ hipError_t launch_kv8_resize(const Kv8View& c, int n_layers, const int32_t* seqs
                              hipStream_t s);
 hipError_t launch_kv8_fork(const Kv8View& c, int n_layers, const int32_t* src, const int32_t* dst, int n, bool copy,
                            void* ws, hipStream_t s);
+size_t kv8_reorder_workspace_bytes(int n_seqs, int seq_pages);
+hipError_t launch_kv8_reorder(const Kv8View& c, const int32_t* src, const int32_t* dst, int n, void* ws, hipStream_t s);
 hipError_t launch_kv8_compact(const Kv8View& c, int n_layers, int32_t* live, void* ws, hipStream_t s);
 // qh_kv8_attn.hip
 // capacity: positions that a sequence can have. oq, od (one entry): the f32 rows of out (without gaps) in 8 bits too, as

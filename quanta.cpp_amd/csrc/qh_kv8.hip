@@ -1,5 +1,5 @@
 // The 8-bit paged key / value cache (layout in qh_kv8.h): rows quantized into it, rows read back, and its pages (resize,
-// fork, compact).
+// fork, reorder, compact).
 #include "qh_device.h"
 #include "qh_kv8.h"
 
@@ -615,6 +615,114 @@ __global__ __launch_bounds__(256) void kv8_share_kernel(Kv8View c, const int32_t
     share_page(c, src[blockIdx.y], dst[blockIdx.y], (int)(blockIdx.x * 256 + threadIdx.x));
 }
 
+// Sequence dst[i] takes what src[i] held (-1: nothing), all at once: src may name sequences of dst, so every new row is read
+// before any is written. Counts only ever move by one for an entry that goes and one for an entry that comes, so their order
+// does not matter. Up to kReorderHere table entries in one workgroup, the rows in its registers; else the rows into the
+// workspace by the whole GPU (its first workgroup checks the lists), and from there in a second launch.
+constexpr int kReorderHere = 8 * kWg;
+struct ReorderWs {
+    int* ok;
+    int *before, *after;  // [n_seqs] lengths of dst and of src
+    int* rows;            // [n_seqs][seq_pages] src's pages
+};
+__host__ __device__ __forceinline__ ReorderWs reorder_ws(void* ws, int n_seqs) {
+    int* p = static_cast<int*>(ws);
+    return {p, p + 4, p + 4 + n_seqs, p + 4 + 2 * (size_t)n_seqs};
+}
+
+__device__ __forceinline__ int seq_at(const int32_t* list, int i) { return list ? list[i] : i; }
+
+// Whether the lists are fit, by one workgroup of kWg threads; seen: n_seqs bits of LDS.
+__device__ bool reorder_lists_ok(const Kv8View& c, const int32_t* src, const int32_t* dst, int n, uint32_t* seen) {
+    const int tid = (int)threadIdx.x;
+    for (int i = tid; i < (c.n_seqs + 31) / 32; i += kWg) seen[i] = 0;
+    __syncthreads();
+    int bad = 0;
+    for (int i = tid; i < n; i += kWg) bad |= !first_seen(seen, seq_at(dst, i), c.n_seqs) || src[i] < -1 || src[i] >= c.n_seqs;
+    bad = __syncthreads_or(bad);
+    if (bad && tid == 0) atomicOr(c.status, QH_KV8_BAD_LIST);
+    return !bad;
+}
+
+// Entry j of sequence d's table row, which held `before` tokens, becomes `page`, its row `after` tokens long.
+__device__ __forceinline__ void replace_page(const Kv8View& c, int d, int j, int before, int after, int page) {
+    int32_t* slot = c.table + (size_t)d * c.seq_pages + j;
+    if (j < pages_of(c, before)) {
+        const int old = *slot;
+        if (old >= 0 && old < c.n_pages) atomicSub(&c.refs[old], 1);
+        if (j >= pages_of(c, after)) *slot = -1;
+    }
+    if (j < pages_of(c, after)) {
+        *slot = page;
+        if (page >= 0 && page < c.n_pages) atomicAdd(&c.refs[page], 1);
+    }
+}
+
+__global__ __launch_bounds__(kWg) void kv8_reorder_here_kernel(Kv8View c, const int32_t* __restrict__ src,
+                                                               const int32_t* __restrict__ dst, int n) {
+    __shared__ uint32_t seen[QH_KV8_MAX_SEQS / 32];
+    if (!reorder_lists_ok(c, src, dst, n, seen)) return;
+    constexpr int kPer = kReorderHere / kWg;
+    const int tid = (int)threadIdx.x, total = n * c.seq_pages;
+    int page[kPer], before[kPer], after[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const int e = k * kWg + tid, i = e / c.seq_pages, j = e - i * c.seq_pages;
+        if (e >= total) break;
+        const int s = src[i];
+        before[k] = kv8_len(c, seq_at(dst, i));
+        after[k] = s < 0 ? 0 : kv8_len(c, s);
+        page[k] = j < pages_of(c, after[k]) ? c.table[(size_t)s * c.seq_pages + j] : -1;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const int e = k * kWg + tid, i = e / c.seq_pages, j = e - i * c.seq_pages;
+        if (e >= total) break;
+        const int d = seq_at(dst, i);
+        if (src[i] == d) continue;
+        replace_page(c, d, j, before[k], after[k], page[k]);
+        if (j == 0) c.lens[d] = after[k];
+    }
+}
+
+__global__ __launch_bounds__(kWg) void kv8_reorder_read_kernel(Kv8View c, const int32_t* __restrict__ src,
+                                                               const int32_t* __restrict__ dst, int n, void* ws) {
+    __shared__ uint32_t seen[QH_KV8_MAX_SEQS / 32];
+    const ReorderWs w = reorder_ws(ws, c.n_seqs);
+    const int tid = (int)threadIdx.x;
+    if (blockIdx.x == 0) {
+        const bool ok = reorder_lists_ok(c, src, dst, n, seen);
+        if (tid == 0) *w.ok = ok;
+        return;
+    }
+    // a wave to a row
+    for (int i = ((int)blockIdx.x - 1) * (kWg / 64) + (tid >> 6); i < n; i += ((int)gridDim.x - 1) * (kWg / 64)) {
+        const int s = src[i], d = seq_at(dst, i);
+        const int after = s >= 0 && s < c.n_seqs ? kv8_len(c, s) : 0;
+        for (int j = tid & 63; j < pages_of(c, after); j += 64)
+            w.rows[(size_t)i * c.seq_pages + j] = c.table[(size_t)s * c.seq_pages + j];
+        if ((tid & 63) == 0) {
+            w.before[i] = d >= 0 && d < c.n_seqs ? kv8_len(c, d) : 0;
+            w.after[i] = after;
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void kv8_reorder_write_kernel(Kv8View c, const int32_t* __restrict__ src,
+                                                                const int32_t* __restrict__ dst, int n, void* ws) {
+    const ReorderWs w = reorder_ws(ws, c.n_seqs);
+    if (*w.ok == 0) return;
+    for (int i = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6); i < n; i += (int)gridDim.x * 4) {
+        const int d = seq_at(dst, i), before = w.before[i], after = w.after[i];
+        if (src[i] == d) continue;
+        const int most = max(pages_of(c, before), pages_of(c, after));
+        for (int j = (int)threadIdx.x & 63; j < most; j += 64)
+            replace_page(c, d, j, before, after, j < pages_of(c, after) ? w.rows[(size_t)i * c.seq_pages + j] : -1);
+        if ((threadIdx.x & 63) == 0) c.lens[d] = after;
+    }
+}
+
 // Which pages move: of L live pages those numbered L and above go, in order, to the free numbers below L, so sources and
 // destinations never meet.
 __global__ __launch_bounds__(kWg) void kv8_compact_kernel(Kv8View c, int32_t* __restrict__ live, void* ws) {
@@ -794,6 +902,23 @@ hipError_t launch_kv8_fork(const Kv8View& c, int n_layers, const int32_t* src, c
     if (mode == kShareHere) return hipSuccess;
     qh_launch(kv8_share_kernel, dim3((unsigned)((c.seq_pages + 255) / 256), (unsigned)n), dim3(256), 0, s, c, src, dst, n,
               ws);
+    return hipGetLastError();
+}
+
+size_t kv8_reorder_workspace_bytes(int n_seqs, int seq_pages) {
+    if ((int64_t)n_seqs * seq_pages <= kReorderHere) return 0;
+    return sizeof(int) * (4 + 2 * (size_t)n_seqs + (size_t)n_seqs * seq_pages);
+}
+
+hipError_t launch_kv8_reorder(const Kv8View& c, const int32_t* src, const int32_t* dst, int n, void* ws, hipStream_t s) {
+    if ((int64_t)n * c.seq_pages <= kReorderHere) {
+        qh_launch(kv8_reorder_here_kernel, dim3(1), dim3(kWg), 0, s, c, src, dst, n);
+        return hipGetLastError();
+    }
+    const int rows = (n + kWg / 64 - 1) / (kWg / 64), waves = (n + 3) / 4;
+    qh_launch(kv8_reorder_read_kernel, dim3((unsigned)(1 + (rows < 1024 ? rows : 1024))), dim3(kWg), 0, s, c, src, dst, n, ws);
+    if (hipError_t e = hipGetLastError()) return e;
+    qh_launch(kv8_reorder_write_kernel, dim3((unsigned)(waves < 2048 ? waves : 2048)), dim3(256), 0, s, c, src, dst, n, ws);
     return hipGetLastError();
 }
 

@@ -1,4 +1,4 @@
-// Row operators between the matmuls of a step of many sequences: norm with residual, and rotary positions.
+// Operators on the rows of a step of many sequences: norm with residual, rotary positions, and beam search's selection.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -36,5 +36,19 @@ struct RopeArgs {
     int hd, rot, n_tok;
 };
 hipError_t launch_rope(const RopeArgs& a, int dtype, bool interleaved, hipStream_t s);
+
+// Beam search's selection (qh_beam.hip): logits [prompts * beams][n_valid], rows ld apart, on their type's alignment; the k
+// best candidates of each prompt, best first.
+struct BeamArgs {
+    const void* logits;
+    const float* scores;  // [prompts * beams], or null: 0
+    int32_t *parent, *token;
+    float* best;
+    void* ws;
+    int64_t ld;
+    int prompts, beams, n_valid, k;
+};
+size_t beam_workspace_bytes(int dtype, int prompts, int beams, int n_valid);
+hipError_t launch_beam_select(const BeamArgs& a, int dtype, hipStream_t s);
 
 }  // namespace qh

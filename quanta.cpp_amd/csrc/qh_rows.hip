@@ -145,8 +145,8 @@ hipError_t rmsnorm_of(const NormArgs& a, hipStream_t s) {
     else if (vecs <= 512) run(integral_constant<int, 4>{}, integral_constant<int, 2>{});
     else if (vecs <= 1024) run(integral_constant<int, 4>{}, integral_constant<int, 4>{});
     else if (vecs <= 2048) run(integral_constant<int, 4>{}, integral_constant<int, 8>{});
-    else if (vecs <= 4096) run(integral_constant<int, 16>{}, integral_constant<int, 4>{});
-    else run(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+    else if (vecs <= 4096) run(integral_constant<int, 16>{}, integral_constant<int, 4>{});  // f16: kMaxNorm elements
+    else if constexpr (kE<T> == 4) run(integral_constant<int, 16>{}, integral_constant<int, 8>{});
     return hipGetLastError();
 }
 
