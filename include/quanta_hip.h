@@ -455,6 +455,24 @@ typedef struct qh_rope_rows {
 int qh_rope(const double* turns, int rot_dim, int interleaved, float magnitude, int head_dim, const qh_rope_rows* q,
             const qh_rope_rows* k, int dtype, const int32_t* pos, int n_tok, void* stream);
 
+/* Attention of prompts over their own keys and values, as the projections give them, before (or without) their rounding into
+ * a cache: out = sum_j p_j v_j with p = softmax(scale * q . k_j) over the keys j that a row sees. Entry b of n has the query rows
+ * [start[b], start[b + 1]) of n_tok and the keys and values [kstart[b], kstart[b + 1]) of n_keys (DEVICE int32 [n + 1] each,
+ * ascending; kstart NULL: start, and n_keys is n_tok). With causal 1 the rows are the entry's last positions: row i of m sees
+ * the keys up to keys - m + i, so that new tokens behind kept ones see those too; with causal 0 every row sees every key of its
+ * entry (states that are not the rows' own). Query head h reads KV head h / (n_heads / n_kv_heads). head_dim is 64 or 128; rows
+ * of dtype QH_F32 or QH_F16, ld elements apart on any alignment of their type, a row's heads contiguous. A row that sees
+ * nothing is 0; rows outside the entries are neither read nor written. Keys and values that a row does not see have no part in
+ * it, whatever they hold. A NaN or an infinity that it sees stays in its dim where it is a value's, and makes the row NaN
+ * where it is the query's; of a key's it becomes NaN, or what the formula gives. f16: weights are rounded to f16 once. f32: products keep 22 bits and more of every value, whatever the others are. Sums in f32. out overlaps no input. The
+ * workspace is 16-byte aligned and needs no initialisation (NULL where the size is 0); calls that overlap must not share one.
+ * No counterpart in the reference, whose prompts attend to its cache in chunks (Model::forward_batch, model.cpp:387-405). */
+size_t qh_attention_workspace_bytes(int dtype, int n_heads, int n_kv_heads, int head_dim, int n, int n_tok, int n_keys);
+int qh_attention(const void* q, const void* k, const void* v, void* out, int dtype, int n_heads, int n_kv_heads,
+                 int head_dim, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, const int32_t* start,
+                 const int32_t* kstart, int n, int n_tok, int n_keys, int causal, float scale, void* workspace,
+                 size_t workspace_bytes, void* stream);
+
 /* Beam search's selection. logits: DEVICE rows [n_prompts * beams][n_valid] of dtype QH_F32 or QH_F16, ld elements apart, on
  * any alignment of their type; scores: DEVICE f32 [n_prompts * beams], what each beam has so far (NULL: 0). A candidate is a
  * beam b of a prompt and an id v, with the score scores[b] + logits[b][v] - log sum_u exp(logits[b][u]); sums, exponentials
@@ -463,8 +481,8 @@ int qh_rope(const double* turns, int rot_dim, int interleaved, float magnitude, 
  * logit of -infinity is no candidate, and neither is any of a row whose score is not finite or whose logits hold a NaN or
  * +infinity or are all -infinity (a beam that ended gets the score -infinity); where there are fewer than k, the places
  * behind them have parent and token -1 and the score -infinity (which is also what a score past f32's range rounds to). beams
- * at most QH_BEAM_MAX_BEAMS, k at most QH_BEAM_MAX_K, n_valid at most QH_SAMPLE_MAX_VOCAB. The workspace is 16-byte aligned and needs no initialisation; calls that overlap must
- * not share one.
+ * at most QH_BEAM_MAX_BEAMS, k at most QH_BEAM_MAX_K, n_valid at most QH_SAMPLE_MAX_VOCAB. The workspace is 16-byte aligned
+ * and needs no initialisation; calls that overlap must not share one.
  * No counterpart in the reference, which samples one sequence (Sampler::sample, sampler.cpp:22-85). */
 #define QH_BEAM_MAX_BEAMS 256
 #define QH_BEAM_MAX_K 256

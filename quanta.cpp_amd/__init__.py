@@ -115,7 +115,8 @@ EXPORTS = ("qh_last_error", "qh_version", "qh_init", "qh_quant_bytes", "qh_tenso
            "qh_kv8_reorder_workspace_bytes", "qh_kv8_reorder",
            "qh_kv8_compact", "qh_kv8_append", "qh_kv8_read", "qh_kv8_attention_workspace_bytes", "qh_kv8_attention",
            "qh_kv8_attention_plan",
-           "qh_rmsnorm", "qh_rope_turns", "qh_rope", "qh_beam_workspace_bytes", "qh_beam_select",
+           "qh_rmsnorm", "qh_rope_turns", "qh_rope", "qh_attention_workspace_bytes",
+           "qh_attention", "qh_beam_workspace_bytes", "qh_beam_select",
            "qh_decoder_create",
            "qh_decoder_destroy",
            "qh_decoder_prefill", "qh_decoder_begin", "qh_decoder_step", "qh_decoder_views",
@@ -172,6 +173,9 @@ def _bind(lib):
                        i32),
         "qh_rope_turns": ([C.POINTER(qh_rope_desc), vp], i32),
         "qh_rope": ([vp, i32, i32, C.c_float, i32, C.POINTER(qh_rope_rows), C.POINTER(qh_rope_rows), i32, vp, i32, vp], i32),
+        "qh_attention_workspace_bytes": ([i32] * 7, sz),
+        "qh_attention": ([vp, vp, vp, vp, i32, i32, i32, i32] + [C.c_int64] * 4 + [vp, vp, i32, i32, i32, i32, C.c_float, vp, sz,
+                          vp], i32),
         "qh_beam_workspace_bytes": ([i32, i32, i32, i32], sz),
         "qh_beam_select": ([vp, i32, C.c_int64, vp, i32, i32, i32, i32, vp, vp, vp, vp, sz, vp], i32),
         "qh_decoder_create": ([C.POINTER(qh_model_desc), C.POINTER(qh_tensor), i32, C.POINTER(vp)], i32),
@@ -729,6 +733,51 @@ class Rope:
         _check(lib().qh_rope(self.turns.data_ptr(), self.rot_dim, self.interleaved, self.magnitude, self.head_dim,
                              C.byref(a), b, dtype, pos.data_ptr(), rows, _here(q.device)))
         return q_out if k is None else (q_out, k_out)
+
+
+def _head_stride(t, what) -> int:
+    """Elements from row to row of [rows][heads][head_dim] with the heads of a row contiguous."""
+    if t.dim() != 3 or (t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]))):
+        raise QHError(f"{what} is {tuple(t.shape)} with strides {t.stride()}, expected [rows][heads][head_dim] with the heads "
+                      "of a row contiguous")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def attention(q, k, v, start=None, kstart=None, causal: bool = True, scale: float | None = None, out=None):
+    """Attention of packed prompts over their own keys and values (qh_attention): q [rows][heads][head_dim], k and v
+    [keys][KV heads][head_dim] (float32 or float16; views of wider rows are fine). start (int32 [n + 1], on the device): the
+    rows of each of n sequences, None: one sequence of all; kstart: their keys, None: the same rows. causal: the rows are
+    each sequence's last positions; scale: 1 / sqrt(head_dim). Rows outside the sequences keep out's values (a new out's are
+    undefined)."""
+    torch = _torch()
+    dtype, ldq = _dtype_of(q, "q"), _head_stride(q, "q")
+    ldk, ldv = _head_stride(k, "k"), _head_stride(v, "v")
+    rows, heads, hd = q.shape
+    keys, kv = k.shape[0], k.shape[1]
+    _like(k, (keys, kv, hd), q, "k")
+    _like(v, (keys, kv, hd), q, "v")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _like(out, q.shape, q, "out")
+    ldo, dev = _head_stride(out, "out"), q.device
+    if start is None:
+        if kstart is not None:
+            raise QHError("kstart without start")
+        start = torch.arange(2, dtype=torch.int32, device=dev) * rows
+        if keys != rows:
+            kstart = torch.arange(2, dtype=torch.int32, device=dev) * keys
+    n = start.shape[0] - 1 if start.dim() == 1 else -1
+    for t, what in ((start, "start"), (kstart, "kstart")):
+        if t is not None and (t.dtype is not torch.int32 or t.device != dev or t.dim() != 1 or t.shape[0] != n + 1 or n < 0 or
+                              not t.is_contiguous()):
+            raise QHError(f"{what} must be a contiguous int32 vector of sequences + 1 on {dev}")
+    need = lib().qh_attention_workspace_bytes(dtype, heads, kv, hd, n, rows, keys)
+    # a tensor for each call: nothing of one call (or captured graph) is shared with the next
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _check(lib().qh_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dtype, heads, kv, hd, ldq, ldk, ldv, ldo,
+                              start.data_ptr(), None if kstart is None else kstart.data_ptr(), n, rows, keys, int(causal),
+                              hd ** -0.5 if scale is None else scale, None if ws is None else ws.data_ptr(), need, _here(dev)))
+    return out
 
 
 def beam_select(logits, scores, beams: int, k: int, n_valid: int | None = None):

@@ -10,6 +10,7 @@
 
 #include "qh_internal.h"
 #include "qh_kv8.h"
+#include "qh_prompt.h"
 #include "qh_rows.h"
 
 namespace qh {
@@ -638,6 +639,60 @@ int qh_rope(const double* turns, int rot_dim, int interleaved, float magnitude, 
     const RopeRows rk = k ? RopeRows{k->x, k->out, k->ld, k->ldo, k->n_heads} : RopeRows{nullptr, nullptr, 0, 0, 0};
     const RopeArgs a{turns, pos, rq, rk, magnitude, head_dim, rot_dim, n_tok};
     return check_hip(launch_rope(a, dtype, interleaved != 0, as_stream(stream)), who);
+}
+
+namespace {
+int validate_prompt(int dtype, int n_heads, int n_kv_heads, int head_dim, int n, int n_tok, int n_keys, const char* who) {
+    if (dtype != QH_F32 && dtype != QH_F16) return fail(QH_ERR_DTYPE, "%s: dtype %d is not f32 (0) or f16 (1)", who, dtype);
+    if ((head_dim != 64 && head_dim != 128) || n_kv_heads < 1 || n_kv_heads > 256 || n_heads < 1 || n_heads % n_kv_heads != 0 ||
+        n_heads > 1 << 16)
+        return fail(QH_ERR_SHAPE, "%s: %d query heads over %d KV heads of %d (64 or 128)", who, n_heads, n_kv_heads, head_dim);
+    if (n < 0 || n_tok < 0 || n_keys < 0) return fail(QH_ERR_ARG, "%s: %d entries over %d rows and %d keys", who, n, n_tok, n_keys);
+    // a launch has fewer than 2^23 workgroups of up to 512: one to 64 rows of a KV head's queries, and one to an entry
+    const int64_t rows = (int64_t)n_heads / n_kv_heads * n_tok;
+    if (rows > 1 << 30 || n_keys > 1 << 30 || (rows / 64 + n) * n_kv_heads >= 1 << 23)
+        return fail(QH_ERR_SHAPE, "%s: %d rows of %d heads in %d entries are too many for one call", who, n_tok, n_heads, n);
+    return QH_OK;
+}
+}  // namespace
+
+size_t qh_attention_workspace_bytes(int dtype, int n_heads, int n_kv_heads, int head_dim, int n, int n_tok, int n_keys) {
+    if (validate_prompt(dtype, n_heads, n_kv_heads, head_dim, n, n_tok, n_keys, "qh_attention_workspace_bytes")) return 0;
+    if (n == 0 || n_tok == 0) return 0;
+    return prompt_workspace_bytes(dtype, n_heads, n_kv_heads, head_dim, n, n_tok, n_keys);
+}
+
+int qh_attention(const void* q, const void* k, const void* v, void* out, int dtype, int n_heads, int n_kv_heads,
+                 int head_dim, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, const int32_t* start,
+                 const int32_t* kstart, int n, int n_tok, int n_keys, int causal, float scale, void* workspace,
+                 size_t workspace_bytes, void* stream) {
+    const char* who = "qh_attention";
+    if (int rc = validate_prompt(dtype, n_heads, n_kv_heads, head_dim, n, n_tok, n_keys, who)) return rc;
+    if (causal != 0 && causal != 1) return fail(QH_ERR_ARG, "%s: causal = %d", who, causal);
+    if (!(fabsf(scale) <= 1e38f)) return fail(QH_ERR_ARG, "%s: scale is not finite", who);
+    if (n == 0 || n_tok == 0) return QH_OK;
+    if (!start) return fail(QH_ERR_ARG, "%s: no starts", who);
+    if (!kstart && n_keys != n_tok) return fail(QH_ERR_ARG, "%s: %d keys for %d rows without starts of their own", who, n_keys, n_tok);
+    const int64_t width = (int64_t)n_heads * head_dim, kv = (int64_t)n_kv_heads * head_dim;
+    if (int rc = validate_rows(q, dtype, ldq, width, "q", who)) return rc;
+    if (int rc = validate_rows(out, dtype, ldo, width, "out", who)) return rc;
+    if (n_keys > 0) {
+        if (int rc = validate_rows(k, dtype, ldk, kv, "k", who)) return rc;
+        if (int rc = validate_rows(v, dtype, ldv, kv, "v", who)) return rc;
+    }
+    if (out == q || out == k || out == v) return fail(QH_ERR_ARG, "%s: out is an input", who);
+    const size_t need = prompt_workspace_bytes(dtype, n_heads, n_kv_heads, head_dim, n, n_tok, n_keys);
+    if (need > (workspace ? workspace_bytes : 0))
+        return fail(QH_ERR_NOMEM, "%s: workspace of %zu bytes, needs %zu", who, workspace ? workspace_bytes : 0, need);
+    if (!aligned16(workspace)) return fail(QH_ERR_ALIGN, "%s: workspace not 16-byte aligned", who);
+    PromptArgs a{};
+    a.q = q, a.k = k, a.v = v, a.out = out;
+    a.ldq = ldq, a.ldk = ldk, a.ldv = ldv, a.ldo = ldo;
+    a.start = start, a.kstart = kstart ? kstart : start;
+    a.n = n, a.n_tok = n_tok, a.n_keys = n_keys, a.n_kv = n_kv_heads, a.group = n_heads / n_kv_heads, a.causal = causal;
+    a.scale_log2e = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504088896340736f;
+    a.sign = scale == 0.0f ? 0.0f : scale < 0.0f ? -1.0f : 1.0f;
+    return check_hip(launch_prompt(a, dtype, head_dim, workspace, as_stream(stream)), who);
 }
 
 namespace {
