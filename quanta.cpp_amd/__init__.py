@@ -218,9 +218,15 @@ def _check(rc: int) -> None:
         raise QHError(f"status {rc}: {lib().qh_last_error().decode()}")
 
 
+_torch_module = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+    return _torch_module
 
 
 def _stream() -> int:
@@ -599,82 +605,99 @@ class KV8Cache:
 
 # ------------------------------------------------------------------------------- rows of a step of many sequences
 
-def _here(device) -> int:
-    """The current stream, on `device` (that of a call's tensors), which has to be the current one."""
-    torch = _torch()
-    if device.type != "cuda" or device.index != torch._C._cuda_getDevice():
-        raise QHError(f"the tensors are on {device}, the current device is cuda:{torch._C._cuda_getDevice()}")
-    return torch._C._cuda_getCurrentRawStream(device.index)
+# What these calls look up is kept short: on a few rows they take a few microseconds, most of them here.
+
+def _here(t) -> int:
+    """The current stream, on the device of a call's tensor t, which has to be the current one."""
+    raw = _torch()._C
+    device = raw._cuda_getDevice()
+    if t.get_device() != device:
+        raise QHError(f"the tensors are on {t.device}, the current device is cuda:{device}")
+    return raw._cuda_getCurrentRawStream(device)
 
 
 def _dtype_of(t, what) -> int:
-    torch = _torch()
-    if t.dtype is torch.float32:
+    torch, dtype = _torch(), t.dtype
+    if dtype is torch.float32:
         return F32
-    if t.dtype is torch.float16:
+    if dtype is torch.float16:
         return F16
-    raise QHError(f"{what} is {t.dtype}, expected float32 or float16")
+    raise QHError(f"{what} is {dtype}, expected float32 or float16")
 
 
 def _like(t, shape, other, what):
     """Checks that a tensor has this shape and another's dtype and device."""
-    if tuple(t.shape) != tuple(shape) or t.dtype is not other.dtype or t.device != other.device:
+    if t.shape != shape or t.dtype is not other.dtype or t.get_device() != other.get_device():
         raise QHError(f"{what} is {tuple(t.shape)} {t.dtype} on {t.device}, expected {tuple(shape)} {other.dtype} on "
                       f"{other.device}")
 
 
 def _row_stride(t, what) -> int:
     """Elements from row to row of a matrix with contiguous rows."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
         raise QHError(f"{what} must be a matrix with contiguous rows")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return stride[0] if shape[0] > 1 else shape[1]
 
 
 def _rmsnorm(x, w, eps, residual, sum, out, q, d):
     torch = _torch()
-    dtype, ldx = _dtype_of(x, "x"), _row_stride(x, "x")
-    rows, n = x.shape
-    if w.dtype is not torch.float32 or tuple(w.shape) != (n,) or w.device != x.device or not w.is_contiguous():
+    dtype, ldx, shape = _dtype_of(x, "x"), _row_stride(x, "x"), x.shape
+    rows, n = shape
+    stream = _here(x)
+    if w.dtype is not torch.float32 or w.shape != (n,) or not w.is_contiguous() or w.get_device() != x.get_device():
         raise QHError(f"w must be a contiguous float32 vector of {n} on {x.device}")
     ldr = lds = ldy = n
+    pr = ps = py = None
     if residual is not None:
-        _like(residual, x.shape, x, "residual")
-        ldr = _row_stride(residual, "residual")
-    if sum is not None:
-        _like(sum, x.shape, x, "sum")
-        lds = _row_stride(sum, "sum")
-    if out is not None:
-        _like(out, x.shape, x, "out")
-        ldy = _row_stride(out, "out")
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    _check(lib().qh_rmsnorm(ptr(x), ptr(residual), ptr(w), dtype, ldx, ldr, rows, n, eps, ptr(sum), lds, ptr(out), ldy,
-                            ptr(q), ptr(d), _here(x.device)))
+        _like(residual, shape, x, "residual")
+        ldr, pr = _row_stride(residual, "residual"), residual.data_ptr()
+        if sum is None:
+            sum = _new_like(x)
+        else:
+            _like(sum, shape, x, "sum")
+            lds = _row_stride(sum, "sum")
+        ps = sum.data_ptr()
+    elif sum is not None:
+        raise QHError("sum without residual")
+    if q is None:
+        if out is None:
+            out = _new_like(x)
+        else:
+            _like(out, shape, x, "out")
+            ldy = _row_stride(out, "out")
+        py = out.data_ptr()
+    rc = (_lib or lib()).qh_rmsnorm(x.data_ptr(), pr, w.data_ptr(), dtype, ldx, ldr, rows, n, eps, ps, lds, py, ldy,
+                                    None if q is None else q.data_ptr(), None if d is None else d.data_ptr(), stream)
+    if rc:
+        _check(rc)
+    return sum, out
+
+
+def _new_like(t):
+    """A new contiguous tensor of t's shape and dtype."""
+    torch = _torch()
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def rmsnorm(x, w, eps: float = 1e-6, residual=None, sum=None, out=None):
     """Root-mean-square norm of the rows x [rows][n] (float32 or float16; views of wider rows are fine) with weight w
     (float32 [n]) -> out. With residual: (sum, out), where sum = x + residual is what is normalized; sum may be x or
     residual itself (in place). See qh_rmsnorm."""
-    torch = _torch()
-    if residual is not None and sum is None:
-        sum = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    _rmsnorm(x, w, eps, residual, sum, out, None, None)
+    sum, out = _rmsnorm(x, w, eps, residual, sum, out, None, None)
     return out if residual is None else (sum, out)
 
 
 def rmsnorm_q8(x, w, eps: float = 1e-6, residual=None, sum=None):
     """The same into the 8-bit blocks that the quantized matmuls take: (q, d), as quantize_q8 makes them of the normalized
     rows in float32; with residual (sum, q, d). n is a multiple of 32."""
-    torch = _torch()
-    if x.dim() != 2 or x.shape[1] % QK:
-        raise QHError(f"x is {tuple(x.shape)}, expected [rows][a multiple of {QK}]")
-    if residual is not None and sum is None:
-        sum = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    d = torch.empty((x.shape[0], x.shape[1] // QK), dtype=torch.float32, device=x.device)
-    _rmsnorm(x, w, eps, residual, sum, None, q, d)
+    torch, shape = _torch(), x.shape
+    if len(shape) != 2 or shape[1] % QK:
+        raise QHError(f"x is {tuple(shape)}, expected [rows][a multiple of {QK}]")
+    dev = x.device
+    q = torch.empty(shape, dtype=torch.int8, device=dev)
+    d = torch.empty((shape[0], shape[1] // QK), dtype=torch.float32, device=dev)
+    sum, _ = _rmsnorm(x, w, eps, residual, sum, None, q, d)
     return (q, d) if residual is None else (sum, q, d)
 
 
@@ -701,46 +724,49 @@ class Rope:
         if turns.dtype is not torch.float64 or turns.numel() != self.rot_dim // 2:
             raise QHError(f"turns must be {self.rot_dim // 2} float64 values")
         self.turns = turns.reshape(-1).to(device).contiguous()
+        self._table, self._index = self.turns.data_ptr(), self.turns.get_device()
 
     def _rows(self, x, out, what):
-        if x.dim() != 3 or x.shape[2] != self.head_dim or x.device != self.turns.device:
-            raise QHError(f"{what} is {tuple(x.shape)} on {x.device}, expected [rows][heads][{self.head_dim}] on "
-                          f"{self.turns.device}")
-        strides = []
-        for t, name in ((x, what), (out, f"{what}_out")):
-            _like(t, x.shape, x, name)
-            if x.numel() and ((self.head_dim > 1 and t.stride(2) != 1) or (t.shape[1] > 1 and t.stride(1) != self.head_dim)):
-                raise QHError(f"the heads of a row of {name} must be contiguous")
-            strides.append(t.stride(0) if t.shape[0] > 1 else t.shape[1] * self.head_dim)
-        return qh_rope_rows(x.data_ptr(), out.data_ptr(), strides[0], strides[1], x.shape[1])
+        hd, shape = self.head_dim, x.shape
+        if len(shape) != 3 or shape[2] != hd or x.get_device() != self._index:
+            raise QHError(f"{what} is {tuple(shape)} on {x.device}, expected [rows][heads][{hd}] on {self.turns.device}")
+        ld = _head_stride(x, what)
+        if out is None:
+            out = _new_like(x)
+            return out, qh_rope_rows(x.data_ptr(), out.data_ptr(), ld, shape[1] * hd, shape[1])
+        _like(out, shape, x, f"{what}_out")
+        return out, qh_rope_rows(x.data_ptr(), out.data_ptr(), ld, _head_stride(out, f"{what}_out"), shape[1])
 
     def __call__(self, q, k=None, *, pos, q_out=None, k_out=None):
         """The rows q and k ([rows][heads][head_dim], float32 or float16; views of one wider row are fine) turned by the
         positions pos (int32 [rows], on the device) -> (q', k'), or q' without k. q_out / k_out may be q / k (in place)."""
-        torch = _torch()
-        rows = q.shape[0]
-        if pos.dtype is not torch.int32 or tuple(pos.shape) != (rows,) or pos.device != q.device or not pos.is_contiguous():
+        torch, rows = _torch(), q.shape[0]
+        stream = _here(q)
+        if (pos.dtype is not torch.int32 or pos.shape != (rows,) or pos.get_device() != q.get_device() or
+                not pos.is_contiguous()):
             raise QHError(f"pos must be a contiguous int32 vector of {rows} on {q.device}")
-        if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        a, b, dtype = self._rows(q, q_out, "q"), None, _dtype_of(q, "q")
+        dtype, b = _dtype_of(q, "q"), None
+        q_out, a = self._rows(q, q_out, "q")
         if k is not None:
             if k.shape[0] != rows or k.dtype is not q.dtype:
                 raise QHError("q and k differ in rows or dtype")
-            if k_out is None:
-                k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-            b = C.byref(self._rows(k, k_out, "k"))
-        _check(lib().qh_rope(self.turns.data_ptr(), self.rot_dim, self.interleaved, self.magnitude, self.head_dim,
-                             C.byref(a), b, dtype, pos.data_ptr(), rows, _here(q.device)))
+            k_out, b = self._rows(k, k_out, "k")
+        rc = (_lib or lib()).qh_rope(self._table, self.rot_dim, self.interleaved, self.magnitude, self.head_dim, a, b, dtype,
+                                     pos.data_ptr(), rows, stream)
+        if rc:
+            _check(rc)
         return q_out if k is None else (q_out, k_out)
 
 
 def _head_stride(t, what) -> int:
     """Elements from row to row of [rows][heads][head_dim] with the heads of a row contiguous."""
-    if t.dim() != 3 or (t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]))):
-        raise QHError(f"{what} is {tuple(t.shape)} with strides {t.stride()}, expected [rows][heads][head_dim] with the heads "
-                      "of a row contiguous")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 3:
+        rows, heads, hd = shape
+        if (stride[2] == 1 or hd == 1) and (stride[1] == hd or heads == 1) or rows * heads * hd == 0:
+            return stride[0] if rows > 1 else heads * hd
+    raise QHError(f"{what} is {tuple(shape)} with strides {stride}, expected [rows][heads][head_dim] with the heads of a row "
+                  "contiguous")
 
 
 def attention(q, k, v, start=None, kstart=None, causal: bool = True, scale: float | None = None, out=None):
@@ -750,16 +776,18 @@ def attention(q, k, v, start=None, kstart=None, causal: bool = True, scale: floa
     each sequence's last positions; scale: 1 / sqrt(head_dim). Rows outside the sequences keep out's values (a new out's are
     undefined)."""
     torch = _torch()
-    dtype, ldq = _dtype_of(q, "q"), _head_stride(q, "q")
+    stream, dtype, ldq = _here(q), _dtype_of(q, "q"), _head_stride(q, "q")
     ldk, ldv = _head_stride(k, "k"), _head_stride(v, "v")
     rows, heads, hd = q.shape
-    keys, kv = k.shape[0], k.shape[1]
+    keys, kv, _ = k.shape
     _like(k, (keys, kv, hd), q, "k")
     _like(v, (keys, kv, hd), q, "v")
+    dev = q.device
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _like(out, q.shape, q, "out")
-    ldo, dev = _head_stride(out, "out"), q.device
+        out, ldo = _new_like(q), heads * hd
+    else:
+        _like(out, q.shape, q, "out")
+        ldo = _head_stride(out, "out")
     if start is None:
         if kstart is not None:
             raise QHError("kstart without start")
@@ -768,15 +796,18 @@ def attention(q, k, v, start=None, kstart=None, causal: bool = True, scale: floa
             kstart = torch.arange(2, dtype=torch.int32, device=dev) * keys
     n = start.shape[0] - 1 if start.dim() == 1 else -1
     for t, what in ((start, "start"), (kstart, "kstart")):
-        if t is not None and (t.dtype is not torch.int32 or t.device != dev or t.dim() != 1 or t.shape[0] != n + 1 or n < 0 or
+        if t is not None and (t.dtype is not torch.int32 or t.shape != (n + 1,) or n < 0 or t.get_device() != q.get_device() or
                               not t.is_contiguous()):
             raise QHError(f"{what} must be a contiguous int32 vector of sequences + 1 on {dev}")
-    need = lib().qh_attention_workspace_bytes(dtype, heads, kv, hd, n, rows, keys)
+    L = _lib or lib()
+    need = L.qh_attention_workspace_bytes(dtype, heads, kv, hd, n, rows, keys)
     # a tensor for each call: nothing of one call (or captured graph) is shared with the next
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _check(lib().qh_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dtype, heads, kv, hd, ldq, ldk, ldv, ldo,
-                              start.data_ptr(), None if kstart is None else kstart.data_ptr(), n, rows, keys, int(causal),
-                              hd ** -0.5 if scale is None else scale, None if ws is None else ws.data_ptr(), need, _here(dev)))
+    rc = L.qh_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dtype, heads, kv, hd, ldq, ldk, ldv, ldo,
+                        start.data_ptr(), None if kstart is None else kstart.data_ptr(), n, rows, keys, int(causal),
+                        hd ** -0.5 if scale is None else scale, None if ws is None else ws.data_ptr(), need, stream)
+    if rc:
+        _check(rc)
     return out
 
 
@@ -786,24 +817,30 @@ def beam_select(logits, scores, beams: int, k: int, n_valid: int | None = None):
     (parent, token, score), each [prompts][k], best first: the row that is continued, the id (both int32) and
     score + log-softmax (float32); -1, -1 and -inf where there are fewer candidates. See qh_beam_select."""
     torch = _torch()
-    dtype, ld = _dtype_of(logits, "logits"), _row_stride(logits, "logits")
+    stream, dtype, ld = _here(logits), _dtype_of(logits, "logits"), _row_stride(logits, "logits")
     rows, n = logits.shape
     n_valid = n if n_valid is None else n_valid
     if beams < 1 or rows % beams or not 1 <= n_valid <= n:
         raise QHError(f"{rows} rows of {beams} beams, {n_valid} of {n} ids")
-    if scores is not None and (scores.dtype is not torch.float32 or tuple(scores.shape) != (rows,) or
-                               scores.device != logits.device or not scores.is_contiguous()):
+    if not 1 <= k <= BEAM_MAX_K:
+        raise QHError(f"k {k} outside [1, {BEAM_MAX_K}]")
+    if scores is not None and (scores.dtype is not torch.float32 or scores.shape != (rows,) or
+                               scores.get_device() != logits.get_device() or not scores.is_contiguous()):
         raise QHError(f"scores must be a contiguous float32 vector of {rows} on {logits.device}")
-    prompts, dev = rows // beams, logits.device
-    parent = torch.empty((prompts, k), dtype=torch.int32, device=dev)
-    token = torch.empty((prompts, k), dtype=torch.int32, device=dev)
-    score = torch.empty((prompts, k), dtype=torch.float32, device=dev)
-    # a tensor for each call: nothing of one call (or captured graph) is shared with the next
-    ws = torch.empty(lib().qh_beam_workspace_bytes(dtype, prompts, beams, n_valid), dtype=torch.uint8, device=dev)
-    _check(lib().qh_beam_select(logits.data_ptr(), dtype, ld, None if scores is None else scores.data_ptr(), prompts, beams,
-                                n_valid, k, parent.data_ptr(), token.data_ptr(), score.data_ptr(), ws.data_ptr(), ws.numel(),
-                                _here(dev)))
-    return parent, token, score
+    prompts, dev, L = rows // beams, logits.device, _lib or lib()
+    need = L.qh_beam_workspace_bytes(dtype, prompts, beams, n_valid)
+    # the results and the workspace in one tensor, a new one for each call: nothing of one call (or captured graph) is shared
+    # with the next
+    each = (prompts * k + 3) // 4 * 4
+    held = torch.empty(3 * each + (need + 3) // 4, dtype=torch.int32, device=dev)
+    parent, token, score, ws = held.split_with_sizes((each, each, each, held.shape[0] - 3 * each))
+    rc = L.qh_beam_select(logits.data_ptr(), dtype, ld, None if scores is None else scores.data_ptr(), prompts, beams, n_valid,
+                          k, parent.data_ptr(), token.data_ptr(), score.data_ptr(), ws.data_ptr(), need, stream)
+    if rc:
+        _check(rc)
+    shape = (prompts, k)
+    return (parent[:prompts * k].view(shape), token[:prompts * k].view(shape),
+            score[:prompts * k].view(torch.float32).view(shape))
 
 
 # ------------------------------------------------------------------------------------------------ decoder

@@ -16,16 +16,19 @@ namespace {
 
 constexpr int kPickThreads = 1024;
 constexpr int kPool = 1024;       // candidates that are ranked
-constexpr int kList = 2 * QH_BEAM_MAX_K + 32;  // groups that are read again, at most
+constexpr int kList = QH_BEAM_MAX_K + 16;  // groups that are read again, at most
 
 template <typename T>
 constexpr int kE = 16 / (int)sizeof(T);
+constexpr int kMostVecs = 4;  // (192 x 151,936 f32: 26.8 us, with 8 28.2, with 16 32.2)
 template <typename T>
 struct Vec {  // at any address of the type's alignment
     typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
 
-// How the rows are cut: a wave's part of a row is `vecs` vectors of 64 * E ids, a group `group` of them.
+// How the rows are cut: a workgroup's part of a row is four waves' `vecs` vectors of 64 * E ids, a group `group` of them: one
+// where that leaves a group to a thread of the picking workgroup, else 1,024 ids (4 x 151,936 f32, of 256: 11.5 us for the
+// picking, of 1,024 8.2), or 2,048 where a thread had more than 32.
 struct BeamCut {
     int vecs, group;
     int parts, groups;  // of a row
@@ -35,20 +38,19 @@ template <typename T>
 BeamCut beam_cut(int rows, int beams, int n_valid) {
     const int v = (n_valid + 64 * kE<T> - 1) / (64 * kE<T>);
     BeamCut c{};
-    c.group = 1;  // groups of a prompt: 8 keys to a thread of the picking workgroup, or 32 where groups cannot be larger
-    while (c.group < 8 && (int64_t)beams * ((v + c.group - 1) / c.group) > 8 * kPickThreads) c.group *= 2;
-    c.vecs = 8;  // the loads that a wave has in flight, fewer where there are not waves enough
-    while (c.vecs > c.group && (int64_t)rows * ((v + c.vecs - 1) / c.vecs) < 4096) c.vecs /= 2;
-    c.parts = (v + c.vecs - 1) / c.vecs;
+    c.group = (int64_t)beams * v <= kPickThreads ? 1 : 1024 / (64 * kE<T>);
+    if ((int64_t)beams * ((v + c.group - 1) / c.group) > 32 * kPickThreads) c.group *= 2;
+    c.vecs = kMostVecs > c.group ? kMostVecs : c.group;  // the loads that a wave has in flight, fewer where there are not workgroups enough
+    while (c.vecs > c.group && (int64_t)rows * ((v + 4 * c.vecs - 1) / (4 * c.vecs)) < 1024) c.vecs /= 2;
+    c.parts = (v + 4 * c.vecs - 1) / (4 * c.vecs);
     c.groups = (v + c.group - 1) / c.group;
     return c;
 }
 
-// exp(d) for d <= 0, off by 2^-38 of it at most: d log2(e) = n + f, and a polynomial for 2^f, |f| <= 1/2, that interpolates
-// (2^f - 1) / f at the Chebyshev nodes; exp(0) is 1. 0 from -800 down.
-__device__ __forceinline__ double exp_below(double d) {
-    const double t = __builtin_fmax(d, -800.0) * 0x1.71547652b82fep+0;
-    const double n = __builtin_rint(t), f = t - n;
+// 2^(n + f) for a polynomial of f, |f| <= 1/2, off by 2^-38 of it at most: it interpolates (2^f - 1) / f at the Chebyshev
+// nodes, and 2^0 is 1. n is the low word of `k`, a number beside 1.5 * 2^52, and goes into the exponent as an integer.
+constexpr double kLog2e = 0x1.71547652b82fep+0, kShift = 0x1.8p+52;
+__device__ __forceinline__ double exp2_parts(double f, double k) {
     double p = 0x1.63b2d7971923fp-20;
     p = __builtin_fma(p, f, 0x1.00c0e4e15189cp-16);
     p = __builtin_fma(p, f, 0x1.4308c7183d6a2p-13);
@@ -58,28 +60,42 @@ __device__ __forceinline__ double exp_below(double d) {
     p = __builtin_fma(p, f, 0x1.ebfbdff82a734p-3);
     p = __builtin_fma(p, f, 0x1.62e42fef9cc69p-1);
     p = __builtin_fma(p, f, 1.0);
-    return __builtin_ldexp(p, (int)n);
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    const u2 w = __builtin_bit_cast(u2, p), n = __builtin_bit_cast(u2, k);
+    return __builtin_bit_cast(double, (u2){w.x, w.y + (n.x << 20)});
+}
+// exp(d) for d <= 1. From -700 down the result stays at 2^-1010, which no sum of logits notices.
+__device__ __forceinline__ double exp_below(double d) {
+    d = __builtin_fmax(d, -700.0);
+    const double k = __builtin_fma(d, kLog2e, kShift);
+    return exp2_parts(__builtin_fma(d, kLog2e, kShift - k), k);
 }
 
 template <typename T, int kVecs>
-__global__ __launch_bounds__(256) void beam_rows_kernel(const T* __restrict__ logits, int64_t ld, int rows, int n_valid,
+__global__ __launch_bounds__(256) void beam_rows_kernel(const T* __restrict__ logits, int64_t ld, int n_valid,
                                                         BeamCut cut, uint32_t part_magic, float* __restrict__ gmax,
                                                         float* __restrict__ pmax, double* __restrict__ psum) {
     constexpr int E = kE<T>;
-    const uint32_t item = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int row = (int)(part_magic ? div_magic(item, part_magic) : item), part = (int)item - row * cut.parts;
-    if (row >= rows) return;
-    const int lane = (int)threadIdx.x & 63, first = part * kVecs;
+    __shared__ float wave_max[4];
+    __shared__ double wave_sum[4];
+    const int row = (int)(part_magic ? div_magic(blockIdx.x, part_magic) : blockIdx.x), part = (int)blockIdx.x - row * cut.parts;
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, first = (4 * part + wave) * kVecs;
     const T* x = logits + (int64_t)row * ld;
     typename Vec<T>::type raw[kVecs];
+    if ((first + kVecs) * 64 * E <= n_valid) {  // (a branch of single lanes would have every load waited for by itself)
 #pragma unroll
-    for (int j = 0; j < kVecs; ++j) {
-        const int i = ((first + j) * 64 + lane) * E;
-        if (i + E <= n_valid) {
-            raw[j] = *reinterpret_cast<const typename Vec<T>::type*>(x + i);
-        } else {
+        for (int j = 0; j < kVecs; ++j)
+            raw[j] = *reinterpret_cast<const typename Vec<T>::type*>(x + ((first + j) * 64 + lane) * E);
+    } else {
 #pragma unroll
-            for (int e = 0; e < E; ++e) raw[j][e] = i + e < n_valid ? x[i + e] : (T)-__builtin_inff();
+        for (int j = 0; j < kVecs; ++j) {
+            const int i = ((first + j) * 64 + lane) * E;
+            if (i + E <= n_valid) {
+                raw[j] = *reinterpret_cast<const typename Vec<T>::type*>(x + i);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) raw[j][e] = i + e < n_valid ? x[i + e] : (T)-__builtin_inff();
+            }
         }
     }
     float m = -__builtin_inff(), g = m;  // maxima pass over a NaN, which the sum does not
@@ -100,17 +116,43 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const T* __restrict__ lo
             g = -__builtin_inff();
         }
     }
-    const double base = (double)__builtin_fmaxf(m, -3.402823466e38f);  // a part without a finite logit sums to 0
     double s = 0.0;
+    if (__builtin_fabsf(m) <= 4096.0f) {
+        // relative to 2^at, the power of two next to exp(m), which n takes up: a logit's product with log2(e) rounds to an integer
+        // beside kShift - at, and the rest of it is exact before its own rounding
+        const double at = __builtin_rint((double)m * kLog2e), a = kShift - at;
+        const float low = m - 690.0f;
 #pragma unroll
-    for (int j = 0; j < kVecs; ++j)
+        for (int j = 0; j < kVecs; ++j)
 #pragma unroll
-        for (int e = 0; e < E; ++e) s += exp_below((double)(float)raw[j][e] - base);
-    s = wave_reduce32x2(s, [](double a, double b) { return a + b; });
+            for (int e = 0; e < E; ++e) {
+                const double x = (double)__builtin_amdgcn_fmed3f((float)raw[j][e], low, __builtin_inff()), k = __builtin_fma(x, kLog2e, a);
+                s += exp2_parts(__builtin_fma(x, kLog2e, a - k), k);
+            }
+        s = wave_reduce32x2(s, [](double p, double q) { return p + q; });
+        s *= exp_below(at * 0x1.62e42fefa39efp-1 - (double)m);  // relative to exp(m)
+    } else {
+        const double base = (double)__builtin_fmaxf(m, -0x1.fffffep127f);  // a part without a finite logit sums to 0 or so
+        for (int j = 0; j < kVecs; ++j)
+            for (int e = 0; e < E; ++e) s += exp_below((double)(float)raw[j][e] - base);
+        s = wave_reduce32x2(s, [](double p, double q) { return p + q; });
+    }
     if (__any(nan) || m == __builtin_inff()) s = __builtin_nan("");
     if (lane == 0) {
-        pmax[(size_t)row * cut.parts + part] = m;
-        psum[(size_t)row * cut.parts + part] = s;
+        wave_max[wave] = m;
+        wave_sum[wave] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {  // lane w takes wave w's
+        const float mine = wave_max[lane & 3];
+        const float top = __builtin_fmaxf(__builtin_fmaxf(wave_max[0], wave_max[1]), __builtin_fmaxf(wave_max[2], wave_max[3]));
+        double all = wave_sum[lane & 3] * exp_below((double)mine - (double)__builtin_fmaxf(top, -0x1.fffffep127f));
+        all += __shfl_xor(all, 1);
+        all += __shfl_xor(all, 2);
+        if (lane == 0) {
+            pmax[(size_t)row * cut.parts + part] = top;
+            psum[(size_t)row * cut.parts + part] = all;
+        }
     }
 }
 
@@ -130,10 +172,9 @@ struct Limit {
     __device__ __forceinline__ bool takes(uint64_t k, uint32_t i) const { return k > key || (k == key && i <= index); }
 };
 
-// Sum of v over the workgroup, for every thread. `red` holds 16 values for each parity of `turn`, so that a call needs one
-// barrier.
+// Sum over the workgroup of what its waves count (the same in a wave's lanes), for every thread. `red` holds 16 values for each
+// parity of `turn`, so that a call needs one barrier.
 __device__ __forceinline__ int wg_sum(int v, int (*red)[16], int& turn) {
-    v = wave_sum_i32(v);
     int* r = red[turn & 1];
     ++turn;
     if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
@@ -148,29 +189,28 @@ __device__ __forceinline__ int wg_sum(int v, int (*red)[16], int& turn) {
 // every thread), or all where there are fewer; top: a key that none is above. Steps down from the top, four times as far
 // each time, halves the keys between the last two steps, and then, where more than `most` share one key, the indexes.
 template <typename Count>
-__device__ __forceinline__ Limit find_limit(uint64_t low, uint64_t top, int k, int most, Count&& count) {
-    Limit all{low, 0xffffffffu};
-    if (count(all) <= most) return all;
-    uint64_t lo = low, hi = top + 1;  // at least k at lo and above, fewer than k at hi and above
-    for (uint64_t step = (uint64_t)1 << 49; hi - lo > step; step = step < (uint64_t)1 << 60 ? 4 * step : ~(uint64_t)0) {
-        const uint64_t at = hi - step;  // 2^49: 2 of a score between 16 and 32
-        const int n = count(Limit{at, 0xffffffffu});
-        if (n < k) {
-            hi = at;
-        } else {
-            if (n <= most) return Limit{at, 0xffffffffu};
+__device__ __forceinline__ Limit find_limit(uint64_t top, int k, int most, Count&& count) {
+    constexpr uint32_t kAny = 0xffffffffu;
+    uint64_t lo = 1, hi = top + 1;  // at least k at lo and above, fewer than k at hi and above
+    for (uint64_t step = (uint64_t)1 << 49;;) {  // 2^49: 2 of a score between 16 and 32
+        const uint64_t at = hi - 1 > step ? hi - step : 1;
+        const int n = count(Limit{at, kAny});
+        if (n <= most && (n >= k || at == 1)) return Limit{at, kAny};
+        if (n >= k) {
             lo = at;
             break;
         }
+        hi = at;
+        step = step < (uint64_t)1 << 60 ? 4 * step : ~(uint64_t)0;
     }
     while (hi - lo > 1) {
         const uint64_t mid = lo + (hi - lo) / 2;
-        const int n = count(Limit{mid, 0xffffffffu});
+        const int n = count(Limit{mid, kAny});
         if (n < k) hi = mid;
-        else if (n <= most) return Limit{mid, 0xffffffffu};
+        else if (n <= most) return Limit{mid, kAny};
         else lo = mid;
     }
-    uint32_t a = 0, b = 0xffffffffu;  // fewer than k up to index a - 1, at least k up to b
+    uint32_t a = 0, b = kAny;  // fewer than k up to index a - 1, at least k up to b
     while (a < b) {
         const uint32_t mid = a + (b - a) / 2;
         const int n = count(Limit{lo, mid});
@@ -181,7 +221,8 @@ __device__ __forceinline__ Limit find_limit(uint64_t low, uint64_t top, int k, i
     return Limit{lo, b};
 }
 
-template <typename T, int kKeys>
+// kKeys: groups to a thread, at most; kGroup: vectors of a group.
+template <typename T, int kKeys, int kGroup>
 __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const T* __restrict__ logits, int64_t ld,
                                                                  const float* __restrict__ scores, int beams, int n_valid,
                                                                  int k, BeamCut cut, uint32_t group_magic,
@@ -193,27 +234,41 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const T* __rest
     __shared__ double row_max[QH_BEAM_MAX_BEAMS], row_add[QH_BEAM_MAX_BEAMS];  // a NaN sum: a row without candidates
     __shared__ uint64_t pool_key[kPool];
     __shared__ uint32_t pool_at[kPool];
-    __shared__ int list[kList];
+    __shared__ int list[kList], rank_of[kPool];
     __shared__ int red[2][16];
-    __shared__ uint64_t ends[2][16];
+    __shared__ uint64_t tops[16];
     __shared__ int n_list, n_pool;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, prompt = (int)blockIdx.x, row0 = prompt * beams;
     if (tid == 0) n_list = n_pool = 0;
+    const int n_groups = beams * cut.groups;
+    float best_of[kKeys];  // in flight while the rows are summed
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j) {
+        const int i = j * kPickThreads + tid;
+        best_of[j] = i < n_groups ? gmax[(size_t)row0 * cut.groups + i] : -__builtin_inff();
+    }
     for (int b = wave; b < beams; b += 16) {
         const float* pm = pmax + (size_t)(row0 + b) * cut.parts;
         const double* ps = psum + (size_t)(row0 + b) * cut.parts;
-        float m = -__builtin_inff();
-        for (int i = lane; i < cut.parts; i += 64) m = __builtin_fmaxf(m, pm[i]);
-        m = wave_reduce32x2(m, [](float a, float c) { return __builtin_fmaxf(a, c); });
-        const double base = (double)__builtin_fmaxf(m, -3.402823466e38f);
-        double s = 0.0;
-        for (int i = lane; i < cut.parts; i += 64) {
-            const double p = ps[i];
-            if (p != 0.0) s += p * exp_below((double)pm[i] - base);
+        constexpr int kHeld = 4;  // parts of a lane: 256 of a row cover every vocabulary at 4 vectors to a wave and more
+        float m[kHeld], top = -__builtin_inff();
+        double p[kHeld];
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            const int i = 64 * j + lane;
+            m[j] = i < cut.parts ? pm[i] : -__builtin_inff();
+            p[j] = i < cut.parts ? ps[i] : 0.0;
         }
-        s = wave_reduce32x2(s, [](double a, double c) { return a + c; });
+        const double score = scores ? (double)scores[row0 + b] : 0.0;
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) top = __builtin_fmaxf(top, m[j]);
+        top = wave_reduce32x2(top, [](float x, float y) { return __builtin_fmaxf(x, y); });
+        const double base = (double)__builtin_fmaxf(top, -0x1.fffffep127f);
+        double s = 0.0;
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) s += p[j] * exp_below((double)m[j] - base);
+        s = wave_reduce32x2(s, [](double x, double y) { return x + y; });
         if (lane == 0) {
-            const double score = scores ? (double)scores[row0 + b] : 0.0;
             const bool fine = s > 0.0 && s < __builtin_inf() && __builtin_fabs(score) < __builtin_inf();
             row_max[b] = base;
             row_add[b] = fine ? score - ::log(s) : __builtin_nan("");
@@ -226,40 +281,24 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const T* __rest
         return __builtin_fabs(v) < __builtin_inf() ? ordered_f64(v) : (uint64_t)0;
     };
     // 1. the groups
-    const int n_groups = beams * cut.groups;
-    uint64_t key[kKeys];
-    uint64_t low = ~(uint64_t)0, top = 0;
+    uint64_t key[kKeys], top = 0;
 #pragma unroll
     for (int j = 0; j < kKeys; ++j) {
         const int i = j * kPickThreads + tid;
         key[j] = 0;
-        if (i < n_groups) {
-            const int b = (int)(group_magic ? div_magic((uint32_t)i, group_magic) : (uint32_t)i);
-            key[j] = key_of(gmax[(size_t)row0 * cut.groups + i], b);
-        }
-        if (key[j]) {
-            low = key[j] < low ? key[j] : low;
-            top = key[j] > top ? key[j] : top;
-        }
+        if (i < n_groups) key[j] = key_of(best_of[j], (int)(group_magic ? div_magic((uint32_t)i, group_magic) : (uint32_t)i));
+        top = key[j] > top ? key[j] : top;
     }
-    low = ~wave_max_u64(~low);
     top = wave_max_u64(top);
-    if (lane == 0) {
-        ends[0][wave] = low;
-        ends[1][wave] = top;
-    }
+    if (lane == 0) tops[wave] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 16; ++w) {
-        low = ends[0][w] < low ? ends[0][w] : low;
-        top = ends[1][w] > top ? ends[1][w] : top;
-    }
-    if (top == 0) low = 1;  // no candidate at all
+    for (int w = 0; w < 16; ++w) top = tops[w] > top ? tops[w] : top;
     int turn = 0;
-    const Limit groups = find_limit(low, top, k, 2 * k + 32, [&](const Limit& l) {
+    const Limit groups = find_limit(top, k, k + 16, [&](const Limit& l) {
         int n = 0;
 #pragma unroll
-        for (int j = 0; j < kKeys; ++j) n += l.takes(key[j], (uint32_t)(j * kPickThreads + tid));
+        for (int j = 0; j < kKeys; ++j) n += __builtin_popcountll(__ballot(l.takes(key[j], (uint32_t)(j * kPickThreads + tid))));
         return wg_sum(n, red, turn);
     });
 #pragma unroll
@@ -269,25 +308,45 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const T* __rest
     }
     __syncthreads();
     // 2. their candidates: where k groups are listed, k of their best are at the limit's key or above, so only such ones count
-    const int listed = n_list, per = 64 * E;
-    auto each = [&](auto&& f) {  // f(key, row * n_valid + id) of every candidate of the listed groups, a wave to a vector of ids
-        for (int w = wave; w < listed * cut.group; w += 16) {
-            const int i = list[w / cut.group], b = (int)(group_magic ? div_magic((uint32_t)i, group_magic) : (uint32_t)i);
-            const int id = ((i - b * cut.groups) * cut.group + w % cut.group) * per + lane * E;
-            const T* x = logits + (int64_t)(row0 + b) * ld + id;
-            if (id + E <= n_valid) {
-                const auto v = *reinterpret_cast<const typename Vec<T>::type*>(x);
+    const int listed = n_list;
+    // f(there, logit, row, id) of every id of the listed groups whose logit can reach the limit, a wave to a group; what reaches it
+    // is at or above the logit whose score the limit is, less what f32 and the sums round off
+    auto each = [&](uint64_t limit_key, auto&& f) {
+        const double goal = limit_key > 1 ? from_ordered_f64(limit_key) : -__builtin_inff();
+        for (int w = wave; w < listed; w += 16) {
+            const int i = list[w], b = (int)(group_magic ? div_magic((uint32_t)i, group_magic) : (uint32_t)i);
+            const int id0 = (i - b * cut.groups) * kGroup * 64 * E;
+            const T* x = logits + (int64_t)(row0 + b) * ld;
+            const double t = goal - row_add[b], u = row_max[b];
+            const float least = (float)(t + u - 0x1p-22 * (__builtin_fabs(t) + __builtin_fabs(u)));
+            typename Vec<T>::type v[kGroup];
+            if (id0 + kGroup * 64 * E <= n_valid) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) f(key_of((float)v[e], b), (uint32_t)(b * n_valid + id + e));
+                for (int g = 0; g < kGroup; ++g)
+                    v[g] = *reinterpret_cast<const typename Vec<T>::type*>(x + id0 + (64 * g + lane) * E);
             } else {
-                for (int e = 0; e < E; ++e)
-                    if (id + e < n_valid) f(key_of((float)x[e], b), (uint32_t)(b * n_valid + id + e));
+#pragma unroll
+                for (int g = 0; g < kGroup; ++g)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const int id = id0 + (64 * g + lane) * E + e;
+                        v[g][e] = id < n_valid ? x[id] : (T)-__builtin_inff();
+                    }
             }
+#pragma unroll
+            for (int g = 0; g < kGroup; ++g)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float l = (float)v[g][e];
+                    if (!(l < least)) f(l, b, id0 + (64 * g + lane) * E + e);
+                }
         }
     };
     Limit limit{listed < k ? (uint64_t)1 : groups.key, 0xffffffffu};  // fewer groups: all that they hold
     auto collect = [&]() {
-        each([&](uint64_t c, uint32_t at) {
+        each(limit.key, [&](float l, int b, int id) {
+            const uint64_t c = key_of(l, b);
+            const uint32_t at = (uint32_t)(b * n_valid + id);
             if (limit.takes(c, at)) {
                 const int i = atomicAdd(&n_pool, 1);
                 if (i < kPool) {
@@ -300,28 +359,52 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const T* __rest
     };
     collect();
     if (n_pool > kPool) {  // many of them next to each other, or equal: the limit from counts of them all
-        limit = find_limit(limit.key, top, k, kPool, [&](const Limit& l) {
+        limit = find_limit(top, k, kPool, [&](const Limit& l) {
             int n = 0;
-            each([&](uint64_t c, uint32_t at) { n += l.takes(c, at); });
-            return wg_sum(n, red, turn);
+            each(l.key, [&](float x, int b, int id) { n += l.takes(key_of(x, b), (uint32_t)(b * n_valid + id)); });
+            return wg_sum(wave_sum_i32(n), red, turn);
         });
         __syncthreads();
         if (tid == 0) n_pool = 0;
         __syncthreads();
         collect();
     }
-    // 3. their ranks, each from a look at all of them
-    const int n = n_pool;
+    if (n_pool > k + 64) {  // those near the k best alone: ranks take their number squared
+        const uint64_t c = tid < n_pool ? pool_key[tid] : 0;
+        const uint32_t at = tid < n_pool ? pool_at[tid] : 0;
+        limit = find_limit(top, k, k + 32, [&](const Limit& l) {
+            return wg_sum((int)__builtin_popcountll(__ballot(l.takes(c, at))), red, turn);
+        });
+        if (tid == 0) n_pool = 0;
+        __syncthreads();
+        if (limit.takes(c, at)) {
+            const int i = atomicAdd(&n_pool, 1);
+            pool_key[i] = c;
+            pool_at[i] = at;
+        }
+        __syncthreads();
+    }
+    // 3. their ranks: how many come before each, a wave's sixteenth of them to each of its lanes' candidates
+    const int n = n_pool, share = (n + 15) / 16, from = wave * share, to = min(from + share, n);
+    for (int i = tid; i < n; i += kPickThreads) rank_of[i] = 0;
+    __syncthreads();
+    for (int i = lane; i < n; i += 64) {
+        const uint64_t c = pool_key[i];
+        const uint32_t at = pool_at[i];
+        int before = 0;
+#pragma unroll 4
+        for (int j = from; j < to; ++j) before += pool_key[j] > c || (pool_key[j] == c && pool_at[j] < at);
+        if (before) atomicAdd(&rank_of[i], before);
+    }
+    __syncthreads();
     if (tid < n) {
-        const uint64_t c = pool_key[tid];
-        const uint32_t at = pool_at[tid];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += pool_key[j] > c || (pool_key[j] == c && pool_at[j] < at);
+        const int rank = rank_of[tid];
         if (rank < k) {
+            const uint32_t at = pool_at[tid];
             const int b = (int)(at / (uint32_t)n_valid);
             parent[(size_t)prompt * k + rank] = row0 + b;
             token[(size_t)prompt * k + rank] = (int)(at - (uint32_t)b * (uint32_t)n_valid);
-            best[(size_t)prompt * k + rank] = (float)from_ordered_f64(c);
+            best[(size_t)prompt * k + rank] = (float)from_ordered_f64(pool_key[tid]);
         }
     }
     for (int i = n + tid; i < k; i += kPickThreads) {  // fewer candidates than k
@@ -342,9 +425,9 @@ hipError_t beam_select_of(const BeamArgs& a, hipStream_t s) {
     float* pmax = reinterpret_cast<float*>(psum + (size_t)rows * c.parts);
     float* gmax = pmax + (size_t)rows * c.parts;
     const T* logits = static_cast<const T*>(a.logits);
-    const dim3 grid((unsigned)(((int64_t)rows * c.parts + 3) / 4));
+    const dim3 grid((unsigned)(rows * c.parts));
     auto go = [&](auto vecs) {
-        qh_launch((beam_rows_kernel<T, decltype(vecs)::value>), grid, dim3(256), 0, s, logits, a.ld, rows, a.n_valid, c,
+        qh_launch((beam_rows_kernel<T, decltype(vecs)::value>), grid, dim3(256), 0, s, logits, a.ld, a.n_valid, c,
                   magic_of(c.parts), gmax, pmax, psum);
     };
     using std::integral_constant;
@@ -353,12 +436,18 @@ hipError_t beam_select_of(const BeamArgs& a, hipStream_t s) {
     else if (c.vecs == 4) go(integral_constant<int, 4>{});
     else go(integral_constant<int, 8>{});
     if (hipError_t e = hipGetLastError()) return e;
-    auto pick = [&](auto keys) {
-        qh_launch((beam_pick_kernel<T, decltype(keys)::value>), dim3((unsigned)a.prompts), dim3(kPickThreads), 0, s, logits,
-                  a.ld, a.scores, a.beams, a.n_valid, a.k, c, magic_of(c.groups), gmax, pmax, psum, a.parent, a.token, a.best);
+    constexpr int kGroup = 1024 / (64 * kE<T>);
+    auto pick = [&](auto keys, auto group) {
+        qh_launch((beam_pick_kernel<T, decltype(keys)::value, decltype(group)::value>), dim3((unsigned)a.prompts),
+                  dim3(kPickThreads), 0, s, logits, a.ld, a.scores, a.beams, a.n_valid, a.k, c, magic_of(c.groups), gmax, pmax,
+                  psum, a.parent, a.token, a.best);
     };
-    if (a.beams * c.groups <= 8 * kPickThreads) pick(integral_constant<int, 8>{});
-    else pick(integral_constant<int, 32>{});
+    const int groups = a.beams * c.groups;
+    if (c.group == 1) pick(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+    else if (c.group != kGroup) pick(integral_constant<int, 32>{}, integral_constant<int, 2 * kGroup>{});
+    else if (groups <= kPickThreads) pick(integral_constant<int, 1>{}, integral_constant<int, kGroup>{});
+    else if (groups <= 4 * kPickThreads) pick(integral_constant<int, 4>{}, integral_constant<int, kGroup>{});
+    else pick(integral_constant<int, 32>{}, integral_constant<int, kGroup>{});
     return hipGetLastError();
 }
 

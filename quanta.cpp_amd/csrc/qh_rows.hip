@@ -69,7 +69,7 @@ __device__ __forceinline__ void quant_lanes(const float (&v)[8], int8_t* q, floa
 // overflows, the order of the sum does not show, and y is rounded once.
 template <typename T, int kWaves, int kVec>
 __global__ __launch_bounds__(kWaves < 4 ? 256 : 64 * kWaves) void rmsnorm_kernel(NormArgs a) {
-    constexpr int E = kE<T>, kRows = kWaves < 4 ? 4 / kWaves : 1;
+    constexpr int E = kE<T>, kRows = kWaves < 4 ? 4 / kWaves : 1, kPass = 64 * kWaves * E;
     const int tid = (int)threadIdx.x % (64 * kWaves);
     const int row = (int)blockIdx.x * kRows + (int)threadIdx.x / (64 * kWaves);
     __shared__ double part[kWaves < 4 ? 4 : kWaves];
@@ -82,12 +82,17 @@ __global__ __launch_bounds__(kWaves < 4 ? 256 : 64 * kWaves) void rmsnorm_kernel
         const T* res = static_cast<const T*>(a.res) + (int64_t)row * a.ldr;
         T* sum = static_cast<T*>(a.sum) + (int64_t)row * a.lds;
         float r[kVec][E];
+        // whole passes of the row without a branch of single lanes, which would have every load waited for by itself
+        auto load = [&](const T* p, float (&v)[kVec][E]) {
 #pragma unroll
-        for (int c = 0; c < kVec; ++c) {
-            const int i = (c * 64 * kWaves + tid) * E;
-            load_e(x + i, a.n - i, h[c]);
-            if (a.res) load_e(res + i, a.n - i, r[c]);
-        }
+            for (int c = 0; c < kVec; ++c) {
+                const int i = (c * 64 * kWaves + tid) * E;
+                if ((c + 1) * kPass <= a.n) load_e(p + i, E, v[c]);
+                else load_e(p + i, a.n - i, v[c]);
+            }
+        };
+        load(x, h);
+        if (a.res) load(res, r);
 #pragma unroll
         for (int c = 0; c < kVec; ++c) {
             const int i = (c * 64 * kWaves + tid) * E;
@@ -95,7 +100,7 @@ __global__ __launch_bounds__(kWaves < 4 ? 256 : 64 * kWaves) void rmsnorm_kernel
 #pragma unroll
                 for (int e = 0; e < E; ++e) h[c][e] = (float)(T)(h[c][e] + r[c][e]);
             }
-            if (a.sum) store_e(sum + i, a.n - i, h[c]);
+            if (a.sum) store_e(sum + i, (c + 1) * kPass <= a.n ? E : a.n - i, h[c]);
 #pragma unroll
             for (int e = 0; e < E; ++e) ss = __builtin_fma((double)h[c][e], (double)h[c][e], ss);
         }
@@ -181,7 +186,8 @@ constexpr int kRopePairs = 512;  // cosines and sines that a workgroup keeps
 // position, less its whole turns), then every head's pairs, E of them to an item, and after them the dims past rot, E to an
 // item, where the result is not written in place. Consecutive lanes take consecutive items of a head, so rows move in one
 // piece.
-template <typename T, bool kInterleaved>
+// kWhole: no item is cut off by the end of the pairs or of the head.
+template <typename T, bool kInterleaved, bool kWhole>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a, int per, int units, int rest, uint32_t unit_magic,
                                                             uint32_t head_magic) {
     constexpr int E = kE<T>;
@@ -205,11 +211,12 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a, int per,
         if (u >= units) {
             const int i = a.rot + (u - units) * E;
             float v[E];
-            load_e(x + i, a.hd - i, v);
-            store_e(out + i, a.hd - i, v);
+            const int m = kWhole ? E : a.hd - i;
+            load_e(x + i, m, v);
+            store_e(out + i, m, v);
             continue;
         }
-        const int p = u * E, m = half - p;
+        const int p = u * E, m = kWhole ? E : half - p;
         const float2* c = cs + t * half + p;
         float f[E], g[E];  // firsts and seconds of the pairs (half), or the pairs in order (interleaved)
         if (kInterleaved) {
@@ -254,8 +261,15 @@ hipError_t rope_of(const RopeArgs& a, bool interleaved, hipStream_t s) {
     per = per < 1 ? 1 : per < kRopePairs / half ? per : kRopePairs / half;
     const dim3 grid((unsigned)((a.n_tok + per - 1) / per));
     const uint32_t um = magic_of(units + rest), hm = magic_of(heads);
-    if (interleaved) qh_launch((rope_kernel<T, true>), grid, dim3(kRopeThreads), 0, s, a, per, units, rest, um, hm);
-    else qh_launch((rope_kernel<T, false>), grid, dim3(kRopeThreads), 0, s, a, per, units, rest, um, hm);
+    const bool whole = half % E == 0 && (rest == 0 || (a.hd - a.rot) % E == 0);
+    auto go = [&](auto inter, auto all) {
+        qh_launch((rope_kernel<T, decltype(inter)::value, decltype(all)::value>), grid, dim3(kRopeThreads), 0, s, a, per, units,
+                  rest, um, hm);
+    };
+    if (interleaved && whole) go(std::true_type{}, std::true_type{});
+    else if (interleaved) go(std::true_type{}, std::false_type{});
+    else if (whole) go(std::false_type{}, std::true_type{});
+    else go(std::false_type{}, std::false_type{});
     return hipGetLastError();
 }
 
