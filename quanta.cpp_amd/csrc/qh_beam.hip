@@ -20,7 +20,7 @@ constexpr int kList = QH_BEAM_MAX_K + 16;  // groups that are read again, at mos
 
 template <typename T>
 constexpr int kE = 16 / (int)sizeof(T);
-constexpr int kMostVecs = 4;  // (192 x 151,936 f32: 26.8 us, with 8 28.2, with 16 32.2)
+constexpr int kMostVecs = 2;  // or a group's (192 x 151,936 f32, groups of 4: 26.8 us, with 8 28.2, with 16 32.2; 512 x 50,257 f16 24.2, with 4 38)
 template <typename T>
 struct Vec {  // at any address of the type's alignment
     typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));

@@ -186,7 +186,7 @@ struct Prompt {
 template <typename T, int kHd, int kTile, int kW>
 __global__ __launch_bounds__(64 * kW, 2) void prompt_kernel(PromptArgs a) {
     typedef Prompt<T, kHd, kTile, kW> P;
-    constexpr int kN = P::kN, kKt = P::kKt, kDt = P::kDt, kKs = P::kKs;
+    constexpr int kN = P::kN, kKt = P::kKt, kDt = P::kDt, kKs = P::kKs, kDeep = 4 / (kN == 3 ? 2 : 1);
     __shared__ __align__(16) uint8_t lds[2 * P::kBuffer];
     __shared__ int odd;  // a value of a tile that is looked at is not finite
     const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5,
@@ -247,13 +247,25 @@ __global__ __launch_bounds__(64 * kW, 2) void prompt_kernel(PromptArgs a) {
     Raw<T> kr[P::kPer], vr[P::kPer];
     const T* const kp = static_cast<const T*>(a.k) + (int64_t)kvh * kHd;
     const T* const vp = static_cast<const T*>(a.v) + (int64_t)kvh * kHd;
+    constexpr int kStep = P::kThreads / P::kChunks;  // rows from a thread's chunk to its next
+    const T* k_at = kp + (int64_t)(e.key0 + tid / P::kChunks) * a.ldk + 8 * (tid % P::kChunks);  // of the next tile to fetch
+    const T* v_at = vp + (int64_t)(e.key0 + tid / P::kChunks) * a.ldv + 8 * (tid % P::kChunks);
     auto fetch = [&](int t) {
+        if ((t + 1) * kTile <= e.keys) {
 #pragma unroll
-        for (int i = 0; i < P::kPer; ++i) {
-            const int c = i * P::kThreads + tid, key = min(t * kTile + c / P::kChunks, e.keys - 1);
-            const int64_t row = e.key0 + key;
-            kr[i].load(kp + row * a.ldk + 8 * (c % P::kChunks));
-            vr[i].load(vp + row * a.ldv + 8 * (c % P::kChunks));
+            for (int i = 0; i < P::kPer; ++i) {
+                kr[i].load(k_at + i * (kStep * a.ldk));
+                vr[i].load(v_at + i * (kStep * a.ldv));
+            }
+            k_at += kTile * a.ldk;
+            v_at += kTile * a.ldv;
+        } else {  // the last tile: rows that are not there are the last one's
+#pragma unroll
+            for (int i = 0; i < P::kPer; ++i) {
+                const int64_t row = e.key0 + min(t * kTile + i * kStep + tid / P::kChunks, e.keys - 1);
+                kr[i].load(kp + row * a.ldk + 8 * (tid % P::kChunks));
+                vr[i].load(vp + row * a.ldv + 8 * (tid % P::kChunks));
+            }
         }
     };
     auto stage = [&](int t, int buf) {
@@ -316,14 +328,27 @@ __global__ __launch_bounds__(64 * kW, 2) void prompt_kernel(PromptArgs a) {
         const uint8_t* buf = lds + cur * P::kBuffer;
         if (t + 1 < tiles) stage(t + 1, cur ^ 1);
         if (t + 2 < tiles) fetch(t + 2);
+        // operands are read kDeep products before their use, and a wave in its products goes before the others of its SIMD
         f16v s[kKt];
+        __builtin_amdgcn_s_setprio(1);
+        {
+            constexpr int kOps = kKt * kKs;
+            Parts<T> ring[kDeep];
 #pragma unroll
-        for (int kt = 0; kt < kKt; ++kt) {
+            for (int r = 0; r < kDeep; ++r) ring[r] = key_op(buf, r % kKt, r / kKt);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[kt][i] = 0.0f;
+            for (int r = 0; r < kOps; ++r) {  // the tiles in turn, so that a product does not wait for the one before
+                const int kt = r % kKt, k = r / kKt;
+                if (k == 0) {
 #pragma unroll
-            for (int k = 0; k < kKs; ++k) s[kt] = product<T>(key_op(buf, kt, k), q[k], s[kt]);
+                    for (int i = 0; i < 16; ++i) s[kt][i] = 0.0f;
+                }
+                s[kt] = product<T>(ring[r % kDeep], q[k], s[kt]);
+                if (r + kDeep < kOps) ring[r % kDeep] = key_op(buf, (r + kDeep) % kKt, (r + kDeep) / kKt);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
+        __builtin_amdgcn_s_setprio(0);
         const int pos0 = t * kTile;
         const bool masked = pos0 + kTile > all_see;
         if (masked) {
@@ -377,10 +402,20 @@ __global__ __launch_bounds__(64 * kW, 2) void prompt_kernel(PromptArgs a) {
             l = weights(base == -__builtin_inff() ? 0.0f : base);
         }
         sum += l;
+        __builtin_amdgcn_s_setprio(1);
+        {
+            constexpr int kOps = 2 * kKt * kDt;
+            Parts<T> ring[kDeep];
 #pragma unroll
-        for (int u = 0; u < 2 * kKt; ++u)
+            for (int r = 0; r < kDeep; ++r) ring[r] = value_op(buf, r / kDt, r % kDt);
 #pragma unroll
-            for (int d = 0; d < kDt; ++d) o[d] = product<T>(value_op(buf, u, d), w[u], o[d]);
+            for (int r = 0; r < kOps; ++r) {
+                o[r % kDt] = product<T>(ring[r % kDeep], w[r / kDt], o[r % kDt]);
+                if (r + kDeep < kOps) ring[r % kDeep] = value_op(buf, (r + kDeep) / kDt, (r + kDeep) % kDt);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        __builtin_amdgcn_s_setprio(0);
         __syncthreads();
     }
 
