@@ -24,6 +24,9 @@
 namespace qh {
 namespace {
 
+constexpr int kSplitKeys = 128;  // keys of a split, at least
+constexpr int kMaxSplits = 64;
+
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -170,9 +173,43 @@ __device__ __forceinline__ int swizzle(int r, int c) {
     else return c ^ ((((r >> 1) & 1) << 2) | ((r >> 2) & 3));
 }
 
+// Entry b: its first query row (token) and rows, its first key and keys, whatever the starts hold inside the arrays.
 struct Entry {
-    int row0, rows, key0, keys;  // first query row (token) and rows, first key and keys
+    int row0, rows, key0, keys;
+    // keys that row r (token * group + head) sees: its token's own position is keys - rows + token
+    __device__ __forceinline__ int visible(const PromptArgs& a, int r) const {
+        return a.causal ? min(max(keys - rows + (int)((unsigned)r / (unsigned)a.group) + 1, 0), keys) : keys;
+    }
 };
+// The entry of row tile `item`, false where there is none; *r0: the tile's first row. Up to 63 entries come with one load of
+// each list, a lane to a start; more are searched for.
+__device__ __forceinline__ bool entry_of(const PromptArgs& a, int item, int tile_rows, Entry* e, int* r0) {
+    const int lane = (int)threadIdx.x & 63;
+    int b, first, q0, q1, k0, k1;
+    if (a.n < 64) {
+        const int i = min(lane, a.n), q = min(max(a.start[i], 0), a.n_tok), k = min(max(a.kstart[i], 0), a.n_keys);
+        const int key = lane < a.n ? (int)((int64_t)q * a.group / tile_rows) + lane : 0x7fffffff;
+        const uint64_t at = __ballot(key <= item);
+        if (at == 0) return false;
+        b = 63 - __builtin_clzll(at);
+        first = __builtin_amdgcn_readlane(key, b);
+        q0 = __builtin_amdgcn_readlane(q, b), q1 = __builtin_amdgcn_readlane(q, b + 1);
+        k0 = __builtin_amdgcn_readlane(k, b), k1 = __builtin_amdgcn_readlane(k, b + 1);
+    } else {
+        b = kv8_entry_of(Kv8Batch{a.start, nullptr, a.n, a.n_tok, 0}, item, a.group, tile_rows, 1, &first);
+        if (b < 0) return false;
+        b = __builtin_amdgcn_readfirstlane(b);
+        q0 = min(max(a.start[b], 0), a.n_tok), q1 = min(max(a.start[b + 1], 0), a.n_tok);
+        k0 = min(max(a.kstart[b], 0), a.n_keys), k1 = min(max(a.kstart[b + 1], 0), a.n_keys);
+    }
+    *e = {q0, max(q1 - q0, 0), k0, max(k1 - k0, 0)};
+    *r0 = (item - first) * tile_rows;
+    return *r0 < e->rows * a.group;
+}
+// The workgroups that share a row tile's key tiles, 128 keys to each at least.
+__device__ __forceinline__ int splits_of(const PromptArgs& a, int tiles, int tile) {
+    return min(a.splits, max(tiles * tile / kSplitKeys, 1));
+}
 
 template <typename T, int kHd, int kTile, int kW>
 struct Prompt {
@@ -183,36 +220,33 @@ struct Prompt {
     static_assert(kPer >= 1 && kTile * kChunks % kThreads == 0, "whole chunks to a thread");
 };
 
-template <typename T, int kHd, int kTile, int kW>
+// 16 bytes to each lane from its address g (a multiple of 16) into shared memory at `to` (the wave's) + 16 * lane, without a
+// register in between. Counted in vmcnt: what reads them is behind wait_loads and a barrier.
+__device__ __forceinline__ void load_to_lds(const void* g, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(to) : "memory", "m0");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// kDirect: f16 keys and values on multiples of 16 bytes, which go into shared memory as they are, past the registers.
+template <typename T, int kHd, int kTile, int kW, bool kDirect>
 __global__ __launch_bounds__(64 * kW, 2) void prompt_kernel(PromptArgs a) {
     typedef Prompt<T, kHd, kTile, kW> P;
-    constexpr int kN = P::kN, kKt = P::kKt, kDt = P::kDt, kKs = P::kKs, kDeep = 4 / (kN == 3 ? 2 : 1);
+    constexpr int kN = P::kN, kKt = P::kKt, kDt = P::kDt, kKs = P::kKs, kDeep = kN == 1 ? 4 : kHd == 64 ? 2 : 1;
     __shared__ __align__(16) uint8_t lds[2 * P::kBuffer];
     __shared__ int odd;  // a value of a tile that is looked at is not finite
     const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5,
               col = lane & 31;
     const int kvh = (int)(blockIdx.x % (unsigned)a.n_kv), item = a.items - 1 - (int)(blockIdx.x / (unsigned)a.n_kv);
-    int from = 0;
-    const int b = kv8_entry_of(Kv8Batch{a.start, nullptr, a.n, a.n_tok, 0}, item, a.group, P::kRows, 1, &from);
-    if (b < 0) return;
     Entry e;
-    {
-        auto span = [&](const int32_t* start, int most, int& first, int& n) {
-            first = min(max(start[b], 0), most);
-            n = max(min(max(start[b + 1], 0), most) - first, 0);
-        };
-        span(a.start, a.n_tok, e.row0, e.rows);
-        span(a.kstart, a.n_keys, e.key0, e.keys);
-        e = {__builtin_amdgcn_readfirstlane(e.row0), __builtin_amdgcn_readfirstlane(e.rows),
-             __builtin_amdgcn_readfirstlane(e.key0), __builtin_amdgcn_readfirstlane(e.keys)};
-    }
-    const int rows = e.rows * a.group, r0 = (item - __builtin_amdgcn_readfirstlane(from)) * P::kRows;
-    if (r0 >= rows) return;
-    // keys that row r sees: its token's own position is keys - rows + token
-    auto visible = [&](int r) {
-        return a.causal ? min(max(e.keys - e.rows + (int)((unsigned)r / (unsigned)a.group) + 1, 0), e.keys) : e.keys;
-    };
-    const int last = min(r0 + P::kRows, rows) - 1, seen = visible(last), tiles = (seen + kTile - 1) / kTile;
+    int r0;
+    if (!entry_of(a, item, P::kRows, &e, &r0)) return;
+    const int rows = e.rows * a.group;
+    auto visible = [&](int r) { return e.visible(a, r); };
+    const int last = min(r0 + P::kRows, rows) - 1, seen = visible(last), all_tiles = (seen + kTile - 1) / kTile;
+    // this workgroup's share of the tiles, where a row tile's are shared out
+    const int splits = splits_of(a, all_tiles, kTile), split = (int)blockIdx.y;
+    if (split >= splits) return;
+    const int tile0 = all_tiles * split / splits, tiles = all_tiles * (split + 1) / splits;
     const int first_sees = visible(r0);  // every row of the workgroup sees these
     const int w0 = r0 + 32 * wave, r = w0 + col;
     const bool valid = r < rows;
@@ -220,18 +254,6 @@ __global__ __launch_bounds__(64 * kW, 2) void prompt_kernel(PromptArgs a) {
     const int head = kvh * a.group + ((valid ? r : r0) - token * a.group);
     const int all_see = w0 < rows ? visible(w0) : e.keys;
 
-    Parts<T> q[kKs];
-    {
-        const T* p = static_cast<const T*>(a.q) + (int64_t)(e.row0 + token) * a.ldq + (int64_t)head * kHd + 8 * half;
-#pragma unroll
-        for (int s = 0; s < kKs; ++s) {
-            Raw<T> raw;
-            raw.load(p + 16 * s);
-            if (a.sign != 1.0f) raw.scale(a.sign);
-            q[s] = raw.parts();
-            if (!valid) q[s] = Parts<T>{};
-        }
-    }
     f16v o[kDt];
 #pragma unroll
     for (int d = 0; d < kDt; ++d)
@@ -244,12 +266,46 @@ __global__ __launch_bounds__(64 * kW, 2) void prompt_kernel(PromptArgs a) {
     const float limit = kN == 1 ? 32768.0f : __builtin_ldexpf((float)(kTile / 2), -shift);
     float base = vis > 0 ? -__builtin_inff() : 0.0f, sum = 0.0f;  // a row that sees nothing asks for no base
 
-    Raw<T> kr[P::kPer], vr[P::kPer];
+    Raw<T> kr[kDirect ? 1 : P::kPer], vr[kDirect ? 1 : P::kPer];
     const T* const kp = static_cast<const T*>(a.k) + (int64_t)kvh * kHd;
     const T* const vp = static_cast<const T*>(a.v) + (int64_t)kvh * kHd;
-    constexpr int kStep = P::kThreads / P::kChunks;  // rows from a thread's chunk to its next
-    const T* k_at = kp + (int64_t)(e.key0 + tid / P::kChunks) * a.ldk + 8 * (tid % P::kChunks);  // of the next tile to fetch
-    const T* v_at = vp + (int64_t)(e.key0 + tid / P::kChunks) * a.ldv + 8 * (tid % P::kChunks);
+    // A thread's chunks: row tid / kChunks and every kStep-th after it; kDirect: the one whose place is the thread's
+    constexpr int kStep = P::kThreads / P::kChunks;
+    static_assert(kStep % 16 == 0, "the same swizzle for all chunks of a thread");
+    const int c_row = tid / P::kChunks, c_at = kDirect ? swizzle<kHd>(c_row, tid % P::kChunks) : tid % P::kChunks;
+    const T* k_at = kp + (int64_t)(e.key0 + tile0 * kTile + c_row) * a.ldk + 8 * c_at;  // of the next tile to fetch
+    const T* v_at = vp + (int64_t)(e.key0 + tile0 * kTile + c_row) * a.ldv + 8 * c_at;
+    auto load_direct = [&](int t, int buf) {
+        const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + buf * P::kBuffer + 1024 * wave;
+        const bool whole = (t + 1) * kTile <= e.keys;
+#pragma unroll
+        for (int i = 0; i < P::kPer; ++i) {
+            const T *k = k_at + i * (kStep * a.ldk), *v = v_at + i * (kStep * a.ldv);
+            if (!whole) {  // the last tile: rows that are not there are the last one's
+                const int64_t row = e.key0 + min(t * kTile + i * kStep + c_row, e.keys - 1);
+                k = kp + row * a.ldk + 8 * c_at;
+                v = vp + row * a.ldv + 8 * c_at;
+            }
+            load_to_lds(k, to + i * (16 * P::kThreads));
+            load_to_lds(v, to + P::kPlane + i * (16 * P::kThreads));
+        }
+        k_at += kTile * a.ldk;
+        v_at += kTile * a.ldv;
+    };
+    // the values of a tile in shared memory that are not finite become 0
+    auto clean_direct = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < P::kPer; ++i) {
+            u4* at = reinterpret_cast<u4*>(lds + buf * P::kBuffer + P::kPlane) + i * P::kThreads + tid;
+            Raw<T> v;
+            if constexpr (kDirect) v.w = *at;
+            if (!v.finite()) {
+                v.clean();
+                if constexpr (kDirect) *at = v.w;
+                odd = 1;
+            }
+        }
+    };
     auto fetch = [&](int t) {
         if ((t + 1) * kTile <= e.keys) {
 #pragma unroll
@@ -262,9 +318,9 @@ __global__ __launch_bounds__(64 * kW, 2) void prompt_kernel(PromptArgs a) {
         } else {  // the last tile: rows that are not there are the last one's
 #pragma unroll
             for (int i = 0; i < P::kPer; ++i) {
-                const int64_t row = e.key0 + min(t * kTile + i * kStep + tid / P::kChunks, e.keys - 1);
-                kr[i].load(kp + row * a.ldk + 8 * (tid % P::kChunks));
-                vr[i].load(vp + row * a.ldv + 8 * (tid % P::kChunks));
+                const int64_t row = e.key0 + min(t * kTile + i * kStep + c_row, e.keys - 1);
+                kr[i].load(kp + row * a.ldk + 8 * c_at);
+                vr[i].load(vp + row * a.ldv + 8 * c_at);
             }
         }
     };
@@ -289,10 +345,30 @@ __global__ __launch_bounds__(64 * kW, 2) void prompt_kernel(PromptArgs a) {
     };
 
     if (tid == 0) odd = 0;
-    if (tiles > 0) fetch(0);
+    if constexpr (kDirect) {
+        if (tiles > tile0) load_direct(tile0, 0);
+    } else {
+        if (tiles > tile0) fetch(tile0);
+    }
+    Parts<T> q[kKs];
+    {
+        const T* p = static_cast<const T*>(a.q) + (int64_t)(e.row0 + token) * a.ldq + (int64_t)head * kHd + 8 * half;
+#pragma unroll
+        for (int s = 0; s < kKs; ++s) {
+            Raw<T> raw;
+            raw.load(p + 16 * s);
+            if (a.sign != 1.0f) raw.scale(a.sign);
+            q[s] = raw.parts();
+            if (!valid) q[s] = Parts<T>{};
+        }
+    }
     __syncthreads();
-    if (tiles > 0) stage(0, 0);
-    if (tiles > 1) fetch(1);
+    if constexpr (kDirect) {
+        wait_loads();
+    } else {
+        if (tiles > tile0) stage(tile0, 0);
+        if (tiles > tile0 + 1) fetch(tile0 + 1);
+    }
     __syncthreads();
 
     // This lane's places in a buffer: row `col` of a key operand, chunk 2 s + half; rows 4 half + lane / 4 % 4 (and 8 more) of
@@ -323,99 +399,130 @@ __global__ __launch_bounds__(64 * kW, 2) void prompt_kernel(PromptArgs a) {
         return r;
     };
 
-    for (int t = 0; t < tiles; ++t) {
-        const int cur = t & 1;
+    for (int t = tile0; t < tiles; ++t) {
+        const int cur = (t - tile0) & 1;
         const uint8_t* buf = lds + cur * P::kBuffer;
-        if (t + 1 < tiles) stage(t + 1, cur ^ 1);
-        if (t + 2 < tiles) fetch(t + 2);
-        // operands are read kDeep products before their use, and a wave in its products goes before the others of its SIMD
-        f16v s[kKt];
-        __builtin_amdgcn_s_setprio(1);
-        {
-            constexpr int kOps = kKt * kKs;
-            Parts<T> ring[kDeep];
-#pragma unroll
-            for (int r = 0; r < kDeep; ++r) ring[r] = key_op(buf, r % kKt, r / kKt);
-#pragma unroll
-            for (int r = 0; r < kOps; ++r) {  // the tiles in turn, so that a product does not wait for the one before
-                const int kt = r % kKt, k = r / kKt;
-                if (k == 0) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[kt][i] = 0.0f;
-                }
-                s[kt] = product<T>(ring[r % kDeep], q[k], s[kt]);
-                if (r + kDeep < kOps) ring[r % kDeep] = key_op(buf, (r + kDeep) % kKt, (r + kDeep) / kKt);
-                __builtin_amdgcn_sched_barrier(0);
+        if constexpr (kDirect) {
+            if ((t + 1) * kTile > first_sees) {  // the same for the whole workgroup
+                clean_direct(cur);
+                __syncthreads();
             }
+            if (t + 1 < tiles) load_direct(t + 1, cur ^ 1);
+        } else {
+            if (t + 1 < tiles) stage(t + 1, cur ^ 1);
+            if (t + 2 < tiles) fetch(t + 2);
         }
-        __builtin_amdgcn_s_setprio(0);
+        // The tile in blocks of 32 keys. Matrix instructions run in the background of a wave, eight issue slots each, so a block's
+        // weights are computed between the products of the next block's scores, and the last block's between the first products
+        // with values; operands are read kDeep products before their use, and a wave in its products goes before the others of
+        // its SIMD.
         const int pos0 = t * kTile;
         const bool masked = pos0 + kTile > all_see;
-        if (masked) {
-#pragma unroll
-            for (int kt = 0; kt < kKt; ++kt)
+        f16v s[kKt];
+        Parts<T> w[kKt][2];  // weights 2^(scale s - base) of a block, two operands of 16 keys
+        float l[kKt];
+        auto mask = [&](int kt) {
+            if (masked) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     s[kt][i] = pos0 + 32 * kt + 8 * (i >> 2) + 4 * half + (i & 3) < vis ? s[kt][i] : -__builtin_inff();
-        }
-        // weights 2^(scale s - base) as operands, and their sum
-        Parts<T> w[2 * kKt];
-        auto weights = [&](float from_base) {
-            float l = 0.0f;
-#pragma unroll
-            for (int u = 0; u < 2 * kKt; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u >> 1][8 * (u & 1) + 2 * i], a.scale_log2e, -from_base));
-                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u >> 1][8 * (u & 1) + 2 * i + 1], a.scale_log2e, -from_base));
-                    if constexpr (kN == 1) {
-                        const h2 h = __builtin_convertvector((f2){x, y}, h2);
-                        w[u].p[0][i] = __builtin_bit_cast(uint32_t, h);
-                        l = __builtin_amdgcn_fdot2(h, (h2){1, 1}, l, false);
-                    } else {
-                        uint32_t p0, p1, p2;
-                        split2<true>(x, y, p0, p1, p2);
-                        w[u].p[0][i] = p0, w[u].p[1][i] = p1, w[u].p[2][i] = p2;
-                        l += x + y;
-                    }
-                }
-            return l;
+            }
         };
-        float l = weights(base);
-        if (__any(!(l <= limit))) {
-            float top = -__builtin_inff();
+        auto weights2 = [&](int kt, int n, float from) {  // values 2 n and 2 n + 1 of the block's 16
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][2 * n], a.scale_log2e, -from));
+            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][2 * n + 1], a.scale_log2e, -from));
+            Parts<T>& to = w[kt][n >> 2];
+            if (n == 0) l[kt] = 0.0f;
+            if constexpr (kN == 1) {
+                const h2 h = __builtin_convertvector((f2){x, y}, h2);
+                to.p[0][n & 3] = __builtin_bit_cast(uint32_t, h);
+                l[kt] = __builtin_amdgcn_fdot2(h, (h2){1, 1}, l[kt], false);
+            } else {
+                uint32_t p0, p1, p2;
+                split2<true>(x, y, p0, p1, p2);
+                to.p[0][n & 3] = p0, to.p[1][n & 3] = p1, to.p[2][n & 3] = p2;
+                l[kt] += x + y;
+            }
+        };
+        // Products n of the block's (scores kKs, values 2 kDt) with a share of the eight pairs of weights of block `of` (-1: none)
+        // after each.
+        auto between = [&](int n, int all, int of) {
+            if (of >= 0) {
 #pragma unroll
-            for (int kt = 0; kt < kKt; ++kt)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, s[kt][i] * a.scale_log2e);
-            top = __builtin_fmaxf(top, other_half(top));
-            // only rows that ask for it (either half of one), so that no row depends on its neighbours
-            const bool asks = !(__builtin_fmaxf(l, other_half(l)) <= limit) || l != l || other_half(l) != other_half(l);
-            const float now = asks ? __builtin_fmaxf(base, top + lift) : base;
-            const float f = now == base ? 1.0f : __builtin_amdgcn_exp2f(base - now);
-            base = now;
-            sum *= f;
-#pragma unroll
-            for (int d = 0; d < kDt; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[d][i] *= f;
-            l = weights(base == -__builtin_inff() ? 0.0f : base);
-        }
-        sum += l;
-        __builtin_amdgcn_s_setprio(1);
-        {
-            constexpr int kOps = 2 * kKt * kDt;
+                for (int p = 0; p < 8; ++p)
+                    if (p * all / 8 == n) weights2(of, p, base);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto scores = [&](int kt, int of) {
             Parts<T> ring[kDeep];
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int r = 0; r < kDeep; ++r) ring[r] = value_op(buf, r / kDt, r % kDt);
+            for (int r = 0; r < kDeep; ++r) ring[r] = key_op(buf, kt, r);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[kt][i] = 0.0f;
+#pragma unroll
+            for (int r = 0; r < kKs; ++r) {
+                s[kt] = product<T>(ring[r % kDeep], q[r], s[kt]);
+                if (r + kDeep < kKs) ring[r % kDeep] = key_op(buf, kt, r + kDeep);
+                between(r, kKs, of);
+            }
+            __builtin_amdgcn_s_setprio(0);
+        };
+        auto values = [&](int kt, int of) {
+            constexpr int kOps = 2 * kDt;
+            Parts<T> ring[kDeep];
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int r = 0; r < kDeep; ++r) ring[r] = value_op(buf, 2 * kt + r / kDt, r % kDt);
 #pragma unroll
             for (int r = 0; r < kOps; ++r) {
-                o[r % kDt] = product<T>(ring[r % kDeep], w[r / kDt], o[r % kDt]);
-                if (r + kDeep < kOps) ring[r % kDeep] = value_op(buf, (r + kDeep) / kDt, (r + kDeep) % kDt);
-                __builtin_amdgcn_sched_barrier(0);
+                o[r % kDt] = product<T>(ring[r % kDeep], w[kt][r / kDt], o[r % kDt]);
+                if (r + kDeep < kOps) ring[r % kDeep] = value_op(buf, 2 * kt + (r + kDeep) / kDt, (r + kDeep) % kDt);
+                between(r, kOps, of);
             }
+            __builtin_amdgcn_s_setprio(0);
+        };
+        // a block's weights stand, or its rows get a new base
+        auto settle = [&](int kt) {
+            if (__any(!(l[kt] <= limit))) {
+                float top = -__builtin_inff();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, s[kt][i] * a.scale_log2e);
+                top = __builtin_fmaxf(top, other_half(top));
+                // only rows that ask for it (either half of one), so that no row depends on its neighbours
+                const float both = other_half(l[kt]);
+                const bool asks = !(l[kt] <= limit) || !(both <= limit);
+                const float now = asks ? __builtin_fmaxf(base, top + lift) : base;
+                const float f = now == base ? 1.0f : __builtin_amdgcn_exp2f(base - now);
+                base = now;
+                sum *= f;
+#pragma unroll
+                for (int d = 0; d < kDt; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[d][i] *= f;
+                const float from = base == -__builtin_inff() ? 0.0f : base;
+#pragma unroll
+                for (int n = 0; n < 8; ++n) weights2(kt, n, from);
+            }
+            sum += l[kt];
+        };
+        scores(0, -1);
+        mask(0);
+        if constexpr (kKt == 1) {
+            between(0, 1, 0);
+            settle(0);
+            values(0, -1);
+        } else {
+            static_assert(kKt <= 2, "a tile of one or two blocks");
+            scores(1, 0);
+            mask(1);
+            settle(0);
+            values(0, 1);
+            settle(1);
+            values(1, -1);
         }
-        __builtin_amdgcn_s_setprio(0);
+        if constexpr (kDirect) wait_loads();
         __syncthreads();
     }
 
@@ -426,7 +533,7 @@ __global__ __launch_bounds__(64 * kW, 2) void prompt_kernel(PromptArgs a) {
         // weights of hidden positions are 0, but 0 times a value that is not finite is NaN, and so are an infinity's products
         // with the parts of a weight: such values, in f16 of the tiles with hidden positions alone, went into the product as
         // zeros, and are added here to the rows that see them
-        for (int j = kN == 3 ? 0 : first_sees / kTile * kTile; j < vis; ++j) {
+        for (int j = max(tile0, kN == 3 ? 0 : first_sees / kTile) * kTile; j < min(vis, tiles * kTile); ++j) {
             const T* v = vp + (int64_t)(e.key0 + j) * a.ldv + 4 * half;
 #pragma unroll
             for (int d = 0; d < kDt; ++d)
@@ -438,6 +545,18 @@ __global__ __launch_bounds__(64 * kW, 2) void prompt_kernel(PromptArgs a) {
                         if (!(__builtin_fabsf((float)x[k]) < __builtin_inff())) o[d][4 * i + k] += (float)x[k];
                 }
         }
+    }
+    if (splits > 1) {  // as they are: the join divides
+        const size_t row = (((size_t)item * a.n_kv + kvh) * a.splits + split) * P::kRows + (r - r0);
+        if (half == 0) reinterpret_cast<float2*>(a.part_ml)[row] = make_float2(base, sum);
+        float* part = a.part_o + row * kHd + 4 * half;
+#pragma unroll
+        for (int d = 0; d < kDt; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<float4*>(part + 32 * d + 8 * i) =
+                    make_float4(o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]);
+        return;
     }
     const float inv = vis > 0 ? 1.0f / sum : 0.0f;
     T* out = static_cast<T*>(a.out) + (int64_t)(e.row0 + token) * a.ldo + (int64_t)head * kHd + 4 * half;
@@ -452,24 +571,108 @@ __global__ __launch_bounds__(64 * kW, 2) void prompt_kernel(PromptArgs a) {
         }
 }
 
+// Joins the parts of the row tiles that were shared out: hd / 4 threads to a row.
+template <typename T, int kHd, int kRows, int kTile>
+__global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a) {
+    constexpr int kThr = kHd / 4, kPer = 256 / kThr;
+    const int kvh = (int)(blockIdx.x % (unsigned)a.n_kv), item = (int)(blockIdx.x / (unsigned)a.n_kv);
+    Entry e;
+    int r0;
+    if (!entry_of(a, item, kRows, &e, &r0)) return;
+    const int rows = e.rows * a.group;
+    const int splits = splits_of(a, (e.visible(a, min(r0 + kRows, rows) - 1) + kTile - 1) / kTile, kTile);
+    const int r = r0 + (int)blockIdx.y * kPer + (int)threadIdx.x / kThr, d = 4 * ((int)threadIdx.x % kThr);
+    if (splits == 1 || r >= rows) return;
+    const size_t first = (((size_t)item * a.n_kv + kvh) * a.splits) * kRows + (r - r0);
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + first;
+    float top = -__builtin_inff();
+    for (int k = 0; k < splits; ++k) top = __builtin_fmaxf(top, ml[(size_t)k * kRows].x);
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    float sum = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) {
+        const float2 m = ml[(size_t)k * kRows];
+        const float4 v = *reinterpret_cast<const float4*>(a.part_o + (first + (size_t)k * kRows) * kHd + d);
+        const float f = __builtin_amdgcn_exp2f(m.x - base);
+        sum = __builtin_fmaf(f, m.y, sum);
+        o.x = __builtin_fmaf(f, v.x, o.x);
+        o.y = __builtin_fmaf(f, v.y, o.y);
+        o.z = __builtin_fmaf(f, v.z, o.z);
+        o.w = __builtin_fmaf(f, v.w, o.w);
+    }
+    const int token = (int)((unsigned)r / (unsigned)a.group), head = kvh * a.group + (r - token * a.group);
+    const float inv = e.visible(a, r) > 0 ? 1.0f / sum : 0.0f;
+    typedef T t4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    *reinterpret_cast<t4*>(static_cast<T*>(a.out) + (int64_t)(e.row0 + token) * a.ldo + (int64_t)head * kHd + d) =
+        (t4){(T)(o.x * inv), (T)(o.y * inv), (T)(o.z * inv), (T)(o.w * inv)};
+}
+
+// Calls f with the element type and, as constants, head_dim, keys of a tile and waves.
+template <typename F>
+void by_shape(int dtype, int hd, F&& f) {
+    using std::integral_constant;
+    typedef integral_constant<int, 32> K32;
+    typedef integral_constant<int, 64> K64;
+    typedef integral_constant<int, 128> K128;
+    typedef integral_constant<int, 4> W4;
+    typedef integral_constant<int, 8> W8;
+    if (dtype == QH_F16 && hd == 128) f((_Float16*)nullptr, K128{}, K64{}, W4{});
+    else if (dtype == QH_F16) f((_Float16*)nullptr, K64{}, K64{}, W4{});
+    else if (hd == 128) f((float*)nullptr, K128{}, K32{}, W8{});
+    else f((float*)nullptr, K64{}, K32{}, W4{});
+}
+
+// Row tiles of a call, and how many workgroups may share one: two workgroups to a compute unit where the row tiles are fewer,
+// as many as the entries' keys are likely to fill.
+struct Plan {
+    int items, splits;
+};
+Plan plan_of(int rows, int group, int n_kv, int n, int n_tok, int n_keys) {
+    Plan p;
+    p.items = (int)((int64_t)n_tok * group / rows) + n;
+    const int64_t wgs = ((int64_t)n_tok * group + rows - 1) / rows * n_kv, want = 2 * device_cus();
+    const int64_t most = n_keys / n / kSplitKeys;
+    int64_t s = want / (wgs > 0 ? wgs : 1);
+    s = s < most ? s : most;
+    p.splits = (int)(s < 1 ? 1 : s < kMaxSplits ? s : kMaxSplits);
+    return p;
+}
+
 }  // namespace
 
-size_t prompt_workspace_bytes(int, int, int, int, int, int, int) { return 0; }
+size_t prompt_workspace_bytes(int dtype, int n_heads, int n_kv, int hd, int n, int n_tok, int n_keys) {
+    size_t bytes = 0;
+    by_shape(dtype, hd, [&](auto*, auto, auto, auto waves) {
+        constexpr int kRows = 32 * decltype(waves)::value;
+        const Plan p = plan_of(kRows, n_heads / n_kv, n_kv, n, n_tok, n_keys);
+        if (p.splits > 1) bytes = (size_t)p.items * n_kv * p.splits * kRows * (hd + 2) * sizeof(float);
+    });
+    return bytes;
+}
 
-hipError_t launch_prompt(PromptArgs a, int dtype, int hd, void*, hipStream_t s) {
-    auto go = [&](auto* type, auto head, auto tile, auto waves) {
+hipError_t launch_prompt(PromptArgs a, int dtype, int hd, void* ws, hipStream_t s) {
+    hipError_t rc = hipSuccess;
+    by_shape(dtype, hd, [&](auto* type, auto head, auto tile, auto waves) {
         using T = std::remove_pointer_t<decltype(type)>;
-        typedef Prompt<T, decltype(head)::value, decltype(tile)::value, decltype(waves)::value> P;
-        a.items = (int)((int64_t)a.n_tok * a.group / P::kRows) + a.n;
-        qh_launch((prompt_kernel<T, decltype(head)::value, decltype(tile)::value, decltype(waves)::value>),
-                  dim3((unsigned)a.items * (unsigned)a.n_kv), dim3(P::kThreads), 0, s, a);
-    };
-    using std::integral_constant;
-    if (dtype == QH_F16 && hd == 128) go((_Float16*)nullptr, integral_constant<int, 128>{}, integral_constant<int, 64>{}, integral_constant<int, 4>{});
-    else if (dtype == QH_F16) go((_Float16*)nullptr, integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 4>{});
-    else if (hd == 128) go((float*)nullptr, integral_constant<int, 128>{}, integral_constant<int, 32>{}, integral_constant<int, 8>{});
-    else go((float*)nullptr, integral_constant<int, 64>{}, integral_constant<int, 32>{}, integral_constant<int, 4>{});
-    return hipGetLastError();
+        constexpr int kHd = decltype(head)::value, kTile = decltype(tile)::value, kW = decltype(waves)::value, kRows = 32 * kW;
+        const Plan p = plan_of(kRows, a.group, a.n_kv, a.n, a.n_tok, a.n_keys);
+        a.items = p.items, a.splits = p.splits;
+        a.part_o = static_cast<float*>(ws);
+        a.part_ml = a.part_o + (size_t)p.items * a.n_kv * p.splits * kRows * hd;
+        const unsigned wgs = (unsigned)p.items * (unsigned)a.n_kv;
+        const dim3 grid(wgs, (unsigned)p.splits);
+        bool direct = false;
+        if constexpr (std::is_same<T, _Float16>::value) {
+            direct = ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) & 15) == 0 && a.ldk % 8 == 0 && a.ldv % 8 == 0;
+            if (direct) qh_launch((prompt_kernel<T, kHd, kTile, kW, true>), grid, dim3(64 * kW), 0, s, a);
+        }
+        if (!direct) qh_launch((prompt_kernel<T, kHd, kTile, kW, false>), grid, dim3(64 * kW), 0, s, a);
+        if ((rc = hipGetLastError()) != hipSuccess || p.splits == 1) return;
+        qh_launch((prompt_join_kernel<T, kHd, kRows, kTile>), dim3(wgs, (unsigned)(kRows * kHd / 1024)), dim3(256), 0, s, a);
+        rc = hipGetLastError();
+    });
+    return rc;
 }
 
 }  // namespace qh
