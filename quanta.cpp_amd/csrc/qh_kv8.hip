@@ -649,6 +649,7 @@ __device__ __forceinline__ void replace_page(const Kv8View& c, int d, int j, int
     int32_t* slot = c.table + (size_t)d * c.seq_pages + j;
     if (j < pages_of(c, before)) {
         const int old = *slot;
+        if (old == page && j < pages_of(c, after)) return;  // beams of one prompt have most of their pages in common
         if (old >= 0 && old < c.n_pages) atomicSub(&c.refs[old], 1);
         if (j >= pages_of(c, after)) *slot = -1;
     }

@@ -608,18 +608,25 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a) {
         (t4){(T)(o.x * inv), (T)(o.y * inv), (T)(o.z * inv), (T)(o.w * inv)};
 }
 
-// Calls f with the element type and, as constants, head_dim, keys of a tile and waves.
+// Calls f with the element type and, as constants, head_dim, keys of a tile and waves: eight where that leaves a row tile to
+// every compute unit, else four (12,001 tokens of 32 heads of 128 over 8, f16: 1,192 us, with four 1,232; 8,000 of 14 heads of
+// 64 over 2 153.6 and 158.6; f32, 300 tokens of 32 heads of 128 over 8: 50 and, with four, 34). f32 heads of 64 stay with four,
+// whose workgroups do not wait for each other (16 prompts of up to 2,000 tokens: 322 us, eight waves over 64 keys 340).
 template <typename F>
-void by_shape(int dtype, int hd, F&& f) {
+void by_shape(int dtype, int hd, int group, int n_kv, int n_tok, F&& f) {
     using std::integral_constant;
     typedef integral_constant<int, 32> K32;
     typedef integral_constant<int, 64> K64;
     typedef integral_constant<int, 128> K128;
     typedef integral_constant<int, 4> W4;
     typedef integral_constant<int, 8> W8;
-    if (dtype == QH_F16 && hd == 128) f((_Float16*)nullptr, K128{}, K64{}, W4{});
+    const bool many = (int64_t)n_tok * group / 256 * n_kv >= device_cus();
+    if (dtype == QH_F16 && hd == 128 && many) f((_Float16*)nullptr, K128{}, K64{}, W8{});
+    else if (dtype == QH_F16 && hd == 128) f((_Float16*)nullptr, K128{}, K64{}, W4{});
+    else if (dtype == QH_F16 && many) f((_Float16*)nullptr, K64{}, K64{}, W8{});
     else if (dtype == QH_F16) f((_Float16*)nullptr, K64{}, K64{}, W4{});
-    else if (hd == 128) f((float*)nullptr, K128{}, K32{}, W8{});
+    else if (hd == 128 && many) f((float*)nullptr, K128{}, K32{}, W8{});
+    else if (hd == 128) f((float*)nullptr, K128{}, K32{}, W4{});
     else f((float*)nullptr, K64{}, K32{}, W4{});
 }
 
@@ -643,7 +650,7 @@ Plan plan_of(int rows, int group, int n_kv, int n, int n_tok, int n_keys) {
 
 size_t prompt_workspace_bytes(int dtype, int n_heads, int n_kv, int hd, int n, int n_tok, int n_keys) {
     size_t bytes = 0;
-    by_shape(dtype, hd, [&](auto*, auto, auto, auto waves) {
+    by_shape(dtype, hd, n_heads / n_kv, n_kv, n_tok, [&](auto*, auto, auto, auto waves) {
         constexpr int kRows = 32 * decltype(waves)::value;
         const Plan p = plan_of(kRows, n_heads / n_kv, n_kv, n, n_tok, n_keys);
         if (p.splits > 1) bytes = (size_t)p.items * n_kv * p.splits * kRows * (hd + 2) * sizeof(float);
@@ -653,7 +660,7 @@ size_t prompt_workspace_bytes(int dtype, int n_heads, int n_kv, int hd, int n, i
 
 hipError_t launch_prompt(PromptArgs a, int dtype, int hd, void* ws, hipStream_t s) {
     hipError_t rc = hipSuccess;
-    by_shape(dtype, hd, [&](auto* type, auto head, auto tile, auto waves) {
+    by_shape(dtype, hd, a.group, a.n_kv, a.n_tok, [&](auto* type, auto head, auto tile, auto waves) {
         using T = std::remove_pointer_t<decltype(type)>;
         constexpr int kHd = decltype(head)::value, kTile = decltype(tile)::value, kW = decltype(waves)::value, kRows = 32 * kW;
         const Plan p = plan_of(kRows, a.group, a.n_kv, a.n, a.n_tok, a.n_keys);

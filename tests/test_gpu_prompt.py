@@ -129,6 +129,25 @@ def test_long(qh, gpu, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("off", [0, 1])
+def test_many_rows(qh, gpu, dtype, hd, off):
+    """Calls whose row tiles are as many as the compute units, which workgroups of eight waves take: ragged lengths, values that
+    are not finite behind rows and between entries, and rows that begin anywhere (keys on multiples of 16 bytes go another way)."""
+    t, heads = TYPES[dtype], 16
+    st = [0, 700, 700, 763, 2900, 4300]
+    gen = torch.Generator(device=gpu).manual_seed(hd + off)
+    buf = torch.randn(4300 * 3 * heads * hd + off, generator=gen, device=gpu).to(t)
+    row = buf[off:].view(4300, 3, heads, hd)
+    q, k, v = row[:, 0], row[:, 1], row[:, 2]
+    v[699, 3, 5], v[1500, 2, hd - 1], v[2899, 0, 0] = math.nan, math.inf, -math.inf
+    assert 4300 // 256 * heads >= 256
+    check(qh.attention(q, k, v, ints(st, gpu)), *formula(q, k, v, st, st, True, hd ** -0.5))
+    v[1500, 2, hd - 1] = 0.5
+    check(qh.attention(q, k, v, ints(st, gpu), causal=False), *formula(q, k, v, st, st, False, hd ** -0.5))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("scale", [0.0, -0.2, 1.0, 1e-8, -1e-30])
 def test_scales(qh, gpu, dtype, scale):
     case(qh, gpu, dtype, 4, 2, 64, [50, 129], scale=scale)
