@@ -436,8 +436,8 @@ typedef struct qh_rope_desc {
  * Host only. Another schedule is as good: qh_rope takes any table. */
 int qh_rope_turns(const qh_rope_desc* r, double* turns_host);
 
-/* The rows' side of qh_rope: n_heads heads of head_dim one after the other, rows ld (out: ldo) elements apart. out may be x
- * (then ldo is ld); they do not overlap otherwise. */
+/* The rows' side of qh_rope: n_heads heads of head_dim one after the other (q's and k's at most 4,096 together), rows ld (out:
+ * ldo) elements apart. out may be x (then ldo is ld); they do not overlap otherwise. */
 typedef struct qh_rope_rows {
     const void* x;
     void* out;

@@ -562,6 +562,7 @@ int qh_rmsnorm(const void* x, const void* res, const float* w, int dtype, int64_
     const char* who = "qh_rmsnorm";
     if (int rc = validate_row_type(dtype, n_tok, who)) return rc;
     if (n <= 0 || n > QH_NORM_MAX) return fail(QH_ERR_SHAPE, "%s: rows of %d, at most %d", who, n, QH_NORM_MAX);
+    if (n > 8192 && n_tok >= 1 << 22) return fail(QH_ERR_SHAPE, "%s: %d rows of %d", who, n_tok, n);  // of 1,024 threads each
     if (!(eps >= 0.0 && eps <= 1e38)) return fail(QH_ERR_ARG, "%s: eps is negative or not finite", who);
     if (q && n % QH_QK != 0) return fail(QH_ERR_SHAPE, "%s: 8-bit blocks of rows of %d (not a multiple of 32)", who, n);
     if (n_tok == 0) return QH_OK;
@@ -632,6 +633,8 @@ int qh_rope(const double* turns, int rot_dim, int interleaved, float magnitude, 
         if (r->x == r->out && n_tok > 1 && r->ld != r->ldo)
             return fail(QH_ERR_ARG, "%s: in place with another row stride", who);
     }
+    if (k && q->n_heads + k->n_heads > 4096)
+        return fail(QH_ERR_SHAPE, "%s: %d heads and %d", who, q->n_heads, k->n_heads);
     if (n_tok == 0) return QH_OK;
     if (k && (q->out == k->out || q->out == k->x || k->out == q->x)) return fail(QH_ERR_ARG, "%s: q's rows are k's", who);
     if (!pos || (reinterpret_cast<uintptr_t>(pos) & 3u) != 0) return fail(QH_ERR_ARG, "%s: no positions", who);

@@ -638,7 +638,7 @@ struct Plan {
 Plan plan_of(int rows, int group, int n_kv, int n, int n_tok, int n_keys) {
     Plan p;
     p.items = (int)((int64_t)n_tok * group / rows) + n;
-    const int64_t wgs = ((int64_t)n_tok * group + rows - 1) / rows * n_kv, want = 2 * device_cus();
+    const int64_t tiles = ((int64_t)n_tok * group + rows - 1) / rows, wgs = (tiles > n ? tiles : n) * n_kv, want = 2 * device_cus();
     const int64_t most = n_keys / n / kSplitKeys;
     int64_t s = want / (wgs > 0 ? wgs : 1);
     s = s < most ? s : most;

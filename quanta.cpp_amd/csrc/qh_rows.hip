@@ -257,13 +257,17 @@ hipError_t rope_of(const RopeArgs& a, bool interleaved, hipStream_t s) {
     const int half = a.rot / 2, units = (half + E - 1) / E, heads = a.q.heads + a.k.heads;
     const bool copies = a.q.x != a.q.out || (a.k.heads > 0 && a.k.x != a.k.out);
     const int rest = copies ? (a.hd - a.rot + E - 1) / E : 0;
-    int per = a.n_tok / 2048;
-    per = per < 1 ? 1 : per < kRopePairs / half ? per : kRopePairs / half;
+    int64_t per = a.n_tok / 2048, items = (int64_t)heads * (units + rest);
+    per = per < kRopePairs / half ? per : kRopePairs / half;
+    // items of a workgroup times what they are divided by stay in 32 bits (at one token: 4,096 heads in all of 65 items)
+    const int64_t most = ((int64_t)1 << 31) / (items * (heads > units + rest ? heads : units + rest));
+    per = per < most ? per : most;
+    per = per < 1 ? 1 : per;
     const dim3 grid((unsigned)((a.n_tok + per - 1) / per));
     const uint32_t um = magic_of(units + rest), hm = magic_of(heads);
     const bool whole = half % E == 0 && (rest == 0 || (a.hd - a.rot) % E == 0);
     auto go = [&](auto inter, auto all) {
-        qh_launch((rope_kernel<T, decltype(inter)::value, decltype(all)::value>), grid, dim3(kRopeThreads), 0, s, a, per, units,
+        qh_launch((rope_kernel<T, decltype(inter)::value, decltype(all)::value>), grid, dim3(kRopeThreads), 0, s, a, (int)per, units,
                   rest, um, hm);
     };
     if (interleaved && whole) go(std::true_type{}, std::true_type{});

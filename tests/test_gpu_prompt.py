@@ -105,7 +105,7 @@ def test_layouts(qh, gpu, dtype, heads, kv, hd):
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("rows", [[1], [2], [31], [32], [33], [63], [64], [65], [127], [128], [129], [500], [1025], [1] * 50, [0, 0, 5, 0],
-                                  [3, 64, 1, 129, 32, 7]])
+                                  [3, 64, 1, 129, 32, 7], [2] * 63, [3] * 64, [5, 0, 1, 33] * 40])
 def test_lengths(qh, gpu, dtype, hd, rows):
     case(qh, gpu, dtype, 4, 2, hd, rows, seed=len(rows) + rows[-1])
 
@@ -115,7 +115,7 @@ def test_lengths(qh, gpu, dtype, hd, rows):
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("rows,keys", [([1], [1]), ([1], [1000]), ([5, 40], [70, 40]), ([64, 3], [65, 300]), ([130], [2000]),
                                        ([20, 7], [5, 0]), ([200], [3]), ([1, 1, 1], [17, 64, 129]), ([33, 0, 9], [31, 64, 900]),
-                                       ([1] * 9, [333] * 9)])
+                                       ([1] * 9, [333] * 9), ([3, 0, 2] * 30, [5, 70, 1] * 30)])
 def test_keys_of_their_own(qh, gpu, dtype, hd, causal, rows, keys):
     """New rows behind kept ones, other states' keys, and more rows than keys: the first of them see nothing then."""
     case(qh, gpu, dtype, 6, 2, hd, rows, keys, causal, seed=sum(keys))

@@ -233,6 +233,20 @@ def test_rope_rows(qh, gpu, rows):
     check_rope(rope(q, pos=pos), q, pos, rope.turns, 64, False)
 
 
+def test_rope_most_heads(qh, gpu):
+    """4,096 heads, nearly all of each a copy: the most items that a token can have."""
+    q, k = torch.randn(2, 4000, 256, device=gpu), torch.randn(2, 96, 256, device=gpu)
+    rope = qh.Rope(256, rot_dim=2, device=gpu)
+    pos = ints_of([5, -7], gpu)
+    q2, k2 = rope(q, k, pos=pos)
+    check_rope(q2, q, pos, rope.turns, 2, False)
+    check_rope(k2, k, pos, rope.turns, 2, False)
+
+
+def ints_of(values, dev):
+    return torch.tensor(values, dtype=torch.int32, device=dev)
+
+
 def test_rope_of_no_rows(qh, gpu):
     rope = qh.Rope(64, device=gpu)
     q = torch.empty(0, 4, 64, device=gpu)

@@ -16,7 +16,7 @@ def norm(qh, x=P, res=A, w=P, dtype=0, ldx=64, ldr=64, n_tok=3, n=64, eps=1e-6, 
 
 @pytest.mark.parametrize("change,code", [
     ({"x": None}, 1), ({"w": None}, 1), ({"dtype": 2}, 2), ({"dtype": -1}, 2), ({"n_tok": -1}, 3), ({"n_tok": 1 << 24}, 3),
-    ({"n": 0}, 3), ({"n": 32769}, 3), ({"n": 48, "ldx": 48}, 3), ({"eps": -1.0}, 1), ({"eps": math.nan}, 1),
+    ({"n_tok": 1 << 22, "n": 8224, "ldx": 8224, "ldr": 8224, "lds": 8224}, 3), ({"n": 0}, 3), ({"n": 32769}, 3), ({"n": 48, "ldx": 48}, 3), ({"eps": -1.0}, 1), ({"eps": math.nan}, 1),
     ({"eps": math.inf}, 1), ({"q": None}, 1), ({"d": None}, 1), ({"q": None, "d": None}, 1), ({"ldx": 63}, 1), ({"ldr": 63}, 1),
     ({"lds": 63}, 1), ({"y": E, "ldy": 63}, 1), ({"x": C.c_void_p(4098)}, 4), ({"dtype": 1, "x": C.c_void_p(4097)}, 4),
     ({"q": C.c_void_p(8200)}, 4), ({"d": C.c_void_p(8194)}, 4), ({"w": C.c_void_p(4098)}, 4), ({"y": P}, 1), ({"y": A}, 1),
@@ -66,6 +66,7 @@ def test_rope_of_shared_rows_and_no_rows(qh):
     assert rope(qh, q=a, k=rows(qh, x=1 << 20)) == 1          # both results in one place
     assert rope(qh, q=a, k=rows(qh, x=1 << 20, out=4096)) == 1  # k's result over q
     assert rope(qh, q=a, k=rows(qh, x=8192, out=1 << 20)) == 1  # q's result over k
+    assert rope(qh, q=rows(qh, heads=2049, ld=1 << 18, ldo=1 << 18), k=rows(qh, x=1 << 20, out=1 << 21, heads=2048, ld=1 << 18, ldo=1 << 18)) == 3
     assert rope(qh, n_tok=0) == 0
     assert qh.lib().qh_rope(P, 64, 0, 1.0, 64, None, None, 0, P, 3, None) == 1
 
