@@ -407,8 +407,8 @@ int qh_kv8_attention_plan(const qh_kv8_cache* c, int n_heads, int n, int n_tok, 
  * y, rows of dtype, and / or q [n_tok][n] with d [n_tok][n / 32], the blocks that qh_quantize_q8 makes of the result in f32
  * (n a multiple of 32 then). w is f32 [n]. Squares are summed in 64 bits and the result is rounded once. Rows are ld elements
  * apart, on any alignment of their type (q: 16 bytes). sum may be x or res, with its row stride; the outputs overlap nothing
- * else. n at most QH_NORM_MAX. A NaN makes its row NaN; an infinity makes its own place NaN and the rest of the row 0 (in
- * blocks: as qh_quantize_q8 takes those).
+ * else. n at most QH_NORM_MAX; n_tok below 2^24, of rows of more than 2,048 below 2^23, of more than 8,192 below 2^22. A NaN
+ * makes its row NaN; an infinity makes its own place NaN and the rest of the row 0 (in blocks: as qh_quantize_q8 takes those).
  * No counterpart among the reference's kernels by itself: its rmsnorm (ops_ref.cpp:194-199) sums in f32 in order, which the
  * decoder's own kernels keep to the bit. */
 #define QH_NORM_MAX 32768
@@ -464,8 +464,9 @@ int qh_rope(const double* turns, int rot_dim, int interleaved, float magnitude, 
  * of dtype QH_F32 or QH_F16, ld elements apart on any alignment of their type, a row's heads contiguous. A row that sees
  * nothing is 0; rows outside the entries are neither read nor written. Keys and values that a row does not see have no part in
  * it, whatever they hold. A NaN or an infinity that it sees stays in its dim where it is a value's, and makes the row NaN
- * where it is the query's; of a key's it becomes NaN, or what the formula gives. f16: weights are rounded to f16 once. f32: products keep 22 bits and more of every value, whatever the others are. Sums in f32. out overlaps no input. The
- * workspace is 16-byte aligned and needs no initialisation (NULL where the size is 0); calls that overlap must not share one.
+ * where it is the query's; of a key's it becomes NaN, or what the formula gives. f16: weights are rounded to f16 once. f32:
+ * products keep 22 bits and more of every value, whatever the others are. Sums in f32. out overlaps no input. The workspace is
+ * 16-byte aligned and needs no initialisation (NULL where the size is 0); calls that overlap must not share one.
  * No counterpart in the reference, whose prompts attend to its cache in chunks (Model::forward_batch, model.cpp:387-405). */
 size_t qh_attention_workspace_bytes(int dtype, int n_heads, int n_kv_heads, int head_dim, int n, int n_tok, int n_keys);
 int qh_attention(const void* q, const void* k, const void* v, void* out, int dtype, int n_heads, int n_kv_heads,
@@ -481,8 +482,8 @@ int qh_attention(const void* q, const void* k, const void* v, void* out, int dty
  * logit of -infinity is no candidate, and neither is any of a row whose score is not finite or whose logits hold a NaN or
  * +infinity or are all -infinity (a beam that ended gets the score -infinity); where there are fewer than k, the places
  * behind them have parent and token -1 and the score -infinity (which is also what a score past f32's range rounds to). beams
- * at most QH_BEAM_MAX_BEAMS, k at most QH_BEAM_MAX_K, n_valid at most QH_SAMPLE_MAX_VOCAB. The workspace is 16-byte aligned
- * and needs no initialisation; calls that overlap must not share one.
+ * at most QH_BEAM_MAX_BEAMS, fewer than 2^17 rows, k at most QH_BEAM_MAX_K, n_valid at most QH_SAMPLE_MAX_VOCAB. The workspace
+ * is 16-byte aligned and needs no initialisation; calls that overlap must not share one.
  * No counterpart in the reference, which samples one sequence (Sampler::sample, sampler.cpp:22-85). */
 #define QH_BEAM_MAX_BEAMS 256
 #define QH_BEAM_MAX_K 256

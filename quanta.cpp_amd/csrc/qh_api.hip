@@ -562,7 +562,9 @@ int qh_rmsnorm(const void* x, const void* res, const float* w, int dtype, int64_
     const char* who = "qh_rmsnorm";
     if (int rc = validate_row_type(dtype, n_tok, who)) return rc;
     if (n <= 0 || n > QH_NORM_MAX) return fail(QH_ERR_SHAPE, "%s: rows of %d, at most %d", who, n, QH_NORM_MAX);
-    if (n > 8192 && n_tok >= 1 << 22) return fail(QH_ERR_SHAPE, "%s: %d rows of %d", who, n_tok, n);  // of 1,024 threads each
+    // a launch has fewer than 2^32 threads, up to 512 of them to a row of more than 2,048 and 1,024 to one of more than 8,192
+    if ((n > 2048 && n_tok >= 1 << 23) || (n > 8192 && n_tok >= 1 << 22))
+        return fail(QH_ERR_SHAPE, "%s: %d rows of %d", who, n_tok, n);
     if (!(eps >= 0.0 && eps <= 1e38)) return fail(QH_ERR_ARG, "%s: eps is negative or not finite", who);
     if (q && n % QH_QK != 0) return fail(QH_ERR_SHAPE, "%s: 8-bit blocks of rows of %d (not a multiple of 32)", who, n);
     if (n_tok == 0) return QH_OK;
@@ -699,11 +701,11 @@ int qh_attention(const void* q, const void* k, const void* v, void* out, int dty
 }
 
 namespace {
-// The shape of a beam selection; up to 2^17 rows, so that its work items are told apart in 32 bits.
+// The shape of a beam selection; fewer than 2^17 rows, of up to 128 workgroups each, so that a launch can tell them apart.
 int validate_beams(int dtype, int n_prompts, int beams, int n_valid, const char* who) {
     if (dtype != QH_F32 && dtype != QH_F16) return fail(QH_ERR_DTYPE, "%s: dtype %d is not f32 (0) or f16 (1)", who, dtype);
     if (beams < 1 || beams > QH_BEAM_MAX_BEAMS || n_valid < 1 || n_valid > QH_SAMPLE_MAX_VOCAB || n_prompts < 0 ||
-        (int64_t)n_prompts * beams > 1 << 17)
+        (int64_t)n_prompts * beams >= 1 << 17)
         return fail(QH_ERR_SHAPE, "%s: %d prompts of %d beams over %d ids", who, n_prompts, beams, n_valid);
     return QH_OK;
 }

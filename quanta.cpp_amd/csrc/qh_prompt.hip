@@ -28,7 +28,6 @@ constexpr int kSplitKeys = 128;  // keys of a split, at least
 constexpr int kMaxSplits = 64;
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
@@ -217,6 +216,7 @@ struct Prompt {
     static constexpr int kRows = 32 * kW, kThreads = 64 * kW, kChunks = kHd / 8;
     static constexpr int kPer = kTile * kChunks / kThreads;  // chunks of keys, and of values, that a thread stages
     static constexpr int kKt = kTile / 32, kDt = kHd / 32, kKs = kHd / 16;
+    static constexpr int kSimdWaves = kThreads / 256 * (160 * 1024 / (2 * kBuffer)) < 2 ? 1 : 2;  // by shared memory, or registers
     static_assert(kPer >= 1 && kTile * kChunks % kThreads == 0, "whole chunks to a thread");
 };
 
@@ -229,7 +229,7 @@ __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)"
 
 // kDirect: f16 keys and values on multiples of 16 bytes, which go into shared memory as they are, past the registers.
 template <typename T, int kHd, int kTile, int kW, bool kDirect>
-__global__ __launch_bounds__(64 * kW, 2) void prompt_kernel(PromptArgs a) {
+__global__ __launch_bounds__(64 * kW, (Prompt<T, kHd, kTile, kW>::kSimdWaves)) void prompt_kernel(PromptArgs a) {
     typedef Prompt<T, kHd, kTile, kW> P;
     constexpr int kN = P::kN, kKt = P::kKt, kDt = P::kDt, kKs = P::kKs, kDeep = kN == 1 ? 4 : kHd == 64 ? 2 : 1;
     __shared__ __align__(16) uint8_t lds[2 * P::kBuffer];

@@ -145,11 +145,14 @@ hipError_t rmsnorm_of(const NormArgs& a, hipStream_t s) {
                   dim3(kWaves < 4 ? 256 : 64 * kWaves), 0, s, a);
     };
     using std::integral_constant;
+    // Loads in flight for waves enough, and one row's lanes not far apart (16,000 x 4,096 f16: 98.5 us, a wave to a row with 8
+    // vectors 162, eight with one 104; 16,000 x 256 f32 with a wave 27.9, with four 33.5; 16,000 x 8,192 f16 197.7, four waves with
+    // four vectors 201.5; 64 x 8,192 f32 5.7 with eight waves, four 6.7; 2,000 x 16,384 f32 176, four waves with 16 vectors 183)
     if (vecs <= 64) run(integral_constant<int, 1>{}, integral_constant<int, 1>{});
     else if (vecs <= 256) run(integral_constant<int, 4>{}, integral_constant<int, 1>{});
     else if (vecs <= 512) run(integral_constant<int, 4>{}, integral_constant<int, 2>{});
-    else if (vecs <= 1024) run(integral_constant<int, 4>{}, integral_constant<int, 4>{});
-    else if (vecs <= 2048) run(integral_constant<int, 4>{}, integral_constant<int, 8>{});
+    else if (vecs <= 1024) run(integral_constant<int, 8>{}, integral_constant<int, 2>{});
+    else if (vecs <= 2048) run(integral_constant<int, 8>{}, integral_constant<int, 4>{});
     else if (vecs <= 4096) run(integral_constant<int, 16>{}, integral_constant<int, 4>{});  // f16: kMaxNorm elements
     else if constexpr (kE<T> == 4) run(integral_constant<int, 16>{}, integral_constant<int, 8>{});
     return hipGetLastError();
@@ -257,7 +260,11 @@ hipError_t rope_of(const RopeArgs& a, bool interleaved, hipStream_t s) {
     const int half = a.rot / 2, units = (half + E - 1) / E, heads = a.q.heads + a.k.heads;
     const bool copies = a.q.x != a.q.out || (a.k.heads > 0 && a.k.x != a.k.out);
     const int rest = copies ? (a.hd - a.rot + E - 1) / E : 0;
-    int64_t per = a.n_tok / 2048, items = (int64_t)heads * (units + rest);
+    // 8,192 workgroups, fewer where a token would leave threads of one without an item and 2,048 are left (8,000 tokens of 40
+    // heads of 128 f16: 28.3 us, by 2,048 workgroups 29.4; 4,096 of 16 heads of 64 f32: 6.8, a token to a workgroup 7.5)
+    const int64_t items = (int64_t)heads * (units + rest), fill = kRopeThreads / items, few = a.n_tok / 2048;
+    int64_t per = a.n_tok / 8192;
+    per = per > (fill < few ? fill : few) ? per : (fill < few ? fill : few);
     per = per < kRopePairs / half ? per : kRopePairs / half;
     // items of a workgroup times what they are divided by stay in 32 bits (at one token: 4,096 heads in all of 65 items)
     const int64_t most = ((int64_t)1 << 31) / (items * (heads > units + rest ? heads : units + rest));

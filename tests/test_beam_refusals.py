@@ -17,7 +17,7 @@ def select(qh, logits=P, dtype=0, ld=1000, scores=A, prompts=2, beams=3, n_valid
 
 @pytest.mark.parametrize("change,code", [
     ({"logits": None}, 1), ({"dtype": 2}, 2), ({"ld": 999}, 1), ({"prompts": -1}, 3), ({"beams": 0}, 3), ({"beams": 257}, 3),
-    ({"n_valid": 0}, 3), ({"n_valid": 262145, "ld": 262145}, 3), ({"prompts": 1 << 16}, 3), ({"prompts": 1 << 30}, 3), ({"k": 0}, 7),
+    ({"n_valid": 0}, 3), ({"n_valid": 262145, "ld": 262145}, 3), ({"prompts": 1 << 16}, 3), ({"prompts": 1 << 17, "beams": 1}, 3), ({"prompts": 1 << 30}, 3), ({"k": 0}, 7),
     ({"k": 257}, 7), ({"parent": None}, 1), ({"token": None}, 1), ({"score": None}, 1), ({"score": A}, 1), ({"ws": None}, 6),
     ({"ws_bytes": 0}, 6), ({"ws": C.c_void_p(65544)}, 4), ({"logits": C.c_void_p(4098)}, 4), ({"scores": C.c_void_p(8194)}, 4),
     ({"dtype": 1, "logits": C.c_void_p(4097)}, 4), ({"token": C.c_void_p(32770)}, 4),

@@ -16,6 +16,7 @@ def norm(qh, x=P, res=A, w=P, dtype=0, ldx=64, ldr=64, n_tok=3, n=64, eps=1e-6, 
 
 @pytest.mark.parametrize("change,code", [
     ({"x": None}, 1), ({"w": None}, 1), ({"dtype": 2}, 2), ({"dtype": -1}, 2), ({"n_tok": -1}, 3), ({"n_tok": 1 << 24}, 3),
+    ({"n_tok": 1 << 23, "n": 2080, "ldx": 2080, "ldr": 2080, "lds": 2080}, 3),
     ({"n_tok": 1 << 22, "n": 8224, "ldx": 8224, "ldr": 8224, "lds": 8224}, 3), ({"n": 0}, 3), ({"n": 32769}, 3), ({"n": 48, "ldx": 48}, 3), ({"eps": -1.0}, 1), ({"eps": math.nan}, 1),
     ({"eps": math.inf}, 1), ({"q": None}, 1), ({"d": None}, 1), ({"q": None, "d": None}, 1), ({"ldx": 63}, 1), ({"ldr": 63}, 1),
     ({"lds": 63}, 1), ({"y": E, "ldy": 63}, 1), ({"x": C.c_void_p(4098)}, 4), ({"dtype": 1, "x": C.c_void_p(4097)}, 4),
