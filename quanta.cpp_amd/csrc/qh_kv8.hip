@@ -486,9 +486,18 @@ __global__ __launch_bounds__(kWg) void kv8_resize_kernel(Kv8View c, const int32_
         if (tid == 0) atomicOr(c.status, QH_KV8_BAD_LIST);
         return;
     }
-    for (int i = tid >> 6; i < n; i += kWg / 64) {
-        const int s = seqs[i], before = pages_of(c, kv8_len(c, s)), after = pages_of(c, want[i]);
-        drop_pages(c, s, after, before);
+    // a lane to a sequence for its lengths, then its wave for the pages of each that gets shorter
+    for (int base = 0; base < n; base += kWg) {
+        const int i = base + (tid & 63) * (kWg / 64) + (tid >> 6);
+        int s = 0, before = 0, after = 0;
+        if (i < n) {
+            s = seqs[i];
+            before = pages_of(c, kv8_len(c, s)), after = pages_of(c, want[i]);
+        }
+        for (uint64_t m = __ballot(after < before); m; m &= m - 1) {
+            const int l = __builtin_ctzll(m);
+            drop_pages(c, __builtin_amdgcn_readlane(s, l), __builtin_amdgcn_readlane(after, l), __builtin_amdgcn_readlane(before, l));
+        }
     }
     __syncthreads();
     int need_all = 0;
