@@ -831,16 +831,15 @@ def beam_select(logits, scores, beams: int, k: int, n_valid: int | None = None):
     need = L.qh_beam_workspace_bytes(dtype, prompts, beams, n_valid)
     # the results and the workspace in one tensor, a new one for each call: nothing of one call (or captured graph) is shared
     # with the next
-    each = (prompts * k + 3) // 4 * 4
+    each, shape, strides = (prompts * k + 3) // 4 * 4, (prompts, k), (k, 1)
     held = torch.empty(3 * each + (need + 3) // 4, dtype=torch.int32, device=dev)
-    parent, token, score, ws = held.split_with_sizes((each, each, each, held.shape[0] - 3 * each))
+    at = held.data_ptr()
     rc = L.qh_beam_select(logits.data_ptr(), dtype, ld, None if scores is None else scores.data_ptr(), prompts, beams, n_valid,
-                          k, parent.data_ptr(), token.data_ptr(), score.data_ptr(), ws.data_ptr(), need, stream)
+                          k, at, at + 4 * each, at + 8 * each, at + 12 * each, need, stream)
     if rc:
         _check(rc)
-    shape = (prompts, k)
-    return (parent[:prompts * k].view(shape), token[:prompts * k].view(shape),
-            score[:prompts * k].view(torch.float32).view(shape))
+    return (held.as_strided(shape, strides), held.as_strided(shape, strides, each),
+            held.view(torch.float32).as_strided(shape, strides, 2 * each))
 
 
 # ------------------------------------------------------------------------------------------------ decoder
