@@ -677,7 +677,7 @@ def _rmsnorm(x, w, eps, residual, sum, out, q, d):
 def _new_like(t):
     """A new contiguous tensor of t's shape and dtype."""
     torch = _torch()
-    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def rmsnorm(x, w, eps: float = 1e-6, residual=None, sum=None, out=None):
@@ -694,9 +694,8 @@ def rmsnorm_q8(x, w, eps: float = 1e-6, residual=None, sum=None):
     torch, shape = _torch(), x.shape
     if len(shape) != 2 or shape[1] % QK:
         raise QHError(f"x is {tuple(shape)}, expected [rows][a multiple of {QK}]")
-    dev = x.device
-    q = torch.empty(shape, dtype=torch.int8, device=dev)
-    d = torch.empty((shape[0], shape[1] // QK), dtype=torch.float32, device=dev)
+    q = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
+    d = torch.empty((shape[0], shape[1] // QK), dtype=torch.float32, device=x.device)
     sum, _ = _rmsnorm(x, w, eps, residual, sum, None, q, d)
     return (q, d) if residual is None else (sum, q, d)
 
