@@ -165,12 +165,40 @@ __device__ __forceinline__ double from_ordered_f64(uint64_t k) {
     return __builtin_bit_cast(double, (k >> 63) ? (k & ~((uint64_t)1 << 63)) : ~k);
 }
 
+// A value that is the same in all lanes, in scalar registers.
+__device__ __forceinline__ uint64_t scalar(uint64_t v) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
+           (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+}
+
 // A candidate's place in the order: a larger key first, then a lower index. Those up to a limit are taken.
 struct Limit {
     uint64_t key;
     uint32_t index;
     __device__ __forceinline__ bool takes(uint64_t k, uint32_t i) const { return k > key || (k == key && i <= index); }
 };
+
+// Sum over the 16 lanes of each row of the wave.
+__device__ __forceinline__ uint32_t sum_row16(uint32_t x) {
+    x += (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x128, 0xF, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x124, 0xF, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x122, 0xF, 0xF, false);
+    return x + (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x121, 0xF, 0xF, false);
+}
+// The largest of the 16 lanes of each row of the wave.
+__device__ __forceinline__ uint64_t max_row16(uint64_t v) {
+    auto step = [&](auto ror) {
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)v, decltype(ror)::value, 0xF, 0xF, false),
+                       hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(v >> 32), decltype(ror)::value, 0xF, 0xF, false);
+        const uint64_t u = (uint64_t)hi << 32 | lo;
+        v = u > v ? u : v;
+    };
+    step(std::integral_constant<int, 0x128>{});
+    step(std::integral_constant<int, 0x124>{});
+    step(std::integral_constant<int, 0x122>{});
+    step(std::integral_constant<int, 0x121>{});
+    return v;
+}
 
 // Sum over the workgroup of what its waves count (the same in a wave's lanes), for every thread. `red` holds 16 values for each
 // parity of `turn`, so that a call needs one barrier.
@@ -179,10 +207,7 @@ __device__ __forceinline__ int wg_sum(int v, int (*red)[16], int& turn) {
     ++turn;
     if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
     __syncthreads();
-    int all = 0;
-#pragma unroll
-    for (int w = 0; w < 16; ++w) all += r[w];
-    return all;
+    return __builtin_amdgcn_readfirstlane((int)sum_row16((uint32_t)r[threadIdx.x & 15]));
 }
 
 // A limit that takes at least k and at most `most` of the candidates that count(limit) counts (the workgroup's, the same for
@@ -234,17 +259,19 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const T* __rest
     __shared__ double row_max[QH_BEAM_MAX_BEAMS], row_add[QH_BEAM_MAX_BEAMS];  // a NaN sum: a row without candidates
     __shared__ uint64_t pool_key[kPool];
     __shared__ uint32_t pool_at[kPool];
-    __shared__ int list[kList], rank_of[kPool];
+    __shared__ int list[kList];
     __shared__ int red[2][16];
-    __shared__ uint64_t tops[16];
+    __shared__ uint64_t cell[64], least_key;
     __shared__ int n_list, n_pool;
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, prompt = (int)blockIdx.x, row0 = prompt * beams;
-    if (tid == 0) n_list = n_pool = 0;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), prompt = (int)blockIdx.x, row0 = prompt * beams;
+    if (tid == 0) least_key = 0, n_list = n_pool = 0;
     const int n_groups = beams * cut.groups;
+    // groups of 16 lanes take every 64th group, so that those of one row, which may hold all the best, are with all of them
+    const int mine = (tid & 15) * 64 + (tid >> 4);
     float best_of[kKeys];  // in flight while the rows are summed
 #pragma unroll
     for (int j = 0; j < kKeys; ++j) {
-        const int i = j * kPickThreads + tid;
+        const int i = j * kPickThreads + mine;
         best_of[j] = i < n_groups ? gmax[(size_t)row0 * cut.groups + i] : -__builtin_inff();
     }
     for (int b = wave; b < beams; b += 16) {
@@ -280,73 +307,118 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const T* __rest
         const double v = ((double)x - row_max[b]) + row_add[b];
         return __builtin_fabs(v) < __builtin_inf() ? ordered_f64(v) : (uint64_t)0;
     };
+    static_assert((int64_t)QH_BEAM_MAX_BEAMS * QH_SAMPLE_MAX_VOCAB <= (int64_t)1 << 32, "an id and its beam in 32 bits");
+    auto index_of = [](int b, int id) { return (uint32_t)b * QH_SAMPLE_MAX_VOCAB + (uint32_t)id; };
     // 1. the groups
-    uint64_t key[kKeys], top = 0;
+    uint64_t key[kKeys], top = 0;  // the largest key is that of a row's largest logit, which is row_add
+    {
+        double t = -__builtin_inff();
+        for (int b = lane; b < beams; b += 64) t = __builtin_fmax(t, row_add[b]);
+        t = wave_reduce32x2(t, [](double x, double y) { return __builtin_fmax(x, y); });
+        if (t > -__builtin_inff()) top = ordered_f64(t);
+        top = scalar(top);
+    }
 #pragma unroll
     for (int j = 0; j < kKeys; ++j) {
-        const int i = j * kPickThreads + tid;
+        const int i = j * kPickThreads + mine;
         key[j] = 0;
         if (i < n_groups) key[j] = key_of(best_of[j], (int)(group_magic ? div_magic((uint32_t)i, group_magic) : (uint32_t)i));
-        top = key[j] > top ? key[j] : top;
     }
-    top = wave_max_u64(top);
-    if (lane == 0) tops[wave] = top;
-    __syncthreads();
+    auto to_list = [&](const Limit& l) {
 #pragma unroll
-    for (int w = 0; w < 16; ++w) top = tops[w] > top ? tops[w] : top;
+        for (int j = 0; j < kKeys; ++j) {
+            const int i = j * kPickThreads + mine;
+            if (l.takes(key[j], (uint32_t)i)) {
+                const int at = atomicAdd(&n_list, 1);
+                if (at < kList) list[at] = i;
+            }
+        }
+        __syncthreads();
+    };
     int turn = 0;
-    const Limit groups = find_limit(top, k, k + 16, [&](const Limit& l) {
-        int n = 0;
+    Limit groups{1, 0xffffffffu};
+    if (k <= 32) {
+        // the k-th largest of the 64 maxima of 16 lanes: k groups or more are at or above it, and rarely more than k + 16
+        uint64_t m = key[0];
 #pragma unroll
-        for (int j = 0; j < kKeys; ++j) n += __builtin_popcountll(__ballot(l.takes(key[j], (uint32_t)(j * kPickThreads + tid))));
-        return wg_sum(n, red, turn);
-    });
+        for (int j = 1; j < kKeys; ++j) m = key[j] > m ? key[j] : m;
+        m = max_row16(m);
+        if ((lane & 15) == 0) cell[tid >> 4] = m;
+        __syncthreads();
+        m = cell[lane];
 #pragma unroll
-    for (int j = 0; j < kKeys; ++j) {
-        const int i = j * kPickThreads + tid;
-        if (groups.takes(key[j], (uint32_t)i)) list[atomicAdd(&n_list, 1)] = i;
+        for (int q = 0; q < 4; ++q) {
+            const uint64_t c = scalar(cell[4 * wave + q]);
+            const int above = __builtin_popcountll(__ballot(m > c)), up_to = __builtin_popcountll(__ballot(m >= c));
+            if (lane == 0 && above < k && up_to >= k) least_key = c;
+        }
+        __syncthreads();
+        const uint64_t least = scalar(least_key);
+        if (least > 1) groups.key = least;
+        to_list(groups);
     }
-    __syncthreads();
+    if (k > 32 || __builtin_amdgcn_readfirstlane(n_list) > k + 16) {
+        groups = find_limit(top, k, k + 16, [&](const Limit& l) {
+            int n = 0;
+#pragma unroll
+            for (int j = 0; j < kKeys; ++j) n += __builtin_popcountll(__ballot(l.takes(key[j], (uint32_t)(j * kPickThreads + mine))));
+            return wg_sum(n, red, turn);
+        });
+        if (tid == 0) n_list = 0;
+        __syncthreads();
+        to_list(groups);
+    }
     // 2. their candidates: where k groups are listed, k of their best are at the limit's key or above, so only such ones count
-    const int listed = n_list;
+    const int listed = __builtin_amdgcn_readfirstlane(n_list);
     // f(there, logit, row, id) of every id of the listed groups whose logit can reach the limit, a wave to a group; what reaches it
     // is at or above the logit whose score the limit is, less what f32 and the sums round off
+    constexpr int kAhead = kKeys <= 4 ? 2 : 1;  // groups of a wave in flight (as many as its registers hold)
     auto each = [&](uint64_t limit_key, auto&& f) {
         const double goal = limit_key > 1 ? from_ordered_f64(limit_key) : -__builtin_inff();
-        for (int w = wave; w < listed; w += 16) {
-            const int i = list[w], b = (int)(group_magic ? div_magic((uint32_t)i, group_magic) : (uint32_t)i);
-            const int id0 = (i - b * cut.groups) * kGroup * 64 * E;
-            const T* x = logits + (int64_t)(row0 + b) * ld;
-            const double t = goal - row_add[b], u = row_max[b];
-            const float least = (float)(t + u - 0x1p-22 * (__builtin_fabs(t) + __builtin_fabs(u)));
-            typename Vec<T>::type v[kGroup];
-            if (id0 + kGroup * 64 * E <= n_valid) {
+        for (int w = wave; w < listed; w += 16 * kAhead) {
+            typename Vec<T>::type v[kAhead][kGroup];
+            int row[kAhead], id0[kAhead];
 #pragma unroll
-                for (int g = 0; g < kGroup; ++g)
-                    v[g] = *reinterpret_cast<const typename Vec<T>::type*>(x + id0 + (64 * g + lane) * E);
-            } else {
+            for (int h = 0; h < kAhead; ++h) {
+                if (w + 16 * h >= listed) break;
+                const int i = __builtin_amdgcn_readfirstlane(list[w + 16 * h]);
+                row[h] = (int)(group_magic ? div_magic((uint32_t)i, group_magic) : (uint32_t)i);
+                id0[h] = (i - row[h] * cut.groups) * kGroup * 64 * E;
+                const T* x = logits + (int64_t)(row0 + row[h]) * ld;
+                if (id0[h] + kGroup * 64 * E <= n_valid) {
+#pragma unroll
+                    for (int g = 0; g < kGroup; ++g)
+                        v[h][g] = *reinterpret_cast<const typename Vec<T>::type*>(x + id0[h] + (64 * g + lane) * E);
+                } else {
+#pragma unroll
+                    for (int g = 0; g < kGroup; ++g)
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            const int id = id0[h] + (64 * g + lane) * E + e;
+                            v[h][g][e] = id < n_valid ? x[id] : (T)-__builtin_inff();
+                        }
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < kAhead; ++h) {
+                if (w + 16 * h >= listed) break;
+                const double t = goal - row_add[row[h]], u = row_max[row[h]];
+                const float least = (float)(t + u - 0x1p-22 * (__builtin_fabs(t) + __builtin_fabs(u)));
 #pragma unroll
                 for (int g = 0; g < kGroup; ++g)
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        const int id = id0 + (64 * g + lane) * E + e;
-                        v[g][e] = id < n_valid ? x[id] : (T)-__builtin_inff();
+                        const float l = (float)v[h][g][e];
+                        if (!(l < least)) f(l, row[h], id0[h] + (64 * g + lane) * E + e);
                     }
             }
-#pragma unroll
-            for (int g = 0; g < kGroup; ++g)
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float l = (float)v[g][e];
-                    if (!(l < least)) f(l, b, id0 + (64 * g + lane) * E + e);
-                }
         }
     };
     Limit limit{listed < k ? (uint64_t)1 : groups.key, 0xffffffffu};  // fewer groups: all that they hold
     auto collect = [&]() {
         each(limit.key, [&](float l, int b, int id) {
             const uint64_t c = key_of(l, b);
-            const uint32_t at = (uint32_t)(b * n_valid + id);
+            const uint32_t at = index_of(b, id);
             if (limit.takes(c, at)) {
                 const int i = atomicAdd(&n_pool, 1);
                 if (i < kPool) {
@@ -361,7 +433,7 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const T* __rest
     if (n_pool > kPool) {  // many of them next to each other, or equal: the limit from counts of them all
         limit = find_limit(top, k, kPool, [&](const Limit& l) {
             int n = 0;
-            each(l.key, [&](float x, int b, int id) { n += l.takes(key_of(x, b), (uint32_t)(b * n_valid + id)); });
+            each(l.key, [&](float x, int b, int id) { n += l.takes(key_of(x, b), index_of(b, id)); });
             return wg_sum(wave_sum_i32(n), red, turn);
         });
         __syncthreads();
@@ -384,27 +456,30 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const T* __rest
         }
         __syncthreads();
     }
-    // 3. their ranks: how many come before each, a wave's sixteenth of them to each of its lanes' candidates
-    const int n = n_pool, share = (n + 15) / 16, from = wave * share, to = min(from + share, n);
-    for (int i = tid; i < n; i += kPickThreads) rank_of[i] = 0;
-    __syncthreads();
-    for (int i = lane; i < n; i += 64) {
-        const uint64_t c = pool_key[i];
-        const uint32_t at = pool_at[i];
-        int before = 0;
-#pragma unroll 4
-        for (int j = from; j < to; ++j) before += pool_key[j] > c || (pool_key[j] == c && pool_at[j] < at);
-        if (before) atomicAdd(&rank_of[i], before);
+    // 3. their ranks: a wave to a candidate, how many come before it. They are k + 64 at most, five to a lane.
+    const int n = __builtin_amdgcn_readfirstlane(n_pool);
+    constexpr int kEach = (QH_BEAM_MAX_K + 64) / 64;
+    uint64_t held[kEach];
+    uint32_t held_at[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        const int i = 64 * j + lane;
+        held[j] = i < n ? pool_key[i] : 0;
+        held_at[j] = i < n ? pool_at[i] : 0;
     }
-    __syncthreads();
-    if (tid < n) {
-        const int rank = rank_of[tid];
-        if (rank < k) {
-            const uint32_t at = pool_at[tid];
-            const int b = (int)(at / (uint32_t)n_valid);
-            parent[(size_t)prompt * k + rank] = row0 + b;
-            token[(size_t)prompt * k + rank] = (int)(at - (uint32_t)b * (uint32_t)n_valid);
-            best[(size_t)prompt * k + rank] = (float)from_ordered_f64(pool_key[tid]);
+    for (int i = wave; i < n; i += 16) {
+        const uint64_t c = scalar(pool_key[i]);
+        const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)pool_at[i]);
+        int rank = 0;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            if (64 * j >= n) break;
+            rank += __builtin_popcountll(__ballot(held[j] > c || (held[j] == c && held_at[j] < at)));
+        }
+        if (lane == 0 && rank < k) {
+            parent[(size_t)prompt * k + rank] = row0 + (int)(at / QH_SAMPLE_MAX_VOCAB);
+            token[(size_t)prompt * k + rank] = (int)(at % QH_SAMPLE_MAX_VOCAB);
+            best[(size_t)prompt * k + rank] = (float)from_ordered_f64(c);
         }
     }
     for (int i = n + tid; i < k; i += kPickThreads) {  // fewer candidates than k

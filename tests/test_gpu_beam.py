@@ -115,6 +115,18 @@ def test_select_neighbouring_logits(qh, gpu, vocab, k):
     check(qh, logits, torch.tensor([-1.0, -2.0, -1.5, -1.1], device=gpu), 2, k)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("beams,k", [(8, 2), (8, 16), (40, 1), (40, 8), (40, 32), (40, 33)])
+def test_select_groups_far_apart(qh, gpu, dtype, beams, k):
+    """The best candidates in every 64th group of 1,024 ids, and every other row without any of them."""
+    logits, scores = make(gpu, beams, 151936, dtype, seed=k)
+    groups = torch.arange(beams, device=gpu)[:, None] * 149 + torch.arange(151936, device=gpu)[None] // 1024
+    best = (groups % 64 == 0) & (torch.arange(151936, device=gpu) % 1024 == 7)
+    check(qh, torch.where(best, logits + 30, logits), None, beams, k)
+    rows = torch.arange(beams, device=gpu)[:, None] % 2 == 0
+    check(qh, torch.where(best & rows, logits + 30, logits), scores, beams, k)
+
+
 def test_select_close_scores(qh, gpu):
     """Beams whose candidates interleave at distances far below f32's: 64-bit scores tell them apart."""
     logits = torch.zeros(4, 2000, device=gpu)
