@@ -2,10 +2,11 @@
 //     score_b + logit_bv - log sum_u exp(logit_bu),
 // ties to the lower (b, v). Two launches:
 //   1. over the whole GPU (beam_rows_kernel): every logit once, for the largest of each group of ids and, wave by wave, the
-//      sum of exponentials. Bound by memory: 192 x 151,936 f32.
+//      sum of exponentials. Bound by memory (192 x 151,936 f32: 26.8 us, 4.4 TB/s with start and end).
 //   2. a workgroup to a prompt (beam_pick_kernel): the rows' sums, then the k best groups by their largest candidate (a
 //      group that is not among them holds none of the k best candidates, for k others have one before its own best), and
-//      the k best of what those groups hold.
+//      the k best of what those groups hold. Bound by latency: sums, groups, their logits and ranks wait for each other, and
+//      what sixteen waves all compute costs each SIMD four times (4 beams 5.6 us, 24 prompts of 8 9.7).
 // Candidates of different rows meet in the order of their scores, so sums, exponentials and scores are 64-bit: rounded to
 // f32, scores that are 2^-20 apart would tie. (A 64-bit multiply-add takes no longer than a 32-bit one here.)
 #include "qh_device.h"
@@ -15,7 +16,7 @@ namespace qh {
 namespace {
 
 constexpr int kPickThreads = 1024;
-constexpr int kPool = 1024;       // candidates that are ranked
+constexpr int kPool = kPickThreads;  // candidates that are held, one to a thread
 constexpr int kList = QH_BEAM_MAX_K + 16;  // groups that are read again, at most
 
 template <typename T>
@@ -277,7 +278,7 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const T* __rest
     for (int b = wave; b < beams; b += 16) {
         const float* pm = pmax + (size_t)(row0 + b) * cut.parts;
         const double* ps = psum + (size_t)(row0 + b) * cut.parts;
-        constexpr int kHeld = 4;  // parts of a lane: 256 of a row cover every vocabulary at 4 vectors to a wave and more
+        constexpr int kHeld = 4;  // parts of a lane: a row has 64 at most, or 256 where a group is one vector
         float m[kHeld], top = -__builtin_inff();
         double p[kHeld];
 #pragma unroll
@@ -405,12 +406,17 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const T* __rest
                 const double t = goal - row_add[row[h]], u = row_max[row[h]];
                 const float least = (float)(t + u - 0x1p-22 * (__builtin_fabs(t) + __builtin_fabs(u)));
 #pragma unroll
-                for (int g = 0; g < kGroup; ++g)
+                for (int g = 0; g < kGroup; ++g) {
+                    float m = (float)v[h][g][0];
+#pragma unroll
+                    for (int e = 1; e < E; ++e) m = __builtin_fmaxf(m, (float)v[h][g][e]);
+                    if (!__any(m >= least)) continue;  // most vectors of a group hold none
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
                         const float l = (float)v[h][g][e];
-                        if (!(l < least)) f(l, row[h], id0[h] + (64 * g + lane) * E + e);
+                        if (l >= least) f(l, row[h], id0[h] + (64 * g + lane) * E + e);
                     }
+                }
             }
         }
     };
@@ -430,31 +436,38 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const T* __rest
         __syncthreads();
     };
     collect();
-    if (n_pool > kPool) {  // many of them next to each other, or equal: the limit from counts of them all
-        limit = find_limit(top, k, kPool, [&](const Limit& l) {
-            int n = 0;
-            each(l.key, [&](float x, int b, int id) { n += l.takes(key_of(x, b), index_of(b, id)); });
-            return wg_sum(wave_sum_i32(n), red, turn);
-        });
-        __syncthreads();
-        if (tid == 0) n_pool = 0;
-        __syncthreads();
-        collect();
-    }
-    if (n_pool > k + 64) {  // those near the k best alone: ranks take their number squared
-        const uint64_t c = tid < n_pool ? pool_key[tid] : 0;
-        const uint32_t at = tid < n_pool ? pool_at[tid] : 0;
-        limit = find_limit(top, k, k + 32, [&](const Limit& l) {
-            return wg_sum((int)__builtin_popcountll(__ballot(l.takes(c, at))), red, turn);
-        });
-        if (tid == 0) n_pool = 0;
-        __syncthreads();
-        if (limit.takes(c, at)) {
-            const int i = atomicAdd(&n_pool, 1);
-            pool_key[i] = c;
-            pool_at[i] = at;
+    // More than the ranks are for: a limit near the k best of those that the pool holds, and where it does not hold all, another
+    // look at the groups. Two such looks suffice but where the pool gets the worst of many first: then the limit comes from
+    // counts of all (64 of 16 beams of 50,257 f16, 8 prompts, where one beam's groups are fewer than 64: 44.9 us, by counts of all
+    // at once 56.2).
+    for (int look = 0; n_pool > k + 64; ++look) {
+        const int held = n_pool;
+        const uint64_t c = tid < held ? pool_key[tid] : 0;
+        const uint32_t at = tid < held ? pool_at[tid] : 0;
+        if (held <= kPool || look < 2) {
+            limit = find_limit(top, k, k + 32, [&](const Limit& l) {
+                return wg_sum((int)__builtin_popcountll(__ballot(l.takes(c, at))), red, turn);
+            });
+        } else {
+            limit = find_limit(top, k, kPool, [&](const Limit& l) {
+                int n = 0;
+                each(l.key, [&](float x, int b, int id) { n += l.takes(key_of(x, b), index_of(b, id)); });
+                return wg_sum(wave_sum_i32(n), red, turn);
+            });
         }
         __syncthreads();
+        if (tid == 0) n_pool = 0;
+        __syncthreads();
+        if (held > kPool) {
+            collect();
+        } else {
+            if (limit.takes(c, at)) {
+                const int i = atomicAdd(&n_pool, 1);
+                pool_key[i] = c;
+                pool_at[i] = at;
+            }
+            __syncthreads();
+        }
     }
     // 3. their ranks: a wave to a candidate, how many come before it. They are k + 64 at most, five to a lane.
     const int n = __builtin_amdgcn_readfirstlane(n_pool);
