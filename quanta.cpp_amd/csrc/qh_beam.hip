@@ -28,18 +28,20 @@ struct Vec {  // at any address of the type's alignment
 };
 
 // How the rows are cut: a workgroup's part of a row is four waves' `vecs` vectors of 64 * E ids, a group `group` of them: one
-// where that leaves a group to a thread of the picking workgroup, else 1,024 ids (4 x 151,936 f32, of 256: 11.5 us for the
-// picking, of 1,024 8.2), or 2,048 where a thread had more than 32.
+// where that leaves a group to a thread of the picking workgroup, or four and the k best may take most of a row's larger ones
+// (64 of 16 beams of 50,257 f16, 8 prompts: 25.5 us, with groups of 1,024 ids 44.9), else 1,024 ids (24 prompts of 4 beams of
+// 151,936 f32: 22.2 us, of 256 28.2), or 2,048 where a thread had more than 32.
 struct BeamCut {
     int vecs, group;
     int parts, groups;  // of a row
 };
 
 template <typename T>
-BeamCut beam_cut(int rows, int beams, int n_valid) {
-    const int v = (n_valid + 64 * kE<T> - 1) / (64 * kE<T>);
+BeamCut beam_cut(int rows, int beams, int n_valid, int k) {
+    const int v = (n_valid + 64 * kE<T> - 1) / (64 * kE<T>), wide = 1024 / (64 * kE<T>);
     BeamCut c{};
-    c.group = (int64_t)beams * v <= kPickThreads ? 1 : 1024 / (64 * kE<T>);
+    const bool small = beams * v <= kPickThreads || (beams * v <= 4 * kPickThreads && 2 * k > (v + wide - 1) / wide);
+    c.group = small ? 1 : wide;
     if ((int64_t)beams * ((v + c.group - 1) / c.group) > 32 * kPickThreads) c.group *= 2;
     c.vecs = kMostVecs > c.group ? kMostVecs : c.group;  // the loads that a wave has in flight, fewer where there are not workgroups enough
     while (c.vecs > c.group && (int64_t)rows * ((v + 4 * c.vecs - 1) / (4 * c.vecs)) < 1024) c.vecs /= 2;
@@ -508,7 +510,7 @@ uint32_t magic_of(int d) { return d == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) 
 template <typename T>
 hipError_t beam_select_of(const BeamArgs& a, hipStream_t s) {
     const int rows = a.prompts * a.beams;
-    const BeamCut c = beam_cut<T>(rows, a.beams, a.n_valid);
+    const BeamCut c = beam_cut<T>(rows, a.beams, a.n_valid, a.k);
     double* psum = static_cast<double*>(a.ws);
     float* pmax = reinterpret_cast<float*>(psum + (size_t)rows * c.parts);
     float* gmax = pmax + (size_t)rows * c.parts;
@@ -531,7 +533,8 @@ hipError_t beam_select_of(const BeamArgs& a, hipStream_t s) {
                   psum, a.parent, a.token, a.best);
     };
     const int groups = a.beams * c.groups;
-    if (c.group == 1) pick(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+    if (c.group == 1 && groups <= kPickThreads) pick(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+    else if (c.group == 1) pick(integral_constant<int, 4>{}, integral_constant<int, 1>{});
     else if (c.group != kGroup) pick(integral_constant<int, 32>{}, integral_constant<int, 2 * kGroup>{});
     else if (groups <= kPickThreads) pick(integral_constant<int, 1>{}, integral_constant<int, kGroup>{});
     else if (groups <= 4 * kPickThreads) pick(integral_constant<int, 4>{}, integral_constant<int, kGroup>{});
@@ -541,10 +544,16 @@ hipError_t beam_select_of(const BeamArgs& a, hipStream_t s) {
 
 }  // namespace
 
+// For any k: the cut of few and of many.
 size_t beam_workspace_bytes(int dtype, int prompts, int beams, int n_valid) {
     const int rows = prompts * beams;
-    const BeamCut c = dtype == QH_F32 ? beam_cut<float>(rows, beams, n_valid) : beam_cut<_Float16>(rows, beams, n_valid);
-    return (size_t)rows * ((size_t)c.parts * 12 + (size_t)c.groups * 4);
+    size_t bytes = 0;
+    for (int k : {1, QH_BEAM_MAX_K}) {
+        const BeamCut c = dtype == QH_F32 ? beam_cut<float>(rows, beams, n_valid, k) : beam_cut<_Float16>(rows, beams, n_valid, k);
+        const size_t need = (size_t)rows * ((size_t)c.parts * 12 + (size_t)c.groups * 4);
+        bytes = need > bytes ? need : bytes;
+    }
+    return bytes;
 }
 
 hipError_t launch_beam_select(const BeamArgs& a, int dtype, hipStream_t s) {

@@ -64,7 +64,7 @@ def make(gpu, rows, vocab, dtype, seed=0, spread=2.0):
 SHAPES = [(1, 1, 1, 1), (1, 1, 1, 5), (3, 2, 1, 4), (1, 4, 3, 8), (2, 1, 255, 1), (2, 3, 256, 7), (2, 3, 257, 7), (1, 2, 511, 40),
           (1, 2, 513, 40), (5, 4, 1000, 8), (1, 1, 1000, 256), (3, 2, 4096, 256), (2, 8, 5003, 16), (1, 5, 32000, 10),
           (2, 4, 50257, 8), (1, 4, 151936, 8), (3, 8, 151936, 16), (1, 32, 50257, 64), (64, 4, 300, 8), (1, 40, 200000, 80),
-          (2, 12, 100, 24), (300, 1, 77, 3)]
+          (2, 12, 100, 24), (300, 1, 77, 3), (2, 8, 50257, 40), (1, 1, 262144, 8)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
