@@ -627,7 +627,8 @@ __global__ __launch_bounds__(256) void kv8_share_kernel(Kv8View c, const int32_t
 // Sequence dst[i] takes what src[i] held (-1: nothing), all at once: src may name sequences of dst, so every new row is read
 // before any is written. Counts only ever move by one for an entry that goes and one for an entry that comes, so their order
 // does not matter. Up to kReorderHere table entries in one workgroup, the rows in its registers; else the rows into the
-// workspace by the whole GPU (its first workgroup checks the lists), and from there in a second launch.
+// workspace by the whole GPU (its first workgroup checks the lists), and from there in a second launch. Bound by latency: 4
+// sequences of 10 pages 3.1 us here (by two launches 2.2 more), 512 of 188 4.2 and 5.2.
 constexpr int kReorderHere = 8 * kWg;
 struct ReorderWs {
     int* ok;

@@ -66,7 +66,8 @@ __device__ __forceinline__ void quant_lanes(const float (&v)[8], int8_t* q, floa
 
 // kWaves waves to a row, kVec vectors of E elements to a lane, 4 / kWaves rows to a workgroup of at least 4 waves. The sum
 // of squares and the scaled products are 64-bit (as fast as 32-bit ones here, and far from the memory's time): no square
-// overflows, the order of the sum does not show, and y is rounded once.
+// overflows, the order of the sum does not show, and y is rounded once. Bound by memory: 4,001 x 5,120 f32 with residual into
+// blocks 51.5-53.5 us, 16,000 x 4,096 f16 with residual 95.7, 5.1 and 5.5 TB/s; 1 x 896 2.4.
 template <typename T, int kWaves, int kVec>
 __global__ __launch_bounds__(kWaves < 4 ? 256 : 64 * kWaves) void rmsnorm_kernel(NormArgs a) {
     constexpr int E = kE<T>, kRows = kWaves < 4 ? 4 / kWaves : 1, kPass = 64 * kWaves * E;
@@ -188,7 +189,7 @@ constexpr int kRopePairs = 512;  // cosines and sines that a workgroup keeps
 // A workgroup takes `per` tokens: their cosines and sines once into LDS (angles in 64 bits: position times turns per
 // position, less its whole turns), then every head's pairs, E of them to an item, and after them the dims past rot, E to an
 // item, where the result is not written in place. Consecutive lanes take consecutive items of a head, so rows move in one
-// piece.
+// piece. Bound by memory: 8,000 tokens of 40 heads of 128 f16 27.6 us, 5.9 TB/s; 48 of 16 heads of 64 f32 2.8.
 // kWhole: no item is cut off by the end of the pairs or of the head.
 template <typename T, bool kInterleaved, bool kWhole>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a, int per, int units, int rest, uint32_t unit_magic,
