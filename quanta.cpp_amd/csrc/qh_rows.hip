@@ -28,13 +28,17 @@ __device__ __forceinline__ void load_e(const T* p, int n, float (&x)[kE<T>]) {
         for (int i = 0; i < kE<T>; ++i) x[i] = i < n ? (float)p[i] : 0.0f;
     }
 }
+// Stores pass by the caches, whose lines the loads of rows to come take: 16,000 x 4,096 f16 norms with residual 84.9 us, by plain
+// stores 98.7, and 161.9 and 166.2 with an addition that reads both results next; 512 x 4,096 5.5 and 6.2, 10.9 and 11.1; 8,000
+// tokens of 40 heads of 128 f16 turned 26.5 and 28.1. (8-bit codes, a quarter of the bytes, do not: 8,000 x 5,120 with their
+// reading back 173, past the caches 200.)
 template <typename T>
 __device__ __forceinline__ void store_e(T* p, int n, const float (&x)[kE<T>]) {
     if (n >= kE<T>) {
         typename Vec<T>::type v;
 #pragma unroll
         for (int i = 0; i < kE<T>; ++i) v[i] = (T)x[i];
-        *reinterpret_cast<typename Vec<T>::type*>(p) = v;
+        __builtin_nontemporal_store(v, reinterpret_cast<typename Vec<T>::type*>(p));
     } else {
 #pragma unroll
         for (int i = 0; i < kE<T>; ++i)
@@ -67,7 +71,7 @@ __device__ __forceinline__ void quant_lanes(const float (&v)[8], int8_t* q, floa
 // kWaves waves to a row, kVec vectors of E elements to a lane, 4 / kWaves rows to a workgroup of at least 4 waves. The sum
 // of squares and the scaled products are 64-bit (as fast as 32-bit ones here, and far from the memory's time): no square
 // overflows, the order of the sum does not show, and y is rounded once. Bound by memory: 4,001 x 5,120 f32 with residual into
-// blocks 51.5-53.5 us, 16,000 x 4,096 f16 with residual 95.7, 5.1 and 5.5 TB/s; 1 x 896 2.4.
+// blocks 49.3 us, 16,000 x 4,096 f16 with residual 91.6, 5.5 and 5.7 TB/s; 1 x 896 2.4.
 template <typename T, int kWaves, int kVec>
 __global__ __launch_bounds__(kWaves < 4 ? 256 : 64 * kWaves) void rmsnorm_kernel(NormArgs a) {
     constexpr int E = kE<T>, kRows = kWaves < 4 ? 4 / kWaves : 1, kPass = 64 * kWaves * E;
@@ -189,7 +193,7 @@ constexpr int kRopePairs = 512;  // cosines and sines that a workgroup keeps
 // A workgroup takes `per` tokens: their cosines and sines once into LDS (angles in 64 bits: position times turns per
 // position, less its whole turns), then every head's pairs, E of them to an item, and after them the dims past rot, E to an
 // item, where the result is not written in place. Consecutive lanes take consecutive items of a head, so rows move in one
-// piece. Bound by memory: 8,000 tokens of 40 heads of 128 f16 27.6 us, 5.9 TB/s; 48 of 16 heads of 64 f32 2.8.
+// piece. Bound by memory: 8,000 tokens of 40 heads of 128 f16 25.9 us, 6.3 TB/s; 48 of 16 heads of 64 f32 2.8.
 // kWhole: no item is cut off by the end of the pairs or of the head.
 template <typename T, bool kInterleaved, bool kWhole>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a, int per, int units, int rest, uint32_t unit_magic,
