@@ -328,6 +328,31 @@ __global__ __launch_bounds__(64 * kW, (Prompt<T, kHd, kTile, kW>::kSimdWaves)) v
             }
         }
     };
+    // f32 heads of 128: the next tile is staged between the products of scores (1,500 tokens of 32 heads over 8: 138.6 us, before
+    // them 153.8; heads of 64, whose two workgroups to a compute unit do so by themselves, 316 and 312 for 16 prompts of up to
+    // 2,000 tokens). A tile's values that are not finite become 0; then chunk p / 2 of its keys (p even) or values, in parts
+    // (behind the last tile the registers hold one that was staged before, and what it writes is not read).
+    constexpr bool kWoven = kN == 3 && kHd == 128;
+    constexpr int kStaging = 2;
+    auto clean = [&]() {
+        bool fine = true;
+#pragma unroll
+        for (int i = 0; i < P::kPer; ++i) fine = fine && vr[kDirect ? 0 : i].finite();
+        if (!fine) {
+#pragma unroll
+            for (int i = 0; i < P::kPer; ++i) vr[kDirect ? 0 : i].clean();
+            odd = 1;
+        }
+    };
+    auto stage_piece = [&](int p, int buf) {
+        if constexpr (kWoven) {
+            const int c = (p >> 1) * P::kThreads + tid, row = c / P::kChunks;
+            uint8_t* at = lds + buf * P::kBuffer + row * P::kRowBytes + 16 * swizzle<kHd>(row, c % P::kChunks) + (p & 1) * kN * P::kPlane;
+            const Parts<T> x = (p & 1) ? vr[p >> 1].parts() : kr[p >> 1].parts();
+#pragma unroll
+            for (int i = 0; i < kN; ++i) *reinterpret_cast<u4*>(at + i * P::kPlane) = x.p[i];
+        }
+    };
     auto stage = [&](int t, int buf) {
         bool fine = true;
 #pragma unroll
@@ -412,9 +437,11 @@ __global__ __launch_bounds__(64 * kW, (Prompt<T, kHd, kTile, kW>::kSimdWaves)) v
                 __syncthreads();
             }
             if (t + 1 < tiles) load_direct(t + 1, cur ^ 1);
-        } else {
+        } else if constexpr (!kWoven) {
             if (t + 1 < tiles) stage(t + 1, cur ^ 1);
             if (t + 2 < tiles) fetch(t + 2);
+        } else {
+            clean();
         }
         // The tile in blocks of 32 keys. Matrix instructions run in the background of a wave, eight issue slots each, so a block's
         // weights are computed between the products of the next block's scores, and the last block's between the first products
@@ -448,10 +475,14 @@ __global__ __launch_bounds__(64 * kW, (Prompt<T, kHd, kTile, kW>::kSimdWaves)) v
                 l[kt] += x + y;
             }
         };
-        // Products n of the block's (scores kKs, values 2 kDt) with a share of the eight pairs of weights of block `of` (-1: none)
-        // after each.
+        // Products n of the block's (scores kKs, values 2 kDt) with a share of the eight pairs of weights of block `of` (-1: none;
+        // kStaging: of the next tile's chunks in their place) after each.
         auto between = [&](int n, int all, int of) {
-            if (of >= 0) {
+            if (of == kStaging) {
+#pragma unroll
+                for (int p = 0; p < 2 * P::kPer; ++p)
+                    if (p * all / (2 * P::kPer) == n) stage_piece(p, cur ^ 1);
+            } else if (of >= 0) {
 #pragma unroll
                 for (int p = 0; p < 8; ++p)
                     if (p * all / 8 == n) weights2(of, p, base);
@@ -511,7 +542,10 @@ __global__ __launch_bounds__(64 * kW, (Prompt<T, kHd, kTile, kW>::kSimdWaves)) v
             }
             sum += l[kt];
         };
-        scores(0, -1);
+        scores(0, kWoven ? kStaging : -1);
+        if constexpr (kWoven) {
+            if (t + 2 < tiles) fetch(t + 2);
+        }
         mask(0);
         if constexpr (kKt == 1) {
             between(0, 1, 0);
