@@ -624,21 +624,38 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a) {
     if (splits == 1 || r >= rows) return;
     const size_t first = (((size_t)item * a.n_kv + kvh) * a.splits) * kRows + (r - r0);
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + first;
-    float top = -__builtin_inff();
-    for (int k = 0; k < splits; ++k) top = __builtin_fmaxf(top, ml[(size_t)k * kRows].x);
-    const float base = top == -__builtin_inff() ? 0.0f : top;
-    float sum = 0.0f;
+    float top = -__builtin_inff(), sum = 0.0f;
     float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-    for (int k = 0; k < splits; ++k) {
-        const float2 m = ml[(size_t)k * kRows];
-        const float4 v = *reinterpret_cast<const float4*>(a.part_o + (first + (size_t)k * kRows) * kHd + d);
-        const float f = __builtin_amdgcn_exp2f(m.x - base);
-        sum = __builtin_fmaf(f, m.y, sum);
-        o.x = __builtin_fmaf(f, v.x, o.x);
-        o.y = __builtin_fmaf(f, v.y, o.y);
-        o.z = __builtin_fmaf(f, v.z, o.z);
-        o.w = __builtin_fmaf(f, v.w, o.w);
+    constexpr int kAhead = 8;  // parts in flight
+    for (int k = 0; k < splits; k += kAhead) {
+        float2 m[kAhead];
+        float4 v[kAhead];
+        float now = top;
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            m[j] = make_float2(-__builtin_inff(), 0.0f);
+            v[j] = make_float4(0, 0, 0, 0);
+            if (k + j < splits) {
+                m[j] = ml[(size_t)(k + j) * kRows];
+                v[j] = *reinterpret_cast<const float4*>(a.part_o + (first + (size_t)(k + j) * kRows) * kHd + d);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) now = __builtin_fmaxf(now, m[j].x);
+        const float base = now == -__builtin_inff() ? 0.0f : now, f = k > 0 ? __builtin_amdgcn_exp2f(top - base) : 1.0f;
+        top = now;
+        sum *= f;
+        o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            if (k + j >= splits) break;
+            const float w = __builtin_amdgcn_exp2f(m[j].x - base);
+            sum = __builtin_fmaf(w, m[j].y, sum);
+            o.x = __builtin_fmaf(w, v[j].x, o.x);
+            o.y = __builtin_fmaf(w, v[j].y, o.y);
+            o.z = __builtin_fmaf(w, v[j].z, o.z);
+            o.w = __builtin_fmaf(w, v[j].w, o.w);
+        }
     }
     const int token = (int)((unsigned)r / (unsigned)a.group), head = kvh * a.group + (r - token * a.group);
     const float inv = e.visible(a, r) > 0 ? 1.0f / sum : 0.0f;
