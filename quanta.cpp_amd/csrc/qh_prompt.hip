@@ -24,7 +24,8 @@
 namespace qh {
 namespace {
 
-constexpr int kSplitKeys = 128;  // keys of a split, at least (512 tokens of 14 heads of 64 f32: 22.0 us, 64 22.7, 256 33.4)
+constexpr int kSplitTiles = 2;  // key tiles of a split, at least (300 tokens of 32 heads of 128 f32: 23.9 us, with one or four 32; 4 x 64 behind 3,000 of 14
+                                // of 64 f16 18.4, with one 21.1)
 constexpr int kMaxSplits = 64;
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -41,13 +42,13 @@ template <typename T>
 struct Parts;
 template <>
 struct Parts<_Float16> {
-    static constexpr int kN = 1;
+    static constexpr int kN = 1, kLong = 20;  // (plan_of)
     typedef h8 Op;
     u4 p[1];
 };
 template <>
 struct Parts<float> {
-    static constexpr int kN = 3;
+    static constexpr int kN = 3, kLong = 12;
     typedef b8 Op;
     u4 p[3];
 };
@@ -205,10 +206,8 @@ __device__ __forceinline__ bool entry_of(const PromptArgs& a, int item, int tile
     *r0 = (item - first) * tile_rows;
     return *r0 < e->rows * a.group;
 }
-// The workgroups that share a row tile's key tiles, 128 keys to each at least.
-__device__ __forceinline__ int splits_of(const PromptArgs& a, int tiles, int tile) {
-    return min(a.splits, max(tiles * tile / kSplitKeys, 1));
-}
+// The workgroups that share a row tile's key tiles.
+__device__ __forceinline__ int splits_of(const PromptArgs& a, int tiles) { return min(a.splits, max(tiles / kSplitTiles, 1)); }
 
 template <typename T, int kHd, int kTile, int kW>
 struct Prompt {
@@ -248,7 +247,7 @@ __global__ __launch_bounds__(64 * kW, (Prompt<T, kHd, kTile, kW>::kSimdWaves)) v
     auto visible = [&](int r) { return e.visible(a, r); };
     const int last = min(r0 + P::kRows, rows) - 1, seen = visible(last), all_tiles = (seen + kTile - 1) / kTile;
     // this workgroup's share of the tiles, where a row tile's are shared out
-    const int splits = splits_of(a, all_tiles, kTile), split = (int)blockIdx.y;
+    const int splits = splits_of(a, all_tiles), split = (int)blockIdx.y;
     if (split >= splits) return;
     const int tile0 = all_tiles * split / splits, tiles = all_tiles * (split + 1) / splits;
     const int first_sees = visible(r0);  // every row of the workgroup sees these
@@ -619,7 +618,7 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a) {
     int r0;
     if (!entry_of(a, item, kRows, &e, &r0)) return;
     const int rows = e.rows * a.group;
-    const int splits = splits_of(a, (e.visible(a, min(r0 + kRows, rows) - 1) + kTile - 1) / kTile, kTile);
+    const int splits = splits_of(a, (e.visible(a, min(r0 + kRows, rows) - 1) + kTile - 1) / kTile);
     const int r = r0 + (int)blockIdx.y * kPer + (int)threadIdx.x / kThr, d = 4 * ((int)threadIdx.x % kThr);
     if (splits == 1 || r >= rows) return;
     const size_t first = (((size_t)item * a.n_kv + kvh) * a.splits) * kRows + (r - r0);
@@ -686,17 +685,20 @@ void by_shape(int dtype, int hd, int group, int n_kv, int n_tok, F&& f) {
     else f((float*)nullptr, K64{}, K32{}, W4{});
 }
 
-// Row tiles of a call, and how many workgroups may share one: two workgroups to a compute unit where the row tiles are fewer,
-// as many as the entries' keys are likely to fill.
+// Row tiles of a call, and how many workgroups may share one where the row tiles are fewer than the compute units: a workgroup to
+// a compute unit, or two where one would still have more than `long_way` key tiles one after the other (f32 12: 512 tokens of 14
+// heads of 64 18.1 us, with two 20.5, 1,000 36.8 and 30.6; f16 20: 8 prompts of up to 300 behind 500 17.3 and 21.4, 1,500 tokens
+// 25.3 and 24.5), by the entries' mean length, which is all that the host knows of them.
 struct Plan {
     int items, splits;
 };
-Plan plan_of(int rows, int group, int n_kv, int n, int n_tok, int n_keys) {
+Plan plan_of(int rows, int tile, int long_way, int group, int n_kv, int n, int n_tok, int n_keys) {
     Plan p;
     p.items = (int)((int64_t)n_tok * group / rows) + n;
-    const int64_t tiles = ((int64_t)n_tok * group + rows - 1) / rows, wgs = (tiles > n ? tiles : n) * n_kv, want = 2 * device_cus();
-    const int64_t most = n_keys / n / kSplitKeys;
-    int64_t s = want / (wgs > 0 ? wgs : 1);
+    const int64_t tiles = ((int64_t)n_tok * group + rows - 1) / rows, wgs = (tiles > n ? tiles : n) * n_kv;
+    const int64_t keys = n_keys / n / tile, most = keys / kSplitTiles;
+    int64_t s = device_cus() / (wgs > 0 ? wgs : 1);
+    if (keys > long_way * (s > 1 ? s : 1)) s = 2 * device_cus() / (wgs > 0 ? wgs : 1);
     s = s < most ? s : most;
     p.splits = (int)(s < 1 ? 1 : s < kMaxSplits ? s : kMaxSplits);
     return p;
@@ -706,9 +708,9 @@ Plan plan_of(int rows, int group, int n_kv, int n, int n_tok, int n_keys) {
 
 size_t prompt_workspace_bytes(int dtype, int n_heads, int n_kv, int hd, int n, int n_tok, int n_keys) {
     size_t bytes = 0;
-    by_shape(dtype, hd, n_heads / n_kv, n_kv, n_tok, [&](auto*, auto, auto, auto waves) {
-        constexpr int kRows = 32 * decltype(waves)::value;
-        const Plan p = plan_of(kRows, n_heads / n_kv, n_kv, n, n_tok, n_keys);
+    by_shape(dtype, hd, n_heads / n_kv, n_kv, n_tok, [&](auto* type, auto, auto tile, auto waves) {
+        constexpr int kRows = 32 * decltype(waves)::value, kLong = Parts<std::remove_pointer_t<decltype(type)>>::kLong;
+        const Plan p = plan_of(kRows, decltype(tile)::value, kLong, n_heads / n_kv, n_kv, n, n_tok, n_keys);
         if (p.splits > 1) bytes = (size_t)p.items * n_kv * p.splits * kRows * (hd + 2) * sizeof(float);
     });
     return bytes;
@@ -719,7 +721,7 @@ hipError_t launch_prompt(PromptArgs a, int dtype, int hd, void* ws, hipStream_t 
     by_shape(dtype, hd, a.group, a.n_kv, a.n_tok, [&](auto* type, auto head, auto tile, auto waves) {
         using T = std::remove_pointer_t<decltype(type)>;
         constexpr int kHd = decltype(head)::value, kTile = decltype(tile)::value, kW = decltype(waves)::value, kRows = 32 * kW;
-        const Plan p = plan_of(kRows, a.group, a.n_kv, a.n, a.n_tok, a.n_keys);
+        const Plan p = plan_of(kRows, kTile, Parts<T>::kLong, a.group, a.n_kv, a.n, a.n_tok, a.n_keys);
         a.items = p.items, a.splits = p.splits;
         a.part_o = static_cast<float*>(ws);
         a.part_ml = a.part_o + (size_t)p.items * a.n_kv * p.splits * kRows * hd;
