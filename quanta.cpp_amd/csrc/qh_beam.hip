@@ -21,7 +21,9 @@ constexpr int kList = QH_BEAM_MAX_K + 16;  // groups that are read again, at mos
 
 template <typename T>
 constexpr int kE = 16 / (int)sizeof(T);
-constexpr int kMostVecs = 2;  // or a group's (192 x 151,936 f32, groups of 4: 26.8 us, with 8 28.2, with 16 32.2; 512 x 50,257 f16 24.2, with 4 38)
+// Loads of a wave in flight, or a group's (192 x 151,936 f32, groups of 4: 26.8 us, with 8 28.2, with 16 32.2; 512 x 50,257 f16
+// 24.2, with 4 38).
+constexpr int kMostVecs = 2;
 template <typename T>
 struct Vec {  // at any address of the type's alignment
     typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
@@ -43,7 +45,7 @@ BeamCut beam_cut(int rows, int beams, int n_valid, int k) {
     const bool small = beams * v <= kPickThreads || (beams * v <= 4 * kPickThreads && 2 * k > (v + wide - 1) / wide);
     c.group = small ? 1 : wide;
     if ((int64_t)beams * ((v + c.group - 1) / c.group) > 32 * kPickThreads) c.group *= 2;
-    c.vecs = kMostVecs > c.group ? kMostVecs : c.group;  // the loads that a wave has in flight, fewer where there are not workgroups enough
+    c.vecs = kMostVecs > c.group ? kMostVecs : c.group;  // fewer where there are not workgroups enough
     while (c.vecs > c.group && (int64_t)rows * ((v + 4 * c.vecs - 1) / (4 * c.vecs)) < 1024) c.vecs /= 2;
     c.parts = (v + 4 * c.vecs - 1) / (4 * c.vecs);
     c.groups = (v + c.group - 1) / c.group;
@@ -129,7 +131,8 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const T* __restrict__ lo
         for (int j = 0; j < kVecs; ++j)
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const double x = (double)__builtin_amdgcn_fmed3f((float)raw[j][e], low, __builtin_inff()), k = __builtin_fma(x, kLog2e, a);
+                const double x = (double)__builtin_amdgcn_fmed3f((float)raw[j][e], low, __builtin_inff());
+                const double k = __builtin_fma(x, kLog2e, a);
                 s += exp2_parts(__builtin_fma(x, kLog2e, a - k), k);
             }
         s = wave_reduce32x2(s, [](double p, double q) { return p + q; });
@@ -266,7 +269,8 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const T* __rest
     __shared__ int red[2][16];
     __shared__ uint64_t cell[64], least_key;
     __shared__ int n_list, n_pool;
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), prompt = (int)blockIdx.x, row0 = prompt * beams;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int prompt = (int)blockIdx.x, row0 = prompt * beams;
     if (tid == 0) least_key = 0, n_list = n_pool = 0;
     const int n_groups = beams * cut.groups;
     // groups of 16 lanes take every 64th group, so that those of one row, which may hold all the best, are with all of them

@@ -24,8 +24,9 @@
 namespace qh {
 namespace {
 
-constexpr int kSplitTiles = 2;  // key tiles of a split, at least (300 tokens of 32 heads of 128 f32: 23.9 us, with one or four 32; 4 x 64 behind 3,000 of 14
-                                // of 64 f16 18.4, with one 21.1)
+// Key tiles of a split, at least (300 tokens of 32 heads of 128 f32: 23.9 us, with one or four 32; 4 x 64 behind 3,000 of 14 heads
+// of 64 f16 18.4, with one 21.1).
+constexpr int kSplitTiles = 2;
 constexpr int kMaxSplits = 64;
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
