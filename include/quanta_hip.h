@@ -477,7 +477,9 @@ int qh_attention(const void* q, const void* k, const void* v, void* out, int dty
 /* Beam search's selection. logits: DEVICE rows [n_prompts * beams][n_valid] of dtype QH_F32 or QH_F16, ld elements apart, on
  * any alignment of their type; scores: DEVICE f32 [n_prompts * beams], what each beam has so far (NULL: 0). A candidate is a
  * beam b of a prompt and an id v, with the score scores[b] + logits[b][v] - log sum_u exp(logits[b][u]); sums, exponentials
- * and the comparison of candidates are 64-bit, and equal ones go to the lower b, then the lower v. For each prompt its k best
+ * and the comparison of candidates are 64-bit, and equal ones go to the lower b, then the lower v. With m the largest logit of the
+ * beam, that is (logits[b][v] - m) + (scores[b] - log sum_u exp(logits[b][u] - m)): beside a score of 2^53 times the logits'
+ * differences and more, all ids of a beam are equal. For each prompt its k best
  * candidates, best first, into DEVICE arrays [n_prompts][k]: parent (the row, prompt * beams + b), token and score (f32). A
  * logit of -infinity is no candidate, and neither is any of a row whose score is not finite or whose logits hold a NaN or
  * +infinity or are all -infinity (a beam that ended gets the score -infinity); where there are fewer than k, the places

@@ -167,6 +167,7 @@ __device__ __forceinline__ uint64_t ordered_f64(double v) {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
     return (u >> 63) ? ~u : (u | ((uint64_t)1 << 63));
 }
+constexpr uint64_t kLeastKey = (uint64_t)1 << 52;  // of the lowest finite f64: those below stand for no number
 __device__ __forceinline__ double from_ordered_f64(uint64_t k) {
     return __builtin_bit_cast(double, (k >> 63) ? (k & ~((uint64_t)1 << 63)) : ~k);
 }
@@ -377,11 +378,14 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const T* __rest
     }
     // 2. their candidates: where k groups are listed, k of their best are at the limit's key or above, so only such ones count
     const int listed = __builtin_amdgcn_readfirstlane(n_list);
-    // f(there, logit, row, id) of every id of the listed groups whose logit can reach the limit, a wave to a group; what reaches it
-    // is at or above the logit whose score the limit is, less what f32 and the sums round off
+    // f(logit, row, id) of every id of the listed groups whose logit can reach the limit, a wave to a group. A logit x is left out
+    // only where its key lies below the limit's, so that counts by f are the counts of the keys themselves (else the search for a
+    // limit below need not end). A key's score (x - u) + row_add reaches `goal` only where x - u >= (goal - row_add), less the
+    // roundings of the sum, at most 2^-53 of goal, and of t, u and x - u, 2^-53 of each and of row_add; 2^-51 and 2^-22 are more.
+    // (The rounding to f32 leaves out nothing: x is an f32.)
     constexpr int kAhead = kKeys <= 4 ? 2 : 1;  // groups of a wave in flight (as many as its registers hold)
     auto each = [&](uint64_t limit_key, auto&& f) {
-        const double goal = limit_key > 1 ? from_ordered_f64(limit_key) : -__builtin_inff();
+        const double goal = limit_key >= kLeastKey ? from_ordered_f64(limit_key) : -__builtin_inff();
         for (int w = wave; w < listed; w += 16 * kAhead) {
             typename Vec<T>::type v[kAhead][kGroup];
             int row[kAhead], id0[kAhead];
@@ -409,8 +413,9 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const T* __rest
 #pragma unroll
             for (int h = 0; h < kAhead; ++h) {
                 if (w + 16 * h >= listed) break;
-                const double t = goal - row_add[row[h]], u = row_max[row[h]];
-                const float least = (float)(t + u - 0x1p-22 * (__builtin_fabs(t) + __builtin_fabs(u)));
+                const double add = row_add[row[h]], t = goal - add, u = row_max[row[h]];
+                const float least = (float)(t + u - (0x1p-22 * (__builtin_fabs(t) + __builtin_fabs(u)) +
+                                                     0x1p-51 * (__builtin_fabs(goal) + __builtin_fabs(add))));
 #pragma unroll
                 for (int g = 0; g < kGroup; ++g) {
                     float m = (float)v[h][g][0];
@@ -444,8 +449,8 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const T* __rest
     collect();
     // More than the ranks are for: a limit near the k best of those that the pool holds, and where it does not hold all, another
     // look at the groups. Two such looks suffice but where the pool gets the worst of many first: then the limit comes from
-    // counts of all (64 of 16 beams of 50,257 f16, 8 prompts, where one beam's groups are fewer than 64: 44.9 us, by counts of all
-    // at once 56.2).
+    // counts of all and takes no more than the pool holds, so that the look after it is the last (64 of 16 beams of 50,257 f16, 8
+    // prompts, where one beam's groups are fewer than 64: 44.9 us, by counts of all at once 56.2).
     for (int look = 0; n_pool > k + 64; ++look) {
         const int held = n_pool;
         const uint64_t c = tid < held ? pool_key[tid] : 0;
