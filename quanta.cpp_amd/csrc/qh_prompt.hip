@@ -567,11 +567,27 @@ __global__ __launch_bounds__(64 * kW, (Prompt<T, kHd, kTile, kW>::kSimdWaves)) v
     sum += other_half(sum);
     if (!valid) return;
     typedef T t4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-    if (odd) {
+    // f16: an infinity of a tile that every row sees went into the product as it is, and is NaN where its weight rounds to 0 or a
+    // later base scales it by 0 (a NaN without one in the sum comes from values alone). Of parts the join looks for such.
+    bool lost = false;
+    if (kN == 1 && splits == 1) {
+#pragma unroll
+        for (int d = 0; d < kDt; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) lost = lost || __builtin_isunordered(o[d][i], o[d][i + 1]);
+        lost = lost && sum == sum;
+        if (lost) {
+#pragma unroll
+            for (int d = 0; d < kDt; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] == o[d][i] ? o[d][i] : 0.0f;
+        }
+    }
+    if (odd || lost) {
         // weights of hidden positions are 0, but 0 times a value that is not finite is NaN, and so are an infinity's products
         // with the parts of a weight: such values, in f16 of the tiles with hidden positions alone, went into the product as
-        // zeros, and are added here to the rows that see them
-        for (int j = max(tile0, kN == 3 ? 0 : first_sees / kTile) * kTile; j < min(vis, tiles * kTile); ++j) {
+        // zeros, and are added here to the rows that see them (an infinity that is there already is not changed by itself)
+        for (int j = max(tile0, kN == 3 || lost ? 0 : first_sees / kTile) * kTile; j < min(vis, tiles * kTile); ++j) {
             const T* v = vp + (int64_t)(e.key0 + j) * a.ldv + 4 * half;
 #pragma unroll
             for (int d = 0; d < kDt; ++d)
@@ -657,9 +673,23 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a) {
             o.w = __builtin_fmaf(w, v[j].w, o.w);
         }
     }
+    typedef T t4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    if ((__builtin_isunordered(o.x, o.y) || __builtin_isunordered(o.z, o.w)) && sum == sum) {
+        // a value that is not finite, in a part or by a weight of 0 (lost, above): what the row sees of such is all that counts
+        float f[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = f[i] == f[i] ? f[i] : 0.0f;
+        const T* v = static_cast<const T*>(a.v) + (int64_t)e.key0 * a.ldv + (int64_t)kvh * kHd + d;
+        for (int j = 0; j < e.visible(a, r); ++j) {
+            const t4 x = *reinterpret_cast<const t4*>(v + (int64_t)j * a.ldv);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (!(__builtin_fabsf((float)x[i]) < __builtin_inff())) f[i] += (float)x[i];
+        }
+        o = make_float4(f[0], f[1], f[2], f[3]);
+    }
     const int token = (int)((unsigned)r / (unsigned)a.group), head = kvh * a.group + (r - token * a.group);
     const float inv = e.visible(a, r) > 0 ? 1.0f / sum : 0.0f;
-    typedef T t4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
     *reinterpret_cast<t4*>(static_cast<T*>(a.out) + (int64_t)(e.row0 + token) * a.ldo + (int64_t)head * kHd + d) =
         (t4){(T)(o.x * inv), (T)(o.y * inv), (T)(o.z * inv), (T)(o.w * inv)};
 }
