@@ -464,7 +464,8 @@ int qh_rope(const double* turns, int rot_dim, int interleaved, float magnitude, 
  * of dtype QH_F32 or QH_F16, ld elements apart on any alignment of their type, a row's heads contiguous. A row that sees
  * nothing is 0; rows outside the entries are neither read nor written. Keys and values that a row does not see have no part in
  * it, whatever they hold. A NaN or an infinity that it sees stays in its dim where it is a value's, however small its weight, and
- * makes the row NaN where it is the query's; of a key's it becomes NaN, or what the formula gives. f16: weights are rounded to f16 once. f32:
+ * makes the row NaN where it is the query's; of a key's it becomes NaN, or what the formula gives. (Values that are not finite
+ * are read once more: such a call takes up to twice its time.) f16: weights are rounded to f16 once. f32:
  * products keep 22 bits and more of every value, whatever the others are. Sums in f32. out overlaps no input. The workspace is
  * 16-byte aligned and needs no initialisation (NULL where the size is 0); calls that overlap must not share one.
  * No counterpart in the reference, whose prompts attend to its cache in chunks (Model::forward_batch, model.cpp:387-405). */

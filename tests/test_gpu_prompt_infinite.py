@@ -75,3 +75,25 @@ def test_batch_of_entries_with_and_without(qh, gpu, dtype):
     got = qh.attention(q, k, v, ints(st, gpu))
     check(got, *formula(q, k, v, st, st, True, 0.125))
     assert torch.equal(got[:95], clean[:95]) and torch.equal(got[180:399], clean[180:399])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("rows,keys", [(150, 150), (3, 2500), (70, 900), (2100, 2100)])
+@pytest.mark.parametrize("share", [0.001, 0.3, 1.0])
+def test_many_values_that_are_not_finite(qh, gpu, dtype, hd, causal, rows, keys, share):
+    """Infinities of both signs and NaN all over, up to every value; large keys among the last, so that early ones weigh nothing."""
+    heads, kv = (32, 16) if rows > 2000 else (4, 2)
+    q, k, v = inputs(gpu, dtype, rows, keys, heads, kv, hd, slice(0, keys // 2))
+    gen = torch.Generator(device=gpu).manual_seed(rows)
+    there = torch.rand(v.shape, generator=gen, device=gpu) < share
+    kinds = torch.tensor([math.nan, math.inf, -math.inf, math.inf, -math.inf, math.inf], device=gpu).to(v.dtype)
+    # dims of +infinity alone, of both, and of all three
+    kind = kinds[torch.randint(0, 6, v.shape, generator=gen, device=gpu)]
+    kind[..., ::3] = math.inf
+    kind[..., 1::3] = kind[..., 1::3].nan_to_num(nan=math.inf, posinf=math.inf, neginf=-math.inf)
+    v.copy_(torch.where(there, kind, v))
+    st, kst = [0, rows], [0, keys]
+    got = qh.attention(q, k, v, ints(st, gpu), ints(kst, gpu), causal=causal)
+    check(got, *formula(q, k, v, st, kst, causal, hd ** -0.5))
