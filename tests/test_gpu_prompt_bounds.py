@@ -1,0 +1,28 @@
+"""Attention of packed prompts (qh_attention): f32 values near the type's smallest.
+
+Small f32 values. The largest weight of a row is 2^-L at least, with 2^L at most 2^10 times the keys (so that f32's largest values do not
+overflow), and their products are summed in f32: where a sum falls below 2^-126 each of the 6 products of a key may round by 2^-150,
+6 keys 2^-150 in all, and the division by a sum of weights of 2^-L and more makes that 6 keys 2^-150 2^10 keys < keys^2 2^-137. The
+three bf16 of a value below 2^-110 end at bf16's smallest, 2^-133: a value is off by 2^-132 at most. Both come on top of the bound that
+holds for other values."""
+import pytest
+import torch
+
+from test_gpu_prompt import check, formula, ints
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows,keys", [(1, 1), (3, 70), (150, 200), (40, 1000), (5, 5000)])
+@pytest.mark.parametrize("wide", [0.0, 1.0, 20.0])
+@pytest.mark.parametrize("size", [-80, -95, -105, -115, -125, -135])
+def test_small_f32_values(qh, gpu, hd, rows, keys, wide, size):
+    """Values of one small size, under equal weights, ordinary ones and one that outweighs the others."""
+    gen = torch.Generator(device=gpu).manual_seed(keys)
+    q = torch.randn(rows, 4, hd, generator=gen, device=gpu) * wide
+    k = torch.randn(keys, 2, hd, generator=gen, device=gpu)
+    v = torch.randn(keys, 2, hd, generator=gen, device=gpu) * 2.0 ** size
+    got = qh.attention(q, k, v, ints([0, rows], gpu), ints([0, keys], gpu))
+    want, err, mine = formula(q, k, v, [0, rows], [0, keys], True, hd ** -0.5)
+    check(got, want, err + keys ** 2 * 2.0 ** -137 + 2.0 ** -132, mine)
