@@ -405,10 +405,11 @@ int qh_kv8_attention_plan(const qh_kv8_cache* c, int n_heads, int n, int n_tok, 
 /* Root-mean-square norm of n_tok rows of n, with a residual's addition before it: h = x + res, rounded to dtype (QH_F32 or
  * QH_F16; res NULL: h = x), goes to sum (NULL: nowhere), and h / sqrt(mean(h^2) + eps) * w to the outputs that are given:
  * y, rows of dtype, and / or q [n_tok][n] with d [n_tok][n / 32], the blocks that qh_quantize_q8 makes of the result in f32
- * (n a multiple of 32 then). w is f32 [n]. Squares are summed in 64 bits and the result is rounded once. Rows are ld elements
- * apart, on any alignment of their type (q: 16 bytes). sum may be x or res, with its row stride; the outputs overlap nothing
- * else. n at most QH_NORM_MAX; n_tok below 2^24, of rows of more than 2,048 below 2^23, of more than 8,192 below 2^22. A NaN
- * makes its row NaN; an infinity makes its own place NaN and the rest of the row 0 (in blocks: as qh_quantize_q8 takes those).
+ * (n a multiple of 32 then). w is f32 [n]. Squares are summed and results computed in 64 bits, rounded to f32, and f16 rows from
+ * there. Rows are ld elements apart, on any alignment of their type (q: 16 bytes). sum may be x or res, with its row stride; the
+ * outputs overlap nothing else. n at most QH_NORM_MAX; n_tok below 2^24, of rows of
+ * more than 2,048 below 2^23, of more than 8,192 below 2^22. A NaN makes its row NaN; an infinity makes its own place NaN and the
+ * rest of the row 0 (in blocks: as qh_quantize_q8 takes those).
  * No counterpart among the reference's kernels by itself: its rmsnorm (ops_ref.cpp:194-199) sums in f32 in order, which the
  * decoder's own kernels keep to the bit. */
 #define QH_NORM_MAX 32768

@@ -70,8 +70,9 @@ __device__ __forceinline__ void quant_lanes(const float (&v)[8], int8_t* q, floa
 
 // kWaves waves to a row, kVec vectors of E elements to a lane, 4 / kWaves rows to a workgroup of at least 4 waves. The sum
 // of squares and the scaled products are 64-bit (as fast as 32-bit ones here, and far from the memory's time): no square
-// overflows, the order of the sum does not show, and y is rounded once. Bound by memory: 4,001 x 5,120 f32 with residual into
-// blocks 49.3 us, 16,000 x 4,096 f16 with residual 91.6, 5.5 and 5.7 TB/s; 1 x 896 2.4.
+// overflows, the order of the sum does not show, and y is rounded to f32 once (f16 rows from there, so by 2^-11 and 2^-24: a
+// single rounding from 64 bits has no instruction). Bound by memory: 4,001 x 5,120 f32 with residual into blocks 49.3 us, 16,000 x
+// 4,096 f16 with residual 91.6, 5.5 and 5.7 TB/s; 1 x 896 2.4.
 template <typename T, int kWaves, int kVec>
 __global__ __launch_bounds__(kWaves < 4 ? 256 : 64 * kWaves) void rmsnorm_kernel(NormArgs a) {
     constexpr int E = kE<T>, kRows = kWaves < 4 ? 4 / kWaves : 1, kPass = 64 * kWaves * E;
