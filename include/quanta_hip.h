@@ -449,8 +449,9 @@ typedef struct qh_rope_rows {
 /* Rotary positions: every head of q's and k's rows (k NULL: q alone) has its first rot_dim dims turned in pairs (a, b) ->
  * (a cos - b sin, a sin + b cos) by the angle 2 pi pos[t] turns[i], cos and sin times `magnitude`; the others are copied. A
  * pair is the dims i and i + rot_dim / 2, or (interleaved 1) 2 i and 2 i + 1. pos: DEVICE int32 [n_tok], of either sign;
- * turns: DEVICE [rot_dim / 2]. Angles are taken in 64 bits less their whole turns, so that far positions lose nothing. Rows
- * of dtype QH_F32 or QH_F16 on any alignment of their type; head_dim at most QH_ROPE_MAX_DIM.
+ * turns: DEVICE [rot_dim / 2]. Angles are taken in 64 bits less their whole turns: with
+ * qh_rope_turns' table they are off by up to some 2^-51 of the angle (2^-49 where rot_dim is no power of two), by the table's
+ * rounding and the product's: below f32's step up to 10^8 positions, 5e-7 radians at int32's ends. Rows of dtype QH_F32 or QH_F16 on any alignment of their type; head_dim at most QH_ROPE_MAX_DIM.
  * Replaces: the rotation in Model::forward (reference model.cpp:187-196), for many sequences' tokens; the decoder's own
  * kernels keep the reference's f32 table to the bit. */
 int qh_rope(const double* turns, int rot_dim, int interleaved, float magnitude, int head_dim, const qh_rope_rows* q,

@@ -167,7 +167,7 @@ hipError_t rmsnorm_of(const NormArgs& a, hipStream_t s) {
 // ------------------------------------------------------------------------------------------------------- rope
 
 // cos and sin of 2 pi t, |t| <= 1/2. t is brought within an eighth of a turn of a multiple of a quarter, exactly; there the
-// power series to x^9 and x^8 are off by less than 2^-27.
+// power series to x^9 and x^10 end less than 2^-29 short.
 __device__ __forceinline__ float2 turn(double t) {
     const double k = __builtin_rint(4.0 * t);
     const float x = (float)((4.0 * t - k) * 1.5707963267948966), z = x * x;
