@@ -423,7 +423,10 @@ int qh_rmsnorm(const void* x, const void* res, const float* w, int dtype, int64_
  *   QH_ROPE_BASE   theta * factor^(rot_dim / (rot_dim - 2)) in theta's place: the slowest pair is divided by factor, the first
  *                  by nothing (rot_dim 2: as it is)
  *   QH_ROPE_PARTS  by parts: pairs that turn at most `low` times over `context` positions are divided by factor, those that
- *                  turn `high` times or more are left, with a ramp linear in the turns between them */
+ *                  turn `high` times or more are left, with a ramp linear in the TURNS between them, as the schedule is
+ *                  published. Programs that ramp linearly in the pair's index between those two ends turn the pairs between
+ *                  them otherwise: for a model that was made with one, give qh_rope that table. What cosines and sines are
+ *                  multiplied by (often 0.1 log(factor) + 1) is qh_rope's `magnitude` */
 enum { QH_ROPE_PLAIN = 0, QH_ROPE_LINEAR = 1, QH_ROPE_BASE = 2, QH_ROPE_PARTS = 3 };
 typedef struct qh_rope_desc {
     double theta;
@@ -449,9 +452,10 @@ typedef struct qh_rope_rows {
 /* Rotary positions: every head of q's and k's rows (k NULL: q alone) has its first rot_dim dims turned in pairs (a, b) ->
  * (a cos - b sin, a sin + b cos) by the angle 2 pi pos[t] turns[i], cos and sin times `magnitude`; the others are copied. A
  * pair is the dims i and i + rot_dim / 2, or (interleaved 1) 2 i and 2 i + 1. pos: DEVICE int32 [n_tok], of either sign;
- * turns: DEVICE [rot_dim / 2]. Angles are taken in 64 bits less their whole turns: with
- * qh_rope_turns' table they are off by up to some 2^-51 of the angle (2^-49 where rot_dim is no power of two), by the table's
- * rounding and the product's: below f32's step up to 10^8 positions, 5e-7 radians at int32's ends. Rows of dtype QH_F32 or QH_F16 on any alignment of their type; head_dim at most QH_ROPE_MAX_DIM.
+ * turns: DEVICE [rot_dim / 2]. Angles are taken in 64 bits less their whole turns: with qh_rope_turns' table they are off by up to
+ * some 2^-51 of the angle (2^-49 where rot_dim is no power of two), by the table's rounding and the product's: below f32's step up
+ * to 10^8 positions, 5e-7 radians at int32's ends. Rows of dtype QH_F32 or QH_F16 on any alignment of their type; head_dim at most
+ * QH_ROPE_MAX_DIM.
  * Replaces: the rotation in Model::forward (reference model.cpp:187-196), for many sequences' tokens; the decoder's own
  * kernels keep the reference's f32 table to the bit. */
 int qh_rope(const double* turns, int rot_dim, int interleaved, float magnitude, int head_dim, const qh_rope_rows* q,

@@ -703,8 +703,9 @@ def rmsnorm_q8(x, w, eps: float = 1e-6, residual=None, sum=None):
 class Rope:
     """Rotary positions of heads of head_dim, the first rot_dim dims of each (all by default) in pairs (i, i + rot_dim / 2),
     or (2 i, 2 i + 1) when interleaved. scaling: None, "linear", "base" or "parts" (qh_rope_desc), with factor and, by
-    parts, context, low and high; magnitude: what cosines and sines are multiplied by. turns: a table of one's own in
-    place of those (float64 [rot_dim / 2]: turns of 2 pi per position)."""
+    parts, context, low and high (the ramp between them is linear in a pair's turns, not in its index); magnitude: what
+    cosines and sines are multiplied by. turns: a table of one's own in place of those (float64 [rot_dim / 2]: turns of 2 pi per
+    position)."""
 
     def __init__(self, head_dim: int, rot_dim: int | None = None, interleaved: bool = False, theta: float = 1e6,
                  scaling: str | None = None, factor: float = 1.0, context: float = 0.0, low: float = 1.0, high: float = 32.0,
