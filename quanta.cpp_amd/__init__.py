@@ -815,7 +815,8 @@ def beam_select(logits, scores, beams: int, k: int, n_valid: int | None = None):
     """The k best continuations of each prompt's beams: logits [prompts * beams][vocabulary] (float32 or float16; views of
     wider rows are fine), scores float32 [prompts * beams] or None (0), n_valid: ids from it on do not count. Returns
     (parent, token, score), each [prompts][k], best first: the row that is continued, the id (both int32) and
-    score + log-softmax (float32); -1, -1 and -inf where there are fewer candidates. See qh_beam_select."""
+    score + log-softmax (float32); -1, -1 and -inf where there are fewer candidates. The three are views of one tensor that also
+    holds the call's workspace (up to a few KB a row): clone what is kept for long. See qh_beam_select."""
     torch = _torch()
     stream, dtype, ld = _here(logits), _dtype_of(logits, "logits"), _row_stride(logits, "logits")
     rows, n = logits.shape
