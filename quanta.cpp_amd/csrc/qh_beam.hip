@@ -2,11 +2,11 @@
 //     score_b + logit_bv - log sum_u exp(logit_bu),
 // ties to the lower (b, v). Two launches:
 //   1. over the whole GPU (beam_rows_kernel): every logit once, for the largest of each group of ids and, wave by wave, the
-//      sum of exponentials. Bound by memory (192 x 151,936 f32: 26.8 us, 4.4 TB/s with start and end).
+//      sum of exponentials. Bound by memory (192 x 151,936 f32: 26.9 us, 4.3 TB/s with start and end).
 //   2. a workgroup to a prompt (beam_pick_kernel): the rows' sums, then the k best groups by their largest candidate (a
 //      group that is not among them holds none of the k best candidates, for k others have one before its own best), and
 //      the k best of what those groups hold. Bound by latency: sums, groups, their logits and ranks wait for each other, and
-//      what sixteen waves all compute costs each SIMD four times (4 beams 5.6 us, 24 prompts of 8 9.7).
+//      what sixteen waves all compute costs each SIMD four times (4 beams 5.3 us, 24 prompts of 8 8.7).
 // Candidates of different rows meet in the order of their scores, so sums, exponentials and scores are 64-bit: rounded to
 // f32, scores that are 2^-20 apart would tie. (A 64-bit multiply-add takes no longer than a 32-bit one here.)
 #include "qh_device.h"

@@ -28,9 +28,9 @@ __device__ __forceinline__ void load_e(const T* p, int n, float (&x)[kE<T>]) {
         for (int i = 0; i < kE<T>; ++i) x[i] = i < n ? (float)p[i] : 0.0f;
     }
 }
-// Stores pass by the caches, whose lines the loads of rows to come take: 16,000 x 4,096 f16 norms with residual 84.9 us, by plain
-// stores 98.7, and 161.9 and 166.2 with an addition that reads both results next; 512 x 4,096 5.5 and 6.2, 10.9 and 11.1; 8,000
-// tokens of 40 heads of 128 f16 turned 26.5 and 28.1. (8-bit codes, a quarter of the bytes, do not: 8,000 x 5,120 with their
+// Stores pass by the caches, whose lines the loads of rows to come take: 16,000 x 4,096 f16 norms with residual 84.0 us replayed one after
+// the other, by plain stores 99.3, and 161.9 and 166.2 with an addition that reads both results next; 512 x 4,096 5.4 and 6.1, 10.9
+// and 11.1; 8,000 tokens of 40 heads of 128 f16 turned 26.5 and 28.2. (8-bit codes, a quarter of the bytes, do not: 8,000 x 5,120 with their
 // reading back 173, past the caches 200.)
 template <typename T>
 __device__ __forceinline__ void store_e(T* p, int n, const float (&x)[kE<T>]) {
@@ -72,7 +72,7 @@ __device__ __forceinline__ void quant_lanes(const float (&v)[8], int8_t* q, floa
 // of squares and the scaled products are 64-bit (as fast as 32-bit ones here, and far from the memory's time): no square
 // overflows, the order of the sum does not show, and y is rounded to f32 once (f16 rows from there, so by 2^-11 and 2^-24: a
 // single rounding from 64 bits has no instruction). Bound by memory: 4,001 x 5,120 f32 with residual into blocks 49.3 us, 16,000 x
-// 4,096 f16 with residual 91.6, 5.5 and 5.7 TB/s; 1 x 896 2.4.
+// 4,096 f16 with residual 91.6 among calls into new rows (84 replayed), 5.5 and 5.7 TB/s; 1 x 896 2.4.
 template <typename T, int kWaves, int kVec>
 __global__ __launch_bounds__(kWaves < 4 ? 256 : 64 * kWaves) void rmsnorm_kernel(NormArgs a) {
     constexpr int E = kE<T>, kRows = kWaves < 4 ? 4 / kWaves : 1, kPass = 64 * kWaves * E;
@@ -151,7 +151,7 @@ hipError_t rmsnorm_of(const NormArgs& a, hipStream_t s) {
                   dim3(kWaves < 4 ? 256 : 64 * kWaves), 0, s, a);
     };
     using std::integral_constant;
-    // Loads in flight for waves enough, and one row's lanes not far apart (16,000 x 4,096 f16: 98.5 us, a wave to a row with 8
+    // Loads in flight for waves enough, and one row's lanes not far apart (all by plain stores: 16,000 x 4,096 f16 98.5 us, a wave to a row with 8
     // vectors 162, eight with one 104; 16,000 x 256 f32 with a wave 27.9, with four 33.5; 16,000 x 8,192 f16 197.7, four waves with
     // four vectors 201.5; 64 x 8,192 f32 5.7 with eight waves, four 6.7; 2,000 x 16,384 f32 176, four waves with 16 vectors 183)
     if (vecs <= 64) run(integral_constant<int, 1>{}, integral_constant<int, 1>{});
