@@ -275,6 +275,12 @@ __global__ __launch_bounds__(64 * kW, (Prompt<T, kHd, kTile, kW>::kSimdWaves)) v
     const float lift = kN == 1 ? -6.0f : (float)(shift + 8);
     const float limit = kN == 1 ? 32768.0f : __builtin_ldexpf((float)(kTile / 2), -shift);
     float base = vis > 0 ? -__builtin_inff() : 0.0f, sum = 0.0f;  // a row that sees nothing asks for no base
+    // A weight is 2^(s * times - base) by one fused step, whose s * times is exact where the base was rounded: they are up to 2^-24 of
+    // the base apart, which is nothing up to some 2^20, and from 2^26 on would make weights of 0 or infinity. Rows with such a base have
+    // their scores multiplied and rounded first, as the base was, and `times` 1.
+    constexpr float kFar = 0x1p20f;
+    float times = a.scale_log2e;
+    bool any_far = false;
 
     Raw<T> kr[kDirect ? 1 : P::kPer], vr[kDirect ? 1 : P::kPer];
     const T* const kp = static_cast<const T*>(a.k) + (int64_t)kvh * kHd;
@@ -459,15 +465,16 @@ __global__ __launch_bounds__(64 * kW, (Prompt<T, kHd, kTile, kW>::kSimdWaves)) v
         Parts<T> w[kKt][2];  // weights 2^(scale s - base) of a block, two operands of 16 keys
         float l[kKt];
         auto mask = [&](int kt) {
-            if (masked) {
+            if (masked || any_far) {
+                const float before = times == 1.0f ? a.scale_log2e : 1.0f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    s[kt][i] = pos0 + 32 * kt + 8 * (i >> 2) + 4 * half + (i & 3) < vis ? s[kt][i] : -__builtin_inff();
+                    s[kt][i] = pos0 + 32 * kt + 8 * (i >> 2) + 4 * half + (i & 3) < vis ? s[kt][i] * before : -__builtin_inff();
             }
         };
         auto weights2 = [&](int kt, int n, float from) {  // values 2 n and 2 n + 1 of the block's 16
-            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][2 * n], a.scale_log2e, -from));
-            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][2 * n + 1], a.scale_log2e, -from));
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][2 * n], times, -from));
+            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][2 * n + 1], times, -from));
             Parts<T>& to = w[kt][n >> 2];
             if (n == 0) l[kt] = 0.0f;
             if constexpr (kN == 1) {
@@ -529,7 +536,7 @@ __global__ __launch_bounds__(64 * kW, (Prompt<T, kHd, kTile, kW>::kSimdWaves)) v
             if (__any(!(l[kt] <= limit))) {
                 float top = -__builtin_inff();
 #pragma unroll
-                for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, s[kt][i] * a.scale_log2e);
+                for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, s[kt][i] * times);
                 top = __builtin_fmaxf(top, other_half(top));
                 // only rows that ask for it (either half of one), so that no row depends on its neighbours
                 const float both = other_half(l[kt]);
@@ -537,6 +544,18 @@ __global__ __launch_bounds__(64 * kW, (Prompt<T, kHd, kTile, kW>::kSimdWaves)) v
                 const float now = asks ? __builtin_fmaxf(base, top + lift) : base;
                 const float f = now == base ? 1.0f : __builtin_amdgcn_exp2f(base - now);
                 base = now;
+                const bool far = times != 1.0f && __builtin_fabsf(base) >= kFar && base != -__builtin_inff();
+                if (__any(far)) {
+                    any_far = true;
+                    if (far) {
+                        times = 1.0f;
+#pragma unroll
+                        for (int b = 0; b < kKt; ++b)  // the blocks whose scores stand (a later one is multiplied by its mask)
+                            if (b >= kt)
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) s[b][i] *= a.scale_log2e;
+                    }
+                }
                 sum *= f;
 #pragma unroll
                 for (int d = 0; d < kDt; ++d)
