@@ -475,7 +475,8 @@ int qh_rope(const double* turns, int rot_dim, int interleaved, float magnitude, 
  * more of every value from 2^-110 up, whatever the others are; of smaller ones what is above 2^-133; and a result of small values
  * is off by up to keys^2 * 2^-137 besides (6e-36 for 1,000 keys). Sums in f32 (a row that sees a score past f32's range may be NaN),
  * in an order that follows the whole call: a sequence's rows have the same bits in every call of the same shape and starts, but
- * not in another batch. out overlaps no input. The workspace is 16-byte aligned and needs no initialisation (NULL where the size is 0); calls that overlap must not share one.
+ * not in another batch. out overlaps no input. The workspace is 16-byte aligned and needs no initialisation (NULL where the size
+ * is 0); calls that overlap must not share one.
  * No counterpart in the reference, whose prompts attend to its cache in chunks (Model::forward_batch, model.cpp:387-405). */
 size_t qh_attention_workspace_bytes(int dtype, int n_heads, int n_kv_heads, int head_dim, int n, int n_tok, int n_keys);
 int qh_attention(const void* q, const void* k, const void* v, void* out, int dtype, int n_heads, int n_kv_heads,

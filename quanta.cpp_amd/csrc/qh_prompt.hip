@@ -270,7 +270,8 @@ __global__ __launch_bounds__(64 * kW, (Prompt<T, kHd, kTile, kW>::kSimdWaves)) v
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
     // A new base puts the largest weight at 2^-lift, and a tile's sum asks for one above `limit`. f32: at most 1 / 2 for all
-    // weights of a row together, so that no sum of weighted values overflows before it is divided.
+    // weights of a row together, so that no sum of weighted values overflows before it is divided (the lift shows in a base up to
+    // 2^28; beyond, weights are at most 1 each).
     const int shift = kN == 1 ? 0 : 33 - __builtin_clz((unsigned)max(e.keys, 1));
     const float lift = kN == 1 ? -6.0f : (float)(shift + 8);
     const float limit = kN == 1 ? 32768.0f : __builtin_ldexpf((float)(kTile / 2), -shift);
