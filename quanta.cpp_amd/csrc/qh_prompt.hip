@@ -237,7 +237,8 @@ __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)"
 // tokens of 32 heads of 128 over 8: 1,198 us, by registers 1,267).
 // Bound by the issue of instructions: that call takes 1,145 to 1,237 us with eight waves on several cards, 1,031 to 954 TFLOP/s, its
 // matrix instructions busy for 49% of the cycles and vector instructions issued in 31%; 16 f32 prompts of up to 2,000 tokens of 14
-// heads of 64 over 2 take 309 to 329, 47% and 39%; the same prompts in f16 110, 467 TFLOP/s, 19% and 27%. A call of few rows is bound by the tiles that a workgroup takes one after the other (512 of those tokens: 14.8 us).
+// heads of 64 over 2 take 309 to 329, 47% and 39%; the same prompts in f16 110, 467 TFLOP/s, 19% and 27%. A call of few rows is bound
+// by the tiles that a workgroup takes one after the other (512 of those tokens: 14.5 us).
 template <typename T, int kHd, int kTile, int kW, bool kDirect>
 __global__ __launch_bounds__(64 * kW, (Prompt<T, kHd, kTile, kW>::kSimdWaves)) void prompt_kernel(PromptArgs a) {
     typedef Prompt<T, kHd, kTile, kW> P;
@@ -757,9 +758,9 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a) {
 }
 
 // Calls f with the element type and, as constants, head_dim, keys of a tile and waves: eight where that leaves a row tile to
-// every compute unit, else four (12,001 tokens of 32 heads of 128 over 8, f16, timed in turn: 1,149 us and, with four,
-// 1,186; on another card 1,237 and 1,284; with fewer row tiles, f16, 1,500 tokens of 14 heads of 64 over 2: 26.7 and, with four, 24.3; f32, 300 of 32 of 128: 28.7 and 24.0). f32 heads of 64
-// stay with four, whose workgroups do not wait for each other (16 prompts of up to 2,000 tokens: 322 us, eight waves over 64 keys
+// every compute unit, else four (12,001 tokens of 32 heads of 128 over 8, f16, timed in turn: 1,149 us and, with four, 1,186; on
+// another card 1,237 and 1,284; with fewer row tiles, f16, 1,500 tokens of 14 heads of 64 over 2: 26.7 and, with four, 24.3; f32, 300
+// of 32 of 128: 28.7 and 24.0). f32 heads of 64 stay with four, whose workgroups do not wait for each other (16 prompts of up to 2,000 tokens: 322 us, eight waves over 64 keys
 // 340).
 template <typename F>
 void by_shape(int dtype, int hd, int group, int n_kv, int n_tok, F&& f) {

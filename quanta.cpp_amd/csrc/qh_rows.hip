@@ -28,10 +28,10 @@ __device__ __forceinline__ void load_e(const T* p, int n, float (&x)[kE<T>]) {
         for (int i = 0; i < kE<T>; ++i) x[i] = i < n ? (float)p[i] : 0.0f;
     }
 }
-// Stores pass by the caches, whose lines the loads of rows to come take: 16,000 x 4,096 f16 norms with residual 84.0 us replayed one after
-// the other, by plain stores 99.3, and 161.9 and 166.2 with an addition that reads both results next; 512 x 4,096 5.4 and 6.1, 10.9
-// and 11.1; 8,000 tokens of 40 heads of 128 f16 turned 26.5 and 28.2. (8-bit codes, a quarter of the bytes, do not: 8,000 x 5,120 with their
-// reading back 173, past the caches 200.)
+// Stores pass by the caches, whose lines the loads of rows to come take: 16,000 x 4,096 f16 norms with residual 84.0 us replayed
+// one after the other, by plain stores 99.3, and 161.9 and 166.2 with an addition that reads both results next; 512 x 4,096 5.4 and
+// 6.1, 10.9 and 11.1; 8,000 tokens of 40 heads of 128 f16 turned 26.5 and 28.2. (8-bit codes, a quarter of the bytes, do not: 8,000 x
+// 5,120 with their reading back 173, past the caches 200.)
 template <typename T>
 __device__ __forceinline__ void store_e(T* p, int n, const float (&x)[kE<T>]) {
     if (n >= kE<T>) {
@@ -151,9 +151,10 @@ hipError_t rmsnorm_of(const NormArgs& a, hipStream_t s) {
                   dim3(kWaves < 4 ? 256 : 64 * kWaves), 0, s, a);
     };
     using std::integral_constant;
-    // Loads in flight for waves enough, and one row's lanes not far apart (all by plain stores: 16,000 x 4,096 f16 98.5 us, a wave to a row with 8
-    // vectors 162, eight with one 104; 16,000 x 256 f32 with a wave 27.9, with four 33.5; 16,000 x 8,192 f16 197.7, four waves with
-    // four vectors 201.5; 64 x 8,192 f32 5.7 with eight waves, four 6.7; 2,000 x 16,384 f32 176, four waves with 16 vectors 183)
+    // Loads in flight for waves enough, and one row's lanes not far apart (all by plain stores: 16,000 x 4,096 f16 98.5 us, a wave to a
+    // row with 8 vectors 162, eight with one 104; 16,000 x 256 f32 with a wave 27.9, with four 33.5; 16,000 x 8,192 f16 197.7, four
+    // waves with four vectors 201.5; 64 x 8,192 f32 5.7 with eight waves, four 6.7; 2,000 x 16,384 f32 176, four waves with 16 vectors
+    // 183)
     if (vecs <= 64) run(integral_constant<int, 1>{}, integral_constant<int, 1>{});
     else if (vecs <= 256) run(integral_constant<int, 4>{}, integral_constant<int, 1>{});
     else if (vecs <= 512) run(integral_constant<int, 4>{}, integral_constant<int, 2>{});

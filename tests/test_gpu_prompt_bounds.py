@@ -37,7 +37,8 @@ def test_a_sequence_alone(qh, gpu, dtype, heads, kv, hd, rows, behind):
     gen = torch.Generator(device=gpu).manual_seed(len(rows))
     keys = [m + behind for m in rows]
     st, kst = starts(rows), starts(keys)
-    q, k, v = (torch.randn(n, h, hd, generator=gen, device=gpu).to(TYPES[dtype]) for n, h in ((st[-1], heads), (kst[-1], kv), (kst[-1], kv)))
+    shapes = ((st[-1], heads, hd), (kst[-1], kv, hd), (kst[-1], kv, hd))
+    q, k, v = (torch.randn(shape, generator=gen, device=gpu).to(TYPES[dtype]) for shape in shapes)
     got = qh.attention(q, k, v, ints(st, gpu), ints(kst, gpu))
     want, err, mine = formula(q, k, v, st, kst, True, hd ** -0.5)
     check(got, want, err, mine)
