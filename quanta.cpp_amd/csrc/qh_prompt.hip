@@ -11,7 +11,7 @@
 //   each). Rows of shared memory are cut in 16-byte chunks whose places are permuted by the row (swizzle), so that neither the
 //   16 rows of a key operand nor the 4 rows of a value operand meet in a bank.
 //   f16: the operands as they are; weights rounded to f16 once, and their sum taken of the rounded ones. (With two f16 of each weight
-//   the error against 64 bits is 2.05e-4, which the rounding of the result alone is, in place of 2.6e-4 to 2.7e-4; but 12,001 tokens
+//   the error against 64 bits is 2.05e-4, which the rounding of the result alone is, in place of 2.3e-4 to 2.9e-4; but 12,001 tokens
 //   of 32 heads of 128 take 1,599 us in place of 1,176, 16 prompts of up to 2,000 of 14 heads of 64 135 in place of 110, and a token
 //   behind 4,000 15.4 in place of 14.4.)
 //   f32: every value as three bf16 (8 bits each: the first cut off, the others rounded, the last exact down to bf16's smallest,

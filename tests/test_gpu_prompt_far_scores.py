@@ -73,3 +73,24 @@ def test_keys_of_one_score_share(qh, gpu, hd, sign, dtype, size):
     got = qh.attention(q, k, v, ints([0, 3], gpu), ints([0, keys], gpu), causal=False)
     part = v[500:] if sign > 0 else v[:500]
     close(got, part.double().mean(0).expand(3, 2, hd), dtype, len(part))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("keys", [150, 1500])
+def test_rows_next_to_far_ones(qh, gpu, hd, dtype, keys):
+    """Rows of ordinary scores have the same bits whether their neighbours' scores are ordinary or far, from the first key on or later."""
+    gen = torch.Generator(device=gpu).manual_seed(keys)
+    q, k, v = (torch.randn(n, 4, hd, generator=gen, device=gpu).to(TYPES[dtype]) for n in (150, keys, keys))
+    q[..., 1] = 0.0
+    k[..., 1] = 0.0
+    k[keys // 2:, :, 1] = 30000.0  # of weight for queries that have this dim alone
+    starts = ints([0, 150], gpu), ints([0, keys], gpu)
+    clean = qh.attention(q, k, v, *starts)
+    q[7, 1, 1], q[40:43, :, 1] = 20000.0, -20000.0
+    q[90, 2] *= 16000.0
+    got = qh.attention(q, k, v, *starts)
+    same = torch.ones(150, 4, dtype=torch.bool, device=gpu)
+    same[7, 1] = same[40:43] = same[90, 2] = False
+    assert torch.equal(got[same], clean[same])
+    assert bool(torch.isfinite(got).all())
